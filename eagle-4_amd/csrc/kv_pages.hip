@@ -1,0 +1,346 @@
+// Rows quantised into fp8-e4m3 pages with one scale per (page, head), and gathered back, on gfx950.
+//
+// Mathematics. A page's scale s is a power of two, the least with amax <= 448 s over the page's rows: value x is held as
+// e4m3(x / s). e4m3 is a floating format, so its relative error (2^-4) is the same at any scale and a power of two costs
+// no precision against amax / 448; x / s is exact, so each value is rounded once, and when later rows make a page's scale
+// grow by 2^k its earlier rows move by k binades: exact but where they leave e4m3's normal range (below 2^-6 of the new
+// scale), as those values lie there in any case. The earlier rows of a page (positions below the context) are re-encoded
+// only when the scale grows; a page that starts at or after the context starts afresh, whatever it held.
+//
+// Both directions are bound by HBM where there is much to move, and by one chain of dependent loads (lengths, page
+// table, rows, scale) where there is little.
+
+#include "common.h"
+
+namespace {
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+constexpr float kMaxE4m3 = 448.f;
+
+// The least power of two s with amax <= 448 s (448 = 1.75 * 2^8), by its bits; at least 2^-126, 0 for 0.
+E4_DEV float page_scale(float amax) {
+  const uint32_t bits = __float_as_uint(amax);
+  if (bits == 0) return 0.f;
+  const int e = static_cast<int>(bits >> 23) - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+  return __uint_as_float(static_cast<uint32_t>(e < 1 ? 1 : e) << 23);
+}
+
+// Two values of magnitude at most 448 (or NaN) rounded to e4m3, nearest even.
+E4_DEV uint32_t encode2(float x, float y) {
+  return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(x, y, 0, false)) & 0xffffu;
+}
+// x / s as e4m3 takes it: an infinity saturates, NaN stays.
+E4_DEV float scaled(float x, float inv) {
+  const float y = x * inv;
+  return __builtin_fabsf(x) == INFINITY ? __builtin_copysignf(kMaxE4m3, x) : y;
+}
+E4_DEV float finite_abs(float x) {
+  const float a = __builtin_fabsf(x);
+  return a < INFINITY ? a : 0.f;
+}
+
+// N values from fp8 (N 8: one 8-byte load) and back.
+template <int N>
+E4_DEV void load_codes(const uint8_t* p, float (&x)[N]) {
+  if constexpr (N == 8) {
+    const u32x2 w = *reinterpret_cast<const u32x2*>(p);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(w[i], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(w[i], true);
+      x[4 * i] = lo[0];
+      x[4 * i + 1] = lo[1];
+      x[4 * i + 2] = hi[0];
+      x[4 * i + 3] = hi[1];
+    }
+  } else {
+    x[0] = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<uint32_t>(*p), false)[0];
+  }
+}
+template <int N>
+E4_DEV void store_codes(uint8_t* p, const float (&x)[N]) {
+  if constexpr (N == 8) {
+    u32x2 w;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) w[i] = encode2(x[4 * i], x[4 * i + 1]) | encode2(x[4 * i + 2], x[4 * i + 3]) << 16;
+    *reinterpret_cast<u32x2*>(p) = w;
+  } else {
+    *p = static_cast<uint8_t>(encode2(x[0], 0.f));
+  }
+}
+
+// A chunk of N elements (8: 16-byte loads) of dtype T as loaded, and widened.
+template <typename T, int N>
+struct Chunk {
+  static constexpr int kWords = N * static_cast<int>(sizeof(typename T::storage)) / 4;
+  u32x4 w[N == 8 ? kWords / 4 : 1];
+  E4_DEV void load(const typename T::storage* p) {
+    if constexpr (N == 8) {
+#pragma unroll
+      for (int i = 0; i < kWords / 4; ++i) w[i] = reinterpret_cast<const u32x4*>(p)[i];
+    } else if constexpr (sizeof(typename T::storage) == 4) {
+      w[0][0] = __float_as_uint(*p);
+    } else {
+      w[0][0] = *p;
+    }
+  }
+  E4_DEV void widen(float (&x)[N]) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if constexpr (sizeof(typename T::storage) == 4)
+        x[i] = __uint_as_float(w[i / 4][i % 4]);
+      else
+        x[i] = T::to_f32(static_cast<uint16_t>(w[0][i / 2] >> (16 * (i % 2))));
+    }
+  }
+};
+
+// One wave per (matrix, head, page, request); waves of a workgroup take adjacent heads. `pages`: pages a request's rows can
+// reach at most. The page's rows stay in registers between the maximum and the rounding where they fit in kHeld chunks a
+// lane (16 rows of 256 elements), else they are read twice.
+template <typename T, int N>
+__global__ __launch_bounds__(256) void write_kernel(const eagle4_write_kv_args a, int pages) {
+  using S = typename T::storage;
+  constexpr int kHeld = N == 8 ? 8 : 4;
+  const int lane = threadIdx.x & 63;
+  const int item = blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int matrices = a.value != nullptr ? 2 : 1;
+  const int p = item / (a.heads * matrices), hm = item % (a.heads * matrices);
+  const int head = hm % a.heads, b = blockIdx.y;
+  const bool second = hm >= a.heads;
+  if (p >= pages) return;
+
+  const int64_t context = e4::ld(a.context_lens, b);
+  const int64_t start = e4::ld(a.query_start_loc, b);
+  const int64_t end = e4::ld(a.query_start_loc, b + 1);
+  int64_t slot = 0, count = end - start;
+  if (a.path.ptr != nullptr) {
+    slot = e4::ld(a.idx_mapping, b);
+    if (slot < 0 || slot >= a.path_slots) return;
+    count = e4::ld(a.path_len, slot);
+    count = count < a.path_width ? count : a.path_width;
+  }
+  count = count < a.max_rows ? count : a.max_rows;
+  if (context < 0 || count <= 0 || start < 0 || end > a.tokens) return;
+  const int64_t index = context / a.page + p, first = index * a.page;
+  const int64_t lo = first > context ? first : context;
+  const int64_t hi = first + a.page < context + count ? first + a.page : context + count;
+  if (lo >= hi || index >= a.max_blocks) return;
+  const int64_t block = e4::ld(a.block_table, b, index);
+  if (block < 0 || block >= a.num_blocks) return;
+
+  const S* const src = static_cast<const S*>(second ? a.value : a.key) + head * (second ? a.stride_vh : a.stride_kh);
+  const int64_t stride_row = second ? a.stride_vt : a.stride_kt;
+  uint8_t* const dst = static_cast<uint8_t*>(second ? a.value_cache : a.key_cache) +
+                       block * (second ? a.stride_vcb : a.stride_kcb) + head * (second ? a.stride_vch : a.stride_kch);
+  const int64_t stride_slot = second ? a.stride_vcs : a.stride_kcs;
+  float* const scale = (second ? a.v_scale : a.k_scale) + block * (second ? a.stride_vsb : a.stride_ksb) +
+                       head * (second ? a.stride_vsh : a.stride_ksh);
+  const float held_scale = *scale;
+
+  const int per_row = a.dim / N, rows = static_cast<int>(hi - lo), chunks = rows * per_row;
+  // the source of chunk c; null where the path names no row of the request
+  auto source = [&](int c) -> const S* {
+    const int r = c / per_row, col = (c - r * per_row) * N;
+    const int64_t j = lo - context + r;
+    const int64_t row = a.path.ptr != nullptr ? e4::ld(a.path, slot, j) : j;
+    if (row < 0 || row >= end - start) return nullptr;
+    return src + (start + row) * stride_row + col;
+  };
+  Chunk<T, N> held[kHeld];
+  const S* from[kHeld];
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) {
+    const int c = lane + 64 * i;
+    from[i] = c < chunks ? source(c) : nullptr;
+  }
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i)
+    if (from[i] != nullptr) held[i].load(from[i]);
+  float amax = 0.f;
+  auto most = [&](const Chunk<T, N>& ch) {
+    float x[N];
+    ch.widen(x);
+#pragma unroll
+    for (int i = 0; i < N; ++i) amax = fmaxf(amax, finite_abs(x[i]));
+  };
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i)
+    if (from[i] != nullptr) most(held[i]);
+  for (int c = lane + 64 * kHeld; c < chunks; c += 64) {
+    const S* const s = source(c);
+    if (s == nullptr) continue;
+    Chunk<T, N> ch;
+    ch.load(s);
+    most(ch);
+  }
+  amax = e4::group_max<64>(amax);
+
+  const int kept = static_cast<int>(lo - first);  // earlier rows of the page
+  const float old = kept > 0 ? held_scale : 0.f;
+  const float now = fmaxf(old, page_scale(amax));
+  const float inv = now > 0.f ? 1.0f / now : 0.f;
+  if (kept > 0 && now > old) {
+    const float ratio = old * inv;
+    for (int c = lane; c < kept * per_row; c += 64) {
+      const int r = c / per_row, col = (c - r * per_row) * N;
+      float x[N];
+      load_codes<N>(dst + r * stride_slot + col, x);
+#pragma unroll
+      for (int i = 0; i < N; ++i) x[i] *= ratio;
+      store_codes<N>(dst + r * stride_slot + col, x);
+    }
+  }
+  auto put = [&](const Chunk<T, N>& ch, int c) {
+    const int r = c / per_row, col = (c - r * per_row) * N;
+    float x[N];
+    ch.widen(x);
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = scaled(x[i], inv);
+    store_codes<N>(dst + (kept + r) * stride_slot + col, x);
+  };
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i)
+    if (from[i] != nullptr) put(held[i], lane + 64 * i);
+  for (int c = lane + 64 * kHeld; c < chunks; c += 64) {
+    const S* const s = source(c);
+    if (s == nullptr) continue;
+    Chunk<T, N> ch;
+    ch.load(s);
+    put(ch, c);
+  }
+  if (lane == 0) *scale = now;
+}
+
+// One workgroup per (run of `rows` positions, request), all heads of both matrices. A page that the table does not have (or
+// names out of range) reads as zeros.
+template <typename T, int N>
+__global__ __launch_bounds__(256) void read_kernel(const eagle4_read_kv_args a, int rows) {
+  using S = typename T::storage;
+  const int b = blockIdx.y;
+  const int64_t start = e4::ld(a.start_loc, b), end = e4::ld(a.start_loc, b + 1);
+  const int64_t lo = static_cast<int64_t>(blockIdx.x) * rows;
+  if (start < 0 || end > a.tokens || lo >= end - start || lo >= a.max_len) return;
+  const int64_t most = end - start < a.max_len ? end - start : a.max_len;
+  const int n = static_cast<int>(most - lo < rows ? most - lo : rows);
+  const int per_head = a.dim / N, per_row = per_head * a.heads, total = n * per_row;
+  const int matrices = a.value != nullptr ? 2 : 1;
+  for (int c = threadIdx.x; c < total * matrices; c += 256) {
+    const bool second = c >= total;
+    const int at = second ? c - total : c;
+    const int r = at / per_row, hc = at - r * per_row, head = hc / per_head, col = (hc - head * per_head) * N;
+    const int64_t pos = lo + r, index = pos / a.page;
+    const int64_t block = index < a.max_blocks ? e4::ld(a.block_table, b, index) : -1;
+    float x[N];
+    if (block >= 0 && block < a.num_blocks) {
+      const uint8_t* const src = static_cast<const uint8_t*>(second ? a.value_cache : a.key_cache) +
+                                 block * (second ? a.stride_vcb : a.stride_kcb) +
+                                 (pos - index * a.page) * (second ? a.stride_vcs : a.stride_kcs) +
+                                 head * (second ? a.stride_vch : a.stride_kch) + col;
+      const float s = second ? a.v_scale[block * a.stride_vsb + head * a.stride_vsh]
+                             : a.k_scale[block * a.stride_ksb + head * a.stride_ksh];
+      load_codes<N>(src, x);
+#pragma unroll
+      for (int i = 0; i < N; ++i) x[i] *= s;
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) x[i] = 0.f;
+    }
+    S* const out = static_cast<S*>(second ? a.value : a.key) + (start + pos) * (second ? a.stride_vt : a.stride_kt) +
+                   head * (second ? a.stride_vh : a.stride_kh) + col;
+    if constexpr (N == 8) {
+      constexpr int kVecs = static_cast<int>(sizeof(S)) / 2;
+#pragma unroll
+      for (int v = 0; v < kVecs; ++v) {
+        u32x4 w;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if constexpr (sizeof(S) == 4)
+            w[i] = __float_as_uint(x[4 * v + i]);
+          else
+            w[i] = T::pack(x[2 * i], x[2 * i + 1]);
+        }
+        reinterpret_cast<u32x4*>(out)[v] = w;
+      }
+    } else {
+      *out = T::from_f32(x[0]);
+    }
+  }
+}
+
+bool tab_ok(const eagle4_itab& t) { return t.ptr != nullptr && e4::is_index_dtype(t.dtype); }
+bool multiple(int64_t v, int64_t of) { return v % of == 0; }
+bool aligned(const void* p, uintptr_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
+
+// Whether rows and pages can be moved eight elements at a time.
+template <typename A>
+bool vectors(const A& a) {
+  const bool v = a.value != nullptr;
+  for (const int64_t s : {int64_t(a.dim), a.stride_kt, a.stride_kh, a.stride_kcb, a.stride_kcs, a.stride_kch,
+                          v ? a.stride_vt : 0, v ? a.stride_vh : 0, v ? a.stride_vcb : 0, v ? a.stride_vcs : 0,
+                          v ? a.stride_vch : 0})
+    if (!multiple(s, 8)) return false;
+  return aligned(a.key, 16) && aligned(a.key_cache, 8) && (!v || (aligned(a.value, 16) && aligned(a.value_cache, 8)));
+}
+
+template <typename A>
+bool pages_ok(const A& a) {
+  return a.key != nullptr && a.key_cache != nullptr && a.k_scale != nullptr &&
+         (a.value == nullptr || (a.value_cache != nullptr && a.v_scale != nullptr)) && tab_ok(a.block_table) &&
+         a.heads > 0 && a.dim > 0 && a.page > 0 && a.max_blocks >= 0 && a.num_blocks >= 0 && a.num_reqs <= 65535 &&
+         int64_t(a.heads) * a.dim <= (1 << 20) && int64_t(a.dim) * a.page <= (1 << 24);
+}
+
+template <typename T>
+int launch_write(const eagle4_write_kv_args& a, hipStream_t s) {
+  // rows from any slot of a first page on reach at most this many pages
+  const int pages = e4::ceil_div(int64_t(a.max_rows) - 1, a.page) + 1;
+  const int64_t items = int64_t(pages) * a.heads * (a.value != nullptr ? 2 : 1);
+  if (items > (int64_t(1) << 30)) return EAGLE4_NOT_COVERED;
+  const dim3 grid(e4::ceil_div(items, 4), a.num_reqs);
+  if (vectors(a))
+    write_kernel<T, 8><<<grid, 256, 0, s>>>(a, pages);
+  else
+    write_kernel<T, 1><<<grid, 256, 0, s>>>(a, pages);
+  return E4_LAUNCH_STATUS();
+}
+
+template <typename T>
+int launch_read(const eagle4_read_kv_args& a, hipStream_t s) {
+  const int rows = 16;
+  const dim3 grid(e4::ceil_div(a.max_len, rows), a.num_reqs);
+  if (vectors(a))
+    read_kernel<T, 8><<<grid, 256, 0, s>>>(a, rows);
+  else
+    read_kernel<T, 1><<<grid, 256, 0, s>>>(a, rows);
+  return E4_LAUNCH_STATUS();
+}
+
+}  // namespace
+
+extern "C" int eagle4_write_kv_pages(const eagle4_write_kv_args* a, void* stream) {
+  if (a->num_reqs == 0 || a->max_rows <= 0) return EAGLE4_OK;
+  if (!pages_ok(*a) || a->num_reqs < 0 || !tab_ok(a->context_lens) || !tab_ok(a->query_start_loc)) return EAGLE4_NOT_COVERED;
+  if (a->path.ptr != nullptr && (!tab_ok(a->path) || !tab_ok(a->path_len) || !tab_ok(a->idx_mapping)))
+    return EAGLE4_NOT_COVERED;
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  switch (a->dtype) {
+    case EAGLE4_BF16: return launch_write<e4::Bf16>(*a, s);
+    case EAGLE4_F16: return launch_write<e4::F16>(*a, s);
+    case EAGLE4_F32: return launch_write<e4::F32>(*a, s);
+    default: return EAGLE4_NOT_COVERED;
+  }
+}
+
+extern "C" int eagle4_read_kv_pages(const eagle4_read_kv_args* a, void* stream) {
+  if (a->num_reqs == 0 || a->max_len <= 0) return EAGLE4_OK;
+  if (!pages_ok(*a) || a->num_reqs < 0 || !tab_ok(a->start_loc)) return EAGLE4_NOT_COVERED;
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  switch (a->dtype) {
+    case EAGLE4_BF16: return launch_read<e4::Bf16>(*a, s);
+    case EAGLE4_F16: return launch_read<e4::F16>(*a, s);
+    case EAGLE4_F32: return launch_read<e4::F32>(*a, s);
+    default: return EAGLE4_NOT_COVERED;
+  }
+}

@@ -23,6 +23,10 @@ extern "C" int64_t eagle4_args_size(int which) {
     case 14: return sizeof(eagle4_chainize_args);
     case 15: return sizeof(eagle4_row_attn_args);
     case 16: return sizeof(eagle4_mamba2_args);
+    case 17: return sizeof(eagle4_write_kv_args);
+    case 18: return sizeof(eagle4_read_kv_args);
+    case 19: return sizeof(eagle4_sample_tree_args);
+    case 20: return sizeof(eagle4_latent_attn_args);
     default: return -1;
   }
 }

@@ -211,7 +211,6 @@ class RowAttnArgs(ctypes.Structure):
     )
 
 
-# entry name -> (args struct, index in eagle4_args_size)
 class Mamba2Args(ctypes.Structure):
     _fields_ = _fields(
         "state:p stride_state_slot:q stride_state_head:q stride_state_dim:q x:p stride_x_tok:q stride_x_head:q dt:p "
@@ -222,6 +221,43 @@ class Mamba2Args(ctypes.Structure):
     )
 
 
+class WriteKvArgs(ctypes.Structure):
+    _fields_ = _fields(
+        "key:p value:p stride_kt:q stride_kh:q stride_vt:q stride_vh:q key_cache:p value_cache:p stride_kcb:q "
+        "stride_kcs:q stride_kch:q stride_vcb:q stride_vcs:q stride_vch:q k_scale:p v_scale:p stride_ksb:q "
+        "stride_ksh:q stride_vsb:q stride_vsh:q block_table:t context_lens:t query_start_loc:t idx_mapping:t path:t "
+        "path_len:t tokens:q num_reqs:i heads:i dim:i page:i max_blocks:i num_blocks:i max_rows:i path_width:i "
+        "path_slots:i dtype:i"
+    )
+
+
+class ReadKvArgs(ctypes.Structure):
+    _fields_ = _fields(
+        "key:p value:p stride_kt:q stride_kh:q stride_vt:q stride_vh:q key_cache:p value_cache:p stride_kcb:q "
+        "stride_kcs:q stride_kch:q stride_vcb:q stride_vcs:q stride_vch:q k_scale:p v_scale:p stride_ksb:q "
+        "stride_ksh:q stride_vsb:q stride_vsh:q block_table:t start_loc:t tokens:q num_reqs:i heads:i dim:i page:i "
+        "max_blocks:i num_blocks:i max_len:i dtype:i"
+    )
+
+
+class SampleTreeArgs(ctypes.Structure):
+    _fields_ = _fields(
+        "logits:p stride_row:q probs:p stride_prob:q drafted:t cu_num_logits:t idx_mapping:t parents:t coins:p "
+        "final_coins:p temperature:p sampled:p stride_sampled:q num_sampled:p path:p stride_path:q path_len:p rows:q "
+        "num_reqs:i width:i vocab:i slots:i dtype:i prob_dtype:i"
+    )
+
+
+class LatentAttnArgs(ctypes.Structure):
+    _fields_ = _fields(
+        "q:p stride_qt:q stride_qh:q latent_new:p stride_nt:q cache:p stride_cb:q stride_cs:q scale_page:p "
+        "stride_sp:q block_table:t context_lens:t query_start_loc:t masks:p stride_mask:q out:p stride_ot:q "
+        "stride_oh:q workspace:p workspace_bytes:q tokens:q scale:f num_reqs:i heads:i rank:i rope:i page:i "
+        "max_query_len:i max_blocks:i num_blocks:i dtype:i cache_dtype:i"
+    )
+
+
+# entry name -> (args struct, index in eagle4_args_size)
 ENTRIES = {
     "eagle4_stage_tree": (StageTreeArgs, 0),
     "eagle4_gdn_tree_ancestors": (AncestorsArgs, 1),
@@ -241,9 +277,13 @@ ENTRIES = {
     "eagle4_chainize": (ChainizeArgs, 14),
     "eagle4_row_attention": (RowAttnArgs, 15),
     "eagle4_mamba2_tree_state_update": (Mamba2Args, 16),
+    "eagle4_write_kv_pages": (WriteKvArgs, 17),
+    "eagle4_read_kv_pages": (ReadKvArgs, 18),
+    "eagle4_sample_tree": (SampleTreeArgs, 19),
+    "eagle4_latent_attention": (LatentAttnArgs, 20),
 }
-EXTRA_SYMBOLS = ("eagle4_verify_attention_workspace", "eagle4_verify_attention_static_bytes", "eagle4_version",
-                 "eagle4_args_size", "eagle4_init")
+EXTRA_SYMBOLS = ("eagle4_verify_attention_workspace", "eagle4_verify_attention_static_bytes",
+                 "eagle4_latent_attention_workspace", "eagle4_version", "eagle4_args_size", "eagle4_init")
 
 
 @functools.lru_cache(maxsize=None)
@@ -268,6 +308,8 @@ def library() -> ctypes.CDLL:
             raise RuntimeError(f"eagle4_amd: {struct.__name__} is {ctypes.sizeof(struct)} bytes here, {native} in {path}")
     lib.eagle4_verify_attention_workspace.argtypes = [ctypes.POINTER(AttnArgs)]
     lib.eagle4_verify_attention_workspace.restype = ctypes.c_int64
+    lib.eagle4_latent_attention_workspace.argtypes = [ctypes.POINTER(LatentAttnArgs)]
+    lib.eagle4_latent_attention_workspace.restype = ctypes.c_int64
     lib.eagle4_verify_attention_static_bytes.argtypes = []
     lib.eagle4_verify_attention_static_bytes.restype = ctypes.c_int64
     lib.eagle4_init.argtypes = []

@@ -77,6 +77,75 @@ def accept_tree(
     return sampled, num_sampled
 
 
+def sample_tree(
+    logits: torch.Tensor,
+    drafted: torch.Tensor,
+    cu_num_logits: torch.Tensor,
+    idx_mapping: torch.Tensor,
+    parents: torch.Tensor,
+    store: TreeStore,
+    coins: torch.Tensor,
+    final_coins: torch.Tensor,
+    temperature: torch.Tensor,
+    draft_probs: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """Verification by sampling, where :func:`greedy_targets` and :func:`accept_tree` take the argmax: the tokens of the
+    walk are distributed as the target's own. ``(sampled [num_reqs, W], num_sampled [num_reqs])`` as
+    :func:`accept_tree`'s, entries of ``sampled`` past ``num_sampled`` -1; the path goes to ``store``.
+
+    ``logits`` [rows, vocab] (bf16 / fp16 / fp32, unit column stride; -inf for a token that may not be drawn); ``coins``
+    [rows] and ``final_coins`` [num_reqs] fp32 uniform numbers in [0, 1), of a drafted row's acceptance and of the
+    token that ends a request's walk; ``temperature`` [num_reqs] fp32 (0: greedy). ``draft_probs`` [rows, vocab] (bf16 /
+    fp16 / fp32): row ``n`` what the children of row ``n`` were drawn from, each independently; None where the
+    children are the draft's choice and not drawn (its most likely tokens).
+
+    A row's children are tried in row order against the residual ``r`` (first ``p = softmax(logits / temperature)``,
+    its mass ``Z = 1``): accepted iff ``coin * q(x) * Z < r(x)``; a rejection leaves ``max(r - Z q, 0)``, or without
+    ``draft_probs`` (``q(x) = 1``) ``r`` without ``x``. Without an accepted child the walk ends with the first token
+    whose running sum of ``r`` exceeds ``final_coin * Z``. A row whose maximum is not finite has all its mass on its
+    argmax. Sums and comparisons are in 64 bits; only the walk's rows are read.
+    """
+    if logits.dim() != 2 or (draft_probs is not None and draft_probs.shape != logits.shape):
+        raise ValueError("sample_tree: logits must be [rows, vocab], draft_probs of the same shape")
+    rows, vocab = logits.shape
+    num_reqs, width = cu_num_logits.shape[0] - 1, store.width
+    if logits.stride(1) != 1 or (draft_probs is not None and draft_probs.stride(1) != 1):
+        raise _native.NotCovered("logits and draft_probs must have a unit column stride")
+    if width > 64:
+        raise _native.NotCovered(f"tree widths above 64 rows ({width})")
+    for t in (logits, draft_probs):
+        if t is not None and t.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+            raise _native.NotCovered(f"logits and draft_probs must be bf16, fp16 or fp32, got {t.dtype}")
+    if drafted.shape != (rows,) or idx_mapping.shape[0] < num_reqs or parents.dim() != 2 or parents.shape[1] < width:
+        raise ValueError(f"sample_tree: drafted must be [{rows}], idx_mapping [>= {num_reqs}], parents [slots, >= {width}]")
+    for name, t, n in (("coins", coins, rows), ("final_coins", final_coins, num_reqs), ("temperature", temperature, num_reqs)):
+        if t.dtype != torch.float32 or t.dim() != 1 or t.shape[0] < n or not t.is_contiguous():
+            raise ValueError(f"sample_tree: {name} must be a contiguous fp32 vector of {n} entries")
+    slots = min(parents.shape[0], store.path.shape[0], store.path_len.shape[0])
+    if (store.path.dtype != torch.int32 or store.path_len.dtype != torch.int32 or store.path.stride(1) != 1
+            or store.path.shape[1] < width or not store.path_len.is_contiguous()):
+        raise ValueError("sample_tree: the store's path and path_len must be int32, contiguous over a slot's entries")
+    for name, t in (("drafted", drafted), ("cu_num_logits", cu_num_logits), ("idx_mapping", idx_mapping), ("parents", parents),
+                    ("coins", coins), ("final_coins", final_coins), ("temperature", temperature), ("draft_probs", draft_probs),
+                    ("the store", store.path), ("the store", store.path_len)):
+        if t is not None and t.device != logits.device:
+            raise ValueError(f"sample_tree: {name} is on {t.device}, logits are on {logits.device}")
+    sampled = torch.empty(num_reqs, width, dtype=torch.int64, device=logits.device)
+    num_sampled = torch.empty(num_reqs, dtype=torch.int32, device=logits.device)
+    args = _native.SampleTreeArgs(
+        logits=logits.data_ptr(), stride_row=logits.stride(0), probs=_native.ptr(draft_probs),
+        stride_prob=0 if draft_probs is None else draft_probs.stride(0), drafted=_native.itab(drafted),
+        cu_num_logits=_native.itab(cu_num_logits), idx_mapping=_native.itab(idx_mapping), parents=_native.itab(parents),
+        coins=coins.data_ptr(), final_coins=final_coins.data_ptr(), temperature=temperature.data_ptr(),
+        sampled=sampled.data_ptr(), stride_sampled=width, num_sampled=num_sampled.data_ptr(), path=store.path.data_ptr(),
+        stride_path=store.path.stride(0), path_len=store.path_len.data_ptr(), rows=rows, num_reqs=num_reqs, width=width,
+        vocab=vocab, slots=slots, dtype=_native.dtype_code(logits.dtype),
+        prob_dtype=0 if draft_probs is None else _native.dtype_code(draft_probs.dtype),
+    )
+    _native.launch("eagle4_sample_tree", args, logits.device)
+    return sampled, num_sampled
+
+
 def accepted_rows_first(
     expanded_idx_mapping: torch.Tensor, expanded_local_pos: torch.Tensor, store: TreeStore
 ) -> torch.Tensor:

@@ -413,7 +413,8 @@ const char* eagle4_version(void);
 int eagle4_init(void);
 /* sizeof() of argument struct `which` (0 stage, 1 ancestors, 2 tail words, 3 conv, 4 gdn, 5 records, 6 records commit,
  * 7 attention, 8 argmax, 9 accept tree, 10 accept tail, 11 compact rows, 12 state commit, 13 compact kv,
- * 14 chainize, 15 row attention, 16 mamba2); -1 past the end. The host binding checks its struct mirrors against these. */
+ * 14 chainize, 15 row attention, 16 mamba2, 17 kv page write, 18 kv page read, 19 sample tree, 20 latent attention); -1 past
+ * the end. The host binding checks its struct mirrors against these. */
 int64_t eagle4_args_size(int which);
 
 /* ---- Mamba2 tree state update: kernels/mamba2_tree.py:41-240 (_tree_ssu_kernel, mamba2_tree_state_update) ------ */
@@ -450,6 +451,111 @@ typedef struct eagle4_mamba2_args {
   int32_t pad_slot_id;
 } eagle4_mamba2_args;
 int eagle4_mamba2_tree_state_update(const eagle4_mamba2_args* args, void* stream);
+
+/* ---- fp8 pages: rows quantised into the cache, and gathered back ------------------------------------------------------ */
+/* A cache is [num_blocks, page, heads, dim] e4m3 with fp32 scales [num_blocks, heads]: an element stands for its code times
+ * its (page, head)'s scale. No counterpart in the reference, whose caches are 16-bit.
+ *
+ * Request b's row j (j < its rows, or < path_len[slot] with `path`, whose entry j names the row that it takes) goes to
+ * position context_lens[b] + j. The scale of a page that rows go to is the least power of two s with amax <= 448 s over
+ * those rows, or the page's own where earlier positions of it are below the context and its scale is larger; where it
+ * grows, those positions are re-encoded. Infinities saturate and take no part in amax; NaN stays NaN. A row whose page
+ * the table does not hold, or names outside num_blocks, is not written. A page belongs to one request. */
+typedef struct eagle4_write_kv_args {
+  const void* key;   /* [tokens, heads, dim], dtype, unit stride over dim */
+  const void* value; /* like key, or null: one matrix (latent rows) */
+  int64_t stride_kt, stride_kh, stride_vt, stride_vh;
+  void *key_cache, *value_cache;
+  int64_t stride_kcb, stride_kcs, stride_kch, stride_vcb, stride_vcs, stride_vch; /* block, slot, head */
+  float *k_scale, *v_scale;
+  int64_t stride_ksb, stride_ksh, stride_vsb, stride_vsh; /* block, head */
+  eagle4_itab block_table;     /* [R, max_blocks] */
+  eagle4_itab context_lens;    /* [R] */
+  eagle4_itab query_start_loc; /* [R + 1] */
+  eagle4_itab idx_mapping;     /* [R], read only with path */
+  eagle4_itab path;            /* [path_slots, path_width] or null: every row, in order */
+  eagle4_itab path_len;        /* [path_slots] */
+  int64_t tokens;
+  int32_t num_reqs, heads, dim, page, max_blocks, num_blocks, max_rows, path_width, path_slots, dtype;
+} eagle4_write_kv_args;
+int eagle4_write_kv_pages(const eagle4_write_kv_args* args, void* stream);
+
+/* Rows start_loc[b] .. start_loc[b + 1] - 1 of key / value take positions 0, 1, .. of request b. A page that the table does
+ * not hold, or names outside num_blocks, reads as zeros. */
+typedef struct eagle4_read_kv_args {
+  void* key;   /* [tokens, heads, dim], dtype, unit stride over dim */
+  void* value; /* like key, or null */
+  int64_t stride_kt, stride_kh, stride_vt, stride_vh;
+  const void *key_cache, *value_cache;
+  int64_t stride_kcb, stride_kcs, stride_kch, stride_vcb, stride_vcs, stride_vch;
+  const float *k_scale, *v_scale;
+  int64_t stride_ksb, stride_ksh, stride_vsb, stride_vsh;
+  eagle4_itab block_table; /* [R, max_blocks] */
+  eagle4_itab start_loc;   /* [R + 1] */
+  int64_t tokens;
+  int32_t num_reqs, heads, dim, page, max_blocks, num_blocks, max_len, dtype;
+} eagle4_read_kv_args;
+int eagle4_read_kv_pages(const eagle4_read_kv_args* args, void* stream);
+
+/* ---- tree acceptance by sampling (no counterpart in the reference's own sources) ------------------------------------------ */
+/* p = softmax(logits[row] / temperature[b]). From the root, a node's children are tried in row order against the residual r
+ * (first p, of mass Z = 1): child of token x is accepted iff coins[child] q(x) Z < r(x). With probs (row n: what the children
+ * of row n were drawn from, independently) q is that row and a rejection leaves r = max(r - Z q, 0); without, q(x) = 1 and
+ * a rejection leaves r(x) = 0. Where no child is accepted the walk ends with the first token whose running sum of r
+ * exceeds final_coins[b] Z (Z = 0: of p). temperature not above 0, or a row whose maximum is not finite: all mass on the
+ * argmax. sampled[b]: the accepted tokens, the last one drawn, then -1; path / path_len as eagle4_accept_tree's. */
+typedef struct eagle4_sample_tree_args {
+  const void* logits; /* [rows, vocab], unit column stride */
+  int64_t stride_row;
+  const void* probs; /* [rows, vocab] or null, unit column stride */
+  int64_t stride_prob;
+  eagle4_itab drafted;       /* [rows] */
+  eagle4_itab cu_num_logits; /* [R + 1] */
+  eagle4_itab idx_mapping;   /* [R] */
+  eagle4_itab parents;       /* [slots, >= width] parent row of each row */
+  const float* coins;        /* [rows] contiguous */
+  const float* final_coins;  /* [R] contiguous */
+  const float* temperature;  /* [R] contiguous */
+  int64_t* sampled;          /* [R, width] */
+  int64_t stride_sampled;
+  int32_t* num_sampled; /* [R] */
+  int32_t* path;        /* [slots, width] */
+  int64_t stride_path;
+  int32_t* path_len; /* [slots] */
+  int64_t rows;
+  int32_t num_reqs, width, vocab, slots, dtype, prob_dtype; /* width <= 64 */
+} eagle4_sample_tree_args;
+int eagle4_sample_tree(const eagle4_sample_tree_args* args, void* stream);
+
+/* ---- tree-verify attention over latent rows (no counterpart in the reference) -------------------------------------------- */
+/* Keys and values are one row of rank + rope elements a token, the values its first `rank` (the absorbed form: q holds each
+ * head's query in the latent space, then its rotary part). Request b's rows see positions below context_lens[b] of its pages
+ * and the round's rows whose bit their mask has; a row that sees nothing gives zeros. A position whose page the table names
+ * outside num_blocks is not seen. */
+typedef struct eagle4_latent_attn_args {
+  const void* q; /* [tokens, heads, rank + rope], dtype */
+  int64_t stride_qt, stride_qh;
+  const void* latent_new; /* [tokens, rank + rope], dtype */
+  int64_t stride_nt;
+  const void* cache; /* [num_blocks, page, rank + rope], cache_dtype: dtype, or e4m3 */
+  int64_t stride_cb, stride_cs;
+  const float* scale_page; /* [num_blocks] scales of an e4m3 cache */
+  int64_t stride_sp;
+  eagle4_itab block_table;     /* [R, max_blocks] int32, unit column stride */
+  eagle4_itab context_lens;    /* [R] */
+  eagle4_itab query_start_loc; /* [R + 1] */
+  const int64_t* masks;        /* [R, >= max_query_len], unit column stride */
+  int64_t stride_mask;
+  void* out; /* [tokens, heads, rank], dtype */
+  int64_t stride_ot, stride_oh;
+  float* workspace; /* eagle4_latent_attention_workspace bytes, 16-byte aligned */
+  int64_t workspace_bytes;
+  int64_t tokens;
+  float scale;
+  int32_t num_reqs, heads, rank, rope, page, max_query_len, max_blocks, num_blocks, dtype, cache_dtype;
+} eagle4_latent_attn_args;
+int64_t eagle4_latent_attention_workspace(const eagle4_latent_attn_args* args); /* bytes; -1: not covered */
+int eagle4_latent_attention(const eagle4_latent_attn_args* args, void* stream);
 
 #ifdef __cplusplus
 }

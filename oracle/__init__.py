@@ -17,6 +17,9 @@ Modules:
 ``attention``       dense tree-verify attention over a paged cache, fp8-e4m3 quantize / dequantize
 ``accept``          greedy tree accept walk, bs1 accept tail, row compaction, first-index argmax
 ``commit``          vLLM linear-state commit (window compaction, accepted state move)
+``sampling``        tree acceptance by sampling, in 64 bits
+``kv_pages``        rows written into fp8 pages with power-of-two scales, and read back
+``latent``          attention over latent rows, in 64 bits, with the bound of 16-bit weights
 ==================  ==============================================================================================
 
 Parity pins: every function is checked in ``tests/test_oracle_*.py`` against the reference tests' known answers
