@@ -40,8 +40,7 @@ HIPCC_FLAGS = [
 # accumulator the chunk and replay kernels' VALU math reads).
 EXTRA_FLAGS = {"verify_attention_stream.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
                "gdn_tree_chunk.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
-               "gdn_tree_replay.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
-               "latent_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
+               "gdn_tree_replay.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
 
 
 def _hipcc() -> str:

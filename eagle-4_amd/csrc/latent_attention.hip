@@ -7,13 +7,14 @@
 // What bounds it. A request's width x heads query rows share every key: 2 (2 RANK + ROPE) operations a row and key against
 // 2 (RANK + ROPE) bytes a key (16-bit pages). From about 128 rows on that is the matrix cores' work, below it HBM's.
 //
-// Split. A workgroup takes ROWS query rows (16 to 128) and a run of 32-key tiles, which all four waves read from LDS:
-//   - RW row waves of NR 16-row tiles each; the 4 / RW waves of the same rows share out the output's columns (and
-//     compute the scores each for itself: with few rows the matrix cores have time for it);
-//   - S^T = C Q^T on v_mfma_f32_16x16x32, so that a lane holds scores of one query row, P^T is the B operand of
-//     O^T = C^T P^T straight from registers, and C^T is read by transposing LDS loads of the same tile: a row of the
-//     cache is brought in once for both products;
-//   - the output (RANK columns of fp32 a row) stays in registers: 128 rows take 256 registers a lane, so one wave a SIMD.
+// Split. A workgroup takes ROWS query rows (16, 32 or 64) and a run of 32-key tiles, which all eight waves read from LDS:
+//   - RW row waves of 16 rows each; the DW = 8 / RW waves of the same rows share out the output's columns, and the scores
+//     between two of them: one takes a tile's keys 0-15, the other 16-31 (with more than two, two sets of them do the
+//     same), and they exchange the weights and their running maxima through LDS;
+//   - S^T = C Q^T on v_mfma_f32_16x16x32, so that a lane holds scores of one query row and P^T is the B operand of
+//     O^T = C^T P^T in the registers' own order; C^T is read by transposing LDS loads of the same tile: a row of the cache
+//     is brought in once for both products;
+//   - a tile's scores are computed beside the last tile's output, so that the exchange costs no wait: one barrier a tile.
 // The launch is one workgroup a CU; each takes an equal run of all (request, row group, tile)s, so requests of any
 // lengths fill the chip. A row group cut by a run's end leaves normalised fp32 partials with their log2-sum-exps (at most two
 // a workgroup), which a second kernel merges.
@@ -25,16 +26,20 @@ namespace {
 using namespace e4attn;
 
 constexpr int kKeys = 32;      // keys of a tile
-constexpr int kWindow = 1024;  // block-table entries held in LDS
-constexpr int kMaxReqs = 2048; // requests of one launch (their tile counts are kept in LDS)
+constexpr int kWindow = 256;   // block-table entries held in LDS
+constexpr int kMaxReqs = 512; // requests of one launch (their tile counts are kept in LDS)
 
 struct LatentPlan {
   int first, reqs;       // requests of this launch
   int groups;            // workgroups
   int least;             // tiles of a workgroup's run at least
   int rows;              // query rows of a workgroup
+  int page_shift;        // of a page size that is a power of two, else -1
+  uint32_t page_inv;     // floor(2^32 / page) of any other
   int64_t pre_off, lse_off, part_off;  // float offsets into the workspace
 };
+
+constexpr float kNone = -3.0e38f;  // the maximum of no score
 
 // Bytes behind keys that are not there: a position past the context, a page outside the cache.
 __device__ __attribute__((aligned(16))) const uint32_t zero_row[640 / 2] = {};
@@ -100,131 +105,213 @@ E4_DEV void split_scale(float scale, float& pow2, float& rest) {
   rest = plain ? scale / pow2 : scale;
 }
 
-// The bits of lanes 0, 8, .., 56 of a ballot, as a byte.
+// A value that all lanes hold, in scalar registers (what comes from LDS or a table is in vector registers otherwise).
+E4_DEV int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+E4_DEV uint32_t uniform(uint32_t x) { return __builtin_amdgcn_readfirstlane(x); }
+E4_DEV int64_t uniform(int64_t x) {
+  return static_cast<int64_t>(static_cast<uint64_t>(uniform(static_cast<uint32_t>(x >> 32))) << 32 |
+                              uniform(static_cast<uint32_t>(x)));
+}
+
+// x, as a value that the compiler cannot have computed before: what follows from it is computed where it is used, not
+// kept in registers over the loop (the 128-row form has none to spare).
+E4_DEV int fresh(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
+// The bits of lanes 0, 8, .., 56 of a ballot, as a byte; those of lanes 0, 4, .., 60, as 16 bits.
 E4_DEV uint8_t every_eighth(uint64_t ballot) {
   return static_cast<uint8_t>(((ballot & 0x0101010101010101ull) * 0x0102040810204080ull) >> 56);
 }
+E4_DEV uint16_t every_fourth(uint64_t x) {
+  x &= 0x1111111111111111ull;
+  x = (x | x >> 3) & 0x0303030303030303ull;
+  x = (x | x >> 6) & 0x000f000f000f000full;
+  x = (x | x >> 12) & 0x000000ff000000ffull;
+  return static_cast<uint16_t>(x | x >> 24);
+}
 
 // A tile in LDS: CB blocks of 64 columns, each 32 keys x 128 bytes, the eight 16-byte chunks of a key's 128 bytes at
-// chunk ^ swz(key). 16 keys at one chunk (the scores' operand) and 8 keys at two adjacent chunks (the transposing
-// reads) then fall on distinct banks; an instruction of direct loads fills 8 keys of a block, so a lane's address is
-// its key's row plus a constant a block.
+// chunk ^ swz(key). Both operand reads then run at the LDS's full rate (256 bytes a cycle): the scores' (16 keys; the four
+// lane groups at chunks 2 g or 2 g + 1) and the transposing one (8 keys at two adjacent chunks). With the lane groups
+// at adjacent chunks instead the scores' reads take twice the cycles. An instruction of direct loads fills 8 keys of a block,
+// so a lane's address is its key's row plus a constant a block.
 E4_DEV int swz(int key) { return 2 * ((key >> 1) & 3) | ((key >> 3) & 1); }
 
-template <int RANK, int ROPE, typename T, bool FP8, int RW, int NR>
+constexpr int kWaves = 8, kThreads = 64 * kWaves;
+
+template <int RANK, int ROPE, typename T_, bool FP8_, int RW_>
 struct Shape {
-  static constexpr int DIM = RANK + ROPE, CB = DIM / 64, KC = DIM / 32, DW = 4 / RW, DT = RANK / 16 / DW;
-  static constexpr int ROWS = RW * NR * 16, TILE = CB * 4096;
-  static constexpr int NBUF = FP8 ? 2 : 4;
+  using T = T_;
+  static constexpr bool FP8 = FP8_;
+  static constexpr int RW = RW_, DW = kWaves / RW, DT = RANK / 16 / DW;
+  static constexpr int DIM = RANK + ROPE, CB = DIM / 64, KC = DIM / 32, ROWS = RW * 16, TILE = CB * 4096;
+  // 16-bit pages: a ring of four tiles, two in use and two on their way. fp8 pages: a ring of four tiles of codes, three on
+  // their way, and two widened ones.
+  static constexpr int NBUF = FP8 ? 2 : 4, RAW = CB * 2048;
+  // blocks of 64 columns that waves 0-3 (each 8 keys of a tile) bring in; waves 4-7 bring in the rest
+  static constexpr int CB0 = (CB + 1) / 2, CB1 = CB - CB0;
+  // LDS operands of the matrix products in registers at a time, the one in use among them. Their loads run that far ahead
+  // in this order, product by product: left to itself the compiler waits for each operand right after its load.
+  static constexpr int AHEAD = 8;
 };
 
-// One tile for a wave's NR x 16 rows; bit k of bits[r]: key k is visible to the lane's row r (`all`: every key to all).
-template <typename S, int NR, typename T, bool FP8>
-E4_DEV void tile_step(const char* tile, const u32x4_t (&q)[NR][S::KC], f32x4_t (&acc)[NR][S::DT], float (&m)[NR],
-                      float (&l)[NR], float scale_log2, const float* key_scale, int dbase, int g, int l16, bool all,
-                      const uint32_t (&bits)[NR]) {
-  f32x4_t s[NR][2];
+// A wave's share of the weights: P^T of one half tile (16 keys x 16 rows) as written by its lanes, and the rows' maxima.
+template <int RW>
+struct Weights {
+  __attribute__((aligned(16))) u32x2_t p[RW][2][64];
+  float m[RW][2][16];
+};
+
+// The scores of keys 16 kt .. of a tile, for a wave's 16 rows.
+template <typename S>
+E4_DEV f32x4_t score_step(const char* tile, const u32x4_t (&q)[S::KC], int kt, int lane) {
+  using T = typename S::T;
+  const int g = lane >> 4, l16 = lane & 15, x = swz(l16);
+  const char* const k0 = tile + kt * 2048 + l16 * 128 + 16 * ((2 * g) ^ x);
+  const char* const k1 = tile + kt * 2048 + l16 * 128 + 16 * ((2 * g + 1) ^ x);
+  u32x4_t ka[S::AHEAD];
+  const auto load = [&](int c) {
+    ka[c % S::AHEAD] = *reinterpret_cast<const u32x4_t*>((c & 1 ? k1 : k0) + (c / 2) * 4096);
+  };
 #pragma unroll
-  for (int r = 0; r < NR; ++r)
-#pragma unroll
-    for (int kt = 0; kt < 2; ++kt) s[r][kt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  const int x = swz(l16);
-  const char* const k0 = tile + l16 * 128 + 16 * (g ^ x);
-  const char* const k1 = tile + l16 * 128 + 16 * ((4 + g) ^ x);
+  for (int c = 0; c < S::AHEAD - 1; ++c) load(c);
+  f32x4_t s[2] = {f32x4_t{0.f, 0.f, 0.f, 0.f}, f32x4_t{0.f, 0.f, 0.f, 0.f}};  // two chains: a product waits for the last but one
 #pragma unroll
   for (int c = 0; c < S::KC; ++c) {
-#pragma unroll
-    for (int kt = 0; kt < 2; ++kt) {
-      const u32x4_t ka = *reinterpret_cast<const u32x4_t*>((c & 1 ? k1 : k0) + (c / 2) * 4096 + kt * 2048);
-#pragma unroll
-      for (int r = 0; r < NR; ++r) s[r][kt] = mfma16<T>(ka, q[r][c], s[r][kt]);
-    }
-    if (c % 3 == 2) __builtin_amdgcn_sched_barrier(0);
+    if (c + S::AHEAD - 1 < S::KC) load(c + S::AHEAD - 1);
+    s[c % 2] = mfma16<T>(ka[c % S::AHEAD], q[c], s[c % 2]);
+    __builtin_amdgcn_sched_barrier(0);
   }
-  float ks[2][4];
-  if constexpr (FP8) {
-#pragma unroll
-    for (int kt = 0; kt < 2; ++kt) {
-      const f32x4_t v = *reinterpret_cast<const f32x4_t*>(key_scale + 16 * kt + 4 * g);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) ks[kt][i] = v[i];
-    }
+  return s[0] + s[1];
+}
+
+// The weights of those scores into `to`, relative to the rows' maximum m; l takes their sum. Bit k of bits: key k of the tile
+// is visible to the lane's row (`all`: every key to every row).
+template <typename S>
+E4_DEV void weight_step(f32x4_t s, Weights<S::RW>& to, int row_wave, int kt, bool writes, float& m, float& l,
+                        float scale_log2, const float* key_scale, int lane, bool all, uint32_t bits) {
+  using T = typename S::T;
+  const int g = lane >> 4;
+  s *= scale_log2;
+  f32x4_t ks = {1.f, 1.f, 1.f, 1.f};
+  if constexpr (S::FP8) {
+    ks = *reinterpret_cast<const f32x4_t*>(key_scale + 16 * kt + 4 * g);
+    s *= ks;
   }
-  u32x4_t pb[NR];
+  if (!all) {
 #pragma unroll
-  for (int r = 0; r < NR; ++r) {
-    float top = -INFINITY;
-#pragma unroll
-    for (int kt = 0; kt < 2; ++kt) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float v = s[r][kt][i] * scale_log2;
-        if constexpr (FP8) v *= ks[kt][i];
-        if (!all) v = (bits[r] >> (16 * kt + 4 * g + i)) & 1 ? v : -INFINITY;
-        s[r][kt][i] = v;
-        top = fmaxf(top, v);
-      }
-    }
-    // The maximum moves only when it grows by more than 2^8: until then p stays below 2^8, which 16 bits hold as well
-    // as values below 1, and the output (up to 256 registers) is not rescaled.
-    if (__any(top > m[r] + 8.f)) {
-      top = fmaxf(top, __shfl_xor(top, 16, 64));
-      top = fmaxf(top, __shfl_xor(top, 32, 64));
-      const float now = fmaxf(m[r], top);
-      const float keep = exp2f(m[r] - now);
-      m[r] = now;
-      l[r] *= keep;
-#pragma unroll
-      for (int dt = 0; dt < S::DT; ++dt) acc[r][dt] *= keep;
-    }
-    uint32_t w[4];
-#pragma unroll
-    for (int p = 0; p < 4; ++p) {  // element i of P^T's operand is key 16 (i / 4) + 4 g + i % 4
-      float p0 = __builtin_amdgcn_exp2f(s[r][p >> 1][2 * (p & 1)] - m[r]);
-      float p1 = __builtin_amdgcn_exp2f(s[r][p >> 1][2 * (p & 1) + 1] - m[r]);
-      l[r] += p0 + p1;
-      if constexpr (FP8) {
-        p0 *= ks[p >> 1][2 * (p & 1)];
-        p1 *= ks[p >> 1][2 * (p & 1) + 1];
-      }
-      w[p] = pack2<T>(p0, p1);
-    }
-    pb[r] = u32x4_t{w[0], w[1], w[2], w[3]};
+    for (int i = 0; i < 4; ++i)
+      if (!((bits >> (16 * kt + 4 * g + i)) & 1)) s[i] = -INFINITY;
   }
-  const int j = l16 >> 2, s4 = l16 & 3, kv = 4 * g + j, xv = swz(kv);
-  const char* const vrow = tile + kv * 128 + 8 * (s4 & 1);
+  float top = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
+  // The maximum moves only when it grows by more than 2^8 (until then p stays below 2^8, which 16 bits hold as well as
+  // values below 1), and to a whole number: what was weighted with the last one is then scaled without rounding.
+  if (__any(top > m + 8.f)) {
+    top = fmaxf(top, __shfl_xor(top, 16, 64));
+    top = fmaxf(top, __shfl_xor(top, 32, 64));
+    const float now = fmaxf(m, ceilf(top));
+    l *= exp2f(m - now);
+    m = now;
+  }
+  float p[4];
 #pragma unroll
-  for (int dt = 0; dt < S::DT; ++dt) {
-    // columns dbase + 16 dt ..: block (dbase / 64) + dt / 4, chunks 2 (dt % 4) and the next (dbase is a multiple of 64)
-    const char* const at = vrow + (dbase / 64 + dt / 4) * 4096 + 16 * ((2 * (dt & 3) + (s4 >> 1)) ^ xv);
-    const v4i16 lo4 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4i16*)(at));
-    const v4i16 hi4 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4i16*)(at + 2048));
-    const u32x2_t lo = __builtin_bit_cast(u32x2_t, lo4), hi = __builtin_bit_cast(u32x2_t, hi4);
-    const u32x4_t va = u32x4_t{lo[0], lo[1], hi[0], hi[1]};
-#pragma unroll
-    for (int r = 0; r < NR; ++r) acc[r][dt] = mfma16<T>(va, pb[r], acc[r][dt]);
-    if (dt % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+  for (int i = 0; i < 4; ++i) {
+    p[i] = __builtin_amdgcn_exp2f(s[i] - m);
+    l += p[i];
+    if constexpr (S::FP8) p[i] *= ks[i];
+  }
+  if (writes) {
+    to.p[row_wave][kt][lane] = u32x2_t{pack2<T>(p[0], p[1]), pack2<T>(p[2], p[3])};
+    if (g == 0) to.m[row_wave][kt][lane & 15] = m;
   }
 }
 
-template <int RANK, int ROPE, typename T, bool FP8, int RW, int NR>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) void latent_kernel(
+// Two packed weights times a power of two.
+template <typename T>
+E4_DEV uint32_t scale2(uint32_t w, float f) {
+  return pack2<T>(T::to_f32(static_cast<uint16_t>(w & 0xffffu)) * f, T::to_f32(static_cast<uint16_t>(w >> 16)) * f);
+}
+
+// The weights of a tile as the operand of its output. macc is what acc is relative to, m what the wave's own next weights
+// are: both move to the largest maximum that the tile's weights bring. (In front of the scores, where no operand of a product
+// is in registers: the compiler then keeps one copy of acc over the branch.)
+template <typename S>
+E4_DEV u32x4_t take_weights(const Weights<S::RW>& from, int row_wave, f32x4_t (&acc)[S::DT], float& macc, float& m, float& l,
+                            int lane) {
+  using T = typename S::T;
+  const int l16 = lane & 15;
+  // element i of P^T's operand is key 16 (i / 4) + 4 g + i % 4
+  u32x2_t p0 = from.p[row_wave][0][lane], p1 = from.p[row_wave][1][lane];
+  const float m0 = from.m[row_wave][0][l16], m1 = from.m[row_wave][1][l16];
+  if (__any(m0 != macc || m1 != macc)) {
+    const float now = fmaxf(macc, fmaxf(m0, m1));
+    const float keep = exp2f(macc - now), f0 = exp2f(m0 - now), f1 = exp2f(m1 - now);
+    l *= exp2f(m - now);  // m <= now: the wave's own maximum is m0 or m1, or that of waves that do the same
+    macc = m = now;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      p0[i] = scale2<T>(p0[i], f0);
+      p1[i] = scale2<T>(p1[i], f1);
+    }
+#pragma unroll
+    for (int dt = 0; dt < S::DT; ++dt) acc[dt] *= keep;
+  }
+  return u32x4_t{p0[0], p0[1], p1[0], p1[1]};
+}
+
+// O^T += C^T P^T of a tile, for a wave's 16 rows and its columns dbase ...
+template <typename S>
+E4_DEV void value_step(const char* tile, u32x4_t pb, f32x4_t (&acc)[S::DT], int dbase, int lane) {
+  using T = typename S::T;
+  const int g = lane >> 4, l16 = lane & 15;
+  const int j = l16 >> 2, s4 = l16 & 3, kv = 4 * g + j, xv = swz(kv);
+  // columns dbase + 16 dt ..: block dbase / 64 + dt / 4, chunks 2 (dt % 4) and the next (waves with fewer than four such
+  // tiles share a block: their first is its tile dt0)
+  const char* const vrow = tile + kv * 128 + 8 * (s4 & 1) + (dbase / 64) * 4096;
+  const int dt0 = dbase % 64 / 16;
+  constexpr int VA = S::AHEAD < S::DT ? S::AHEAD : S::DT;
+  u32x4_t va[VA];
+  const auto load = [&](int dt) {
+    const char* const at = vrow + (dt / 4) * 4096 + 16 * ((2 * (dt0 + (dt & 3)) + (s4 >> 1)) ^ xv);
+    const v4i16 lo4 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4i16*)(at));
+    const v4i16 hi4 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4i16*)(at + 2048));
+    const u32x2_t lo = __builtin_bit_cast(u32x2_t, lo4), hi = __builtin_bit_cast(u32x2_t, hi4);
+    va[dt % VA] = u32x4_t{lo[0], lo[1], hi[0], hi[1]};
+  };
+#pragma unroll
+  for (int dt = 0; dt < VA - 1; ++dt) load(dt);
+#pragma unroll
+  for (int dt = 0; dt < S::DT; ++dt) {
+    if (dt + VA - 1 < S::DT) load(dt + VA - 1);
+    acc[dt] = mfma16<T>(va[dt % VA], pb, acc[dt]);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
+template <int RANK, int ROPE, typename T, bool FP8, int RW>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void latent_kernel(
     const eagle4_latent_attn_args a, const LatentPlan p) {
-  using S = Shape<RANK, ROPE, T, FP8, RW, NR>;
+  using S = Shape<RANK, ROPE, T, FP8, RW>;
   __shared__ __attribute__((aligned(1024))) char smem[S::NBUF][S::TILE];
+  __shared__ __attribute__((aligned(1024))) char s_raw[FP8 ? 4 : 1][FP8 ? S::RAW : 16];
+  __shared__ Weights<RW> s_w[2];
   __shared__ uint32_t s_pre[kMaxReqs + 1];
   __shared__ int32_t s_win[kWindow];
   __shared__ float s_winscale[FP8 ? kWindow : 1];
-  __shared__ __attribute__((aligned(16))) float s_ks[S::NBUF][kKeys];
-  __shared__ uint32_t s_vis[S::NBUF];  // a bit a key: it is there
+  // by tile % 4 (up to three tiles are under way beside the one in use): a bit a key that is there, and its scale's parts
+  __shared__ uint32_t s_vis[4];
+  __shared__ __attribute__((aligned(16))) float s_rest[4][kKeys], s_pow2[FP8 ? 4 : 1][kKeys];
   __shared__ uint32_t s_bad;           // a bit a new key: it holds a value that is not finite
-  __shared__ uint32_t s_tot[4];
+  __shared__ uint32_t s_tot[kWaves];
+  __shared__ float s_sum[RW][2][16];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 4, l16 = lane & 15;
 
   // tiles before each request
   uint32_t run = 0;
-  for (int b0 = 0; b0 < p.reqs; b0 += 256) {
+  for (int b0 = 0; b0 < p.reqs; b0 += kThreads) {
     uint32_t n = 0;
     if (b0 + tid < p.reqs) {
       const Unit u = unit_of(a, p.first + b0 + tid, S::ROWS);
@@ -239,7 +326,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
     if (lane == 63) s_tot[wave] = sum;
     __syncthreads();
     uint32_t before = run;
-    for (int w = 0; w < 4; ++w) {
+    for (int w = 0; w < kWaves; ++w) {
       if (w < wave) before += s_tot[w];
       run += s_tot[w];
     }
@@ -248,77 +335,68 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
   }
   if (tid == 0) s_pre[0] = 0;
   __syncthreads();
-  const uint32_t total = run;
+  const uint32_t total = uniform(run);
   uint32_t share = (total + p.groups - 1) / p.groups;
   share = share < static_cast<uint32_t>(p.least) ? p.least : share;
   // adjacent runs on one XCD (workgroups go to the eight in turn): row groups of a request share its tiles in the L2
   const int wg = p.groups % 8 == 0 ? (blockIdx.x % 8) * (p.groups / 8) + blockIdx.x / 8 : blockIdx.x;
   if (wg == 0) {  // for the merge
     uint32_t* const pre = reinterpret_cast<uint32_t*>(a.workspace + p.pre_off);
-    for (int i = tid; i <= p.reqs; i += 256) pre[i] = s_pre[i];
+    for (int i = tid; i <= p.reqs; i += kThreads) pre[i] = s_pre[i];
   }
   uint32_t pos = wg * share;
   const uint32_t stop = pos + share < total ? pos + share : total;
   if (pos >= stop) return;
   int at = 0;  // the request of tile `pos`: the last with s_pre <= pos
-  for (int step = 1 << 11; step > 0; step >>= 1)
-    if (at + step < p.reqs && s_pre[at + step] <= pos) at += step;
+  for (int step = kMaxReqs / 2; step > 0; step >>= 1)
+    if (at + step < p.reqs && uniform(s_pre[at + step]) <= pos) at += step;
 
-  const int row_wave = wave / S::DW, dbase = (wave % S::DW) * S::DT * 16;
+  const int row_wave = wave / S::DW, column_wave = wave % S::DW, kt = column_wave % 2, dbase = column_wave * S::DT * 16;
   const float scale_log2 = a.scale * 1.4426950408889634f;
   constexpr int EB = FP8 ? 1 : 2;
   const char* const cache = static_cast<const char*>(a.cache);
   const int64_t scb = a.stride_cb * EB, scs = a.stride_cs * EB;
-  const int page_shift = (a.page & (a.page - 1)) == 0 ? __builtin_ctz(a.page) : -1;
-  const auto page_of = [&](int pos) {
-    return page_shift >= 0 ? pos >> page_shift
-                           : static_cast<int>(static_cast<uint32_t>(pos) / static_cast<uint32_t>(a.page));
+  const auto page_of = [&](int pos) {  // pos / page: by the inverse it comes out right or one short
+    if (p.page_shift >= 0) return pos >> p.page_shift;
+    const int n = static_cast<int>(__umulhi(static_cast<uint32_t>(pos), p.page_inv));
+    return n + (pos - n * a.page >= a.page ? 1 : 0);
   };
-  // this lane's key of a tile and where its chunks go: a wave brings in 8 keys, 8 lanes a key
-  const int my_key = 8 * wave + lane / 8;
-  const int my_chunk = (lane % 8) ^ swz(my_key);
+  // a wave brings in 8 keys of a tile, 8 lanes a key, half the blocks of columns
+  const int octet = wave % 4;
+  const bool second_half = wave >= 4;
+  const int cb_first = second_half ? S::CB0 : 0;
 
   while (pos < stop) {
-    while (s_pre[at + 1] <= pos) ++at;
+    while (uniform(s_pre[at + 1]) <= pos) ++at;
     const int b = p.first + at;
-    const Unit u = unit_of(a, b, S::ROWS);
-    const uint32_t within = pos - s_pre[at];
+    Unit u = unit_of(a, b, S::ROWS);
+    u = Unit{uniform(u.start), uniform(u.width), uniform(u.context), uniform(u.ctx_tiles), uniform(u.tiles),
+             uniform(u.row_groups)};
+    const uint32_t within = pos - uniform(s_pre[at]);
     const int rg = static_cast<int>(within / u.tiles), t0 = static_cast<int>(within % u.tiles);
     const int t1 = static_cast<int>(static_cast<uint32_t>(u.tiles - t0) < stop - pos ? u.tiles : t0 + (stop - pos));
     const int32_t* const table = static_cast<const int32_t*>(a.block_table.ptr) + b * a.block_table.s0;
 
-    u32x4_t q[NR][S::KC];
-    f32x4_t acc[NR][S::DT];
-    float m[NR], l[NR];
-    uint64_t mask[NR];
-    int rho[NR];
-    bool ok[NR], computes = false;
-#pragma unroll
-    for (int r = 0; r < NR; ++r) {
-      rho[r] = rg * S::ROWS + (row_wave * NR + r) * 16 + l16;
-      ok[r] = rho[r] < u.width * a.heads;
-      computes |= rg * S::ROWS + (row_wave * NR + r) * 16 < u.width * a.heads;
-      const int t = ok[r] ? rho[r] / a.heads : 0, head = ok[r] ? rho[r] % a.heads : 0;
-      const uint16_t* const qrow = static_cast<const uint16_t*>(a.q) + (u.start + t) * a.stride_qt + head * a.stride_qh;
-#pragma unroll
-      for (int c = 0; c < S::KC; ++c)
-        q[r][c] = ok[r] ? *reinterpret_cast<const u32x4_t*>(qrow + 32 * c + 8 * g) : u32x4_t{0u, 0u, 0u, 0u};
-      mask[r] = ok[r] ? static_cast<uint64_t>(a.masks[b * a.stride_mask + t]) : 0;
-      m[r] = -3.0e38f;
-      l[r] = 0.f;
-#pragma unroll
-      for (int dt = 0; dt < S::DT; ++dt) acc[r][dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    }
-
+    const int row0 = rg * S::ROWS + row_wave * 16;
+    const bool computes = row0 < u.width * a.heads;
+    // the lane's row: its place among the request's rows, its draft token and head (0, 0 for none)
+    const auto my_row = [&](int& rho, int& t, int& head) {
+      rho = row0 + (fresh(lane) & 15);
+      const bool ok = rho < u.width * a.heads;
+      t = ok ? rho / a.heads : 0;
+      head = ok ? rho - t * a.heads : 0;
+      return ok;
+    };
     int win0 = 0, win1 = 0;  // the block-table entries in LDS
     const auto window = [&](int tile) {  // makes those of context tile `tile` be there; every thread calls it
-      const int lo = page_of(tile * kKeys);
+      const int lo = uniform(page_of(tile * kKeys));
       const int last = tile * kKeys + kKeys < u.context ? tile * kKeys + kKeys - 1 : u.context - 1;
       if (lo >= win0 && page_of(last) < win1) return;
       __syncthreads();
       win0 = lo;
       win1 = lo + kWindow;
-      for (int i = tid; i < kWindow; i += 256) {
+#pragma unroll 1
+      for (int i = fresh(tid); i < kWindow; i += kThreads) {
         int32_t blk = -1;
         if (win0 + i < a.max_blocks) blk = table[win0 + i];
         if (blk < 0 || blk >= a.num_blocks) blk = -1;
@@ -328,7 +406,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
       __syncthreads();
     };
     // the lane's key row of a tile; null where there is none
-    const auto key_row = [&](int tile, float& scale) -> const char* {
+    const auto key_row = [&](int tile, int my_key, float& scale) -> const char* {
       scale = 1.f;
       if (tile >= u.ctx_tiles) {
         const int j = (tile - u.ctx_tiles) * kKeys + my_key;
@@ -341,160 +419,221 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
       if constexpr (FP8) scale = s_winscale[page - win0];
       return blk >= 0 ? cache + blk * scb + static_cast<int64_t>(k - page * a.page) * scs : nullptr;
     };
-    const auto mark = [&](int buf, bool there, float scale) {
-      const uint8_t byte = every_eighth(__ballot(there));
-      if (lane == 0) reinterpret_cast<uint8_t*>(&s_vis[buf])[wave] = byte;
-      if (FP8 && lane % 8 == 0) s_ks[buf][my_key] = scale;
-    };
-    // a tile of 16-bit rows by direct loads
-    const auto issue = [&](int tile, int buf) {
-      float scale;
-      const char* row = key_row(tile, scale);
-      mark(buf, row != nullptr, 1.f);
-      if (row == nullptr) row = reinterpret_cast<const char*>(zero_row);
-      const char* const src = row + 16 * my_chunk;
-      const uint32_t dst = lds_addr(smem[buf]) + 1024 * wave;
-#pragma unroll
-      for (int c = 0; c < S::CB; ++c) dma16(src + 128 * c, dst + 4096 * c);
-    };
-    // a tile of fp8 rows through registers: raw codes now, widened into LDS a tile later
-    u32x2_t raw[FP8 ? S::CB : 1];
-    float raw_scale = 1.f;
-    bool raw_there = false;
-    const auto load8 = [&](int tile) {
-      const char* const row = key_row(tile, raw_scale);
-      raw_there = row != nullptr;
-#pragma unroll
-      for (int c = 0; c < S::CB; ++c)
-        raw[FP8 ? c : 0] = raw_there ? *reinterpret_cast<const u32x2_t*>(row + 64 * c + 8 * (lane % 8)) : u32x2_t{0u, 0u};
-    };
-    const auto store8 = [&](int buf) {
-      float pow2, rest;
-      split_scale(raw_scale, pow2, rest);
-      mark(buf, raw_there, rest);
-#pragma unroll
-      for (int c = 0; c < S::CB; ++c)
-        *reinterpret_cast<u32x4_t*>(smem[buf] + 4096 * c + my_key * 128 + 16 * my_chunk) =
-            widen8<T>(raw[FP8 ? c : 0], pow2);
-    };
     const auto is_ctx = [&](int tile) { return tile < u.ctx_tiles; };
+    // a tile of 16-bit rows by direct loads
+    const auto issue = [&](int tile) {
+      const int ln = fresh(lane), my_key = 8 * octet + ln / 8, my_chunk = (ln % 8) ^ swz(my_key);
+      float scale;
+      const char* row = key_row(tile, my_key, scale);
+      const uint8_t there = every_eighth(__ballot(row != nullptr));
+      if (!second_half && ln == 0) reinterpret_cast<uint8_t*>(&s_vis[tile % 4])[octet] = there;
+      if (FP8 && !second_half) s_rest[tile % 4][my_key] = 1.f;  // eight lanes, one value
+      if (row == nullptr) row = reinterpret_cast<const char*>(zero_row);
+      const char* const src = row + 16 * my_chunk + 128 * cb_first;
+      const uint32_t dst = __builtin_amdgcn_readfirstlane(lds_addr(smem[tile % S::NBUF]) + 1024 * octet + 4096 * cb_first);
+#pragma unroll
+      for (int c = 0; c < S::CB1; ++c) dma16(src + 128 * c, dst + 4096 * c);
+      if (S::CB0 > S::CB1 && !second_half) dma16(src + 128 * S::CB1, dst + 4096 * S::CB1);
+    };
+    // a tile of fp8 codes by direct loads: a block of 64 columns is 32 keys x 64 bytes, an instruction 16 keys of it; wave w
+    // brings in keys 16 (w % 2) .. of blocks w / 2, w / 2 + kWaves / 2, ..
+    const auto issue8 = [&](int tile) {
+      const int ln = fresh(lane), my_key = 16 * (wave % 2) + ln / 4;
+      float scale, pow2, rest;
+      const char* row = key_row(tile, my_key, scale);
+      const uint16_t there = every_fourth(__ballot(row != nullptr));
+      split_scale(scale, pow2, rest);
+      if (wave < 2) {
+        if (ln == 0) reinterpret_cast<uint16_t*>(&s_vis[tile % 4])[wave] = there;
+        s_pow2[FP8 ? tile % 4 : 0][my_key] = pow2;
+        s_rest[tile % 4][my_key] = rest;
+      }
+      if (row == nullptr) row = reinterpret_cast<const char*>(zero_row);
+      const char* const src = row + 16 * (ln % 4);
+      const uint32_t dst = __builtin_amdgcn_readfirstlane(lds_addr(s_raw[FP8 ? tile % 4 : 0]) + 1024 * (wave % 2));
+#pragma unroll
+      for (int c0 = 0; c0 < S::CB; c0 += kWaves / 2)
+        if (wave / 2 + c0 < S::CB) dma16(src + 64 * (wave / 2 + c0), dst + 2048 * (wave / 2 + c0));
+    };
+    const auto widen = [&](int tile) {
+      const int ln = fresh(lane), my_key = 8 * octet + ln / 8, my_chunk = (ln % 8) ^ swz(my_key);
+      const float pow2 = s_pow2[FP8 ? tile % 4 : 0][my_key];
+      const char* const src = s_raw[FP8 ? tile % 4 : 0] + 2048 * cb_first + my_key * 64 + 8 * (ln % 8);
+      char* const dst = smem[tile % S::NBUF] + 4096 * cb_first + my_key * 128 + 16 * my_chunk;
+      const int blocks = second_half ? S::CB1 : S::CB0;
+#pragma unroll
+      for (int c = 0; c < S::CB0; ++c)
+        if (c < blocks)
+          *reinterpret_cast<u32x4_t*>(dst + 4096 * c) = widen8<T>(*reinterpret_cast<const u32x2_t*>(src + 2048 * c), pow2);
+    };
 
     __syncthreads();  // the last piece's tiles have been read
-    if constexpr (FP8) {
-      if (is_ctx(t0)) {
-        window(t0);
-        load8(t0);
-        store8(t0 & 1);
-      } else {
-        issue(t0, t0 & 1);
-      }
-      if (t0 + 1 < t1 && is_ctx(t0 + 1)) {
-        window(t0 + 1);
-        load8(t0 + 1);
-      }
-    } else {
-      for (int i = 0; i < S::NBUF - 1 && t0 + i < t1; ++i) {
-        if (is_ctx(t0 + i)) window(t0 + i);
-        issue(t0 + i, (t0 + i) % S::NBUF);
-      }
+    // the tiles behind the first start after it, so that two (fp8: three) are under way in the loop
+    const auto start = [&](int tile) {
+      if (tile >= t1 || (FP8 && !is_ctx(tile))) return;
+      if constexpr (FP8) issue8(tile); else issue(tile);
+    };
+#pragma unroll 1
+    for (int i = 0; i < (FP8 ? 3 : 2); ++i) {
+      if (t0 + i < t1 && is_ctx(t0 + i)) window(t0 + i);
+      start(t0 + i);
     }
-    for (int tile = t0; tile < t1; ++tile) {
-      const int buf = tile % S::NBUF;
+    // Waits until a tile (fp8: its codes) is there for every wave, the last tile's weights too; the buffer of the tile before
+    // that is free.
+    const auto arrive = [&](int tile) {
       if constexpr (FP8) {
-        wait_vm<0>();
-      } else {
-        if (tile + 2 < t1)
-          wait_vm<2 * S::CB>();
-        else if (tile + 1 < t1)
-          wait_vm<S::CB>();
-        else
-          wait_vm<0>();
-      }
-      __syncthreads();  // the tile is there for every wave, and the buffer of the last one is free
-      if constexpr (FP8) {
-        if (tile + 1 < t1) {
-          if (is_ctx(tile + 1))
-            store8((tile + 1) & 1);
-          else
-            issue(tile + 1, (tile + 1) & 1);
-        }
+        // instructions a tile of waves below 2 (CB % 4); the others one less
+        constexpr int kMost = (S::CB + 3) / 4;
+        const bool less = S::CB % 4 != 0 && wave >= 2 * (S::CB % 4);
         if (tile + 2 < t1 && is_ctx(tile + 2)) {
-          window(tile + 2);
-          load8(tile + 2);
+          if (less) wait_vm<2 * (kMost - 1)>(); else wait_vm<2 * kMost>();
+        } else if (tile + 1 < t1 && is_ctx(tile + 1)) {
+          if (less) wait_vm<kMost - 1>(); else wait_vm<kMost>();
+        } else {
+          wait_vm<0>();
         }
       } else {
-        const int ahead = tile + S::NBUF - 1;
-        if (ahead < t1) {
-          if (is_ctx(ahead)) window(ahead);
-          issue(ahead, ahead % S::NBUF);
+        if (tile + 1 < t1) {
+          if (second_half) wait_vm<S::CB1>(); else wait_vm<S::CB0>();
+        } else {
+          wait_vm<0>();
         }
       }
-      const char* const data = smem[buf];
-      const uint32_t vis = __builtin_amdgcn_readfirstlane(s_vis[buf]);
-      uint32_t bits[NR];
-      if (is_ctx(tile)) {
-#pragma unroll
-        for (int r = 0; r < NR; ++r) bits[r] = vis;
-      } else {
-        // The round's rows. One that is not finite must not reach the rows that do not see it through 0 x NaN: it is
-        // cleared, and the rows that see it become NaN.
-        bool bad = false;
-        char* const mine = smem[buf] + my_key * 128 + 16 * (lane % 8);
+      __syncthreads();
+    };
+    // The round's rows. One that is not finite must not reach the rows that do not see it through 0 x NaN: it is cleared, and
+    // the rows that see it become NaN. Gives a bit a row that was cleared; every wave calls it.
+    const auto clean = [&](int tile) {
+      if (tid == 0) s_bad = 0;
+      __syncthreads();
+      const int ln = fresh(lane), my_key = 8 * octet + ln / 8;
+      char* const mine = smem[tile % S::NBUF] + 4096 * cb_first + my_key * 128 + 16 * (ln % 8);
+      bool bad = false;
 #pragma unroll 1
-        for (int c = 0; c < S::CB; ++c) {
-          const u32x4_t w = *reinterpret_cast<const u32x4_t*>(mine + 4096 * c);
-          constexpr uint32_t kExp = T::code == EAGLE4_BF16 ? 0x7f80u : 0x7c00u;
+      for (int c = 0; c < (second_half ? S::CB1 : S::CB0); ++c) {
+        const u32x4_t w = *reinterpret_cast<const u32x4_t*>(mine + 4096 * c);
+        constexpr uint32_t kExp = T::code == EAGLE4_BF16 ? 0x7f80u : 0x7c00u;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) bad |= (w[i] & kExp) == kExp || ((w[i] >> 16) & kExp) == kExp;
-        }
-        uint64_t any = __ballot(bad);
-        any |= any >> 4;
-        any |= any >> 2;
-        any |= any >> 1;
-        const uint8_t byte = every_eighth(any);
-        if (lane == 0) reinterpret_cast<uint8_t*>(&s_bad)[wave] = byte;
-        if ((byte >> (lane / 8)) & 1) {
+        for (int i = 0; i < 4; ++i) bad |= (w[i] & kExp) == kExp || ((w[i] >> 16) & kExp) == kExp;
+      }
+      if (bad) atomicOr(&s_bad, 1u << my_key);
+      __syncthreads();
+      const uint32_t poison = __builtin_amdgcn_readfirstlane(s_bad);
+      if (poison != 0) {
+        if ((poison >> my_key) & 1) {
 #pragma unroll 1
-          for (int c = 0; c < S::CB; ++c) *reinterpret_cast<u32x4_t*>(mine + 4096 * c) = u32x4_t{0u, 0u, 0u, 0u};
+          for (int c = 0; c < (second_half ? S::CB1 : S::CB0); ++c)
+            *reinterpret_cast<u32x4_t*>(mine + 4096 * c) = u32x4_t{0u, 0u, 0u, 0u};
         }
         __syncthreads();
-        const uint32_t poison = __builtin_amdgcn_readfirstlane(s_bad);
-        const int first_new = (tile - u.ctx_tiles) * kKeys;
-#pragma unroll
-        for (int r = 0; r < NR; ++r) {
-          bits[r] = static_cast<uint32_t>(mask[r] >> first_new) & vis;
-          if (bits[r] & poison) l[r] = __builtin_nanf("");
-        }
       }
-      if (computes)
-        tile_step<S, NR, T, FP8>(data, q, acc, m, l, scale_log2, s_ks[buf], dbase, g, l16,
-                                 is_ctx(tile) && vis == 0xffffffffu, bits);
+      return poison;
+    };
+    // The first iteration's output: no weights over a tile of zeros.
+    for (int i = tid; i < S::TILE / 16; i += kThreads)
+      *reinterpret_cast<u32x4_t*>(smem[(t0 + S::NBUF - 1) % S::NBUF] + 16 * i) = u32x4_t{0u, 0u, 0u, 0u};
+    if (tid < RW * 64) {
+      s_w[(t0 + 1) % 2].p[tid / 64][0][lane] = s_w[(t0 + 1) % 2].p[tid / 64][1][lane] = u32x2_t{0u, 0u};
+      if (lane < 32) s_w[(t0 + 1) % 2].m[tid / 64][lane / 16][l16] = kNone;
     }
+    // What every wave does in iteration `tile`, before its products and after: the tile's arrival, the loads of a later one.
+    const auto begin = [&](int tile) {
+      arrive(tile);
+      const int ahead = tile + (FP8 ? 3 : 2);
+      if (ahead < t1 && is_ctx(ahead)) window(ahead);
+      // 16-bit pages: waves 0-3 start the tile two ahead before their products, waves 4-7 after, so that of the two waves
+      // of a SIMD one has the matrix cores while the other is at its loads.
+      if (FP8 || !second_half) start(ahead);
+      if (FP8 && tile < t1) {
+        if (is_ctx(tile)) widen(tile);
+        else issue(tile);  // the round's rows are 16-bit: brought in here, there are few of them
+      }
+    };
+    const auto widened = [&](int tile) {
+      if (!is_ctx(tile)) wait_vm<0>();
+      __syncthreads();
+    };
+    if (!computes) {  // no rows of this row group: a share of the loads alone
+      for (int tile = t0; tile <= t1; ++tile) {
+        begin(tile);
+        if (FP8 && tile < t1) widened(tile);
+        if (tile < t1 && !is_ctx(tile)) clean(tile);
+        if (!FP8 && second_half) start(tile + 2);
+      }
+      __syncthreads();
+      pos += t1 - t0;
+      continue;
+    }
+    u32x4_t q[S::KC];
+    f32x4_t acc[S::DT];
+    float m = kNone, macc = kNone, l = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < S::DT; ++dt) acc[dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    {
+      int rho, t, head;
+      const bool ok = my_row(rho, t, head);
+      const uint16_t* const qrow = static_cast<const uint16_t*>(a.q) + (u.start + t) * a.stride_qt + head * a.stride_qh;
+#pragma unroll
+      for (int c = 0; c < S::KC; ++c)  // the columns of the lane's chunk of the scores' operand
+        q[c] = ok ? *reinterpret_cast<const u32x4_t*>(qrow + 64 * (c / 2) + 8 * (2 * g + (c & 1))) : u32x4_t{0u, 0u, 0u, 0u};
+      // Settled here, once: a wait for them inside the loop would wait for the tiles on their way too.
+#pragma unroll
+      for (int c = 0; c < S::KC; ++c) asm volatile("" : "+v"(q[c]));
+    }
+    // Iteration `tile`: its scores and weights, and the output of the tile before it.
+    for (int tile = t0; tile <= t1; ++tile) {
+      begin(tile);
+      uint32_t bits = 0xffffffffu;
+      bool all = true;
+      f32x4_t s = {0.f, 0.f, 0.f, 0.f};
+      const auto score = [&] {
+        const uint32_t vis = __builtin_amdgcn_readfirstlane(s_vis[tile % 4]);
+        bits = vis;
+        all = is_ctx(tile) && vis == 0xffffffffu;
+        if (!is_ctx(tile)) {
+          const uint32_t poison = clean(tile);
+          int rho, t, head;
+          const uint64_t mask = my_row(rho, t, head) ? static_cast<uint64_t>(a.masks[b * a.stride_mask + t]) : 0;
+          bits = static_cast<uint32_t>(mask >> ((tile - u.ctx_tiles) * kKeys)) & vis;
+          if (bits & poison) l = __builtin_nanf("");
+        }
+        s = score_step<S>(smem[tile % S::NBUF], q, kt, fresh(lane));
+      };
+      const u32x4_t pb = take_weights<S>(s_w[(tile + 1) % 2], row_wave, acc, macc, m, l, fresh(lane));
+      if (!FP8 && tile < t1) score();
+      value_step<S>(smem[(tile + S::NBUF - 1) % S::NBUF], pb, acc, dbase, fresh(lane));
+      if (FP8 && tile < t1) {
+        widened(tile);
+        score();
+      }
+      if (tile < t1)
+        weight_step<S>(s, s_w[tile % 2], row_wave, kt, column_wave < 2, m, l, scale_log2, s_rest[tile % 4], fresh(lane), all,
+                       bits);
+      if (!FP8 && second_half) start(tile + 2);
+    }
+    // the sum over both halves of the keys: each wave's own is relative to the last maximum by now
+    float sum = l + __shfl_xor(l, 16, 64);
+    sum += __shfl_xor(sum, 32, 64);
+    if (column_wave < 2 && g == 0) s_sum[row_wave][kt][l16] = sum;
+    __syncthreads();
+    sum = s_sum[row_wave][0][l16] + s_sum[row_wave][1][l16];
 
     const bool whole = t0 == 0 && t1 == u.tiles;
-    const int64_t slot = 2 * static_cast<int64_t>(wg) + (t0 == 0 ? 1 : 0);
-    if (computes) {
+    const float inv = sum == 0.f ? 0.f : 1.0f / sum;  // nothing seen: zeros
+    int rho, t, head;
+    const bool ok = my_row(rho, t, head);
+    if (ok && whole) {
+      uint16_t* const o = static_cast<uint16_t*>(a.out) + (u.start + t) * a.stride_ot + head * a.stride_oh + dbase;
 #pragma unroll
-      for (int r = 0; r < NR; ++r) {
-        float sum = l[r] + __shfl_xor(l[r], 16, 64);
-        sum += __shfl_xor(sum, 32, 64);
-        const float inv = sum == 0.f ? 0.f : 1.0f / sum;  // nothing seen: zeros
-        if (!ok[r]) continue;
-        if (whole) {
-          const int t = rho[r] / a.heads, head = rho[r] % a.heads;
-          uint16_t* const o = static_cast<uint16_t*>(a.out) + (u.start + t) * a.stride_ot + head * a.stride_oh + dbase;
+      for (int dt = 0; dt < S::DT; ++dt)
+        *reinterpret_cast<u32x2_t*>(o + 16 * dt + 4 * g) =
+            u32x2_t{pack2<T>(acc[dt][0] * inv, acc[dt][1] * inv), pack2<T>(acc[dt][2] * inv, acc[dt][3] * inv)};
+    } else if (ok) {
+      const int64_t part = (2 * static_cast<int64_t>(wg) + (t0 == 0 ? 1 : 0)) * S::ROWS + rho - rg * S::ROWS;
+      float* const o = a.workspace + p.part_off + part * RANK + dbase;
 #pragma unroll
-          for (int dt = 0; dt < S::DT; ++dt)
-            *reinterpret_cast<u32x2_t*>(o + 16 * dt + 4 * g) =
-                u32x2_t{pack2<T>(acc[r][dt][0] * inv, acc[r][dt][1] * inv), pack2<T>(acc[r][dt][2] * inv, acc[r][dt][3] * inv)};
-        } else {
-          const int64_t part = slot * S::ROWS + rho[r] - rg * S::ROWS;
-          float* const o = a.workspace + p.part_off + part * RANK + dbase;
-#pragma unroll
-          for (int dt = 0; dt < S::DT; ++dt) *reinterpret_cast<f32x4_t*>(o + 16 * dt + 4 * g) = acc[r][dt] * inv;
-          if (g == 0 && dbase == 0) a.workspace[p.lse_off + part] = sum == 0.f ? -INFINITY : m[r] + log2f(sum);
-        }
-      }
+      for (int dt = 0; dt < S::DT; ++dt) *reinterpret_cast<f32x4_t*>(o + 16 * dt + 4 * g) = acc[dt] * inv;
+      if (g == 0 && dbase == 0) a.workspace[p.lse_off + part] = sum == 0.f ? -INFINITY : macc + log2f(sum);
     }
     pos += t1 - t0;
   }
@@ -547,6 +686,7 @@ bool covered(const eagle4_latent_attn_args& a) {
   if (static_cast<int64_t>(a.max_blocks) * a.page >= (int64_t(1) << 31) - kKeys) return false;  // 32-bit positions
   for (const int64_t s : {a.stride_qt, a.stride_qh, a.stride_nt, a.stride_cb, a.stride_cs, a.stride_ot, a.stride_oh})
     if (s % 8 != 0) return false;
+  if (a.cache_dtype == EAGLE4_FP8_E4M3 && (a.stride_cb % 16 != 0 || a.stride_cs % 16 != 0)) return false;
   for (const void* p : {a.q, a.latent_new, a.cache, static_cast<const void*>(a.out)})
     if (reinterpret_cast<uintptr_t>(p) % 16 != 0) return false;
   return true;
@@ -571,6 +711,8 @@ LatentPlan plan(const eagle4_latent_attn_args& a) {
   p.groups = kGroups;
   p.least = 4;
   p.first = 0;
+  p.page_shift = (a.page & (a.page - 1)) == 0 ? __builtin_ctz(a.page) : -1;
+  p.page_inv = a.page > 1 ? static_cast<uint32_t>((uint64_t(1) << 32) / a.page) : 0;
   const int fit = reqs_of(a, p.rows);
   p.reqs = a.num_reqs < fit ? a.num_reqs : fit;
   p.pre_off = 0;
@@ -582,9 +724,9 @@ LatentPlan plan(const eagle4_latent_attn_args& a) {
 template <int RANK, typename T, bool FP8>
 int launch(const eagle4_latent_attn_args& a, const LatentPlan& p, hipStream_t s) {
   switch (p.rows) {
-    case 16: latent_kernel<RANK, 64, T, FP8, 1, 1><<<p.groups, 256, 0, s>>>(a, p); break;
-    case 32: latent_kernel<RANK, 64, T, FP8, 1, 2><<<p.groups, 256, 0, s>>>(a, p); break;
-    default: latent_kernel<RANK, 64, T, FP8, 2, 2><<<p.groups, 256, 0, s>>>(a, p); break;
+    case 16: latent_kernel<RANK, 64, T, FP8, 1><<<p.groups, kThreads, 0, s>>>(a, p); break;
+    case 32: latent_kernel<RANK, 64, T, FP8, 2><<<p.groups, kThreads, 0, s>>>(a, p); break;
+    default: latent_kernel<RANK, 64, T, FP8, 4><<<p.groups, kThreads, 0, s>>>(a, p); break;
   }
   const int status = E4_LAUNCH_STATUS();
   if (status != EAGLE4_OK) return status;
