@@ -26,8 +26,8 @@ namespace {
 using namespace e4attn;
 
 constexpr int kKeys = 32;      // keys of a tile
-constexpr int kWindow = 256;   // block-table entries held in LDS
-constexpr int kMaxReqs = 512; // requests of one launch (their tile counts are kept in LDS)
+constexpr int kBatch = 4;      // tiles whose keys' addresses are looked up together
+constexpr int kMaxReqs = 512; // requests of one launch (a thread counts the tiles of each)
 
 struct LatentPlan {
   int first, reqs;       // requests of this launch
@@ -73,6 +73,10 @@ E4_DEV uint32_t lds_addr(const void* p) {
 // 64 lanes x 16 bytes from per-lane addresses into LDS [lds, lds + 1024), lane p at lds + 16 p.
 E4_DEV void dma16(const void* src, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(lds) : "memory", "m0");
+}
+// The same with 4 bytes a lane.
+E4_DEV void dma4(const void* src, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(src), "s"(lds) : "memory", "m0");
 }
 template <int N>
 E4_DEV void wait_vm() {
@@ -120,18 +124,6 @@ E4_DEV int fresh(int x) {
   return x;
 }
 
-// The bits of lanes 0, 8, .., 56 of a ballot, as a byte; those of lanes 0, 4, .., 60, as 16 bits.
-E4_DEV uint8_t every_eighth(uint64_t ballot) {
-  return static_cast<uint8_t>(((ballot & 0x0101010101010101ull) * 0x0102040810204080ull) >> 56);
-}
-E4_DEV uint16_t every_fourth(uint64_t x) {
-  x &= 0x1111111111111111ull;
-  x = (x | x >> 3) & 0x0303030303030303ull;
-  x = (x | x >> 6) & 0x000f000f000f000full;
-  x = (x | x >> 12) & 0x000000ff000000ffull;
-  return static_cast<uint16_t>(x | x >> 24);
-}
-
 // A tile in LDS: CB blocks of 64 columns, each 32 keys x 128 bytes, the eight 16-byte chunks of a key's 128 bytes at
 // chunk ^ swz(key). Both operand reads then run at the LDS's full rate (256 bytes a cycle): the scores' (16 keys; the four
 // lane groups at chunks 2 g or 2 g + 1) and the transposing one (8 keys at two adjacent chunks). With the lane groups
@@ -147,15 +139,23 @@ struct Shape {
   static constexpr bool FP8 = FP8_;
   static constexpr int RW = RW_, DW = kWaves / RW, DT = RANK / 16 / DW;
   static constexpr int DIM = RANK + ROPE, CB = DIM / 64, KC = DIM / 32, ROWS = RW * 16, TILE = CB * 4096;
-  // 16-bit pages: a ring of four tiles, two in use and two on their way. fp8 pages: a ring of four tiles of codes, three on
-  // their way, and two widened ones.
-  static constexpr int NBUF = FP8 ? 2 : 4, RAW = CB * 2048;
+  // 16-bit pages: a ring of four tiles, two in use and two on their way. fp8 pages: a ring of three, two in use and one being
+  // widened, and one of two tiles of codes, the one that is widened and one on its way.
+  static constexpr int NBUF = FP8 ? 3 : 4, RAW = CB * 2048;
   // blocks of 64 columns that waves 0-3 (each 8 keys of a tile) bring in; waves 4-7 bring in the rest
   static constexpr int CB0 = (CB + 1) / 2, CB1 = CB - CB0;
   // LDS operands of the matrix products in registers at a time, the one in use among them. Their loads run that far ahead
   // in this order, product by product: left to itself the compiler waits for each operand right after its load.
   static constexpr int AHEAD = 8;
 };
+
+// The larger of a lane's value and that of lane ^ 16 or lane ^ 32: swaps of rows of lanes, no LDS trip.
+template <int N>
+E4_DEV float other_max(float x) {
+  const uint32_t w = __float_as_uint(x);
+  const auto r = N == 16 ? __builtin_amdgcn_permlane16_swap(w, w, false, false) : __builtin_amdgcn_permlane32_swap(w, w, false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
 
 // A wave's share of the weights: P^T of one half tile (16 keys x 16 rows) as written by its lanes, and the rows' maxima.
 template <int RW>
@@ -164,9 +164,10 @@ struct Weights {
   float m[RW][2][16];
 };
 
-// The scores of keys 16 kt .. of a tile, for a wave's 16 rows.
-template <typename S>
-E4_DEV f32x4_t score_step(const char* tile, const u32x4_t (&q)[S::KC], int kt, int lane) {
+// The scores of keys 16 kt .. of a tile, for a wave's 16 rows. between(c) follows product c: other work, which the matrix
+// core's time covers.
+template <typename S, typename F>
+E4_DEV f32x4_t score_step(const char* tile, const u32x4_t (&q)[S::KC], int kt, int lane, F between) {
   using T = typename S::T;
   const int g = lane >> 4, l16 = lane & 15, x = swz(l16);
   const char* const k0 = tile + kt * 2048 + l16 * 128 + 16 * ((2 * g) ^ x);
@@ -182,51 +183,59 @@ E4_DEV f32x4_t score_step(const char* tile, const u32x4_t (&q)[S::KC], int kt, i
   for (int c = 0; c < S::KC; ++c) {
     if (c + S::AHEAD - 1 < S::KC) load(c + S::AHEAD - 1);
     s[c % 2] = mfma16<T>(ka[c % S::AHEAD], q[c], s[c % 2]);
+    between(c);
     __builtin_amdgcn_sched_barrier(0);
   }
   return s[0] + s[1];
 }
 
 // The weights of those scores into `to`, relative to the rows' maximum m; l takes their sum. Bit k of bits: key k of the tile
-// is visible to the lane's row (`all`: every key to every row).
+// is visible to the lane's row. In kPhases phases without a branch, for the places between the products of the output.
 template <typename S>
-E4_DEV void weight_step(f32x4_t s, Weights<S::RW>& to, int row_wave, int kt, bool writes, float& m, float& l,
-                        float scale_log2, const float* key_scale, int lane, bool all, uint32_t bits) {
+struct WeightStep {
   using T = typename S::T;
-  const int g = lane >> 4;
-  s *= scale_log2;
-  f32x4_t ks = {1.f, 1.f, 1.f, 1.f};
-  if constexpr (S::FP8) {
-    ks = *reinterpret_cast<const f32x4_t*>(key_scale + 16 * kt + 4 * g);
-    s *= ks;
-  }
-  if (!all) {
+  static constexpr int kPhases = 8;
+  f32x4_t s, ks;
+  float top, p[4];
+  E4_DEV void phase(int i, Weights<S::RW>& to, int row_wave, int kt, bool writes, float& m, float& l, float scale_log2,
+                    const float* key_scale, int lane, uint32_t bits) {
+    const int g = lane >> 4;
+    if (i == 0) {
+      s *= scale_log2;
+      if constexpr (S::FP8) {
+        ks = *reinterpret_cast<const f32x4_t*>(key_scale + 16 * kt + 4 * g);
+        s *= ks;
+      }
+    } else if (i == 1) {
+      const uint32_t mine = bits >> (16 * kt + 4 * g);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (!((bits >> (16 * kt + 4 * g + i)) & 1)) s[i] = -INFINITY;
-  }
-  float top = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
-  // The maximum moves only when it grows by more than 2^8 (until then p stays below 2^8, which 16 bits hold as well as
-  // values below 1), and to a whole number: what was weighted with the last one is then scaled without rounding.
-  if (__any(top > m + 8.f)) {
-    top = fmaxf(top, __shfl_xor(top, 16, 64));
-    top = fmaxf(top, __shfl_xor(top, 32, 64));
-    const float now = fmaxf(m, ceilf(top));
-    l *= exp2f(m - now);
-    m = now;
-  }
-  float p[4];
+      for (int k = 0; k < 4; ++k) s[k] = (mine >> k) & 1 ? s[k] : -INFINITY;
+    } else if (i == 2) {
+      top = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
+      top = other_max<16>(top);
+    } else if (i == 3) {
+      top = other_max<32>(top);
+    } else if (i == 4) {
+      // The maximum moves only when it grows by more than 2^8 (until then p stays below 2^8, which 16 bits hold as well as
+      // values below 1), and to a whole number: what was weighted with the last one is then scaled without rounding.
+      const float now = top > m + 8.f ? ceilf(top) : m;
+      l *= __builtin_amdgcn_exp2f(m - now);
+      m = now;
+    } else if (i == 5) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    p[i] = __builtin_amdgcn_exp2f(s[i] - m);
-    l += p[i];
-    if constexpr (S::FP8) p[i] *= ks[i];
+      for (int k = 0; k < 4; ++k) p[k] = __builtin_amdgcn_exp2f(s[k] - m);
+    } else if (i == 6) {
+      l += (p[0] + p[1]) + (p[2] + p[3]);
+      if constexpr (S::FP8) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) p[k] *= ks[k];
+      }
+    } else if (writes) {
+      to.p[row_wave][kt][lane] = u32x2_t{pack2<T>(p[0], p[1]), pack2<T>(p[2], p[3])};
+      if (g == 0) to.m[row_wave][kt][lane & 15] = m;
+    }
   }
-  if (writes) {
-    to.p[row_wave][kt][lane] = u32x2_t{pack2<T>(p[0], p[1]), pack2<T>(p[2], p[3])};
-    if (g == 0) to.m[row_wave][kt][lane & 15] = m;
-  }
-}
+};
 
 // Two packed weights times a power of two.
 template <typename T>
@@ -261,9 +270,9 @@ E4_DEV u32x4_t take_weights(const Weights<S::RW>& from, int row_wave, f32x4_t (&
   return u32x4_t{p0[0], p0[1], p1[0], p1[1]};
 }
 
-// O^T += C^T P^T of a tile, for a wave's 16 rows and its columns dbase ...
-template <typename S>
-E4_DEV void value_step(const char* tile, u32x4_t pb, f32x4_t (&acc)[S::DT], int dbase, int lane) {
+// O^T += C^T P^T of a tile, for a wave's 16 rows and its columns dbase ...; between(dt) follows product dt.
+template <typename S, typename F>
+E4_DEV void value_step(const char* tile, u32x4_t pb, f32x4_t (&acc)[S::DT], int dbase, int lane, F between) {
   using T = typename S::T;
   const int g = lane >> 4, l16 = lane & 15;
   const int j = l16 >> 2, s4 = l16 & 3, kv = 4 * g + j, xv = swz(kv);
@@ -286,6 +295,7 @@ E4_DEV void value_step(const char* tile, u32x4_t pb, f32x4_t (&acc)[S::DT], int 
   for (int dt = 0; dt < S::DT; ++dt) {
     if (dt + VA - 1 < S::DT) load(dt + VA - 1);
     acc[dt] = mfma16<T>(va[dt % VA], pb, acc[dt]);
+    between(dt);
     __builtin_amdgcn_sched_barrier(0);
   }
 }
@@ -295,61 +305,65 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
     const eagle4_latent_attn_args a, const LatentPlan p) {
   using S = Shape<RANK, ROPE, T, FP8, RW>;
   __shared__ __attribute__((aligned(1024))) char smem[S::NBUF][S::TILE];
-  __shared__ __attribute__((aligned(1024))) char s_raw[FP8 ? 4 : 1][FP8 ? S::RAW : 16];
+  __shared__ __attribute__((aligned(1024))) char s_raw[FP8 ? 2 : 1][FP8 ? S::RAW : 16];
   __shared__ Weights<RW> s_w[2];
-  __shared__ uint32_t s_pre[kMaxReqs + 1];
-  __shared__ int32_t s_win[kWindow];
-  __shared__ float s_winscale[FP8 ? kWindow : 1];
-  // by tile % 4 (up to three tiles are under way beside the one in use): a bit a key that is there, and its scale's parts
-  __shared__ uint32_t s_vis[4];
-  __shared__ __attribute__((aligned(16))) float s_rest[4][kKeys], s_pow2[FP8 ? 4 : 1][kKeys];
+  // The keys of two batches of tiles: their table entries and scales as loaded, then the addresses of their rows, a bit a key
+  // that is there, and the two parts of its scale.
+  constexpr int kBatchKeys = kBatch * kKeys;
+  __shared__ __attribute__((aligned(16))) int32_t s_ent[kBatchKeys];
+  __shared__ __attribute__((aligned(16))) float s_entscale[FP8 ? kBatchKeys : 1];
+  __shared__ uint64_t s_row[2][kBatchKeys];
+  __shared__ uint32_t s_vis[2][kBatch];
+  __shared__ __attribute__((aligned(16))) float s_rest[FP8 ? 2 : 1][kBatchKeys], s_pow2[FP8 ? 2 : 1][kBatchKeys];
   __shared__ uint32_t s_bad;           // a bit a new key: it holds a value that is not finite
   __shared__ uint32_t s_tot[kWaves];
   __shared__ float s_sum[RW][2][16];
+  __shared__ int s_at;
+  __shared__ uint32_t s_before;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 4, l16 = lane & 15;
 
-  // tiles before each request
-  uint32_t run = 0;
-  for (int b0 = 0; b0 < p.reqs; b0 += kThreads) {
-    uint32_t n = 0;
-    if (b0 + tid < p.reqs) {
-      const Unit u = unit_of(a, p.first + b0 + tid, S::ROWS);
-      n = static_cast<uint32_t>(u.tiles) * static_cast<uint32_t>(u.row_groups);
-    }
-    uint32_t sum = n;
-#pragma unroll
-    for (int k = 1; k < 64; k <<= 1) {
-      const uint32_t o = __shfl_up(sum, k, 64);
-      if (lane >= k) sum += o;
-    }
-    if (lane == 63) s_tot[wave] = sum;
-    __syncthreads();
-    uint32_t before = run;
-    for (int w = 0; w < kWaves; ++w) {
-      if (w < wave) before += s_tot[w];
-      run += s_tot[w];
-    }
-    if (b0 + tid < p.reqs) s_pre[b0 + tid + 1] = before + sum;
-    __syncthreads();
+  // tiles before each request (one a thread)
+  static_assert(kMaxReqs <= kThreads, "requests of a launch");
+  uint32_t mine = 0, sum_tiles = 0;
+  if (tid < p.reqs) {
+    const Unit u = unit_of(a, p.first + tid, S::ROWS);
+    mine = static_cast<uint32_t>(u.tiles) * static_cast<uint32_t>(u.row_groups);
   }
-  if (tid == 0) s_pre[0] = 0;
+  sum_tiles = mine;
+#pragma unroll
+  for (int k = 1; k < 64; k <<= 1) {
+    const uint32_t o = __shfl_up(sum_tiles, k, 64);
+    if (lane >= k) sum_tiles += o;
+  }
+  if (lane == 63) s_tot[wave] = sum_tiles;
   __syncthreads();
-  const uint32_t total = uniform(run);
+  uint32_t all_tiles = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    if (w < wave) sum_tiles += s_tot[w];
+    all_tiles += s_tot[w];
+  }
+  const uint32_t total = uniform(all_tiles);
   uint32_t share = (total + p.groups - 1) / p.groups;
   share = share < static_cast<uint32_t>(p.least) ? p.least : share;
   // adjacent runs on one XCD (workgroups go to the eight in turn): row groups of a request share its tiles in the L2
   const int wg = p.groups % 8 == 0 ? (blockIdx.x % 8) * (p.groups / 8) + blockIdx.x / 8 : blockIdx.x;
-  if (wg == 0) {  // for the merge
-    uint32_t* const pre = reinterpret_cast<uint32_t*>(a.workspace + p.pre_off);
-    for (int i = tid; i <= p.reqs; i += kThreads) pre[i] = s_pre[i];
-  }
   uint32_t pos = wg * share;
   const uint32_t stop = pos + share < total ? pos + share : total;
+  if (sum_tiles - mine <= pos && pos < sum_tiles) {  // the request of tile `pos`
+    s_at = tid;
+    s_before = sum_tiles - mine;
+  }
+  if (wg == 0 && tid < p.reqs) {  // for the merge
+    uint32_t* const pre = reinterpret_cast<uint32_t*>(a.workspace + p.pre_off);
+    pre[tid + 1] = sum_tiles;
+    if (tid == 0) pre[0] = 0;
+  }
+  __syncthreads();
   if (pos >= stop) return;
-  int at = 0;  // the request of tile `pos`: the last with s_pre <= pos
-  for (int step = kMaxReqs / 2; step > 0; step >>= 1)
-    if (at + step < p.reqs && uniform(s_pre[at + step]) <= pos) at += step;
+  int at = uniform(s_at);
+  uint32_t before = uniform(s_before);  // tiles before request `at`
 
   const int row_wave = wave / S::DW, column_wave = wave % S::DW, kt = column_wave % 2, dbase = column_wave * S::DT * 16;
   const float scale_log2 = a.scale * 1.4426950408889634f;
@@ -367,12 +381,16 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
   const int cb_first = second_half ? S::CB0 : 0;
 
   while (pos < stop) {
-    while (uniform(s_pre[at + 1]) <= pos) ++at;
     const int b = p.first + at;
     Unit u = unit_of(a, b, S::ROWS);
     u = Unit{uniform(u.start), uniform(u.width), uniform(u.context), uniform(u.ctx_tiles), uniform(u.tiles),
              uniform(u.row_groups)};
-    const uint32_t within = pos - uniform(s_pre[at]);
+    const uint32_t within = pos - before, its_tiles = static_cast<uint32_t>(u.tiles) * static_cast<uint32_t>(u.row_groups);
+    if (within >= its_tiles) {
+      before += its_tiles;
+      ++at;
+      continue;
+    }
     const int rg = static_cast<int>(within / u.tiles), t0 = static_cast<int>(within % u.tiles);
     const int t1 = static_cast<int>(static_cast<uint32_t>(u.tiles - t0) < stop - pos ? u.tiles : t0 + (stop - pos));
     const int32_t* const table = static_cast<const int32_t*>(a.block_table.ptr) + b * a.block_table.s0;
@@ -387,134 +405,158 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
       head = ok ? rho - t * a.heads : 0;
       return ok;
     };
-    int win0 = 0, win1 = 0;  // the block-table entries in LDS
-    const auto window = [&](int tile) {  // makes those of context tile `tile` be there; every thread calls it
-      const int lo = uniform(page_of(tile * kKeys));
-      const int last = tile * kKeys + kKeys < u.context ? tile * kKeys + kKeys - 1 : u.context - 1;
-      if (lo >= win0 && page_of(last) < win1) return;
-      __syncthreads();
-      win0 = lo;
-      win1 = lo + kWindow;
-#pragma unroll 1
-      for (int i = fresh(tid); i < kWindow; i += kThreads) {
-        int32_t blk = -1;
-        if (win0 + i < a.max_blocks) blk = table[win0 + i];
-        if (blk < 0 || blk >= a.num_blocks) blk = -1;
-        s_win[i] = blk;
-        if constexpr (FP8) s_winscale[i] = blk >= 0 ? a.scale_page[blk * a.stride_sp] : 0.f;
+    const int tiles = t1 - t0;
+    const auto is_ctx = [&](uint32_t i) { return t0 + static_cast<int>(i) < u.ctx_tiles; };  // tile i of the piece
+    // The keys of batch n of the piece (tiles kBatch n ..), one a thread of waves 0 and 1: the table entry of a context key
+    // (a key behind the context: the last one's), ...
+    const auto entry_of = [&](int n, int i) -> const int32_t* {
+      const int k = (t0 + kBatch * n) * kKeys + i;
+      return table + page_of(k < u.context ? k : (u.context > 0 ? u.context - 1 : 0));
+    };
+    // ... and from it the key's address, its mark and its scale. What is not there reads zeros.
+    const auto fill = [&](int n, int i, int32_t blk, float scale) {
+      const int tile = kBatch * n + i / kKeys, key = i % kKeys;
+      const char* row = nullptr;
+      if (tile < tiles && is_ctx(tile)) {
+        const int k = (t0 + tile) * kKeys + key, page = page_of(k);
+        if (k < u.context && blk >= 0 && blk < a.num_blocks)
+          row = cache + blk * scb + static_cast<int64_t>(k - page * a.page) * scs;
+      } else if (tile < tiles) {
+        const int j = (t0 + tile - u.ctx_tiles) * kKeys + key;
+        scale = 1.f;
+        if (j < u.width) row = static_cast<const char*>(a.latent_new) + (u.start + j) * a.stride_nt * 2;
       }
-      __syncthreads();
+      if (row == nullptr) scale = 1.f;
+      const uint64_t there = __ballot(row != nullptr);
+      if (key == 0) s_vis[n % 2][i / kKeys] = static_cast<uint32_t>(there >> (i & 32));
+      s_row[n % 2][i] = reinterpret_cast<uint64_t>(row != nullptr ? row : reinterpret_cast<const char*>(zero_row));
+      if constexpr (FP8) split_scale(scale, s_pow2[n % 2][i], s_rest[n % 2][i]);
     };
-    // the lane's key row of a tile; null where there is none
-    const auto key_row = [&](int tile, int my_key, float& scale) -> const char* {
-      scale = 1.f;
-      if (tile >= u.ctx_tiles) {
-        const int j = (tile - u.ctx_tiles) * kKeys + my_key;
-        return j < u.width ? static_cast<const char*>(a.latent_new) + (u.start + j) * a.stride_nt * 2 : nullptr;
+    // In the loop the lookups are direct loads too, two iterations ahead of the fill, which is two ahead of the first use.
+    const auto lookup = [&](int i) {
+      if (wave >= 2) return;
+      const int n = i / kBatch, key = fresh(tid), k0 = 64 * wave;
+      if (i % kBatch == 2) {
+        if ((t0 + kBatch * (n + 2)) * kKeys < u.context) dma4(entry_of(n + 2, key), uniform(lds_addr(&s_ent[k0])));
+      } else if (FP8 && i % kBatch == 3) {  // (an entry that was not loaded is none of a key's, and in its bounds or not used)
+        const int32_t blk = s_ent[key];
+        dma4(a.scale_page + (blk >= 0 && blk < a.num_blocks ? blk : 0) * a.stride_sp,
+             uniform(lds_addr(&s_entscale[FP8 ? k0 : 0])));
+      } else if (i % kBatch == 0 && i > 0) {
+        fill(n + 1, key, s_ent[key], FP8 ? s_entscale[FP8 ? key : 0] : 1.f);
       }
-      const int k = tile * kKeys + my_key;
-      if (k >= u.context) return nullptr;
-      const int page = page_of(k);
-      const int32_t blk = s_win[page - win0];
-      if constexpr (FP8) scale = s_winscale[page - win0];
-      return blk >= 0 ? cache + blk * scb + static_cast<int64_t>(k - page * a.page) * scs : nullptr;
     };
-    const auto is_ctx = [&](int tile) { return tile < u.ctx_tiles; };
-    // a tile of 16-bit rows by direct loads
-    const auto issue = [&](int tile) {
-      const int ln = fresh(lane), my_key = 8 * octet + ln / 8, my_chunk = (ln % 8) ^ swz(my_key);
-      float scale;
-      const char* row = key_row(tile, my_key, scale);
-      const uint8_t there = every_eighth(__ballot(row != nullptr));
-      if (!second_half && ln == 0) reinterpret_cast<uint8_t*>(&s_vis[tile % 4])[octet] = there;
-      if (FP8 && !second_half) s_rest[tile % 4][my_key] = 1.f;  // eight lanes, one value
-      if (row == nullptr) row = reinterpret_cast<const char*>(zero_row);
-      const char* const src = row + 16 * my_chunk + 128 * cb_first;
-      const uint32_t dst = __builtin_amdgcn_readfirstlane(lds_addr(smem[tile % S::NBUF]) + 1024 * octet + 4096 * cb_first);
+    // Direct loads of a tile, in two parts: the address, then the loads one by one. A tile past the piece (and, for fp8, one
+    // of the round's rows) brings in zeros, so that every iteration has the same loads.
+    struct Loads {
+      const char* src;
+      uint32_t dst;
+    };
+    // 16-bit rows: block c of the wave's CB0 (waves 4-7: CB1) blocks
+    const auto prepare = [&](int i) {
+      const int ln = fresh(lane), key = 8 * octet + (ln >> 3), chunk = (ln & 7) ^ swz(key);
+      const char* const row = reinterpret_cast<const char*>(s_row[i / kBatch % 2][i % kBatch * kKeys + key]);
+      return Loads{row + (16 * chunk + 128 * cb_first),
+                   uniform(lds_addr(smem[i % S::NBUF]) + 1024 * octet + 4096 * cb_first)};
+    };
+    const auto load = [&](const Loads& to, int c) { dma16(to.src + 128 * c, to.dst + 4096 * c); };
+    // fp8 codes: a block of 64 columns is 32 keys x 64 bytes, an instruction 16 keys of it; wave w brings in keys 16 (w % 2) ..
+    // of blocks w / 2, w / 2 + 4, ..
+    const auto prepare8 = [&](int i) {
+      const int ln = fresh(lane), key = 16 * (wave % 2) + (ln >> 2);
+      const char* row = reinterpret_cast<const char*>(s_row[i / kBatch % 2][i % kBatch * kKeys + key]);
+      if (!is_ctx(i)) row = reinterpret_cast<const char*>(zero_row);
+      return Loads{row + (16 * (ln & 3) + 64 * (wave / 2)),
+                   uniform(lds_addr(s_raw[FP8 ? i % 2 : 0]) + 1024 * (wave % 2) + 2048 * (wave / 2))};
+    };
+    const auto load8 = [&](const Loads& to, int c) { dma16(to.src + 256 * c, to.dst + 8192 * c); };
+    // the loads that every wave has, and the ones that some have beyond them
+    constexpr int kLoads = FP8 ? S::CB / 4 : S::CB1;
+    const bool more = FP8 ? wave / 2 + 4 * kLoads < S::CB : S::CB0 > S::CB1 && !second_half;
+    const auto prepare_next = [&](int i) {
+      if constexpr (FP8) return prepare8(i); else return prepare(i);
+    };
+    const auto load_next = [&](const Loads& to, int c) {
+      if constexpr (FP8) load8(to, c); else load(to, c);
+    };
+    const auto load_all = [&](const Loads& to) {
 #pragma unroll
-      for (int c = 0; c < S::CB1; ++c) dma16(src + 128 * c, dst + 4096 * c);
-      if (S::CB0 > S::CB1 && !second_half) dma16(src + 128 * S::CB1, dst + 4096 * S::CB1);
+      for (int c = 0; c < kLoads; ++c) load_next(to, c);
+      if (more) load_next(to, kLoads);
     };
-    // a tile of fp8 codes by direct loads: a block of 64 columns is 32 keys x 64 bytes, an instruction 16 keys of it; wave w
-    // brings in keys 16 (w % 2) .. of blocks w / 2, w / 2 + kWaves / 2, ..
-    const auto issue8 = [&](int tile) {
-      const int ln = fresh(lane), my_key = 16 * (wave % 2) + ln / 4;
-      float scale, pow2, rest;
-      const char* row = key_row(tile, my_key, scale);
-      const uint16_t there = every_fourth(__ballot(row != nullptr));
-      split_scale(scale, pow2, rest);
-      if (wave < 2) {
-        if (ln == 0) reinterpret_cast<uint16_t*>(&s_vis[tile % 4])[wave] = there;
-        s_pow2[FP8 ? tile % 4 : 0][my_key] = pow2;
-        s_rest[tile % 4][my_key] = rest;
+    // widens the codes of block c of the wave's CB0 / CB1 blocks
+    struct Codes {
+      const char* src;
+      char* dst;
+      float pow2;
+    };
+    const auto codes_of = [&](int i) {
+      const int ln = fresh(lane), key = 8 * octet + (ln >> 3), chunk = (ln & 7) ^ swz(key);
+      return Codes{s_raw[FP8 ? i % 2 : 0] + 2048 * cb_first + key * 64 + 8 * (ln & 7),
+                   smem[i % S::NBUF] + 4096 * cb_first + key * 128 + 16 * chunk,
+                   s_pow2[FP8 ? i / kBatch % 2 : 0][i % kBatch * kKeys + key]};
+    };
+    const auto widen = [&](const Codes& x, int c) {
+      *reinterpret_cast<u32x4_t*>(x.dst + 4096 * c) = widen8<T>(*reinterpret_cast<const u32x2_t*>(x.src + 2048 * c), x.pow2);
+    };
+    // fp8, what a tile needs of every wave an iteration ahead: its codes widened, or (the round's rows are 16-bit, and few)
+    // its rows brought in
+    const auto next_rows = [&](int i) {
+      if (i >= tiles) return;
+      if (is_ctx(i)) {
+        const Codes x = codes_of(i);
+#pragma unroll
+        for (int c = 0; c < S::CB1; ++c) widen(x, c);
+        if (S::CB0 > S::CB1 && !second_half) widen(x, S::CB1);
+      } else {
+        const Loads to = prepare(i);
+#pragma unroll
+        for (int c = 0; c < S::CB1; ++c) load(to, c);
+        if (S::CB0 > S::CB1 && !second_half) load(to, S::CB1);
       }
-      if (row == nullptr) row = reinterpret_cast<const char*>(zero_row);
-      const char* const src = row + 16 * (ln % 4);
-      const uint32_t dst = __builtin_amdgcn_readfirstlane(lds_addr(s_raw[FP8 ? tile % 4 : 0]) + 1024 * (wave % 2));
-#pragma unroll
-      for (int c0 = 0; c0 < S::CB; c0 += kWaves / 2)
-        if (wave / 2 + c0 < S::CB) dma16(src + 64 * (wave / 2 + c0), dst + 2048 * (wave / 2 + c0));
-    };
-    const auto widen = [&](int tile) {
-      const int ln = fresh(lane), my_key = 8 * octet + ln / 8, my_chunk = (ln % 8) ^ swz(my_key);
-      const float pow2 = s_pow2[FP8 ? tile % 4 : 0][my_key];
-      const char* const src = s_raw[FP8 ? tile % 4 : 0] + 2048 * cb_first + my_key * 64 + 8 * (ln % 8);
-      char* const dst = smem[tile % S::NBUF] + 4096 * cb_first + my_key * 128 + 16 * my_chunk;
-      const int blocks = second_half ? S::CB1 : S::CB0;
-#pragma unroll
-      for (int c = 0; c < S::CB0; ++c)
-        if (c < blocks)
-          *reinterpret_cast<u32x4_t*>(dst + 4096 * c) = widen8<T>(*reinterpret_cast<const u32x2_t*>(src + 2048 * c), pow2);
     };
 
     __syncthreads();  // the last piece's tiles have been read
-    // the tiles behind the first start after it, so that two (fp8: three) are under way in the loop
-    const auto start = [&](int tile) {
-      if (tile >= t1 || (FP8 && !is_ctx(tile))) return;
-      if constexpr (FP8) issue8(tile); else issue(tile);
-    };
-#pragma unroll 1
-    for (int i = 0; i < (FP8 ? 3 : 2); ++i) {
-      if (t0 + i < t1 && is_ctx(t0 + i)) window(t0 + i);
-      start(t0 + i);
+    if (tid < 2 * kBatchKeys) {  // batches 0 and 1
+      const int n = tid / kBatchKeys, i = tid % kBatchKeys;
+      int32_t blk = -1;
+      if ((t0 + kBatch * n) * kKeys + i < u.context) blk = *entry_of(n, i);
+      float scale = 1.f;
+      if (FP8 && blk >= 0 && blk < a.num_blocks) scale = a.scale_page[blk * a.stride_sp];
+      fill(n, i, blk, scale);
     }
-    // Waits until a tile (fp8: its codes) is there for every wave, the last tile's weights too; the buffer of the tile before
-    // that is free.
-    const auto arrive = [&](int tile) {
-      if constexpr (FP8) {
-        // instructions a tile of waves below 2 (CB % 4); the others one less
-        constexpr int kMost = (S::CB + 3) / 4;
-        const bool less = S::CB % 4 != 0 && wave >= 2 * (S::CB % 4);
-        if (tile + 2 < t1 && is_ctx(tile + 2)) {
-          if (less) wait_vm<2 * (kMost - 1)>(); else wait_vm<2 * kMost>();
-        } else if (tile + 1 < t1 && is_ctx(tile + 1)) {
-          if (less) wait_vm<kMost - 1>(); else wait_vm<kMost>();
-        } else {
-          wait_vm<0>();
-        }
-      } else {
-        if (tile + 1 < t1) {
-          if (second_half) wait_vm<S::CB1>(); else wait_vm<S::CB0>();
-        } else {
-          wait_vm<0>();
-        }
+    __syncthreads();
+#pragma unroll 1
+    for (int i = 0; i < 2; ++i) load_all(prepare_next(i));
+    if constexpr (FP8) {
+      wait_vm<0>();
+      __syncthreads();
+      next_rows(0);
+    }
+    // Waits until tile i (fp8: the codes of the one after it too) is there for every wave, the last tile's weights too; the
+    // buffer of the tile before that is free.
+    const auto arrive = [&](int i) {
+      if (FP8 || i == tiles) {
+        wait_vm<0>();
+      } else {  // the loads of the tile behind it may be outstanding
+        if (second_half) wait_vm<S::CB1>(); else wait_vm<S::CB0>();
       }
       __syncthreads();
     };
     // The round's rows. One that is not finite must not reach the rows that do not see it through 0 x NaN: it is cleared, and
     // the rows that see it become NaN. Gives a bit a row that was cleared; every wave calls it.
-    const auto clean = [&](int tile) {
+    const auto clean = [&](int i) {
       if (tid == 0) s_bad = 0;
       __syncthreads();
-      const int ln = fresh(lane), my_key = 8 * octet + ln / 8;
-      char* const mine = smem[tile % S::NBUF] + 4096 * cb_first + my_key * 128 + 16 * (ln % 8);
+      const int ln = fresh(lane), my_key = 8 * octet + (ln >> 3);
+      char* const mine = smem[i % S::NBUF] + 4096 * cb_first + my_key * 128 + 16 * (ln & 7);
       bool bad = false;
 #pragma unroll 1
       for (int c = 0; c < (second_half ? S::CB1 : S::CB0); ++c) {
         const u32x4_t w = *reinterpret_cast<const u32x4_t*>(mine + 4096 * c);
         constexpr uint32_t kExp = T::code == EAGLE4_BF16 ? 0x7f80u : 0x7c00u;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) bad |= (w[i] & kExp) == kExp || ((w[i] >> 16) & kExp) == kExp;
+        for (int k = 0; k < 4; ++k) bad |= (w[k] & kExp) == kExp || ((w[k] >> 16) & kExp) == kExp;
       }
       if (bad) atomicOr(&s_bad, 1u << my_key);
       __syncthreads();
@@ -531,37 +573,23 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
     };
     // The first iteration's output: no weights over a tile of zeros.
     for (int i = tid; i < S::TILE / 16; i += kThreads)
-      *reinterpret_cast<u32x4_t*>(smem[(t0 + S::NBUF - 1) % S::NBUF] + 16 * i) = u32x4_t{0u, 0u, 0u, 0u};
+      *reinterpret_cast<u32x4_t*>(smem[S::NBUF - 1] + 16 * i) = u32x4_t{0u, 0u, 0u, 0u};
     if (tid < RW * 64) {
-      s_w[(t0 + 1) % 2].p[tid / 64][0][lane] = s_w[(t0 + 1) % 2].p[tid / 64][1][lane] = u32x2_t{0u, 0u};
-      if (lane < 32) s_w[(t0 + 1) % 2].m[tid / 64][lane / 16][l16] = kNone;
+      s_w[1].p[tid / 64][0][lane] = s_w[1].p[tid / 64][1][lane] = u32x2_t{0u, 0u};
+      if (lane < 32) s_w[1].m[tid / 64][lane / 16][l16] = kNone;
     }
-    // What every wave does in iteration `tile`, before its products and after: the tile's arrival, the loads of a later one.
-    const auto begin = [&](int tile) {
-      arrive(tile);
-      const int ahead = tile + (FP8 ? 3 : 2);
-      if (ahead < t1 && is_ctx(ahead)) window(ahead);
-      // 16-bit pages: waves 0-3 start the tile two ahead before their products, waves 4-7 after, so that of the two waves
-      // of a SIMD one has the matrix cores while the other is at its loads.
-      if (FP8 || !second_half) start(ahead);
-      if (FP8 && tile < t1) {
-        if (is_ctx(tile)) widen(tile);
-        else issue(tile);  // the round's rows are 16-bit: brought in here, there are few of them
-      }
-    };
-    const auto widened = [&](int tile) {
-      if (!is_ctx(tile)) wait_vm<0>();
-      __syncthreads();
-    };
     if (!computes) {  // no rows of this row group: a share of the loads alone
-      for (int tile = t0; tile <= t1; ++tile) {
-        begin(tile);
-        if (FP8 && tile < t1) widened(tile);
-        if (tile < t1 && !is_ctx(tile)) clean(tile);
-        if (!FP8 && second_half) start(tile + 2);
+      for (int i = 0; i <= tiles; ++i) {
+        arrive(i);
+        if (i == tiles) break;
+        lookup(i);
+        const Loads to = prepare_next(i + 2);
+        if (!is_ctx(i)) clean(i);
+        load_all(to);
+        if constexpr (FP8) next_rows(i + 1);
       }
       __syncthreads();
-      pos += t1 - t0;
+      pos += tiles;
       continue;
     }
     u32x4_t q[S::KC];
@@ -580,38 +608,43 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
 #pragma unroll
       for (int c = 0; c < S::KC; ++c) asm volatile("" : "+v"(q[c]));
     }
-    // Iteration `tile`: its scores and weights, and the output of the tile before it.
-    for (int tile = t0; tile <= t1; ++tile) {
-      begin(tile);
-      uint32_t bits = 0xffffffffu;
-      bool all = true;
-      f32x4_t s = {0.f, 0.f, 0.f, 0.f};
-      const auto score = [&] {
-        const uint32_t vis = __builtin_amdgcn_readfirstlane(s_vis[tile % 4]);
-        bits = vis;
-        all = is_ctx(tile) && vis == 0xffffffffu;
-        if (!is_ctx(tile)) {
-          const uint32_t poison = clean(tile);
+    // Iteration i: the scores of tile i, beside them the loads of the tile two ahead; the output of the tile before it, beside
+    // that the scores' weights.
+    for (int i = 0; i <= tiles; ++i) {
+      arrive(i);
+      const u32x4_t pb = take_weights<S>(s_w[(i + 1) % 2], row_wave, acc, macc, m, l, fresh(lane));
+      WeightStep<S> w;
+      w.s = f32x4_t{0.f, 0.f, 0.f, 0.f};
+      uint32_t bits = 0;
+      if (i < tiles) {
+        lookup(i);
+        const Loads to = prepare_next(i + 2);
+        bits = uniform(s_vis[i / kBatch % 2][i % kBatch]);
+        if (!is_ctx(i)) {
+          const uint32_t poison = clean(i);
           int rho, t, head;
           const uint64_t mask = my_row(rho, t, head) ? static_cast<uint64_t>(a.masks[b * a.stride_mask + t]) : 0;
-          bits = static_cast<uint32_t>(mask >> ((tile - u.ctx_tiles) * kKeys)) & vis;
+          bits &= static_cast<uint32_t>(mask >> ((t0 + i - u.ctx_tiles) * kKeys));
           if (bits & poison) l = __builtin_nanf("");
         }
-        s = score_step<S>(smem[tile % S::NBUF], q, kt, fresh(lane));
-      };
-      const u32x4_t pb = take_weights<S>(s_w[(tile + 1) % 2], row_wave, acc, macc, m, l, fresh(lane));
-      if (!FP8 && tile < t1) score();
-      value_step<S>(smem[(tile + S::NBUF - 1) % S::NBUF], pb, acc, dbase, fresh(lane));
-      if (FP8 && tile < t1) {
-        widened(tile);
-        score();
+        w.s = score_step<S>(smem[i % S::NBUF], q, kt, fresh(lane), [&](int c) {
+          if (c % 2 == 1 && c / 2 < kLoads) load_next(to, c / 2);
+        });
+        if (more) load_next(to, kLoads);
+        if constexpr (FP8) next_rows(i + 1);
       }
-      if (tile < t1)
-        weight_step<S>(s, s_w[tile % 2], row_wave, kt, column_wave < 2, m, l, scale_log2, s_rest[tile % 4], fresh(lane), all,
-                       bits);
-      if (!FP8 && second_half) start(tile + 2);
+      const int ln = fresh(lane);
+      const float* const rest = s_rest[FP8 ? i / kBatch % 2 : 0] + i % kBatch * kKeys;
+      value_step<S>(smem[(i + S::NBUF - 1) % S::NBUF], pb, acc, dbase, ln, [&](int dt) {
+        constexpr int kPhases = WeightStep<S>::kPhases;
+#pragma unroll
+        for (int ph = 0; ph < kPhases; ++ph)
+          if (ph * S::DT / kPhases == dt)
+            w.phase(ph, s_w[i % 2], row_wave, kt, column_wave < 2, m, l, scale_log2, rest, ln, bits);
+      });
     }
     // the sum over both halves of the keys: each wave's own is relative to the last maximum by now
+    const int ln = fresh(lane), g = ln >> 4, l16 = ln & 15;
     float sum = l + __shfl_xor(l, 16, 64);
     sum += __shfl_xor(sum, 32, 64);
     if (column_wave < 2 && g == 0) s_sum[row_wave][kt][l16] = sum;
@@ -635,7 +668,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
       for (int dt = 0; dt < S::DT; ++dt) *reinterpret_cast<f32x4_t*>(o + 16 * dt + 4 * g) = acc[dt] * inv;
       if (g == 0 && dbase == 0) a.workspace[p.lse_off + part] = sum == 0.f ? -INFINITY : macc + log2f(sum);
     }
-    pos += t1 - t0;
+    pos += tiles;
   }
 }
 
