@@ -250,7 +250,7 @@ template <typename S>
 E4_DEV u32x4_t take_weights(const Weights<S::RW>& from, int row_wave, f32x4_t (&acc)[S::DT], float& macc, float& m, float& l,
                             int lane) {
   using T = typename S::T;
-  const int l16 = lane & 15;
+  const int g = lane >> 4, l16 = lane & 15;
   // element i of P^T's operand is key 16 (i / 4) + 4 g + i % 4
   u32x2_t p0 = from.p[row_wave][0][lane], p1 = from.p[row_wave][1][lane];
   const float m0 = from.m[row_wave][0][l16], m1 = from.m[row_wave][1][l16];
@@ -321,7 +321,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
   __shared__ int s_at;
   __shared__ uint32_t s_before;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int g = lane >> 4, l16 = lane & 15;
+  const int l16 = lane & 15;
 
   // tiles before each request (one a thread)
   static_assert(kMaxReqs <= kThreads, "requests of a launch");
@@ -452,19 +452,23 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
       const char* src;
       uint32_t dst;
     };
+    const auto row_of = [&](int i) {  // of the lane's key of tile i
+      const int ln = fresh(lane), key = FP8 ? 16 * (wave % 2) + (ln >> 2) : 8 * octet + (ln >> 3);
+      return s_row[i / kBatch % 2][i % kBatch * kKeys + key];
+    };
     // 16-bit rows: block c of the wave's CB0 (waves 4-7: CB1) blocks
-    const auto prepare = [&](int i) {
+    const auto prepare = [&](int i, uint64_t at) {
       const int ln = fresh(lane), key = 8 * octet + (ln >> 3), chunk = (ln & 7) ^ swz(key);
-      const char* const row = reinterpret_cast<const char*>(s_row[i / kBatch % 2][i % kBatch * kKeys + key]);
+      const char* const row = reinterpret_cast<const char*>(at);
       return Loads{row + (16 * chunk + 128 * cb_first),
                    uniform(lds_addr(smem[i % S::NBUF]) + 1024 * octet + 4096 * cb_first)};
     };
     const auto load = [&](const Loads& to, int c) { dma16(to.src + 128 * c, to.dst + 4096 * c); };
     // fp8 codes: a block of 64 columns is 32 keys x 64 bytes, an instruction 16 keys of it; wave w brings in keys 16 (w % 2) ..
     // of blocks w / 2, w / 2 + 4, ..
-    const auto prepare8 = [&](int i) {
-      const int ln = fresh(lane), key = 16 * (wave % 2) + (ln >> 2);
-      const char* row = reinterpret_cast<const char*>(s_row[i / kBatch % 2][i % kBatch * kKeys + key]);
+    const auto prepare8 = [&](int i, uint64_t at) {
+      const int ln = fresh(lane);
+      const char* row = reinterpret_cast<const char*>(at);
       if (!is_ctx(i)) row = reinterpret_cast<const char*>(zero_row);
       return Loads{row + (16 * (ln & 3) + 64 * (wave / 2)),
                    uniform(lds_addr(s_raw[FP8 ? i % 2 : 0]) + 1024 * (wave % 2) + 2048 * (wave / 2))};
@@ -473,8 +477,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
     // the loads that every wave has, and the ones that some have beyond them
     constexpr int kLoads = FP8 ? S::CB / 4 : S::CB1;
     const bool more = FP8 ? wave / 2 + 4 * kLoads < S::CB : S::CB0 > S::CB1 && !second_half;
-    const auto prepare_next = [&](int i) {
-      if constexpr (FP8) return prepare8(i); else return prepare(i);
+    const auto prepare_next = [&](int i, uint64_t at) {
+      if constexpr (FP8) return prepare8(i, at); else return prepare(i, at);
     };
     const auto load_next = [&](const Loads& to, int c) {
       if constexpr (FP8) load8(to, c); else load(to, c);
@@ -509,7 +513,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
         for (int c = 0; c < S::CB1; ++c) widen(x, c);
         if (S::CB0 > S::CB1 && !second_half) widen(x, S::CB1);
       } else {
-        const Loads to = prepare(i);
+        const int key = 8 * octet + (fresh(lane) >> 3);
+        const Loads to = prepare(i, s_row[i / kBatch % 2][i % kBatch * kKeys + key]);
 #pragma unroll
         for (int c = 0; c < S::CB1; ++c) load(to, c);
         if (S::CB0 > S::CB1 && !second_half) load(to, S::CB1);
@@ -517,6 +522,22 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
     };
 
     __syncthreads();  // the last piece's tiles have been read
+    // The queries come in through the last two tiles' place, whole lines once for all waves: a lane's own loads would be 16
+    // bytes of every row, twice. 8 rows x 64 columns an instruction, in the layout of a tile.
+    char* const s_q = smem[S::NBUF - 2];
+    static_assert(S::KC / 2 * S::ROWS * 128 <= 2 * S::TILE, "the queries' place");
+    {
+      const int ln = fresh(lane), row = 8 * (wave % (2 * RW)) + (ln >> 3), rho = rg * S::ROWS + row;
+      const bool ok = rho < u.width * a.heads;
+      const int t = ok ? rho / a.heads : 0, head = ok ? rho - t * a.heads : 0;
+      const char* const src = ok ? reinterpret_cast<const char*>(static_cast<const uint16_t*>(a.q) + (u.start + t) * a.stride_qt +
+                                                                 head * a.stride_qh)
+                                 : reinterpret_cast<const char*>(zero_row);
+      const int chunk = 16 * ((ln & 7) ^ swz(row % kKeys));
+      const uint32_t dst = uniform(lds_addr(s_q) + 1024 * (wave % (2 * RW)));
+#pragma unroll 1
+      for (int cb = wave / (2 * RW); cb < S::KC / 2; cb += 4 / RW) dma16(src + 128 * cb + chunk, dst + cb * S::ROWS * 128);
+    }
     if (tid < 2 * kBatchKeys) {  // batches 0 and 1
       const int n = tid / kBatchKeys, i = tid % kBatchKeys;
       int32_t blk = -1;
@@ -525,9 +546,10 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
       if (FP8 && blk >= 0 && blk < a.num_blocks) scale = a.scale_page[blk * a.stride_sp];
       fill(n, i, blk, scale);
     }
+    wait_vm<0>();
     __syncthreads();
 #pragma unroll 1
-    for (int i = 0; i < 2; ++i) load_all(prepare_next(i));
+    for (int i = 0; i < 2; ++i) load_all(prepare_next(i, row_of(i)));
     if constexpr (FP8) {
       wait_vm<0>();
       __syncthreads();
@@ -571,6 +593,19 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
       }
       return poison;
     };
+    u32x4_t q[S::KC];
+    {
+      const int ln = fresh(lane), row = 16 * row_wave + (ln & 15);
+      const char* const from = s_q + row * 128;
+#pragma unroll
+      for (int c = 0; c < S::KC; ++c)  // the columns of the lane's chunk of the scores' operand
+        q[c] = *reinterpret_cast<const u32x4_t*>(from + c / 2 * (S::ROWS * 128) +
+                                                 16 * ((2 * (ln >> 4) + (c & 1)) ^ swz(row % kKeys)));
+      // Settled here, once: a wait for them inside the loop would wait for the tiles on their way too.
+#pragma unroll
+      for (int c = 0; c < S::KC; ++c) asm volatile("" : "+v"(q[c]));
+    }
+    __syncthreads();
     // The first iteration's output: no weights over a tile of zeros.
     for (int i = tid; i < S::TILE / 16; i += kThreads)
       *reinterpret_cast<u32x4_t*>(smem[S::NBUF - 1] + 16 * i) = u32x4_t{0u, 0u, 0u, 0u};
@@ -583,7 +618,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
         arrive(i);
         if (i == tiles) break;
         lookup(i);
-        const Loads to = prepare_next(i + 2);
+        const Loads to = prepare_next(i + 2, row_of(i + 2));
         if (!is_ctx(i)) clean(i);
         load_all(to);
         if constexpr (FP8) next_rows(i + 1);
@@ -592,22 +627,10 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
       pos += tiles;
       continue;
     }
-    u32x4_t q[S::KC];
     f32x4_t acc[S::DT];
     float m = kNone, macc = kNone, l = 0.f;
 #pragma unroll
     for (int dt = 0; dt < S::DT; ++dt) acc[dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    {
-      int rho, t, head;
-      const bool ok = my_row(rho, t, head);
-      const uint16_t* const qrow = static_cast<const uint16_t*>(a.q) + (u.start + t) * a.stride_qt + head * a.stride_qh;
-#pragma unroll
-      for (int c = 0; c < S::KC; ++c)  // the columns of the lane's chunk of the scores' operand
-        q[c] = ok ? *reinterpret_cast<const u32x4_t*>(qrow + 64 * (c / 2) + 8 * (2 * g + (c & 1))) : u32x4_t{0u, 0u, 0u, 0u};
-      // Settled here, once: a wait for them inside the loop would wait for the tiles on their way too.
-#pragma unroll
-      for (int c = 0; c < S::KC; ++c) asm volatile("" : "+v"(q[c]));
-    }
     // Iteration i: the scores of tile i, beside them the loads of the tile two ahead; the output of the tile before it, beside
     // that the scores' weights.
     for (int i = 0; i <= tiles; ++i) {
@@ -617,9 +640,10 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
       w.s = f32x4_t{0.f, 0.f, 0.f, 0.f};
       uint32_t bits = 0;
       if (i < tiles) {
+        const uint64_t next_row = row_of(i + 2);
+        bits = s_vis[i / kBatch % 2][i % kBatch];
         lookup(i);
-        const Loads to = prepare_next(i + 2);
-        bits = uniform(s_vis[i / kBatch % 2][i % kBatch]);
+        const Loads to = prepare_next(i + 2, next_row);
         if (!is_ctx(i)) {
           const uint32_t poison = clean(i);
           int rho, t, head;
