@@ -14,8 +14,15 @@
 // an element at the rate of 32-bit ones, against about 10 with the hardware's 32-bit exp2, whose error would flip one
 // comparison in 10^7, and of a flat row's running sums far more).
 //
-// Only rows on the walk are read. One workgroup per request; a wave sums one contiguous region of the row, so that the
-// regions' sums, which the walk needs for Z anyway, also lead the final token's search to one region.
+// Split: a wave takes 4096 elements of a row, a chunk. Three kinds of launches:
+//   - statistics: of every chunk of every row its maximum and its mass relative to that. All rows of all trees at once: the
+//     walk visits a few of them, but one after another, and a workgroup that reads rows on its own reads them at a
+//     hundredth of the memory's rate. PLACEHOLDER
+//   - the walk, a workgroup per request: the rows' sums out of the chunks', then the decisions, a lane a child. Ends with the
+//     final token: the chunks' running sum leads to one chunk, which is read. With draft probabilities a rejection needs the
+//     residual's mass: the walk stops there and leaves its state,
+//   - the residual's launch sums max(p - s q, 0) over the chunks of the stopped walks, and the walk is launched again.
+// After kPairs such pairs a walk reads the rows of its further rejections itself.
 
 #include "common.h"
 
@@ -136,28 +143,208 @@ E4_DEV double wave_sum(double x) {
   return x;
 }
 
-// (value, index) with the first index on ties; NaN is the largest value.
-E4_DEV bool better(float v, int i, float bv, int bi) {
-  const bool vn = v != v, bn = bv != bv;
-  if (vn || bn) return vn && (!bn || i < bi);
-  return v > bv || (v == bv && i < bi);
+constexpr int kMaxRows = 64;  // of a tree: a lane each
+constexpr int kPairs = 3;     // residual and walk launches behind the first walk
+constexpr int kChunk = 4096;  // elements
+constexpr int kThreads = 256, kWaves = kThreads / 64;
+
+// A stopped walk. `count` rows are on its path, the last one `node`, whose child `child` was rejected last.
+struct State {
+  int32_t stopped, node, child, count;
+  double spent;
+};
+
+struct Split {
+  int chunks;  // of a row
+  int64_t maxes_off, masses_off, state_off;  // in the workspace, bytes; the chunks' sums come first
+};
+
+struct Work {  // a row's parts of the workspace
+  const double* sums;
+  const float* maxes;
+  E4_DEV Work(const eagle4_sample_tree_args& a, const Split& s, int64_t row) {
+    sums = reinterpret_cast<const double*>(a.workspace) + row * s.chunks;
+    maxes = reinterpret_cast<const float*>(static_cast<const char*>(a.workspace) + s.maxes_off) + row * s.chunks;
+  }
+};
+
+// The request of a logits row: how many of them end at it or before. 64 probes at a time.
+E4_DEV int request_of(const eagle4_sample_tree_args& a, int64_t row, int lane) {
+  int lo = 0, n = a.num_reqs;  // it is lo .. lo + n, the last one: none
+  while (n > 0) {
+    const int step = (n + 63) / 64, at = lo + lane * step + step - 1;  // ends at row or before: lo is behind it
+    const bool past = at < lo + n && e4::ld(a.cu_num_logits, at + 1) <= row;
+    const int whole = __popcll(__ballot(past));
+    lo += whole * step;
+    n = n - whole * step < step - 1 ? n - whole * step : step - 1;
+  }
+  return lo;
 }
 
-constexpr int kMaxRows = 64;
+E4_DEV float wave_max(float x) {  // NaN the largest
+#pragma unroll
+  for (int k = 1; k < 64; k <<= 1) x = __builtin_elementwise_maximum(x, __shfl_xor(x, k, 64));
+  return x;
+}
 
-template <typename T, typename Q, int NT>
-__global__ __launch_bounds__(NT) void sample_tree_kernel(const eagle4_sample_tree_args a) {
-  constexpr int NW = NT / 64, VEC = Row<T>::VEC;
+E4_DEV int wave_min(int x) {
+#pragma unroll
+  for (int k = 1; k < 64; k <<= 1) {
+    const int o = __shfl_xor(x, k, 64);
+    x = o < x ? o : x;
+  }
+  return x;
+}
+
+E4_DEV double scale_of(float temperature) { return 1.4426950408889634 / static_cast<double>(temperature); }
+
+// Maximum and mass of a chunk, a wave each. Where all mass is on one element (T = 0, a maximum of +inf or NaN) the place of
+// the sum holds the first index of the maximum.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void sample_chunks(const eagle4_sample_tree_args a, const Split s) {
+  constexpr int VEC = Row<T>::VEC, NV = kChunk / VEC / 64;
+  const int lane = threadIdx.x & 63;
+  const uint32_t id = blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t n = id / static_cast<uint32_t>(s.chunks);
+  const int chunk = id % static_cast<uint32_t>(s.chunks);
+  if (n >= a.rows) return;
+  const Row<T> row(a.logits, n, a.stride_row, a.vocab);
+  const int v0 = chunk * (64 * NV) + lane;
+  float x[NV][VEC];
+  if (row.first(chunk * (64 * NV)) >= 0 && row.first((chunk + 1) * (64 * NV)) <= row.vocab) {  // wholly inside
+    u32x4 w[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) w[i] = row.raw(v0 + 64 * i);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) Row<T>::widen(w[i], x[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) row.load(v0 + 64 * i, x[i]);
+  }
+  const int b = __builtin_amdgcn_readfirstlane(request_of(a, n, lane));
+  if (b >= a.num_reqs || n - e4::ld(a.cu_num_logits, b) >= a.width) return;  // a row that no walk visits
+  const float temperature = a.temperature[b];
+
+  float m = x[0][0];
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) m = __builtin_elementwise_maximum(m, x[i][k]);
+  m = wave_max(m);
+  double sum = 0.0;
+  if (!(temperature > 0.f) || !(m < INFINITY)) {
+    int at = INT32_MAX;
+#pragma unroll
+    for (int i = NV - 1; i >= 0; --i)
+#pragma unroll
+      for (int k = VEC - 1; k >= 0; --k) {
+        const int e = row.first(v0 + 64 * i) + k;
+        if (e >= 0 && e < row.vocab && (m != m ? x[i][k] != x[i][k] : x[i][k] == m)) at = e;
+      }
+    sum = wave_min(at);
+  } else {
+    const double c = scale_of(temperature), off = -static_cast<double>(m) * c;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      double part = 0.0;
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) part += exp2_64(__builtin_fma(static_cast<double>(x[i][k]), c, off));
+      sum += part;
+    }
+    sum = wave_sum(sum);
+  }
+  if (lane == 0) {
+    const Work out(a, s, n);
+    const_cast<double*>(out.sums)[chunk] = sum;
+    const_cast<float*>(out.maxes)[chunk] = m;
+  }
+}
+
+// The residual of a vector's elements, times the row's total: off = -maximum c.
+template <typename T, typename Q>
+E4_DEV void residual(const Row<T>& row, const QRow<Q, Row<T>::VEC>& qrow, int v, double c, double off, double spent,
+                     double (&r)[Row<T>::VEC]) {
+  constexpr int VEC = Row<T>::VEC;
+  float x[VEC];
+  row.load(v, x);
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) r[i] = exp2_64(__builtin_fma(static_cast<double>(x[i]), c, off));
+  if constexpr (Q::code >= 0) {
+    if (spent > 0.0) {
+      float q[VEC];
+      qrow.load(row.first(v), row.vocab, q);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) r[i] = __builtin_fmax(r[i] - spent * static_cast<double>(q[i]), 0.0);
+    }
+  }
+}
+
+// A chunk's mass of it, by one wave.
+template <typename T, typename Q>
+E4_DEV double chunk_mass(const Row<T>& row, const QRow<Q, Row<T>::VEC>& qrow, int chunk, double c, double off, double spent,
+                         int lane) {
+  constexpr int VEC = Row<T>::VEC, NV = kChunk / VEC / 64;
+  double sum = 0.0;
+#pragma unroll 2
+  for (int i = 0; i < NV; ++i) {
+    const int v = (chunk * NV + i) * 64 + lane;
+    if (v >= row.vectors) continue;
+    double r[VEC];
+    residual<T, Q>(row, qrow, v, c, off, spent, r);
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) sum += r[k];
+  }
+  return wave_sum(sum);
+}
+
+E4_DEV float row_max(const float* maxes, int chunks, int lane) {
+  float top = -INFINITY;
+  for (int k = lane; k < chunks; k += 64) top = __builtin_elementwise_maximum(top, maxes[k]);
+  return wave_max(top);
+}
+
+template <typename T, typename Q>
+__global__ __launch_bounds__(kThreads) void sample_residual(const eagle4_sample_tree_args a, const Split s) {
+  const int lane = threadIdx.x & 63, b = blockIdx.y, chunk = blockIdx.x * kWaves + (threadIdx.x >> 6);
+  char* const work = static_cast<char*>(a.workspace);
+  const State st = reinterpret_cast<const State*>(work + s.state_off)[b];
+  if (st.stopped == 0 || chunk >= s.chunks) return;
+  const int64_t n = e4::ld(a.cu_num_logits, b) + st.node;
+  const Row<T> row(a.logits, n, a.stride_row, a.vocab);
+  const QRow<Q, Row<T>::VEC> qrow(a.probs, n, a.stride_prob, row.past);
+  const double c = scale_of(a.temperature[b]);
+  const double off = -static_cast<double>(row_max(Work(a, s, n).maxes, s.chunks, lane)) * c;
+  const double mass = chunk_mass<T, Q>(row, qrow, chunk, c, off, st.spent, lane);
+  if (lane == 0) reinterpret_cast<double*>(work + s.masses_off)[static_cast<int64_t>(b) * s.chunks + chunk] = mass;
+}
+
+// The walk. Every wave takes the decisions, lane j for row j of the tree; the waves part for the rows' sums and for the
+// final token's chunk.
+template <typename T, typename Q>
+__global__ __launch_bounds__(kThreads) void sample_walk(const eagle4_sample_tree_args a, const Split s, int first, int last) {
+  constexpr int VEC = Row<T>::VEC, NV = kChunk / VEC / kThreads;  // vectors of a thread in the final token's chunk
   constexpr bool kProbs = Q::code >= 0;
-  __shared__ int s_parent[kMaxRows];
-  __shared__ int64_t s_draft[kMaxRows];
-  __shared__ float s_coin[kMaxRows];
-  __shared__ int s_rejected[kMaxRows];  // tokens taken out of the residual (no draft probabilities)
-  __shared__ float s_max[NW];
-  __shared__ int s_arg[NW];
-  __shared__ double s_p[NW], s_r[NW], s_scan[NW];  // a region's mass of p, of the residual; scan totals
+  static_assert(NV >= 1, "a chunk");
+  __shared__ float s_top[kMaxRows];
+  __shared__ double s_total[kMaxRows];
+  __shared__ int s_lost_chunk[kMaxRows];
+  __shared__ double s_lost_mass[kMaxRows];
+  __shared__ double s_scan[kWaves];
   __shared__ int s_token, s_last;
-  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  char* const work = static_cast<char*>(a.workspace);
+  State* const state = reinterpret_cast<State*>(work + s.state_off) + b;
+  double* const masses = reinterpret_cast<double*>(work + s.masses_off) + static_cast<int64_t>(b) * s.chunks;
+  int node = 0, count = 0, resumed = 0;
+  double spent = 0.0;
+  if (!first) {
+    const State st = *state;
+    if (st.stopped == 0) return;
+    node = st.node;
+    count = st.count;
+    resumed = st.child;
+    spent = st.spent;
+  }
 
   const int64_t slot = e4::ld(a.idx_mapping, b);
   const int64_t start = e4::ld(a.cu_num_logits, b);
@@ -166,310 +353,321 @@ __global__ __launch_bounds__(NT) void sample_tree_kernel(const eagle4_sample_tre
   const int limit = !valid ? 0 : static_cast<int>(rows < a.width ? rows : a.width);
   const float temperature = a.temperature[b];
   const bool greedy = !(temperature > 0.f);
-  const double c = 1.4426950408889634 / static_cast<double>(temperature);
-  if (tid < limit) {
-    s_parent[tid] = static_cast<int>(e4::ld(a.parents, slot, tid));
-    s_draft[tid] = e4::ld(a.drafted, start + tid);
-    s_coin[tid] = a.coins[start + tid];
+  const double c = scale_of(temperature);
+
+  // lane j: row j's parent, token, coin, and of its parent's row the token's logit and draft probability
+  int parent = -1;
+  int64_t token = -1;
+  float coin = 0.f, logit = 0.f, drawn = 1.f;
+  if (lane < limit) {
+    parent = static_cast<int>(e4::ld(a.parents, slot, lane));
+    token = e4::ld(a.drafted, start + lane);
+    coin = a.coins[start + lane];
+  }
+  const bool child = lane > 0 && lane < limit && parent >= 0 && parent < limit && token >= 0 && token < a.vocab;
+  if (child) {
+    logit = T::to_f32(static_cast<const typename T::storage*>(a.logits)[(start + parent) * a.stride_row + token]);
+    if constexpr (kProbs)
+      drawn = Q::to_f32(static_cast<const typename Q::storage*>(a.probs)[(start + parent) * a.stride_prob + token]);
+  }
+
+  // The rows' maxima and totals out of the chunks', 16 lanes a row; a row with all mass on one element: its index.
+  for (int r = tid / 16; r < limit; r += kThreads / 16) {
+    const Work w(a, s, start + r);
+    const int l16 = lane & 15;
+    float top = -INFINITY;
+    for (int k = l16; k < s.chunks; k += 16) top = __builtin_elementwise_maximum(top, w.maxes[k]);
+#pragma unroll
+    for (int k = 1; k < 16; k <<= 1) top = __builtin_elementwise_maximum(top, __shfl_xor(top, k, 64));
+    double total = 0.0;
+    if (greedy || !(__builtin_fabsf(top) < INFINITY)) {
+      int at = INT32_MAX;  // its first chunk's; a row of -inf: 0
+      for (int k = l16; k < s.chunks; k += 16)
+        if (at == INT32_MAX && (top != top ? w.maxes[k] != w.maxes[k] : w.maxes[k] == top)) at = k;
+#pragma unroll
+      for (int k = 1; k < 16; k <<= 1) {
+        const int o = __shfl_xor(at, k, 64);
+        at = o < at ? o : at;
+      }
+      total = top == -INFINITY ? 0.0 : w.sums[at];
+    } else {
+      for (int k = l16; k < s.chunks; k += 16)
+        total += w.sums[k] * exp2_64((static_cast<double>(w.maxes[k]) - static_cast<double>(top)) * c);
+#pragma unroll
+      for (int k = 1; k < 16; k <<= 1) total += __shfl_xor(total, k, 64);
+    }
+    if (l16 == 0) {
+      s_top[r] = top;
+      s_total[r] = total;
+    }
   }
   __syncthreads();
+  // exp2((l - top) c), the parent's p of the token times the parent's total
+  const double p = exp2_64(__builtin_fma(static_cast<double>(logit), c,
+                                         child ? -static_cast<double>(s_top[parent]) * c : 0.0));
 
-  int node = 0, count = 0;
-  for (int step = 0; step < limit; ++step) {
+  const auto lane_f64 = [](double x, int j) {
+    const uint64_t bits = __builtin_bit_cast(uint64_t, x);
+    const uint32_t lo = __builtin_amdgcn_readlane(static_cast<uint32_t>(bits), j);
+    const uint32_t hi = __builtin_amdgcn_readlane(static_cast<uint32_t>(bits >> 32), j);
+    return __builtin_bit_cast(double, (static_cast<uint64_t>(hi) << 32) | lo);
+  };
+  const auto out_token = [&](int64_t x) {
+    if (tid == 0) a.sampled[b * a.stride_sampled + count - 1] = x;
+  };
+  const auto sum_of_masses = [&] {
+    double sum = 0.0;
+    for (int k = lane; k < s.chunks; k += 64) sum += masses[k];
+    return wave_sum(sum);
+  };
+
+  while (count < limit || resumed > 0) {
     const Row<T> row(a.logits, start + node, a.stride_row, a.vocab);
     const QRow<Q, VEC> qrow(a.probs, start + node, a.stride_prob, row.past);
-    const int per = (row.vectors + NW - 1) / NW;
-    const auto region = [&](int w, int& lo, int& hi) {
-      lo = w * per < row.vectors ? w * per : row.vectors;
-      hi = lo + per < row.vectors ? lo + per : row.vectors;
-    };
-
-    // the row's maximum and every region's mass, relative to it
-    float top = -INFINITY;
-    bool single = greedy;  // all mass on the argmax
-    if (!greedy) {
-      float m = -INFINITY;
-      double sum = 0.0;
-      const auto take = [&](const float (&x)[VEC]) {
-        float vm = x[0];
-#pragma unroll
-        for (int i = 1; i < VEC; ++i) vm = __builtin_elementwise_maximum(vm, x[i]);
-        if (!(vm <= m)) {
-          sum *= exp2_64((static_cast<double>(m) - static_cast<double>(vm)) * c);
-          m = vm;
-        }
-        const double off = -static_cast<double>(m) * c;
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) sum += exp2_64(__builtin_fma(static_cast<double>(x[i]), c, off));
-      };
-      int lo, hi;
-      region(wave, lo, hi);
-      for (int v = lo + lane; v < hi; v += 64) {
-        float x[VEC];
-        row.load(v, x);
-        take(x);
-      }
-      float wm = m;
-#pragma unroll
-      for (int k = 1; k < 64; k <<= 1) wm = __builtin_elementwise_maximum(wm, __shfl_xor(wm, k, 64));
-      sum = wave_sum(sum * exp2_64((static_cast<double>(m) - static_cast<double>(wm)) * c));
-      if (lane == 0) {
-        s_max[wave] = wm;
-        s_p[wave] = sum;
-      }
-      __syncthreads();
-      top = s_max[0];
-#pragma unroll
-      for (int w = 1; w < NW; ++w) top = __builtin_elementwise_maximum(top, s_max[w]);
-      single = !(__builtin_fabsf(top) < INFINITY);
-      if (!single && tid < NW)
-        s_p[tid] *= exp2_64((static_cast<double>(s_max[tid]) - static_cast<double>(top)) * c);
-      __syncthreads();
+    const Work w(a, s, start + node);
+    const float top = s_top[node];
+    const double total = s_total[node], off = -static_cast<double>(top) * c;
+    const bool single = greedy || !(__builtin_fabsf(top) < INFINITY);
+    double mass = total;   // Z, and above s, times the total
+    uint64_t rejected = 0; // tokens taken out of the residual (no draft probabilities)
+    uint64_t kids = __ballot(child && parent == node);
+    if (resumed > 0) {
+      kids &= resumed < 63 ? ~0ull << (resumed + 1) : 0ull;
+      mass = sum_of_masses();
+      resumed = 0;
+    } else {
+      if (tid == 0) a.path[slot * a.stride_path + count] = node;
+      ++count;
+      spent = 0.0;
     }
-    int arg = 0;
-    if (single) {
-      float bv = -INFINITY;
-      int bi = INT32_MAX;
-      for (int v = tid; v < row.vectors; v += NT) {
-        float x[VEC];
-        row.load(v, x);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          const int e = row.first(v) + i;
-          if (e >= 0 && e < row.vocab && better(x[i], e, bv, bi)) {
-            bv = x[i];
-            bi = e;
-          }
-        }
-      }
-#pragma unroll
-      for (int k = 1; k < 64; k <<= 1) {
-        const float ov = __shfl_xor(bv, k, 64);
-        const int oi = __shfl_xor(bi, k, 64);
-        if (better(ov, oi, bv, bi)) {
-          bv = ov;
-          bi = oi;
-        }
-      }
-      if (lane == 0) {
-        s_max[wave] = bv;
-        s_arg[wave] = bi;
-      }
-      __syncthreads();
-      bv = s_max[0];
-      arg = s_arg[0];
-      for (int w = 1; w < NW; ++w)
-        if (better(s_max[w], s_arg[w], bv, arg)) {
-          bv = s_max[w];
-          arg = s_arg[w];
-        }
-      __syncthreads();
-    }
-
-    // exp2((l - top) c), the row's p times `total`
-    const double off = -static_cast<double>(top) * c;
-    const auto weight = [&](float l) { return exp2_64(__builtin_fma(static_cast<double>(l), c, off)); };
-    double total = 0.0;
-    if (!single) {
-#pragma unroll
-      for (int w = 0; w < NW; ++w) total += s_p[w];
-    }
-    double spent = 0.0, mass = total;  // s and Z, times `total`
-    int rejected = 0;
-    // the residual of a vector's elements, times `total`
-    const auto residual = [&](int v, double (&r)[VEC]) {
-      float x[VEC];
-      row.load(v, x);
-      if constexpr (kProbs) {
-        float q[VEC];
-        if (spent > 0.0) qrow.load(row.first(v), row.vocab, q);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          r[i] = weight(x[i]);
-          if (spent > 0.0) r[i] = __builtin_fmax(r[i] - spent * static_cast<double>(q[i]), 0.0);
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) r[i] = weight(x[i]);
-        for (int k = 0; k < rejected; ++k) {
-          const int at = s_rejected[k] - row.first(v);
-#pragma unroll
-          for (int i = 0; i < VEC; ++i)
-            if (i == at) r[i] = 0.0;
-        }
-      }
-    };
-    const auto region_mass = [&](int w) {
-      int lo, hi;
-      region(w, lo, hi);
-      double sum = 0.0;
-      for (int v = lo + lane; v < hi; v += 64) {
-        double r[VEC];
-        residual(v, r);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) sum += r[i];
-      }
-      return wave_sum(sum);
-    };
 
     // the children, in row order
     int next = -1;
-    for (int child = 1; child < limit && next < 0; ++child) {
-      if (s_parent[child] != node) continue;
-      const int64_t token = s_draft[child];
-      if (token < 0 || token >= row.vocab) continue;
-      if (single) {
-        if (token == arg) next = child;
-        continue;
-      }
-      double r = weight(T::to_f32(row.p[token])), drawn = 1.0;
+    if (single) {
+      const uint64_t fits = kids & __ballot(token == static_cast<int64_t>(total));
+      if (fits != 0 && count < limit) next = __builtin_ctzll(fits);
+      kids = 0;
+    }
+    while (kids != 0 && count < limit) {
+      const int j = __builtin_ctzll(kids);
+      kids &= kids - 1;
+      double r = lane_f64(p, j), q = 1.0;
       if constexpr (kProbs) {
-        drawn = static_cast<double>(Q::to_f32(qrow.p[token]));
-        if (spent > 0.0) r = __builtin_fmax(r - spent * drawn, 0.0);
+        q = static_cast<double>(__builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, drawn), j)));
+        if (spent > 0.0) r = __builtin_fmax(r - spent * q, 0.0);
       } else {
-        for (int k = 0; k < rejected; ++k)
-          if (s_rejected[k] == token) r = 0.0;
+        const int x = __builtin_amdgcn_readlane(static_cast<int>(token), j);
+        if ((__ballot(static_cast<int>(token) == x) & rejected) != 0) r = 0.0;
       }
-      if (static_cast<double>(s_coin[child]) * drawn * mass < r) {
-        next = child;
-      } else if constexpr (kProbs) {
+      const float u = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, coin), j));
+      if (static_cast<double>(u) * q * mass < r) {
+        next = j;
+        break;
+      }
+      if constexpr (kProbs) {
         spent += mass;
-        const double mine = region_mass(wave);
-        __syncthreads();  // the last residual's masses have been read
-        if (lane == 0) s_r[wave] = mine;
+        if (!last) {
+          if (tid == 0) *state = State{1, node, j, count, spent};
+          return;
+        }
+        __syncthreads();  // the last masses have been read
+        for (int k = wave; k < s.chunks; k += kWaves) {
+          const double m = chunk_mass<T, Q>(row, qrow, k, c, off, spent, lane);
+          if (lane == 0) masses[k] = m;
+        }
         __syncthreads();
-        mass = 0.0;
-#pragma unroll
-        for (int w = 0; w < NW; ++w) mass += s_r[w];
+        mass = sum_of_masses();
       } else if (r > 0.0) {
-        if (tid == 0) s_rejected[rejected] = static_cast<int>(token);
-        ++rejected;
+        rejected |= 1ull << j;
         mass = __builtin_fmax(mass - r, 0.0);
-        __syncthreads();
       }
     }
-    if (tid == 0) a.path[slot * a.stride_path + step] = node;
-    ++count;
     if (next >= 0) {
-      if (tid == 0) a.sampled[b * a.stride_sampled + step] = s_draft[next];
+      out_token(__shfl(token, next, 64));
       node = next;
-      __syncthreads();  // s_max, s_p, s_rejected have been read
       continue;
     }
 
     // no child accepted: the token of the final coin
-    int64_t token = arg;
+    int64_t found = static_cast<int64_t>(total);
     if (!single) {
-      if constexpr (!kProbs) {
-        if (rejected > 0) {  // the regions that lost a token, summed again; the others' masses are p's
-          int lo, hi;
-          region(wave, lo, hi);
-          bool lost = false;
-          for (int k = 0; k < rejected; ++k) {
-            const int v = (s_rejected[k] + row.past) / VEC;
-            lost |= v >= lo && v < hi;
-          }
-          const double mine = lost ? region_mass(wave) : s_p[wave];
-          if (lane == 0) s_r[wave] = mine;
-          __syncthreads();
-          mass = 0.0;
+      int lost = 0;
+      if constexpr (!kProbs) {  // the chunks that lost a token, summed again
+        uint64_t left = rejected;
+        const int my_chunk = static_cast<int>((token + row.past) / kChunk);
+        while (left != 0) {
+          const int k = __builtin_amdgcn_readlane(my_chunk, __builtin_ctzll(left));
+          left &= ~__ballot(my_chunk == k);
+          if (lost % kWaves == wave) {
+            double sum = 0.0;
+            for (int v = k * (kChunk / VEC) + lane; v < (k + 1) * (kChunk / VEC) && v < row.vectors; v += 64) {
+              double r[VEC];
+              residual<T, Q>(row, qrow, v, c, off, 0.0, r);
+              for (uint64_t x = rejected; x != 0; x &= x - 1) {
+                const int at = __builtin_amdgcn_readlane(static_cast<int>(token), __builtin_ctzll(x)) - row.first(v);
 #pragma unroll
-          for (int w = 0; w < NW; ++w) mass += s_r[w];
+                for (int i = 0; i < VEC; ++i)
+                  if (i == at) r[i] = 0.0;
+              }
+#pragma unroll
+              for (int i = 0; i < VEC; ++i) sum += r[i];
+            }
+            sum = wave_sum(sum);
+            if (lane == 0) {
+              s_lost_chunk[lost] = k;
+              s_lost_mass[lost] = sum;
+            }
+          }
+          ++lost;
         }
+        if (lost > 0) __syncthreads();
       }
-      bool whole = spent == 0.0 && rejected == 0;
-      if (!whole && !(mass > 0.0)) {
-        whole = true;
+      const auto mass_of = [&](int k) {
+        if (spent > 0.0) return masses[k];
+        double m = w.sums[k] * exp2_64((static_cast<double>(w.maxes[k]) - static_cast<double>(top)) * c);
+        for (int i = 0; i < lost; ++i)
+          if (s_lost_chunk[i] == k) m = s_lost_mass[i];
+        return m;
+      };
+      if (lost > 0) {
+        mass = 0.0;
+        for (int k = lane; k < s.chunks; k += 64) mass += mass_of(k);
+        mass = wave_sum(mass);
+      }
+      if (!(mass > 0.0)) {  // p again
         spent = 0.0;
         rejected = 0;
+        lost = 0;
         mass = total;
       }
-      const double* const masses = whole ? s_p : s_r;
       const double target = static_cast<double>(a.final_coins[b]) * mass;
-      double base = 0.0, before = 0.0;
-      int at = -1, last = 0;
-      bool sought = true;
-      for (int w = 0; w < NW; ++w) {
-        const double after = before + masses[w];
-        if (masses[w] > 0.0) last = w;
-        if (at < 0 && after > target) {
-          at = w;
-          base = before;
-        }
-        before = after;
-      }
-      if (at < 0) {  // a coin that no running sum passes: the last token that has mass
-        at = last;
-        sought = false;
-      }
-      if (tid == 0) {
-        s_token = INT32_MAX;
-        s_last = -1;
-      }
-      __syncthreads();
-      int lo, hi;
-      region(at, lo, hi);
-      for (int v0 = lo; v0 < hi; v0 += NT) {
-        const int v = v0 + tid;
-        double r[VEC];
-        double mine = 0.0;
-        int end = -1;  // the last element that has mass
-        if (v < hi) {
-          residual(v, r);
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) {
-            mine += r[i];
-            if (r[i] > 0.0) end = row.first(v) + i;
-          }
-        }
-        double run = mine;
+      double base = 0.0;
+      int at = -1, full = 0;  // the chunk in which the running sum passes the target, the last one that has mass
+      for (int k0 = 0; k0 < s.chunks && at < 0; k0 += 64) {
+        const double m = k0 + lane < s.chunks ? mass_of(k0 + lane) : 0.0;
+        double run = m;
 #pragma unroll
         for (int k = 1; k < 64; k <<= 1) {
           const double o = __shfl_up(run, k, 64);
           if (lane >= k) run += o;
         }
-        if (lane == 63) s_scan[wave] = run;
-        __syncthreads();
-        double from = base;
-        for (int w = 0; w < wave; ++w) from += s_scan[w];
-        const double left = __shfl_up(run, 1, 64);
-        const double begin = lane == 0 ? from : from + left, stop = from + run;
-        if (sought && begin <= target && stop > target) {
-          double acc = begin;
-          int found = end;
-          bool open = true;
+        const uint64_t passed = __ballot(base + run > target), any = __ballot(m > 0.0);
+        if (any != 0) full = k0 + 63 - __builtin_clzll(any);
+        if (passed != 0) {
+          const int f = __builtin_ctzll(passed);
+          at = k0 + f;
+          base += lane_f64(run, f) - lane_f64(m, f);
+        } else {
+          base += lane_f64(run, 63);
+        }
+      }
+      const bool sought = at >= 0;  // else: a coin that no running sum passes; the last token that has mass
+      if (!sought) at = full;
+      if (tid == 0) {
+        s_token = INT32_MAX;
+        s_last = -1;
+      }
+      double r[NV][VEC];
+      double mine = 0.0;
+      int end = -1;  // the thread's last element that has mass
+      const int v0 = (at * kThreads + tid) * NV;
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) {
-            acc += r[i];
-            if (open && acc > target && r[i] > 0.0) {
-              found = row.first(v) + i;
+      for (int i = 0; i < NV; ++i) {
+        if (v0 + i < row.vectors) {
+          residual<T, Q>(row, qrow, v0 + i, c, off, spent, r[i]);
+        } else {
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) r[i][k] = 0.0;
+        }
+        if constexpr (!kProbs)
+          for (uint64_t x = rejected; x != 0; x &= x - 1) {
+            const int gone = __builtin_amdgcn_readlane(static_cast<int>(token), __builtin_ctzll(x)) - row.first(v0 + i);
+#pragma unroll
+            for (int k = 0; k < VEC; ++k)
+              if (k == gone) r[i][k] = 0.0;
+          }
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) {
+          mine += r[i][k];
+          if (r[i][k] > 0.0) end = row.first(v0 + i) + k;
+        }
+      }
+      double run = mine;
+#pragma unroll
+      for (int k = 1; k < 64; k <<= 1) {
+        const double o = __shfl_up(run, k, 64);
+        if (lane >= k) run += o;
+      }
+      if (lane == 63) s_scan[wave] = run;
+      __syncthreads();
+      double from = base;
+      for (int k = 0; k < wave; ++k) from += s_scan[k];
+      const double left = __shfl_up(run, 1, 64);
+      const double begin = lane == 0 ? from : from + left, stop = from + run;
+      if (sought && begin <= target && stop > target) {
+        double acc = begin;
+        int hit = end;
+        bool open = true;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) {
+            acc += r[i][k];
+            if (open && acc > target && r[i][k] > 0.0) {
+              hit = row.first(v0 + i) + k;
               open = false;
             }
           }
-          atomicMin(&s_token, found);
-        }
-        if (end >= 0) atomicMax(&s_last, end);
-        for (int w = 0; w < NW; ++w) base += s_scan[w];
-        __syncthreads();
-        if (s_token != INT32_MAX) break;
+        atomicMin(&s_token, hit);
       }
-      token = s_token != INT32_MAX ? s_token : (s_last >= 0 ? s_last : 0);
+      if (end >= 0) atomicMax(&s_last, end);
+      __syncthreads();
+      found = s_token != INT32_MAX ? s_token : (s_last >= 0 ? s_last : 0);
     }
-    if (tid == 0) a.sampled[b * a.stride_sampled + step] = token;
+    out_token(found);
     break;
   }
-  for (int i = count + tid; i < a.width; i += NT) a.sampled[b * a.stride_sampled + i] = -1;
+  for (int i = count + tid; i < a.width; i += kThreads) a.sampled[b * a.stride_sampled + i] = -1;
   if (tid == 0) {
+    state->stopped = 0;
     a.num_sampled[b] = count;
     if (slot >= 0 && slot < a.slots) a.path_len[slot] = count;
   }
+}
+
+Split split_of(const eagle4_sample_tree_args& a) {
+  const int vec = a.dtype == EAGLE4_F32 ? 4 : 8;
+  Split s;
+  // a row may start up to vec - 1 elements behind a 16-byte boundary
+  s.chunks = static_cast<int>(e4::ceil_div(e4::ceil_div(static_cast<int64_t>(a.vocab) + vec - 1, vec), kChunk / vec));
+  const int64_t stats = a.rows * s.chunks;
+  s.masses_off = stats * 8;
+  s.state_off = s.masses_off + (a.probs != nullptr ? static_cast<int64_t>(a.num_reqs) * s.chunks * 8 : 0);
+  s.maxes_off = s.state_off + static_cast<int64_t>(a.num_reqs) * static_cast<int64_t>(sizeof(State));
+  return s;
+}
+
+int64_t workspace_of(const eagle4_sample_tree_args& a) {
+  const Split s = split_of(a);
+  return s.maxes_off + a.rows * s.chunks * 4;
 }
 
 bool tab_ok(const eagle4_itab& t) { return t.ptr != nullptr && e4::is_index_dtype(t.dtype); }
 
 template <typename T, typename Q>
 int launch(const eagle4_sample_tree_args& a, hipStream_t s) {
-  sample_tree_kernel<T, Q, 512><<<a.num_reqs, 512, 0, s>>>(a);
+  const Split split = split_of(a);
+  const int64_t waves = a.rows * split.chunks;
+  if (waves >= (1 << 25)) return EAGLE4_NOT_COVERED;  // 2^31 threads
+  const int pairs = a.probs == nullptr ? 0 : (a.width - 1 < kPairs ? a.width - 1 : kPairs);
+  if (waves > 0) sample_chunks<T><<<static_cast<uint32_t>(e4::ceil_div(waves, kWaves)), kThreads, 0, s>>>(a, split);
+  sample_walk<T, Q><<<a.num_reqs, kThreads, 0, s>>>(a, split, 1, pairs == 0);
+  if constexpr (Q::code >= 0) {
+    for (int i = 1; i <= pairs; ++i) {
+      sample_residual<T, Q><<<dim3(e4::ceil_div(split.chunks, kWaves), a.num_reqs), kThreads, 0, s>>>(a, split);
+      sample_walk<T, Q><<<a.num_reqs, kThreads, 0, s>>>(a, split, 0, i == pairs);
+    }
+  }
   return E4_LAUNCH_STATUS();
 }
 
@@ -484,13 +682,21 @@ int launch_t(const eagle4_sample_tree_args& a, hipStream_t s) {
   }
 }
 
+bool covered(const eagle4_sample_tree_args* a) {
+  return a->num_reqs > 0 && a->num_reqs <= 65535 && a->rows >= 0 && a->vocab >= 1 && a->vocab <= (1 << 30) && a->width >= 1 &&
+         a->width <= kMaxRows && a->slots >= 1;
+}
+
 }  // namespace
+
+extern "C" int64_t eagle4_sample_tree_workspace(const eagle4_sample_tree_args* a) {
+  return covered(a) ? workspace_of(*a) : -1;
+}
 
 extern "C" int eagle4_sample_tree(const eagle4_sample_tree_args* a, void* stream) {
   if (a->num_reqs == 0) return EAGLE4_OK;
-  if (a->num_reqs < 0 || a->rows < 0 || a->vocab < 1 || a->vocab > (1 << 30) || a->width < 1 || a->width > kMaxRows ||
-      a->slots < 1 || !tab_ok(a->drafted) || !tab_ok(a->cu_num_logits) || !tab_ok(a->idx_mapping) || !tab_ok(a->parents) ||
-      a->coins == nullptr || a->final_coins == nullptr || a->temperature == nullptr || a->logits == nullptr)
+  if (!covered(a) || a->workspace == nullptr || a->workspace_bytes < workspace_of(*a) || !tab_ok(a->drafted) ||
+      !tab_ok(a->cu_num_logits) || !tab_ok(a->idx_mapping) || !tab_ok(a->parents) || a->coins == nullptr || a->final_coins == nullptr || a->temperature == nullptr || a->logits == nullptr)
     return EAGLE4_NOT_COVERED;
   const hipStream_t s = static_cast<hipStream_t>(stream);
   switch (a->dtype) {

@@ -243,8 +243,8 @@ class ReadKvArgs(ctypes.Structure):
 class SampleTreeArgs(ctypes.Structure):
     _fields_ = _fields(
         "logits:p stride_row:q probs:p stride_prob:q drafted:t cu_num_logits:t idx_mapping:t parents:t coins:p "
-        "final_coins:p temperature:p sampled:p stride_sampled:q num_sampled:p path:p stride_path:q path_len:p rows:q "
-        "num_reqs:i width:i vocab:i slots:i dtype:i prob_dtype:i"
+        "final_coins:p temperature:p sampled:p stride_sampled:q num_sampled:p path:p stride_path:q path_len:p workspace:p "
+        "workspace_bytes:q rows:q num_reqs:i width:i vocab:i slots:i dtype:i prob_dtype:i"
     )
 
 
@@ -283,7 +283,8 @@ ENTRIES = {
     "eagle4_latent_attention": (LatentAttnArgs, 20),
 }
 EXTRA_SYMBOLS = ("eagle4_verify_attention_workspace", "eagle4_verify_attention_static_bytes",
-                 "eagle4_latent_attention_workspace", "eagle4_version", "eagle4_args_size", "eagle4_init")
+                 "eagle4_latent_attention_workspace", "eagle4_sample_tree_workspace", "eagle4_version",
+                 "eagle4_args_size", "eagle4_init")
 
 
 @functools.lru_cache(maxsize=None)
@@ -310,6 +311,8 @@ def library() -> ctypes.CDLL:
     lib.eagle4_verify_attention_workspace.restype = ctypes.c_int64
     lib.eagle4_latent_attention_workspace.argtypes = [ctypes.POINTER(LatentAttnArgs)]
     lib.eagle4_latent_attention_workspace.restype = ctypes.c_int64
+    lib.eagle4_sample_tree_workspace.argtypes = [ctypes.POINTER(SampleTreeArgs)]
+    lib.eagle4_sample_tree_workspace.restype = ctypes.c_int64
     lib.eagle4_verify_attention_static_bytes.argtypes = []
     lib.eagle4_verify_attention_static_bytes.restype = ctypes.c_int64
     lib.eagle4_init.argtypes = []

@@ -103,7 +103,7 @@ def sample_tree(
     its mass ``Z = 1``): accepted iff ``coin * q(x) * Z < r(x)``; a rejection leaves ``max(r - Z q, 0)``, or without
     ``draft_probs`` (``q(x) = 1``) ``r`` without ``x``. Without an accepted child the walk ends with the first token
     whose running sum of ``r`` exceeds ``final_coin * Z``. A row whose maximum is not finite has all its mass on its
-    argmax. Sums and comparisons are in 64 bits; only the walk's rows are read.
+    argmax. Sums and comparisons are in 64 bits.
     """
     if logits.dim() != 2 or (draft_probs is not None and draft_probs.shape != logits.shape):
         raise ValueError("sample_tree: logits must be [rows, vocab], draft_probs of the same shape")
@@ -142,6 +142,10 @@ def sample_tree(
         vocab=vocab, slots=slots, dtype=_native.dtype_code(logits.dtype),
         prob_dtype=0 if draft_probs is None else _native.dtype_code(draft_probs.dtype),
     )
+    need = _native.library().eagle4_sample_tree_workspace(args)
+    if need > 0:  # the torch caching allocator's
+        workspace = torch.empty(need, dtype=torch.uint8, device=logits.device)
+        args.workspace, args.workspace_bytes = workspace.data_ptr(), need
     _native.launch("eagle4_sample_tree", args, logits.device)
     return sampled, num_sampled
 

@@ -522,9 +522,13 @@ typedef struct eagle4_sample_tree_args {
   int32_t* path;        /* [slots, width] */
   int64_t stride_path;
   int32_t* path_len; /* [slots] */
+  void* workspace;   /* eagle4_sample_tree_workspace bytes, 16-byte aligned */
+  int64_t workspace_bytes;
   int64_t rows;
   int32_t num_reqs, width, vocab, slots, dtype, prob_dtype; /* width <= 64 */
 } eagle4_sample_tree_args;
+/* Bytes of workspace that a launch needs, or -1 where it is not covered. */
+int64_t eagle4_sample_tree_workspace(const eagle4_sample_tree_args* args);
 int eagle4_sample_tree(const eagle4_sample_tree_args* args, void* stream);
 
 /* ---- tree-verify attention over latent rows (no counterpart in the reference) -------------------------------------------- */
