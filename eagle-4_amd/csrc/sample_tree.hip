@@ -82,18 +82,36 @@ struct Row {
         x[i] = T::to_f32(static_cast<S>(w[i / 2] >> (16 * (i % 2))));
     }
   }
-  E4_DEV void edge(int v, float (&x)[VEC]) const {
+  E4_DEV u32x4 load(int v) const {
+    if (inside(v)) return raw(v);
     const int e0 = first(v);
+    u32x4 w = {0u, 0u, 0u, 0u};
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) x[i] = e0 + i >= 0 && e0 + i < vocab ? T::to_f32(p[e0 + i]) : -INFINITY;
-  }
-  E4_DEV void load(int v, float (&x)[VEC]) const {
-    if (inside(v))
-      widen(raw(v), x);
-    else
-      edge(v, x);
+    for (int i = 0; i < VEC; ++i) {
+      const S x = e0 + i >= 0 && e0 + i < vocab ? p[e0 + i] : T::from_f32(-INFINITY);
+      if constexpr (sizeof(S) == 4)
+        w[i] = __float_as_uint(x);
+      else
+        w[i / 2] |= static_cast<uint32_t>(x) << (16 * (i % 2));
+    }
+    return w;
   }
 };
+
+constexpr int kChunk = 4096;  // elements
+
+// A chunk of a row, 64 lanes: lane l has vectors l, l + 64, ..; all loads are in flight together. -inf outside the row.
+template <typename T, int NV = kChunk / Row<T>::VEC / 64>
+E4_DEV void load_chunk(const Row<T>& row, int chunk, int lane, u32x4 (&w)[NV]) {
+  const int v0 = chunk * (64 * NV) + lane;
+  if (row.first(chunk * (64 * NV)) >= 0 && row.first((chunk + 1) * (64 * NV)) <= row.vocab) {  // wholly inside
+#pragma unroll
+    for (int i = 0; i < NV; ++i) w[i] = row.raw(v0 + 64 * i);
+  } else {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) w[i] = row.load(v0 + 64 * i);
+  }
+}
 
 // The draft's probabilities of the same elements; `wide` where their vectors lie on vector boundaries too (rows of one
 // stride over bases on 16 bytes do).
@@ -145,13 +163,13 @@ E4_DEV double wave_sum(double x) {
 
 constexpr int kMaxRows = 64;  // of a tree: a lane each
 constexpr int kPairs = 3;     // residual and walk launches behind the first walk
-constexpr int kChunk = 4096;  // elements
 constexpr int kThreads = 256, kWaves = kThreads / 64;
 
 // A stopped walk. `count` rows are on its path, the last one `node`, whose child `child` was rejected last.
 struct State {
   int32_t stopped, node, child, count;
   double spent;
+  float top;  // the row's maximum
 };
 
 struct Split {
@@ -205,31 +223,24 @@ __global__ __launch_bounds__(kThreads) void sample_chunks(const eagle4_sample_tr
   constexpr int VEC = Row<T>::VEC, NV = kChunk / VEC / 64;
   const int lane = threadIdx.x & 63;
   const uint32_t id = blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t n = id / static_cast<uint32_t>(s.chunks);
-  const int chunk = id % static_cast<uint32_t>(s.chunks);
+  const uint32_t n = id / static_cast<uint32_t>(s.chunks);
+  const int chunk = static_cast<int>(id - n * s.chunks);
   if (n >= a.rows) return;
   const Row<T> row(a.logits, n, a.stride_row, a.vocab);
-  const int v0 = chunk * (64 * NV) + lane;
-  float x[NV][VEC];
-  if (row.first(chunk * (64 * NV)) >= 0 && row.first((chunk + 1) * (64 * NV)) <= row.vocab) {  // wholly inside
-    u32x4 w[NV];
-#pragma unroll
-    for (int i = 0; i < NV; ++i) w[i] = row.raw(v0 + 64 * i);
-#pragma unroll
-    for (int i = 0; i < NV; ++i) Row<T>::widen(w[i], x[i]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < NV; ++i) row.load(v0 + 64 * i, x[i]);
-  }
+  u32x4 w[NV];
+  load_chunk<T>(row, chunk, lane, w);
   const int b = __builtin_amdgcn_readfirstlane(request_of(a, n, lane));
   if (b >= a.num_reqs || n - e4::ld(a.cu_num_logits, b) >= a.width) return;  // a row that no walk visits
   const float temperature = a.temperature[b];
 
-  float m = x[0][0];
+  float x[NV][VEC];
+  float m = -INFINITY;
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
+  for (int i = 0; i < NV; ++i) {
+    Row<T>::widen(w[i], x[i]);
 #pragma unroll
     for (int k = 0; k < VEC; ++k) m = __builtin_elementwise_maximum(m, x[i][k]);
+  }
   m = wave_max(m);
   double sum = 0.0;
   if (!(temperature > 0.f) || !(m < INFINITY)) {
@@ -238,19 +249,16 @@ __global__ __launch_bounds__(kThreads) void sample_chunks(const eagle4_sample_tr
     for (int i = NV - 1; i >= 0; --i)
 #pragma unroll
       for (int k = VEC - 1; k >= 0; --k) {
-        const int e = row.first(v0 + 64 * i) + k;
+        const int e = row.first((chunk * NV + i) * 64 + lane) + k;
         if (e >= 0 && e < row.vocab && (m != m ? x[i][k] != x[i][k] : x[i][k] == m)) at = e;
       }
     sum = wave_min(at);
   } else {
     const double c = scale_of(temperature), off = -static_cast<double>(m) * c;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      double part = 0.0;
+    for (int i = 0; i < NV; ++i)
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) part += exp2_64(__builtin_fma(static_cast<double>(x[i][k]), c, off));
-      sum += part;
-    }
+      for (int k = 0; k < VEC; ++k) sum += exp2_64(__builtin_fma(static_cast<double>(x[i][k]), c, off));
     sum = wave_sum(sum);
   }
   if (lane == 0) {
@@ -260,47 +268,55 @@ __global__ __launch_bounds__(kThreads) void sample_chunks(const eagle4_sample_tr
   }
 }
 
-// The residual of a vector's elements, times the row's total: off = -maximum c.
-template <typename T, typename Q>
-E4_DEV void residual(const Row<T>& row, const QRow<Q, Row<T>::VEC>& qrow, int v, double c, double off, double spent,
-                     double (&r)[Row<T>::VEC]) {
-  constexpr int VEC = Row<T>::VEC;
-  float x[VEC];
-  row.load(v, x);
-#pragma unroll
-  for (int i = 0; i < VEC; ++i) r[i] = exp2_64(__builtin_fma(static_cast<double>(x[i]), c, off));
+// The residual of a vector's elements out of its logits, times the row's total: off = -maximum c.
+template <typename Q, int VEC>
+E4_DEV void residual(const float (&x)[VEC], const QRow<Q, VEC>& qrow, int first, int vocab, double c, double off, double spent,
+                     double (&r)[VEC]) {
   if constexpr (Q::code >= 0) {
-    if (spent > 0.0) {
-      float q[VEC];
-      qrow.load(row.first(v), row.vocab, q);
+    float q[VEC];
+    if (spent > 0.0) qrow.load(first, vocab, q);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) r[i] = __builtin_fmax(r[i] - spent * static_cast<double>(q[i]), 0.0);
+    for (int i = 0; i < VEC; ++i) {
+      r[i] = exp2_64(__builtin_fma(static_cast<double>(x[i]), c, off));
+      if (spent > 0.0) r[i] = __builtin_fmax(r[i] - spent * static_cast<double>(q[i]), 0.0);
     }
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) r[i] = exp2_64(__builtin_fma(static_cast<double>(x[i]), c, off));
   }
 }
 
-// A chunk's mass of it, by one wave.
+// Those elements of a vector away that are the `token` of a lane of `gone`.
+template <int VEC>
+E4_DEV void take_out(float (&x)[VEC], int first, uint64_t gone, int token) {
+  for (; gone != 0; gone &= gone - 1) {
+    const int at = __builtin_amdgcn_readlane(token, __builtin_ctzll(gone)) - first;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i)
+      if (i == at) x[i] = -INFINITY;
+  }
+}
+
+// A chunk's mass of it, by one wave. `gone`: the lanes whose `token` is taken out.
 template <typename T, typename Q>
 E4_DEV double chunk_mass(const Row<T>& row, const QRow<Q, Row<T>::VEC>& qrow, int chunk, double c, double off, double spent,
-                         int lane) {
+                         int lane, uint64_t gone, int token) {
   constexpr int VEC = Row<T>::VEC, NV = kChunk / VEC / 64;
+  const int v0 = chunk * (64 * NV) + lane;
+  u32x4 w[NV];
+  load_chunk<T>(row, chunk, lane, w);
   double sum = 0.0;
-#pragma unroll 2
+#pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int v = (chunk * NV + i) * 64 + lane;
-    if (v >= row.vectors) continue;
+    float x[VEC];
+    Row<T>::widen(w[i], x);
+    if constexpr (Q::code < 0) take_out<VEC>(x, row.first(v0 + 64 * i), gone, token);
     double r[VEC];
-    residual<T, Q>(row, qrow, v, c, off, spent, r);
+    residual<Q, VEC>(x, qrow, row.first(v0 + 64 * i), row.vocab, c, off, spent, r);
 #pragma unroll
     for (int k = 0; k < VEC; ++k) sum += r[k];
   }
   return wave_sum(sum);
-}
-
-E4_DEV float row_max(const float* maxes, int chunks, int lane) {
-  float top = -INFINITY;
-  for (int k = lane; k < chunks; k += 64) top = __builtin_elementwise_maximum(top, maxes[k]);
-  return wave_max(top);
 }
 
 template <typename T, typename Q>
@@ -313,8 +329,8 @@ __global__ __launch_bounds__(kThreads) void sample_residual(const eagle4_sample_
   const Row<T> row(a.logits, n, a.stride_row, a.vocab);
   const QRow<Q, Row<T>::VEC> qrow(a.probs, n, a.stride_prob, row.past);
   const double c = scale_of(a.temperature[b]);
-  const double off = -static_cast<double>(row_max(Work(a, s, n).maxes, s.chunks, lane)) * c;
-  const double mass = chunk_mass<T, Q>(row, qrow, chunk, c, off, st.spent, lane);
+  const double off = -static_cast<double>(st.top) * c;
+  const double mass = chunk_mass<T, Q>(row, qrow, chunk, c, off, st.spent, lane, 0, 0);
   if (lane == 0) reinterpret_cast<double*>(work + s.masses_off)[static_cast<int64_t>(b) * s.chunks + chunk] = mass;
 }
 
@@ -375,11 +391,26 @@ __global__ __launch_bounds__(kThreads) void sample_walk(const eagle4_sample_tree
   for (int r = tid / 16; r < limit; r += kThreads / 16) {
     const Work w(a, s, start + r);
     const int l16 = lane & 15;
-    float top = -INFINITY;
-    for (int k = l16; k < s.chunks; k += 16) top = __builtin_elementwise_maximum(top, w.maxes[k]);
+    float top = -INFINITY;  // the lane's chunks', then the row's
+    double total = 0.0;
+    for (int k0 = l16; k0 < s.chunks; k0 += 64) {
+      float m[4], most = top;
+      double sum[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const bool in = k0 + 16 * i < s.chunks;
+        m[i] = in ? w.maxes[k0 + 16 * i] : -INFINITY;
+        sum[i] = in ? w.sums[k0 + 16 * i] : 0.0;
+        most = __builtin_elementwise_maximum(most, m[i]);
+      }
+      total *= exp2_64((static_cast<double>(top) - static_cast<double>(most)) * c);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) total += sum[i] * exp2_64((static_cast<double>(m[i]) - static_cast<double>(most)) * c);
+      top = most;
+    }
+    const float mine = top;
 #pragma unroll
     for (int k = 1; k < 16; k <<= 1) top = __builtin_elementwise_maximum(top, __shfl_xor(top, k, 64));
-    double total = 0.0;
     if (greedy || !(__builtin_fabsf(top) < INFINITY)) {
       int at = INT32_MAX;  // its first chunk's; a row of -inf: 0
       for (int k = l16; k < s.chunks; k += 16)
@@ -391,8 +422,7 @@ __global__ __launch_bounds__(kThreads) void sample_walk(const eagle4_sample_tree
       }
       total = top == -INFINITY ? 0.0 : w.sums[at];
     } else {
-      for (int k = l16; k < s.chunks; k += 16)
-        total += w.sums[k] * exp2_64((static_cast<double>(w.maxes[k]) - static_cast<double>(top)) * c);
+      total *= exp2_64((static_cast<double>(mine) - static_cast<double>(top)) * c);
 #pragma unroll
       for (int k = 1; k < 16; k <<= 1) total += __shfl_xor(total, k, 64);
     }
@@ -467,12 +497,12 @@ __global__ __launch_bounds__(kThreads) void sample_walk(const eagle4_sample_tree
       if constexpr (kProbs) {
         spent += mass;
         if (!last) {
-          if (tid == 0) *state = State{1, node, j, count, spent};
+          if (tid == 0) *state = State{1, node, j, count, spent, top};
           return;
         }
         __syncthreads();  // the last masses have been read
         for (int k = wave; k < s.chunks; k += kWaves) {
-          const double m = chunk_mass<T, Q>(row, qrow, k, c, off, spent, lane);
+          const double m = chunk_mass<T, Q>(row, qrow, k, c, off, spent, lane, 0, 0);
           if (lane == 0) masses[k] = m;
         }
         __syncthreads();
@@ -499,20 +529,7 @@ __global__ __launch_bounds__(kThreads) void sample_walk(const eagle4_sample_tree
           const int k = __builtin_amdgcn_readlane(my_chunk, __builtin_ctzll(left));
           left &= ~__ballot(my_chunk == k);
           if (lost % kWaves == wave) {
-            double sum = 0.0;
-            for (int v = k * (kChunk / VEC) + lane; v < (k + 1) * (kChunk / VEC) && v < row.vectors; v += 64) {
-              double r[VEC];
-              residual<T, Q>(row, qrow, v, c, off, 0.0, r);
-              for (uint64_t x = rejected; x != 0; x &= x - 1) {
-                const int at = __builtin_amdgcn_readlane(static_cast<int>(token), __builtin_ctzll(x)) - row.first(v);
-#pragma unroll
-                for (int i = 0; i < VEC; ++i)
-                  if (i == at) r[i] = 0.0;
-              }
-#pragma unroll
-              for (int i = 0; i < VEC; ++i) sum += r[i];
-            }
-            sum = wave_sum(sum);
+            const double sum = chunk_mass<T, Q>(row, qrow, k, c, off, 0.0, lane, rejected, static_cast<int>(token));
             if (lane == 0) {
               s_lost_chunk[lost] = k;
               s_lost_mass[lost] = sum;
@@ -573,19 +590,10 @@ __global__ __launch_bounds__(kThreads) void sample_walk(const eagle4_sample_tree
       const int v0 = (at * kThreads + tid) * NV;
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        if (v0 + i < row.vectors) {
-          residual<T, Q>(row, qrow, v0 + i, c, off, spent, r[i]);
-        } else {
-#pragma unroll
-          for (int k = 0; k < VEC; ++k) r[i][k] = 0.0;
-        }
-        if constexpr (!kProbs)
-          for (uint64_t x = rejected; x != 0; x &= x - 1) {
-            const int gone = __builtin_amdgcn_readlane(static_cast<int>(token), __builtin_ctzll(x)) - row.first(v0 + i);
-#pragma unroll
-            for (int k = 0; k < VEC; ++k)
-              if (k == gone) r[i][k] = 0.0;
-          }
+        float x[VEC];
+        Row<T>::widen(row.load(v0 + i), x);
+        if constexpr (!kProbs) take_out<VEC>(x, row.first(v0 + i), rejected, static_cast<int>(token));
+        residual<Q, VEC>(x, qrow, row.first(v0 + i), row.vocab, c, off, spent, r[i]);
 #pragma unroll
         for (int k = 0; k < VEC; ++k) {
           mine += r[i][k];
@@ -657,10 +665,11 @@ bool tab_ok(const eagle4_itab& t) { return t.ptr != nullptr && e4::is_index_dtyp
 template <typename T, typename Q>
 int launch(const eagle4_sample_tree_args& a, hipStream_t s) {
   const Split split = split_of(a);
-  const int64_t waves = a.rows * split.chunks;
-  if (waves >= (1 << 25)) return EAGLE4_NOT_COVERED;  // 2^31 threads
+  const int64_t stats = a.rows * split.chunks;
+  if (stats >= 1 << 25) return EAGLE4_NOT_COVERED;  // 64 threads each: under 2^32
   const int pairs = a.probs == nullptr ? 0 : (a.width - 1 < kPairs ? a.width - 1 : kPairs);
-  if (waves > 0) sample_chunks<T><<<static_cast<uint32_t>(e4::ceil_div(waves, kWaves)), kThreads, 0, s>>>(a, split);
+  if (stats > 0)
+    sample_chunks<T><<<e4::ceil_div(stats, kWaves), kThreads, 0, s>>>(a, split);
   sample_walk<T, Q><<<a.num_reqs, kThreads, 0, s>>>(a, split, 1, pairs == 0);
   if constexpr (Q::code >= 0) {
     for (int i = 1; i <= pairs; ++i) {
