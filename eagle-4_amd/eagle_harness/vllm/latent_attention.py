@@ -42,15 +42,14 @@ def latent_verify_attention(
     if q.dim() != 3 or latent_new.dim() != 2 or latent_cache.dim() != 3 or out.dim() != 3:
         raise ValueError("latent_verify_attention: q [tokens, heads, dim], latent_new [tokens, dim], latent_cache "
                          "[blocks, page, dim] and out [tokens, heads, rank]")
-    tokens, heads, dim = q.shape
-    blocks, page, _ = latent_cache.shape
-    rank, num_reqs = out.shape[2], query_start_loc.shape[0] - 1
-    if latent_new.shape != (tokens, dim) or latent_cache.shape[2] != dim or out.shape[:2] != (tokens, heads) or rank >= dim:
+    (tokens, heads, dim), (blocks, page, cached), (out_tokens, out_heads, rank) = q.shape, latent_cache.shape, out.shape
+    num_reqs, dtype, device = query_start_loc.shape[0] - 1, q.dtype, q.device
+    if latent_new.shape != (tokens, dim) or cached != dim or out_tokens != tokens or out_heads != heads or rank >= dim:
         raise ValueError(f"latent_verify_attention: q {tuple(q.shape)}, latent_new {tuple(latent_new.shape)}, latent_cache "
                          f"{tuple(latent_cache.shape)} and out {tuple(out.shape)} do not fit")
     fp8 = latent_cache.dtype == torch.float8_e4m3fn
-    if q.dtype not in (torch.bfloat16, torch.float16) or q.dtype != latent_new.dtype or q.dtype != out.dtype or not (
-            fp8 or latent_cache.dtype == q.dtype):
+    if dtype not in (torch.bfloat16, torch.float16) or dtype != latent_new.dtype or dtype != out.dtype or not (
+            fp8 or latent_cache.dtype == dtype):
         raise _native.NotCovered("q, latent_new and out must share a dtype (bf16 or fp16), the cache be of it or float8_e4m3fn")
     if fp8:
         if latent_scale is None:
@@ -58,36 +57,35 @@ def latent_verify_attention(
         if latent_scale.dtype != torch.float32 or latent_scale.dim() not in (1, 2) or latent_scale.shape[0] < blocks or (
                 latent_scale.dim() == 2 and latent_scale.shape[1] < 1):
             raise ValueError(f"latent_scale must be fp32 [blocks >= {blocks}], got {tuple(latent_scale.shape)}")
+        if latent_scale.device != device:
+            raise ValueError("latent_verify_attention: every tensor must be on q's device")
     if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.stride(1) != 1:
         raise _native.NotCovered("the block table must be int32 [requests, blocks] with a unit column stride")
     if masks.dtype != torch.int64 or masks.dim() != 2 or masks.stride(1) != 1:
         raise _native.NotCovered("masks must be int64 with unit row stride")
-    if (block_table.shape[0] < num_reqs or context_lens.shape[0] < num_reqs or masks.shape[0] < num_reqs
-            or masks.shape[1] < max_query_len):
+    (requests, max_blocks), (mask_rows, mask_columns) = block_table.shape, masks.shape
+    if requests < num_reqs or context_lens.shape[0] < num_reqs or mask_rows < num_reqs or mask_columns < max_query_len:
         raise ValueError(f"latent_verify_attention: block_table, context_lens and masks must have {num_reqs} rows, masks "
                          f"{max_query_len} columns")
-    for name, t in (("q", q), ("latent_new", latent_new), ("latent_cache", latent_cache), ("out", out)):
-        if t.stride(-1) != 1:
-            raise _native.NotCovered(f"{name} must have a unit stride over its last dim")
-    for t in (latent_new, latent_cache, out, block_table, context_lens, query_start_loc, masks, latent_scale if fp8 else None):
-        if t is not None and t.device != q.device:
+    (q_token, q_head, q_unit), (new_token, new_unit) = q.stride(), latent_new.stride()
+    (cache_block, cache_slot, cache_unit), (out_token, out_head, out_unit) = latent_cache.stride(), out.stride()
+    if q_unit != 1 or new_unit != 1 or cache_unit != 1 or out_unit != 1:
+        raise _native.NotCovered("q, latent_new, latent_cache and out must have a unit stride over their last dim")
+    for t in (latent_new, latent_cache, out, block_table, context_lens, query_start_loc, masks):
+        if t.device != device:
             raise ValueError("latent_verify_attention: every tensor must be on q's device")
+    itab = _native.itab
     args = _native.LatentAttnArgs(
-        q=q.data_ptr(), stride_qt=q.stride(0), stride_qh=q.stride(1), latent_new=latent_new.data_ptr(),
-        stride_nt=latent_new.stride(0), cache=latent_cache.data_ptr(), stride_cb=latent_cache.stride(0),
-        stride_cs=latent_cache.stride(1), scale_page=latent_scale.data_ptr() if fp8 else 0,
-        stride_sp=latent_scale.stride(0) if fp8 else 0, block_table=_native.itab(block_table),
-        context_lens=_native.itab(context_lens), query_start_loc=_native.itab(query_start_loc), masks=masks.data_ptr(),
-        stride_mask=masks.stride(0), out=out.data_ptr(), stride_ot=out.stride(0), stride_oh=out.stride(1), tokens=tokens,
-        scale=scale, num_reqs=num_reqs, heads=heads, rank=rank, rope=dim - rank, page=page, max_query_len=max_query_len,
-        max_blocks=block_table.shape[1], num_blocks=blocks, dtype=_native.dtype_code(q.dtype),
-        cache_dtype=_native.dtype_code(latent_cache.dtype),
-    )
+        q.data_ptr(), q_token, q_head, latent_new.data_ptr(), new_token, latent_cache.data_ptr(), cache_block, cache_slot,
+        latent_scale.data_ptr() if fp8 else 0, latent_scale.stride(0) if fp8 else 0, itab(block_table), itab(context_lens),
+        itab(query_start_loc), masks.data_ptr(), masks.stride(0), out.data_ptr(), out_token, out_head, None, 0, tokens, scale,
+        num_reqs, heads, rank, dim - rank, page, max_query_len, max_blocks, blocks, _native.dtype_code(dtype),
+        _native.dtype_code(latent_cache.dtype))
     need = _native.library().eagle4_latent_attention_workspace(args)
     if need < 0:
         raise _native.NotCovered("eagle4_amd: latent_verify_attention does not cover this launch (shape, dtype or layout)")
     if need > 0:
-        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)  # the torch caching allocator's
+        workspace = torch.empty(need, dtype=torch.uint8, device=device)  # the torch caching allocator's
         args.workspace, args.workspace_bytes = workspace.data_ptr(), need
-    _native.launch("eagle4_latent_attention", args, q.device)
+    _native.launch("eagle4_latent_attention", args, device)
     return out

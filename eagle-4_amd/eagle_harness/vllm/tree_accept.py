@@ -77,6 +77,9 @@ def accept_tree(
     return sampled, num_sampled
 
 
+_LOGIT_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
+
+
 def sample_tree(
     logits: torch.Tensor,
     drafted: torch.Tensor,
@@ -107,46 +110,44 @@ def sample_tree(
     """
     if logits.dim() != 2 or (draft_probs is not None and draft_probs.shape != logits.shape):
         raise ValueError("sample_tree: logits must be [rows, vocab], draft_probs of the same shape")
-    rows, vocab = logits.shape
-    num_reqs, width = cu_num_logits.shape[0] - 1, store.width
-    if logits.stride(1) != 1 or (draft_probs is not None and draft_probs.stride(1) != 1):
+    (rows, vocab), device = logits.shape, logits.device
+    path, path_len, width = store.path, store.path_len, store.width
+    num_reqs = cu_num_logits.shape[0] - 1
+    row_stride, column = logits.stride()
+    prob_stride, prob_column = (0, 1) if draft_probs is None else draft_probs.stride()
+    if column != 1 or prob_column != 1:
         raise _native.NotCovered("logits and draft_probs must have a unit column stride")
     if width > 64:
         raise _native.NotCovered(f"tree widths above 64 rows ({width})")
-    for t in (logits, draft_probs):
-        if t is not None and t.dtype not in (torch.bfloat16, torch.float16, torch.float32):
-            raise _native.NotCovered(f"logits and draft_probs must be bf16, fp16 or fp32, got {t.dtype}")
+    if logits.dtype not in _LOGIT_DTYPES or (draft_probs is not None and draft_probs.dtype not in _LOGIT_DTYPES):
+        raise _native.NotCovered("logits and draft_probs must be bf16, fp16 or fp32, got "
+                                 f"{logits.dtype}{'' if draft_probs is None else f', {draft_probs.dtype}'}")
     if drafted.shape != (rows,) or idx_mapping.shape[0] < num_reqs or parents.dim() != 2 or parents.shape[1] < width:
         raise ValueError(f"sample_tree: drafted must be [{rows}], idx_mapping [>= {num_reqs}], parents [slots, >= {width}]")
     for name, t, n in (("coins", coins, rows), ("final_coins", final_coins, num_reqs), ("temperature", temperature, num_reqs)):
         if t.dtype != torch.float32 or t.dim() != 1 or t.shape[0] < n or not t.is_contiguous():
             raise ValueError(f"sample_tree: {name} must be a contiguous fp32 vector of {n} entries")
-    slots = min(parents.shape[0], store.path.shape[0], store.path_len.shape[0])
-    if (store.path.dtype != torch.int32 or store.path_len.dtype != torch.int32 or store.path.stride(1) != 1
-            or store.path.shape[1] < width or not store.path_len.is_contiguous()):
+    (path_slots, path_width), (path_stride, path_column) = path.shape, path.stride()
+    if (path.dtype != torch.int32 or path_len.dtype != torch.int32 or path_column != 1 or path_width < width
+            or not path_len.is_contiguous()):
         raise ValueError("sample_tree: the store's path and path_len must be int32, contiguous over a slot's entries")
-    for name, t in (("drafted", drafted), ("cu_num_logits", cu_num_logits), ("idx_mapping", idx_mapping), ("parents", parents),
-                    ("coins", coins), ("final_coins", final_coins), ("temperature", temperature), ("draft_probs", draft_probs),
-                    ("the store", store.path), ("the store", store.path_len)):
-        if t is not None and t.device != logits.device:
-            raise ValueError(f"sample_tree: {name} is on {t.device}, logits are on {logits.device}")
-    sampled = torch.empty(num_reqs, width, dtype=torch.int64, device=logits.device)
-    num_sampled = torch.empty(num_reqs, dtype=torch.int32, device=logits.device)
+    for t in (drafted, cu_num_logits, idx_mapping, parents, coins, final_coins, temperature, draft_probs, path, path_len):
+        if t is not None and t.device != device:
+            raise ValueError(f"sample_tree: every tensor must be on the logits' device, {device}, got {t.device}")
+    itab = _native.itab
+    sampled = torch.empty((num_reqs, width), dtype=torch.int64, device=device)
+    num_sampled = torch.empty(num_reqs, dtype=torch.int32, device=device)
     args = _native.SampleTreeArgs(
-        logits=logits.data_ptr(), stride_row=logits.stride(0), probs=_native.ptr(draft_probs),
-        stride_prob=0 if draft_probs is None else draft_probs.stride(0), drafted=_native.itab(drafted),
-        cu_num_logits=_native.itab(cu_num_logits), idx_mapping=_native.itab(idx_mapping), parents=_native.itab(parents),
-        coins=coins.data_ptr(), final_coins=final_coins.data_ptr(), temperature=temperature.data_ptr(),
-        sampled=sampled.data_ptr(), stride_sampled=width, num_sampled=num_sampled.data_ptr(), path=store.path.data_ptr(),
-        stride_path=store.path.stride(0), path_len=store.path_len.data_ptr(), rows=rows, num_reqs=num_reqs, width=width,
-        vocab=vocab, slots=slots, dtype=_native.dtype_code(logits.dtype),
-        prob_dtype=0 if draft_probs is None else _native.dtype_code(draft_probs.dtype),
-    )
+        logits.data_ptr(), row_stride, _native.ptr(draft_probs), prob_stride, itab(drafted), itab(cu_num_logits),
+        itab(idx_mapping), itab(parents), coins.data_ptr(), final_coins.data_ptr(), temperature.data_ptr(), sampled.data_ptr(),
+        width, num_sampled.data_ptr(), path.data_ptr(), path_stride, path_len.data_ptr(), None, 0, rows, num_reqs, width, vocab,
+        min(parents.shape[0], path_slots, path_len.shape[0]), _native.dtype_code(logits.dtype),
+        0 if draft_probs is None else _native.dtype_code(draft_probs.dtype))
     need = _native.library().eagle4_sample_tree_workspace(args)
-    if need > 0:  # the torch caching allocator's
-        workspace = torch.empty(need, dtype=torch.uint8, device=logits.device)
+    if need > 0:
+        workspace = torch.empty(need, dtype=torch.uint8, device=device)  # the torch caching allocator's
         args.workspace, args.workspace_bytes = workspace.data_ptr(), need
-    _native.launch("eagle4_sample_tree", args, logits.device)
+    _native.launch("eagle4_sample_tree", args, device)
     return sampled, num_sampled
 
 
