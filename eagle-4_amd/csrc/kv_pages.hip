@@ -41,23 +41,31 @@ E4_DEV float finite_abs(float x) {
   return a < INFINITY ? a : 0.f;
 }
 
-// N values from fp8 (N 8: one 8-byte load) and back.
+// N values in fp8 (N 8: one 8-byte load), widened, and back.
 template <int N>
-E4_DEV void load_codes(const uint8_t* p, float (&x)[N]) {
-  if constexpr (N == 8) {
-    const u32x2 w = *reinterpret_cast<const u32x2*>(p);
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(w[i], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(w[i], true);
-      x[4 * i] = lo[0];
-      x[4 * i + 1] = lo[1];
-      x[4 * i + 2] = hi[0];
-      x[4 * i + 3] = hi[1];
-    }
-  } else {
-    x[0] = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<uint32_t>(*p), false)[0];
+struct Codes {
+  u32x2 w;
+  E4_DEV void load(const uint8_t* p) {
+    if constexpr (N == 8)
+      w = *reinterpret_cast<const u32x2*>(p);
+    else
+      w[0] = *p;
   }
-}
+  E4_DEV void widen(float (&x)[N]) const {
+    if constexpr (N == 8) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(w[i], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(w[i], true);
+        x[4 * i] = lo[0];
+        x[4 * i + 1] = lo[1];
+        x[4 * i + 2] = hi[0];
+        x[4 * i + 3] = hi[1];
+      }
+    } else {
+      x[0] = __builtin_amdgcn_cvt_pk_f32_fp8(w[0], false)[0];
+    }
+  }
+};
 template <int N>
 E4_DEV void store_codes(uint8_t* p, const float (&x)[N]) {
   if constexpr (N == 8) {
@@ -96,6 +104,12 @@ struct Chunk {
   }
 };
 
+// A position's page; the division is a 32-bit one for all but the longest.
+E4_DEV int64_t page_of(int64_t position, int page) {
+  if (position >> 32 == 0) return static_cast<uint32_t>(position) / static_cast<uint32_t>(page);
+  return position / page;
+}
+
 // One wave per (matrix, head, page, request); waves of a workgroup take adjacent heads. `pages`: pages a request's rows can
 // reach at most. The page's rows stay in registers between the maximum and the rounding where they fit in kHeld chunks a
 // lane (16 rows of 256 elements), else they are read twice.
@@ -123,7 +137,7 @@ __global__ __launch_bounds__(256) void write_kernel(const eagle4_write_kv_args a
   }
   count = count < a.max_rows ? count : a.max_rows;
   if (context < 0 || count <= 0 || start < 0 || end > a.tokens) return;
-  const int64_t index = context / a.page + p, first = index * a.page;
+  const int64_t index = page_of(context, a.page) + p, first = index * a.page;
   const int64_t lo = first > context ? first : context;
   const int64_t hi = first + a.page < context + count ? first + a.page : context + count;
   if (lo >= hi || index >= a.max_blocks) return;
@@ -186,7 +200,9 @@ __global__ __launch_bounds__(256) void write_kernel(const eagle4_write_kv_args a
     for (int c = lane; c < kept * per_row; c += 64) {
       const int r = c / per_row, col = (c - r * per_row) * N;
       float x[N];
-      load_codes<N>(dst + r * stride_slot + col, x);
+      Codes<N> codes;
+      codes.load(dst + r * stride_slot + col);
+      codes.widen(x);
 #pragma unroll
       for (int i = 0; i < N; ++i) x[i] *= ratio;
       store_codes<N>(dst + r * stride_slot + col, x);
@@ -213,58 +229,87 @@ __global__ __launch_bounds__(256) void write_kernel(const eagle4_write_kv_args a
   if (lane == 0) *scale = now;
 }
 
-// One workgroup per (run of `rows` positions, request), all heads of both matrices. A page that the table does not have (or
-// names out of range) reads as zeros.
+// One workgroup per (run of `rows` positions, request, matrix), all heads. kAhead chunks of N elements a lane are on their way
+// together: table entries, then codes and scales, then the stores. A page that the table does not have (or names out of
+// range) reads as zeros.
 template <typename T, int N>
 __global__ __launch_bounds__(256) void read_kernel(const eagle4_read_kv_args a, int rows) {
   using S = typename T::storage;
+  constexpr int kAhead = 4;
   const int b = blockIdx.y;
+  const bool second = blockIdx.z != 0;
   const int64_t start = e4::ld(a.start_loc, b), end = e4::ld(a.start_loc, b + 1);
-  const int64_t lo = static_cast<int64_t>(blockIdx.x) * rows;
+  const int lo = static_cast<int>(blockIdx.x) * rows;
   if (start < 0 || end > a.tokens || lo >= end - start || lo >= a.max_len) return;
   const int64_t most = end - start < a.max_len ? end - start : a.max_len;
   const int n = static_cast<int>(most - lo < rows ? most - lo : rows);
   const int per_head = a.dim / N, per_row = per_head * a.heads, total = n * per_row;
-  const int matrices = a.value != nullptr ? 2 : 1;
-  for (int c = threadIdx.x; c < total * matrices; c += 256) {
-    const bool second = c >= total;
-    const int at = second ? c - total : c;
-    const int r = at / per_row, hc = at - r * per_row, head = hc / per_head, col = (hc - head * per_head) * N;
-    const int64_t pos = lo + r, index = pos / a.page;
-    const int64_t block = index < a.max_blocks ? e4::ld(a.block_table, b, index) : -1;
-    float x[N];
-    if (block >= 0 && block < a.num_blocks) {
-      const uint8_t* const src = static_cast<const uint8_t*>(second ? a.value_cache : a.key_cache) +
-                                 block * (second ? a.stride_vcb : a.stride_kcb) +
-                                 (pos - index * a.page) * (second ? a.stride_vcs : a.stride_kcs) +
-                                 head * (second ? a.stride_vch : a.stride_kch) + col;
-      const float s = second ? a.v_scale[block * a.stride_vsb + head * a.stride_vsh]
-                             : a.k_scale[block * a.stride_ksb + head * a.stride_ksh];
-      load_codes<N>(src, x);
+  const uint8_t* const cache = static_cast<const uint8_t*>(second ? a.value_cache : a.key_cache);
+  const int64_t stride_block = second ? a.stride_vcb : a.stride_kcb, stride_slot = second ? a.stride_vcs : a.stride_kcs,
+                stride_head = second ? a.stride_vch : a.stride_kch;
+  const float* const scales = second ? a.v_scale : a.k_scale;
+  const int64_t stride_sb = second ? a.stride_vsb : a.stride_ksb, stride_sh = second ? a.stride_vsh : a.stride_ksh;
+  S* const rows_out = static_cast<S*>(second ? a.value : a.key) + (start + lo) * (second ? a.stride_vt : a.stride_kt);
+  const int64_t stride_t = second ? a.stride_vt : a.stride_kt, stride_h = second ? a.stride_vh : a.stride_kh;
+  // chunk c is row c / per_row; the lane's next one is 256 on
+  const int step_row = 256 / per_row, step_col = 256 % per_row;
+  int r = static_cast<int>(threadIdx.x) / per_row, hc = static_cast<int>(threadIdx.x) % per_row;
+  for (int c0 = threadIdx.x; c0 < total; c0 += 256 * kAhead) {
+    int64_t block[kAhead];
+    int row[kAhead], head[kAhead], col[kAhead], slot[kAhead];
 #pragma unroll
-      for (int i = 0; i < N; ++i) x[i] *= s;
-    } else {
-#pragma unroll
-      for (int i = 0; i < N; ++i) x[i] = 0.f;
-    }
-    S* const out = static_cast<S*>(second ? a.value : a.key) + (start + pos) * (second ? a.stride_vt : a.stride_kt) +
-                   head * (second ? a.stride_vh : a.stride_kh) + col;
-    if constexpr (N == 8) {
-      constexpr int kVecs = static_cast<int>(sizeof(S)) / 2;
-#pragma unroll
-      for (int v = 0; v < kVecs; ++v) {
-        u32x4 w;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if constexpr (sizeof(S) == 4)
-            w[i] = __float_as_uint(x[4 * v + i]);
-          else
-            w[i] = T::pack(x[2 * i], x[2 * i + 1]);
-        }
-        reinterpret_cast<u32x4*>(out)[v] = w;
+    for (int i = 0; i < kAhead; ++i) {
+      row[i] = r;
+      head[i] = static_cast<int>(static_cast<uint32_t>(hc) / static_cast<uint32_t>(per_head));
+      col[i] = (hc - head[i] * per_head) * N;
+      const int index = static_cast<int>(static_cast<uint32_t>(lo + r) / static_cast<uint32_t>(a.page));
+      slot[i] = lo + r - index * a.page;
+      block[i] = c0 + 256 * i < total && index < a.max_blocks ? e4::ld(a.block_table, b, index) : -1;
+      r += step_row;
+      hc += step_col;
+      if (hc >= per_row) {
+        hc -= per_row;
+        ++r;
       }
-    } else {
-      *out = T::from_f32(x[0]);
+    }
+    Codes<N> codes[kAhead];
+    float s[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      s[i] = 0.f;
+      codes[i] = Codes<N>{};
+      if (block[i] >= 0 && block[i] < a.num_blocks) {
+        codes[i].load(cache + block[i] * stride_block + slot[i] * stride_slot + head[i] * stride_head + col[i]);
+        s[i] = scales[block[i] * stride_sb + head[i] * stride_sh];
+      } else {
+        block[i] = -1;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      if (c0 + 256 * i >= total) break;
+      float x[N];
+      codes[i].widen(x);
+#pragma unroll
+      for (int k = 0; k < N; ++k) x[k] = block[i] < 0 ? 0.f : x[k] * s[i];
+      S* const out = rows_out + row[i] * stride_t + head[i] * stride_h + col[i];
+      if constexpr (N == 8) {
+        constexpr int kVecs = static_cast<int>(sizeof(S)) / 2;
+#pragma unroll
+        for (int v = 0; v < kVecs; ++v) {
+          u32x4 w;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            if constexpr (sizeof(S) == 4)
+              w[k] = __float_as_uint(x[4 * v + k]);
+            else
+              w[k] = T::pack(x[2 * k], x[2 * k + 1]);
+          }
+          reinterpret_cast<u32x4*>(out)[v] = w;
+        }
+      } else {
+        *out = T::from_f32(x[0]);
+      }
     }
   }
 }
@@ -309,7 +354,7 @@ int launch_write(const eagle4_write_kv_args& a, hipStream_t s) {
 template <typename T>
 int launch_read(const eagle4_read_kv_args& a, hipStream_t s) {
   const int rows = 16;
-  const dim3 grid(e4::ceil_div(a.max_len, rows), a.num_reqs);
+  const dim3 grid(e4::ceil_div(a.max_len, rows), a.num_reqs, a.value != nullptr ? 2 : 1);
   if (vectors(a))
     read_kernel<T, 8><<<grid, 256, 0, s>>>(a, rows);
   else
