@@ -113,10 +113,9 @@ E4_DEV int64_t page_of(int64_t position, int page) {
 // One wave per (matrix, head, page, request); waves of a workgroup take adjacent heads. `pages`: pages a request's rows can
 // reach at most. The page's rows stay in registers between the maximum and the rounding where they fit in kHeld chunks a
 // lane (16 rows of 256 elements), else they are read twice.
-template <typename T, int N>
+template <typename T, int N, int kHeld>
 __global__ __launch_bounds__(256) void write_kernel(const eagle4_write_kv_args a, int pages) {
   using S = typename T::storage;
-  constexpr int kHeld = N == 8 ? 8 : 4;
   const int lane = threadIdx.x & 63;
   const int item = blockIdx.x * 4 + (threadIdx.x >> 6);
   const int matrices = a.value != nullptr ? 2 : 1;
@@ -344,10 +343,12 @@ int launch_write(const eagle4_write_kv_args& a, hipStream_t s) {
   const int64_t items = int64_t(pages) * a.heads * (a.value != nullptr ? 2 : 1);
   if (items > (int64_t(1) << 30)) return EAGLE4_NOT_COVERED;
   const dim3 grid(e4::ceil_div(items, 4), a.num_reqs);
-  if (vectors(a))
-    write_kernel<T, 8><<<grid, 256, 0, s>>>(a, pages);
+  if (!vectors(a))
+    write_kernel<T, 1, 4><<<grid, 256, 0, s>>>(a, pages);
+  else if (int64_t(a.page) * a.dim <= 4 * 64 * 8)
+    write_kernel<T, 8, 4><<<grid, 256, 0, s>>>(a, pages);
   else
-    write_kernel<T, 1><<<grid, 256, 0, s>>>(a, pages);
+    write_kernel<T, 8, 8><<<grid, 256, 0, s>>>(a, pages);
   return E4_LAUNCH_STATUS();
 }
 
