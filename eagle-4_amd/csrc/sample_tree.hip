@@ -16,13 +16,20 @@
 //
 // Split: a wave takes 4096 elements of a row, a chunk. Three kinds of launches:
 //   - statistics: of every chunk of every row its maximum and its mass relative to that. All rows of all trees at once: the
-//     walk visits a few of them, but one after another, and a workgroup that reads rows on its own reads them at a
-//     hundredth of the memory's rate. PLACEHOLDER
+//     walk visits a few of them, but one after another, and a workgroup that reads its request's rows on its own has one
+//     CU's rate (vocabulary 151936, bf16: one tree of 16 rows 105 to 232 us that way, by the walk's length, against 19;
+//     64 trees of up to 16 rows 228 against 102);
 //   - the walk, a workgroup per request: the rows' sums out of the chunks', then the decisions, a lane a child. Ends with the
 //     final token: the chunks' running sum leads to one chunk, which is read. With draft probabilities a rejection needs the
-//     residual's mass: the walk stops there and leaves its state,
+//     residual's mass: the walk stops there and leaves its state;
 //   - the residual's launch sums max(p - s q, 0) over the chunks of the stopped walks, and the walk is launched again.
-// After kPairs such pairs a walk reads the rows of its further rejections itself.
+// After kPairs such pairs a walk reads the rows of its further rejections itself. 2: a pair that finds nothing to do costs
+// 5 us (32 chains 68.6 us with two, 70.9 with three), a pass by one workgroup 15 to 40 (12 trees of 50257 tokens 64.1 and
+// 72.1 us with two and three). Continuing the walk in the residual's last workgroup instead of a launch of its own takes a fence
+// of every workgroup, and those cost more (95 us instead of 71).
+// What bounds it: the statistics by their 64-bit operations (64 trees: 82 us for 750 rows, 44 of them the logits' own; a table
+// of 32 roots with a polynomial of degree 4 has a third fewer operations and is no faster for its lookups; one chunk
+// loaded ahead of another, 93 us), the walk by its chain of dependent loads (12 us for one request, 22 among 64).
 
 #include "common.h"
 
@@ -100,16 +107,16 @@ struct Row {
 
 constexpr int kChunk = 4096;  // elements
 
-// A chunk of a row, 64 lanes: lane l has vectors l, l + 64, ..; all loads are in flight together. -inf outside the row.
-template <typename T, int NV = kChunk / Row<T>::VEC / 64>
-E4_DEV void load_chunk(const Row<T>& row, int chunk, int lane, u32x4 (&w)[NV]) {
-  const int v0 = chunk * (64 * NV) + lane;
-  if (row.first(chunk * (64 * NV)) >= 0 && row.first((chunk + 1) * (64 * NV)) <= row.vocab) {  // wholly inside
+// 64 NV vectors of a row from `v0` on: lane l has v0 + l, v0 + l + 64, ..; all loads are in flight together. -inf outside
+// the row.
+template <typename T, int NV>
+E4_DEV void load_vectors(const Row<T>& row, int v0, int lane, u32x4 (&w)[NV]) {
+  if (row.first(v0) >= 0 && row.first(v0 + 64 * NV) <= row.vocab) {  // wholly inside
 #pragma unroll
-    for (int i = 0; i < NV; ++i) w[i] = row.raw(v0 + 64 * i);
+    for (int i = 0; i < NV; ++i) w[i] = row.raw(v0 + lane + 64 * i);
   } else {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) w[i] = row.load(v0 + 64 * i);
+    for (int i = 0; i < NV; ++i) w[i] = row.load(v0 + lane + 64 * i);
   }
 }
 
@@ -162,7 +169,7 @@ E4_DEV double wave_sum(double x) {
 }
 
 constexpr int kMaxRows = 64;  // of a tree: a lane each
-constexpr int kPairs = 3;     // residual and walk launches behind the first walk
+constexpr int kPairs = 2;     // residual and walk launches behind the first walk
 constexpr int kThreads = 256, kWaves = kThreads / 64;
 
 // A stopped walk. `count` rows are on its path, the last one `node`, whose child `child` was rejected last.
@@ -228,7 +235,7 @@ __global__ __launch_bounds__(kThreads) void sample_chunks(const eagle4_sample_tr
   if (n >= a.rows) return;
   const Row<T> row(a.logits, n, a.stride_row, a.vocab);
   u32x4 w[NV];
-  load_chunk<T>(row, chunk, lane, w);
+  load_vectors<T, NV>(row, chunk * (64 * NV), lane, w);
   const int b = __builtin_amdgcn_readfirstlane(request_of(a, n, lane));
   if (b >= a.num_reqs || n - e4::ld(a.cu_num_logits, b) >= a.width) return;  // a row that no walk visits
   const float temperature = a.temperature[b];
@@ -301,20 +308,24 @@ E4_DEV void take_out(float (&x)[VEC], int first, uint64_t gone, int token) {
 template <typename T, typename Q>
 E4_DEV double chunk_mass(const Row<T>& row, const QRow<Q, Row<T>::VEC>& qrow, int chunk, double c, double off, double spent,
                          int lane, uint64_t gone, int token) {
-  constexpr int VEC = Row<T>::VEC, NV = kChunk / VEC / 64;
-  const int v0 = chunk * (64 * NV) + lane;
-  u32x4 w[NV];
-  load_chunk<T>(row, chunk, lane, w);
+  constexpr int VEC = Row<T>::VEC, NV = kChunk / VEC / 64, kAtOnce = 4;  // vectors whose loads are in flight together
   double sum = 0.0;
+#pragma unroll 1
+  for (int i0 = 0; i0 < NV; i0 += kAtOnce) {
+    const int v0 = (chunk * NV + i0) * 64;
+    u32x4 w[kAtOnce];
+    load_vectors<T, kAtOnce>(row, v0, lane, w);
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    float x[VEC];
-    Row<T>::widen(w[i], x);
-    if constexpr (Q::code < 0) take_out<VEC>(x, row.first(v0 + 64 * i), gone, token);
-    double r[VEC];
-    residual<Q, VEC>(x, qrow, row.first(v0 + 64 * i), row.vocab, c, off, spent, r);
+    for (int i = 0; i < kAtOnce; ++i) {
+      const int first = row.first(v0 + lane + 64 * i);
+      float x[VEC];
+      Row<T>::widen(w[i], x);
+      if constexpr (Q::code < 0) take_out<VEC>(x, first, gone, token);
+      double r[VEC];
+      residual<Q, VEC>(x, qrow, first, row.vocab, c, off, spent, r);
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) sum += r[k];
+      for (int k = 0; k < VEC; ++k) sum += r[k];
+    }
   }
   return wave_sum(sum);
 }
