@@ -23,10 +23,11 @@
 //     final token: the chunks' running sum leads to one chunk, which is read. With draft probabilities a rejection needs the
 //     residual's mass: the walk stops there and leaves its state;
 //   - the residual's launch sums max(p - s q, 0) over the chunks of the stopped walks, and the walk is launched again.
-// After kPairs such pairs a walk reads the rows of its further rejections itself. 2: a pair that finds nothing to do costs
-// 5 us (32 chains 68.6 us with two, 70.9 with three), a pass by one workgroup 15 to 40 (12 trees of 50257 tokens 64.1 and
-// 72.1 us with two and three). Continuing the walk in the residual's last workgroup instead of a launch of its own takes a fence
-// of every workgroup, and those cost more (95 us instead of 71).
+// After kPairs such pairs a walk reads the rows of its further rejections itself. None, one and two pairs take 87, 62 and
+// 65 us for 32 chains of 6 (one rejection each at most), 80, 78 and 76 for 12 trees of 12 over 50257 tokens, 200, 176 and 151
+// for 16 trees of 16 over 151936. Continuing the walk in the residual's last workgroup instead of a launch of its own takes a
+// fence of every workgroup, and those cost more (95 us instead of 71). The walk's workgroup has 512 threads for those rows:
+// with 256, 89 us instead of 76 for the 12 trees; with 1024, 3% off the trees and 10% on single users' walks.
 // What bounds it: the statistics by their 64-bit operations (64 trees: 82 us for 750 rows, 44 of them the logits' own; a table
 // of 32 roots with a polynomial of degree 4 has a third fewer operations and is no faster for its lookups; one chunk
 // loaded ahead of another, 93 us), the walk by its chain of dependent loads (12 us for one request, 22 among 64).
@@ -106,6 +107,8 @@ struct Row {
 };
 
 constexpr int kChunk = 4096;  // elements
+constexpr int kPart = 1024;   // of a residual's masses
+constexpr int kParts = kChunk / kPart;
 
 // 64 NV vectors of a row from `v0` on: lane l has v0 + l, v0 + l + 64, ..; all loads are in flight together. -inf outside
 // the row.
@@ -171,6 +174,7 @@ E4_DEV double wave_sum(double x) {
 constexpr int kMaxRows = 64;  // of a tree: a lane each
 constexpr int kPairs = 2;     // residual and walk launches behind the first walk
 constexpr int kThreads = 256, kWaves = kThreads / 64;
+constexpr int kWalkThreads = 512, kWalkWaves = kWalkThreads / 64;
 
 // A stopped walk. `count` rows are on its path, the last one `node`, whose child `child` was rejected last.
 struct State {
@@ -293,6 +297,10 @@ E4_DEV void residual(const float (&x)[VEC], const QRow<Q, VEC>& qrow, int first,
   }
 }
 
+E4_DEV double* masses_of(const eagle4_sample_tree_args& a, const Split& s, int b) {  // of request b's stopped row
+  return reinterpret_cast<double*>(static_cast<char*>(a.workspace) + s.masses_off) + static_cast<int64_t>(b) * s.chunks * kParts;
+}
+
 // Those elements of a vector away that are the `token` of a lane of `gone`.
 template <int VEC>
 E4_DEV void take_out(float (&x)[VEC], int first, uint64_t gone, int token) {
@@ -304,64 +312,62 @@ E4_DEV void take_out(float (&x)[VEC], int first, uint64_t gone, int token) {
   }
 }
 
-// A chunk's mass of it, by one wave. `gone`: the lanes whose `token` is taken out.
-template <typename T, typename Q>
-E4_DEV double chunk_mass(const Row<T>& row, const QRow<Q, Row<T>::VEC>& qrow, int chunk, double c, double off, double spent,
-                         int lane, uint64_t gone, int token) {
-  constexpr int VEC = Row<T>::VEC, NV = kChunk / VEC / 64, kAtOnce = 4;  // vectors whose loads are in flight together
+// The mass of it in 64 NV vectors from v0 on, by one wave; their loads are in flight together. `gone`: the lanes whose `token`
+// is taken out.
+template <typename T, typename Q, int NV>
+E4_DEV double residual_mass(const Row<T>& row, const QRow<Q, Row<T>::VEC>& qrow, int v0, double c, double off, double spent,
+                            int lane, uint64_t gone, int token) {
+  constexpr int VEC = Row<T>::VEC;
+  u32x4 w[NV];
+  load_vectors<T, NV>(row, v0, lane, w);
   double sum = 0.0;
-#pragma unroll 1
-  for (int i0 = 0; i0 < NV; i0 += kAtOnce) {
-    const int v0 = (chunk * NV + i0) * 64;
-    u32x4 w[kAtOnce];
-    load_vectors<T, kAtOnce>(row, v0, lane, w);
 #pragma unroll
-    for (int i = 0; i < kAtOnce; ++i) {
-      const int first = row.first(v0 + lane + 64 * i);
-      float x[VEC];
-      Row<T>::widen(w[i], x);
-      if constexpr (Q::code < 0) take_out<VEC>(x, first, gone, token);
-      double r[VEC];
-      residual<Q, VEC>(x, qrow, first, row.vocab, c, off, spent, r);
+  for (int i = 0; i < NV; ++i) {
+    const int first = row.first(v0 + lane + 64 * i);
+    float x[VEC];
+    Row<T>::widen(w[i], x);
+    if constexpr (Q::code < 0) take_out<VEC>(x, first, gone, token);
+    double r[VEC];
+    residual<Q, VEC>(x, qrow, first, row.vocab, c, off, spent, r);
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) sum += r[k];
-    }
+    for (int k = 0; k < VEC; ++k) sum += r[k];
   }
   return wave_sum(sum);
 }
 
 template <typename T, typename Q>
 __global__ __launch_bounds__(kThreads) void sample_residual(const eagle4_sample_tree_args a, const Split s) {
-  const int lane = threadIdx.x & 63, b = blockIdx.y, chunk = blockIdx.x * kWaves + (threadIdx.x >> 6);
+  constexpr int VEC = Row<T>::VEC;
+  const int lane = threadIdx.x & 63, b = blockIdx.y;
+  const int part = blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   char* const work = static_cast<char*>(a.workspace);
   const State st = reinterpret_cast<const State*>(work + s.state_off)[b];
-  if (st.stopped == 0 || chunk >= s.chunks) return;
+  if (st.stopped == 0 || part >= s.chunks * kParts) return;
   const int64_t n = e4::ld(a.cu_num_logits, b) + st.node;
   const Row<T> row(a.logits, n, a.stride_row, a.vocab);
   const QRow<Q, Row<T>::VEC> qrow(a.probs, n, a.stride_prob, row.past);
   const double c = scale_of(a.temperature[b]);
   const double off = -static_cast<double>(st.top) * c;
-  const double mass = chunk_mass<T, Q>(row, qrow, chunk, c, off, st.spent, lane, 0, 0);
-  if (lane == 0) reinterpret_cast<double*>(work + s.masses_off)[static_cast<int64_t>(b) * s.chunks + chunk] = mass;
+  const double mass = residual_mass<T, Q, kPart / VEC / 64>(row, qrow, part * (kPart / VEC), c, off, st.spent, lane, 0, 0);
+  if (lane == 0) masses_of(a, s, b)[part] = mass;
 }
 
 // The walk. Every wave takes the decisions, lane j for row j of the tree; the waves part for the rows' sums and for the
 // final token's chunk.
 template <typename T, typename Q>
-__global__ __launch_bounds__(kThreads) void sample_walk(const eagle4_sample_tree_args a, const Split s, int first, int last) {
-  constexpr int VEC = Row<T>::VEC, NV = kChunk / VEC / kThreads;  // vectors of a thread in the final token's chunk
+__global__ __launch_bounds__(kWalkThreads) void sample_walk(const eagle4_sample_tree_args a, const Split s, int first, int last) {
+  constexpr int VEC = Row<T>::VEC, NV = (kChunk / VEC + kWalkThreads - 1) / kWalkThreads;  // vectors of a thread in the final token's chunk
   constexpr bool kProbs = Q::code >= 0;
-  static_assert(NV >= 1, "a chunk");
   __shared__ float s_top[kMaxRows];
   __shared__ double s_total[kMaxRows];
   __shared__ int s_lost_chunk[kMaxRows];
   __shared__ double s_lost_mass[kMaxRows];
-  __shared__ double s_scan[kWaves];
+  __shared__ double s_scan[kWalkWaves];
   __shared__ int s_token, s_last;
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   char* const work = static_cast<char*>(a.workspace);
   State* const state = reinterpret_cast<State*>(work + s.state_off) + b;
-  double* const masses = reinterpret_cast<double*>(work + s.masses_off) + static_cast<int64_t>(b) * s.chunks;
+  double* const masses = masses_of(a, s, b);
   int node = 0, count = 0, resumed = 0;
   double spent = 0.0;
   if (!first) {
@@ -399,7 +405,7 @@ __global__ __launch_bounds__(kThreads) void sample_walk(const eagle4_sample_tree
   }
 
   // The rows' maxima and totals out of the chunks', 16 lanes a row; a row with all mass on one element: its index.
-  for (int r = tid / 16; r < limit; r += kThreads / 16) {
+  for (int r = tid / 16; r < limit; r += kWalkThreads / 16) {
     const Work w(a, s, start + r);
     const int l16 = lane & 15;
     float top = -INFINITY;  // the lane's chunks', then the row's
@@ -458,7 +464,7 @@ __global__ __launch_bounds__(kThreads) void sample_walk(const eagle4_sample_tree
   };
   const auto sum_of_masses = [&] {
     double sum = 0.0;
-    for (int k = lane; k < s.chunks; k += 64) sum += masses[k];
+    for (int k = lane; k < s.chunks * kParts; k += 64) sum += masses[k];
     return wave_sum(sum);
   };
 
@@ -512,8 +518,8 @@ __global__ __launch_bounds__(kThreads) void sample_walk(const eagle4_sample_tree
           return;
         }
         __syncthreads();  // the last masses have been read
-        for (int k = wave; k < s.chunks; k += kWaves) {
-          const double m = chunk_mass<T, Q>(row, qrow, k, c, off, spent, lane, 0, 0);
+        for (int k = wave; k < s.chunks * kParts; k += kWalkWaves) {
+          const double m = residual_mass<T, Q, kPart / VEC / 64>(row, qrow, k * (kPart / VEC), c, off, spent, lane, 0, 0);
           if (lane == 0) masses[k] = m;
         }
         __syncthreads();
@@ -539,8 +545,9 @@ __global__ __launch_bounds__(kThreads) void sample_walk(const eagle4_sample_tree
         while (left != 0) {
           const int k = __builtin_amdgcn_readlane(my_chunk, __builtin_ctzll(left));
           left &= ~__ballot(my_chunk == k);
-          if (lost % kWaves == wave) {
-            const double sum = chunk_mass<T, Q>(row, qrow, k, c, off, 0.0, lane, rejected, static_cast<int>(token));
+          if (lost % kWalkWaves == wave) {
+            const double sum = residual_mass<T, Q, kChunk / VEC / 64>(row, qrow, k * (kChunk / VEC), c, off, 0.0, lane, rejected,
+                                                                               static_cast<int>(token));
             if (lane == 0) {
               s_lost_chunk[lost] = k;
               s_lost_mass[lost] = sum;
@@ -550,6 +557,7 @@ __global__ __launch_bounds__(kThreads) void sample_walk(const eagle4_sample_tree
         }
         if (lost > 0) __syncthreads();
       }
+      // a chunk's mass, or of a residual a part's
       const auto mass_of = [&](int k) {
         if (spent > 0.0) return masses[k];
         double m = w.sums[k] * exp2_64((static_cast<double>(w.maxes[k]) - static_cast<double>(top)) * c);
@@ -569,10 +577,11 @@ __global__ __launch_bounds__(kThreads) void sample_walk(const eagle4_sample_tree
         mass = total;
       }
       const double target = static_cast<double>(a.final_coins[b]) * mass;
+      const int units = spent > 0.0 ? s.chunks * kParts : s.chunks, unit = (spent > 0.0 ? kPart : kChunk) / VEC;
       double base = 0.0;
-      int at = -1, full = 0;  // the chunk in which the running sum passes the target, the last one that has mass
-      for (int k0 = 0; k0 < s.chunks && at < 0; k0 += 64) {
-        const double m = k0 + lane < s.chunks ? mass_of(k0 + lane) : 0.0;
+      int at = -1, full = 0;  // the unit in which the running sum passes the target, the last one that has mass
+      for (int k0 = 0; k0 < units && at < 0; k0 += 64) {
+        const double m = k0 + lane < units ? mass_of(k0 + lane) : 0.0;
         double run = m;
 #pragma unroll
         for (int k = 1; k < 64; k <<= 1) {
@@ -598,11 +607,16 @@ __global__ __launch_bounds__(kThreads) void sample_walk(const eagle4_sample_tree
       double r[NV][VEC];
       double mine = 0.0;
       int end = -1;  // the thread's last element that has mass
-      const int v0 = (at * kThreads + tid) * NV;
+      const int v0 = at * unit + tid * NV;
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         float x[VEC];
-        Row<T>::widen(row.load(v0 + i), x);
+        if (tid * NV + i < unit) {
+          Row<T>::widen(row.load(v0 + i), x);
+        } else {
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) x[k] = -INFINITY;
+        }
         if constexpr (!kProbs) take_out<VEC>(x, row.first(v0 + i), rejected, static_cast<int>(token));
         residual<Q, VEC>(x, qrow, row.first(v0 + i), row.vocab, c, off, spent, r[i]);
 #pragma unroll
@@ -646,7 +660,7 @@ __global__ __launch_bounds__(kThreads) void sample_walk(const eagle4_sample_tree
     out_token(found);
     break;
   }
-  for (int i = count + tid; i < a.width; i += kThreads) a.sampled[b * a.stride_sampled + i] = -1;
+  for (int i = count + tid; i < a.width; i += kWalkThreads) a.sampled[b * a.stride_sampled + i] = -1;
   if (tid == 0) {
     state->stopped = 0;
     a.num_sampled[b] = count;
@@ -661,7 +675,7 @@ Split split_of(const eagle4_sample_tree_args& a) {
   s.chunks = static_cast<int>(e4::ceil_div(e4::ceil_div(static_cast<int64_t>(a.vocab) + vec - 1, vec), kChunk / vec));
   const int64_t stats = a.rows * s.chunks;
   s.masses_off = stats * 8;
-  s.state_off = s.masses_off + (a.probs != nullptr ? static_cast<int64_t>(a.num_reqs) * s.chunks * 8 : 0);
+  s.state_off = s.masses_off + (a.probs != nullptr ? static_cast<int64_t>(a.num_reqs) * s.chunks * kParts * 8 : 0);
   s.maxes_off = s.state_off + static_cast<int64_t>(a.num_reqs) * static_cast<int64_t>(sizeof(State));
   return s;
 }
@@ -681,11 +695,11 @@ int launch(const eagle4_sample_tree_args& a, hipStream_t s) {
   const int pairs = a.probs == nullptr ? 0 : (a.width - 1 < kPairs ? a.width - 1 : kPairs);
   if (stats > 0)
     sample_chunks<T><<<e4::ceil_div(stats, kWaves), kThreads, 0, s>>>(a, split);
-  sample_walk<T, Q><<<a.num_reqs, kThreads, 0, s>>>(a, split, 1, pairs == 0);
+  sample_walk<T, Q><<<a.num_reqs, kWalkThreads, 0, s>>>(a, split, 1, pairs == 0);
   if constexpr (Q::code >= 0) {
     for (int i = 1; i <= pairs; ++i) {
-      sample_residual<T, Q><<<dim3(e4::ceil_div(split.chunks, kWaves), a.num_reqs), kThreads, 0, s>>>(a, split);
-      sample_walk<T, Q><<<a.num_reqs, kThreads, 0, s>>>(a, split, 0, i == pairs);
+      sample_residual<T, Q><<<dim3(e4::ceil_div(split.chunks * kParts, kWaves), a.num_reqs), kThreads, 0, s>>>(a, split);
+      sample_walk<T, Q><<<a.num_reqs, kWalkThreads, 0, s>>>(a, split, 0, i == pairs);
     }
   }
   return E4_LAUNCH_STATUS();
