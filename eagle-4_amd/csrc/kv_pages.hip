@@ -8,7 +8,10 @@
 // only when the scale grows; a page that starts at or after the context starts afresh, whatever it held.
 //
 // Both directions are bound by HBM where there is much to move, and by one chain of dependent loads (lengths, page
-// table, rows, scale) where there is little.
+// table, rows, scale) where there is little. Measured (bf16 rows): 4 prompts of 8 heads x 128, K and V, written in 22 us (3.3
+// TB/s read and written, latency's more than HBM's: each wave's chain is five loads long, and 28 waves a CU hide most of
+// it); 64 rounds' accepted rows in 6.4 us, nearly all of it that chain and the launch; 8 long requests read in 35 us (5.6
+// TB/s, what a large copy reaches; with one chunk a lane in flight 56 us); one latent request in 5.4 us.
 
 #include "common.h"
 
@@ -343,6 +346,8 @@ int launch_write(const eagle4_write_kv_args& a, hipStream_t s) {
   const int64_t items = int64_t(pages) * a.heads * (a.value != nullptr ? 2 : 1);
   if (items > (int64_t(1) << 30)) return EAGLE4_NOT_COVERED;
   const dim3 grid(e4::ceil_div(items, 4), a.num_reqs);
+  // where a page's rows fit four chunks a lane, twice the waves fit a CU (72 registers instead of 108): 22.0 instead of
+  // 24.7 us for 4 prompts of 16 x 128 pages
   if (!vectors(a))
     write_kernel<T, 1, 4><<<grid, 256, 0, s>>>(a, pages);
   else if (int64_t(a.page) * a.dim <= 4 * 64 * 8)
