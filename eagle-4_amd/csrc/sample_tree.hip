@@ -15,10 +15,10 @@
 // comparison in 10^7, and of a flat row's running sums far more).
 //
 // Split: a wave takes 4096 elements of a row, a chunk. Three kinds of launches:
-//   - statistics: of every chunk of every row its maximum and its mass relative to that. All rows of all trees at once: the
-//     walk visits a few of them, but one after another, and a workgroup that reads its request's rows on its own has one
-//     CU's rate (vocabulary 151936, bf16: one tree of 16 rows 105 to 232 us that way, by the walk's length, against 19;
-//     64 trees of up to 16 rows 228 against 102);
+//   - statistics: of every chunk of a row its maximum and its mass relative to that. All rows of all trees at once, or the
+//     trees' first rows and later those that may still be visited: the walk visits a few of them, but one after another,
+//     and a workgroup that reads its request's rows on its own has one CU's rate (vocabulary 151936, bf16: one tree of
+//     16 rows 105 to 232 us that way, by the walk's length, against 19; 64 trees of up to 16 rows 228 against 85);
 //   - the walk, a workgroup per request: the rows' sums out of the chunks', then the decisions, a lane a child. Ends with the
 //     final token: the chunks' running sum leads to one chunk, which is read. With draft probabilities a rejection needs the
 //     residual's mass: the walk stops there and leaves its state;
@@ -28,7 +28,7 @@
 // for 16 trees of 16 over 151936. Continuing the walk in the residual's last workgroup instead of a launch of its own takes a
 // fence of every workgroup, and those cost more (95 us instead of 71). The walk's workgroup has 512 threads for those rows:
 // with 256, 89 us instead of 76 for the 12 trees; with 1024, 3% off the trees and 10% on single users' walks.
-// What bounds it: the statistics by their 64-bit operations (64 trees: 82 us for 750 rows, 44 of them the logits' own; a table
+// What bounds it: the statistics by their 64-bit operations (82 us for 750 rows, 44 of them the logits' own; a table
 // of 32 roots with a polynomial of degree 4 has a third fewer operations and is no faster for its lookups; one chunk
 // loaded ahead of another, 93 us), the walk by its chain of dependent loads (12 us for one request, 22 among 64).
 
@@ -172,14 +172,18 @@ E4_DEV double wave_sum(double x) {
 }
 
 constexpr int kMaxRows = 64;  // of a tree: a lane each
+constexpr int64_t kTwoSteps = 1 << 14;  // chunks of a launch
 constexpr int kPairs = 2;     // residual and walk launches behind the first walk
 constexpr int kThreads = 256, kWaves = kThreads / 64;
 constexpr int kWalkThreads = 512, kWalkWaves = kWalkThreads / 64;
 
-// A stopped walk. `count` rows are on its path, the last one `node`, whose child `child` was rejected last.
+// A stopped walk, `count` rows on its path. kForMass: the last one is `node`, whose child `child` was rejected last. kForRows:
+// it goes on with `node`; `rows` has a bit for it and for each of its descendants.
+constexpr int kForMass = 1, kForRows = 2;
 struct State {
   int32_t stopped, node, child, count;
   double spent;
+  uint64_t rows;
   float top;  // the row's maximum
 };
 
@@ -227,23 +231,12 @@ E4_DEV int wave_min(int x) {
 
 E4_DEV double scale_of(float temperature) { return 1.4426950408889634 / static_cast<double>(temperature); }
 
-// Maximum and mass of a chunk, a wave each. Where all mass is on one element (T = 0, a maximum of +inf or NaN) the place of
-// the sum holds the first index of the maximum.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void sample_chunks(const eagle4_sample_tree_args a, const Split s) {
-  constexpr int VEC = Row<T>::VEC, NV = kChunk / VEC / 64;
-  const int lane = threadIdx.x & 63;
-  const uint32_t id = blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const uint32_t n = id / static_cast<uint32_t>(s.chunks);
-  const int chunk = static_cast<int>(id - n * s.chunks);
-  if (n >= a.rows) return;
-  const Row<T> row(a.logits, n, a.stride_row, a.vocab);
-  u32x4 w[NV];
-  load_vectors<T, NV>(row, chunk * (64 * NV), lane, w);
-  const int b = __builtin_amdgcn_readfirstlane(request_of(a, n, lane));
-  if (b >= a.num_reqs || n - e4::ld(a.cu_num_logits, b) >= a.width) return;  // a row that no walk visits
-  const float temperature = a.temperature[b];
-
+// Maximum and mass of a chunk of row n, by one wave, from its vectors as loaded. Where all mass is on one element (T = 0, a
+// maximum of +inf or NaN) the place of the sum holds the first index of the maximum.
+template <typename T, int NV>
+E4_DEV void chunk_statistics(const eagle4_sample_tree_args& a, const Split& s, int64_t n, int chunk, const Row<T>& row,
+                             const u32x4 (&w)[NV], float temperature, int lane) {
+  constexpr int VEC = Row<T>::VEC;
   float x[NV][VEC];
   float m = -INFINITY;
 #pragma unroll
@@ -277,6 +270,42 @@ __global__ __launch_bounds__(kThreads) void sample_chunks(const eagle4_sample_tr
     const_cast<double*>(out.sums)[chunk] = sum;
     const_cast<float*>(out.maxes)[chunk] = m;
   }
+}
+
+// Of every row that a walk can visit.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void sample_chunks(const eagle4_sample_tree_args a, const Split s) {
+  constexpr int NV = kChunk / Row<T>::VEC / 64;
+  const int lane = threadIdx.x & 63;
+  const uint32_t id = blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t n = id / static_cast<uint32_t>(s.chunks);
+  const int chunk = static_cast<int>(id - n * s.chunks);
+  if (n >= a.rows) return;
+  const Row<T> row(a.logits, n, a.stride_row, a.vocab);
+  u32x4 w[NV];
+  load_vectors<T, NV>(row, chunk * (64 * NV), lane, w);
+  const int b = __builtin_amdgcn_readfirstlane(request_of(a, n, lane));
+  if (b >= a.num_reqs || n - e4::ld(a.cu_num_logits, b) >= a.width) return;  // a row that no walk visits
+  chunk_statistics<T, NV>(a, s, n, chunk, row, w, a.temperature[b], lane);
+}
+
+// Of the trees' first rows (first != 0), or of the rows that the stopped walks may still visit.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void sample_chunks_of(const eagle4_sample_tree_args a, const Split s, int first) {
+  constexpr int NV = kChunk / Row<T>::VEC / 64;
+  const int lane = threadIdx.x & 63, r = blockIdx.y, b = blockIdx.z;
+  const int chunk = blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (chunk >= s.chunks) return;
+  if (!first) {
+    const State* const st = reinterpret_cast<const State*>(static_cast<char*>(a.workspace) + s.state_off) + b;
+    if (st->stopped != kForRows || !(st->rows >> r & 1)) return;
+  }
+  const int64_t start = e4::ld(a.cu_num_logits, b), end = e4::ld(a.cu_num_logits, b + 1), n = start + r;
+  if (start < 0 || n >= end || end > a.rows) return;
+  const Row<T> row(a.logits, n, a.stride_row, a.vocab);
+  u32x4 w[NV];
+  load_vectors<T, NV>(row, chunk * (64 * NV), lane, w);
+  chunk_statistics<T, NV>(a, s, n, chunk, row, w, a.temperature[b], lane);
 }
 
 // The residual of a vector's elements out of its logits, times the row's total: off = -maximum c.
@@ -342,7 +371,7 @@ __global__ __launch_bounds__(kThreads) void sample_residual(const eagle4_sample_
   const int part = blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   char* const work = static_cast<char*>(a.workspace);
   const State st = reinterpret_cast<const State*>(work + s.state_off)[b];
-  if (st.stopped == 0 || part >= s.chunks * kParts) return;
+  if (st.stopped != kForMass || part >= s.chunks * kParts) return;
   const int64_t n = e4::ld(a.cu_num_logits, b) + st.node;
   const Row<T> row(a.logits, n, a.stride_row, a.vocab);
   const QRow<Q, Row<T>::VEC> qrow(a.probs, n, a.stride_prob, row.past);
@@ -355,7 +384,7 @@ __global__ __launch_bounds__(kThreads) void sample_residual(const eagle4_sample_
 // The walk. Every wave takes the decisions, lane j for row j of the tree; the waves part for the rows' sums and for the
 // final token's chunk.
 template <typename T, typename Q>
-__global__ __launch_bounds__(kWalkThreads) void sample_walk(const eagle4_sample_tree_args a, const Split s, int first, int last) {
+__global__ __launch_bounds__(kWalkThreads) void sample_walk(const eagle4_sample_tree_args a, const Split s, int first, int last, int roots) {
   constexpr int VEC = Row<T>::VEC, NV = (kChunk / VEC + kWalkThreads - 1) / kWalkThreads;  // vectors of a thread in the final token's chunk
   constexpr bool kProbs = Q::code >= 0;
   __shared__ float s_top[kMaxRows];
@@ -370,6 +399,7 @@ __global__ __launch_bounds__(kWalkThreads) void sample_walk(const eagle4_sample_
   double* const masses = masses_of(a, s, b);
   int node = 0, count = 0, resumed = 0;
   double spent = 0.0;
+  uint64_t have = roots ? 1 : ~0ull;  // rows whose statistics are there
   if (!first) {
     const State st = *state;
     if (st.stopped == 0) return;
@@ -377,6 +407,7 @@ __global__ __launch_bounds__(kWalkThreads) void sample_walk(const eagle4_sample_
     count = st.count;
     resumed = st.child;
     spent = st.spent;
+    if (st.stopped == kForRows) have = st.rows;
   }
 
   const int64_t slot = e4::ld(a.idx_mapping, b);
@@ -406,6 +437,7 @@ __global__ __launch_bounds__(kWalkThreads) void sample_walk(const eagle4_sample_
 
   // The rows' maxima and totals out of the chunks', 16 lanes a row; a row with all mass on one element: its index.
   for (int r = tid / 16; r < limit; r += kWalkThreads / 16) {
+    if (!(have >> r & 1)) continue;
     const Work w(a, s, start + r);
     const int l16 = lane & 15;
     float top = -INFINITY;  // the lane's chunks', then the row's
@@ -514,7 +546,7 @@ __global__ __launch_bounds__(kWalkThreads) void sample_walk(const eagle4_sample_
       if constexpr (kProbs) {
         spent += mass;
         if (!last) {
-          if (tid == 0) *state = State{1, node, j, count, spent, top};
+          if (tid == 0) *state = State{kForMass, node, j, count, spent, 0, top};
           return;
         }
         __syncthreads();  // the last masses have been read
@@ -532,6 +564,15 @@ __global__ __launch_bounds__(kWalkThreads) void sample_walk(const eagle4_sample_
     if (next >= 0) {
       out_token(__shfl(token, next, 64));
       node = next;
+      if (!(have >> node & 1)) {
+        uint64_t under = 1ull << node, before = 0;
+        while (under != before) {
+          before = under;
+          under |= __ballot(lane > 0 && lane < limit && parent >= 0 && parent < limit && (before >> parent & 1));
+        }
+        if (tid == 0) *state = State{kForRows, node, 0, count, 0.0, under, 0.f};
+        return;
+      }
       continue;
     }
 
@@ -693,13 +734,26 @@ int launch(const eagle4_sample_tree_args& a, hipStream_t s) {
   const int64_t stats = a.rows * split.chunks;
   if (stats >= 1 << 25) return EAGLE4_NOT_COVERED;  // 64 threads each: under 2^32
   const int pairs = a.probs == nullptr ? 0 : (a.width - 1 < kPairs ? a.width - 1 : kPairs);
-  if (stats > 0)
+  // Without draft probabilities a walk of many rows goes in two: the trees' first rows, then what is left of each tree under
+  // the child that was accepted. Two launches more, but a fraction of the rows (64 requests, vocabulary 151936, trees of
+  // 16, 39000 chunks: 95 instead of 135 us; trees of 8, 19000: 76 and 79; 16 requests, trees of 16, 9700: 58 and 51).
+  const bool two = a.probs == nullptr && a.width > 1 && stats >= kTwoSteps;
+  const auto chunks_of = [&](int rows, int first) {
+    sample_chunks_of<T><<<dim3(e4::ceil_div(split.chunks, kWaves), rows, a.num_reqs), kThreads, 0, s>>>(a, split, first);
+  };
+  if (two)
+    chunks_of(1, 1);
+  else if (stats > 0)
     sample_chunks<T><<<e4::ceil_div(stats, kWaves), kThreads, 0, s>>>(a, split);
-  sample_walk<T, Q><<<a.num_reqs, kWalkThreads, 0, s>>>(a, split, 1, pairs == 0);
+  sample_walk<T, Q><<<a.num_reqs, kWalkThreads, 0, s>>>(a, split, 1, pairs == 0, two);
+  if (two) {
+    chunks_of(a.width, 0);
+    sample_walk<T, Q><<<a.num_reqs, kWalkThreads, 0, s>>>(a, split, 0, 1, 0);
+  }
   if constexpr (Q::code >= 0) {
     for (int i = 1; i <= pairs; ++i) {
       sample_residual<T, Q><<<dim3(e4::ceil_div(split.chunks * kParts, kWaves), a.num_reqs), kThreads, 0, s>>>(a, split);
-      sample_walk<T, Q><<<a.num_reqs, kWalkThreads, 0, s>>>(a, split, 0, i == pairs);
+      sample_walk<T, Q><<<a.num_reqs, kWalkThreads, 0, s>>>(a, split, 0, i == pairs, 0);
     }
   }
   return E4_LAUNCH_STATUS();

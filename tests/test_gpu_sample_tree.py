@@ -231,3 +231,15 @@ def test_streams_and_graphs(dev):
         torch.cuda.synchronize()
         check(x, (sampled, count, store))
         launch(x, dev)  # eager work between the replays
+
+
+@pytest.mark.parametrize("requests,width,vocab,dtype", [(2300, 8, 40, F32), (220, 8, 45000, BF16)])
+def test_many_rows(dev, requests, width, vocab, dtype):
+    """Batches of more than 2^14 pieces of rows: the trees' first rows are read before the rest."""
+    announce(f"sample tree {requests} requests of up to {width} rows, vocab {vocab} {dtype}")
+    x = inputs([0 if b % 40 == 7 else 1 + b % 3 if b % 20 == 3 else width for b in range(requests)], width, vocab, dtype, None, seed=9)
+    x["temperature"][::9] = 0.0
+    x["parents"][x["slots"][5].long(), 2:] = torch.tensor([0, 7, 1, 2, 3, 40][: width - 2], dtype=torch.int32)  # no tree
+    chunks = -(-(vocab + 7) // 4096) * int(x["cu"][-1])
+    assert chunks >= 1 << 14
+    check(x, launch(x, dev))
