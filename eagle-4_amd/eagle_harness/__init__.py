@@ -6,8 +6,9 @@ signatures:
 - ``eagle_harness.kernels``: ``gdn_tree`` (tree tables), ``gdn_tree_conv``, ``gdn_tree_recurrence``,
   ``gdn_tree_records``, ``accept_tail``, ``verify_prep``, ``row_attention``, ``mamba2_tree``;
 - ``eagle_harness.vllm``: ``verify_attention``, ``verify_layout`` (the verify stage), ``tree_attention`` (the CUSTOM
-  backend), ``tree_accept`` (the greedy walk), ``gdn_tree_verify`` (the layer hook and the accepted-path state
-  commit) and ``round_commit``.
+  backend), ``tree_accept`` (the greedy and the sampled walk), ``gdn_tree_verify`` (the layer hook and the
+  accepted-path state commit) and ``round_commit``; ``latent_attention`` and ``kv_pages`` (verify attention over latent rows,
+  fp8 pages written and read) are this package's own.
 
 Every launch of these modules goes to hand-written gfx950 HIP kernels in ``kernels/libeagle4_amd.so`` through a plain
 C ABI; nothing here falls back to another implementation.

@@ -14,8 +14,9 @@
  * no fallback path: "not covered" is an error for the caller.
  *
  * The library never allocates and never synchronises: launches are asynchronous on `stream` (a hipStream_t), read
- * and write only caller-owned memory, and can be captured in a HIP graph. The one scratch buffer (verify attention's
- * split partials) is passed in by the caller; eagle4_verify_attention_workspace() gives its size.
+ * and write only caller-owned memory, and can be captured in a HIP graph. Scratch buffers (verify and latent attention's
+ * split partials, the sampled walk's row statistics) are passed in by the caller; eagle4_verify_attention_workspace(),
+ * eagle4_latent_attention_workspace() and eagle4_sample_tree_workspace() give their sizes.
  *
  * dtype codes follow the reference's (candidate.cu:566): 0 bfloat16, 1 float16, 2 float32; then 3 float8_e4m3fn
  * (OCP), 4 int32, 5 int64, 6 uint8/bool.
