@@ -184,3 +184,16 @@ def test_the_library_refuses_what_reaches_it():
     for over in (dict(key=0), dict(num_blocks=-1), dict(dtype=5), dict(value=16), dict(num_reqs=70000)):
         assert lib.eagle4_read_kv_pages(_native.ReadKvArgs(**{**kv, **over}), None) == -1, over
     assert lib.eagle4_read_kv_pages(_native.ReadKvArgs(**{**kv, "max_len": 0}), None) == 0
+
+
+def test_capacities_near_the_positions_limit():
+    """Tables whose pages reach up to 2^31 positions leave no room for the tiles that are looked up ahead."""
+    from eagle_harness.kernels import _native
+
+    lib, tab = _native.library(), _native.itab(torch.zeros(4, 4, dtype=I32))
+    args = dict(q=16, latent_new=16, cache=16, out=16, workspace=16, workspace_bytes=1 << 40, block_table=tab, context_lens=tab,
+                query_start_loc=tab, masks=16, num_reqs=1, heads=16, rank=512, rope=64, max_query_len=1, num_blocks=4)
+    for page, blocks, ok in ((1 << 16, (1 << 15) - 1, True), (1, (1 << 31) - 2049, True), (1, (1 << 31) - 2048, False),
+                             (1 << 16, 1 << 15, False)):
+        need = lib.eagle4_latent_attention_workspace(_native.LatentAttnArgs(**args, page=page, max_blocks=blocks))
+        assert (need > 0) == ok, (page, blocks)
