@@ -333,7 +333,7 @@ bool vectors(const A& a) {
 
 template <typename A>
 bool pages_ok(const A& a) {
-  return a.key != nullptr && a.key_cache != nullptr && a.k_scale != nullptr &&
+  return (a.key != nullptr || a.tokens == 0) && a.key_cache != nullptr && a.k_scale != nullptr &&
          (a.value == nullptr || (a.value_cache != nullptr && a.v_scale != nullptr)) && tab_ok(a.block_table) &&
          a.heads > 0 && a.dim > 0 && a.page > 0 && a.max_blocks >= 0 && a.num_blocks >= 0 && a.num_reqs <= 65535 &&
          int64_t(a.heads) * a.dim <= (1 << 20) && int64_t(a.dim) * a.page <= (1 << 24);

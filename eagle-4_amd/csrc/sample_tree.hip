@@ -783,9 +783,11 @@ extern "C" int64_t eagle4_sample_tree_workspace(const eagle4_sample_tree_args* a
 
 extern "C" int eagle4_sample_tree(const eagle4_sample_tree_args* a, void* stream) {
   if (a->num_reqs == 0) return EAGLE4_OK;
-  if (!covered(a) || a->workspace == nullptr || a->workspace_bytes < workspace_of(*a) || !tab_ok(a->drafted) ||
-      !tab_ok(a->cu_num_logits) || !tab_ok(a->idx_mapping) || !tab_ok(a->parents) || a->coins == nullptr || a->final_coins == nullptr || a->temperature == nullptr || a->logits == nullptr)
+  if (!covered(a) || a->workspace == nullptr || a->workspace_bytes < workspace_of(*a) || !tab_ok(a->cu_num_logits) ||
+      !tab_ok(a->idx_mapping) || !tab_ok(a->parents) || a->final_coins == nullptr || a->temperature == nullptr)
     return EAGLE4_NOT_COVERED;
+  // (of no rows nothing is read)
+  if (a->rows > 0 && (a->logits == nullptr || a->coins == nullptr || !tab_ok(a->drafted))) return EAGLE4_NOT_COVERED;
   const hipStream_t s = static_cast<hipStream_t>(stream);
   switch (a->dtype) {
     case EAGLE4_BF16: return launch_t<e4::Bf16>(*a, s);

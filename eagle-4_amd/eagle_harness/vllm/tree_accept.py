@@ -5,6 +5,9 @@ from the root to the lowest-index child whose draft token equals the current nod
 child; the accepted rows are the path (root first) and the sampled tokens are the path rows' target tokens, the last
 of which is the bonus token.
 
+Where the target samples, :func:`sample_tree` takes that walk's place: it accepts children and draws the bonus token so that
+every token is distributed as the target's own.
+
 The reference's module also holds ``TreeRejectionSampler``, vLLM's rejection sampler with the chain rule replaced by
 the tree walk (engine glue: it applies the engine's sampling parameters and Gumbel sampling, then calls
 :func:`accept_tree`). It is not rewritten here: importing ``TreeRejectionSampler`` from this module runs the installed

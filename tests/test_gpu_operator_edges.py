@@ -133,3 +133,18 @@ def test_empty_batches(dev):
     z["starts"] = torch.zeros(1, dtype=torch.int32)
     got = kv.write(z, dev)
     assert kv.same(got[0], z["cache"]) and torch.equal(got[1].cpu(), z["scale"])
+
+
+def test_batches_of_no_rows(dev):
+    """Requests, but no row among them: the walks are empty, pages and scales stay."""
+    announce("batches of no rows")
+    y = st.inputs([0, 0], 4, 50, F32, F32, seed=42)
+    st.check(y, st.launch(y, dev))
+    z = kv.batch([5, 40], [0, 0], 4, 128, 16, BF16, seed=43)
+    got = kv.write(z, dev)
+    assert kv.same(got[0], z["cache"]) and torch.equal(got[1].cpu(), z["scale"])
+    from eagle_harness.vllm.kv_pages import read_kv_pages
+
+    out = torch.empty(0, 4, 128, dtype=BF16, device=dev)
+    read_kv_pages(z["cache"].to(dev), None, z["scale"].to(dev), None, z["table"].to(dev), z["starts"].to(dev), out, None,
+                  max_len=8)
