@@ -24,9 +24,8 @@
 // the products are 1100 and their operands' LDS reads about as much; the rest is the barrier (250 to 650), the exchange of
 // weights and the lookups (900 to 1600, with the lookups of each tile on their own instead of four tiles at once: 281 us).
 // 128 requests of 4 tokens, 16 heads, fp8 pages: 177 us; widening the codes is a fourth of a tile. 64 single tokens of 16
-// heads: 68 us, 4.5 TB/s. One token of 128 heads over 2048 keys: 35 us, a chain of lookups, queries and first tiles
-// (15000 cycles), four tiles a workgroup, the partials (7000), and 6 us of merge. Queries loaded by each lane on its own, 16
-// bytes of every row: 41 us.
+// heads: 68 us, 4.5 TB/s. One token of 128 heads over 2048 keys: 26 us, a chain of lookups, queries and first tiles, two tiles
+// a workgroup, the partials, and 6 us of merge. Queries loaded by each lane on its own, 16 bytes of every row: 6 us more.
 
 #include "attention_tile.h"
 
@@ -759,9 +758,16 @@ bool covered(const eagle4_latent_attn_args& a) {
   return true;
 }
 
+// Query rows of a workgroup: 64 share a tile's loads best, but where the tables leave at most two such tiles a workgroup, 16
+// rows spread the work over more of them, with less to bring in, to leave and to merge (RANK 512; the tiles of 64 rows, the
+// times with 64 and 16: one token of 128 heads over 2048 keys, 128 tiles: 36.7 and 26.2 us; 8192 keys, 512: 47.1 and 36.0;
+// 16384 keys, 1024: 52.2 and 46.2; 32768 keys, 2048: 60.8 and 66.4; 4 trees of 16 x 16 heads over 512 keys, 256: 36.3 and
+// 27.0; over 2048 keys, 1024: 34.1 and 40.6).
 int rows_of(const eagle4_latent_attn_args& a) {
   const int rows = a.max_query_len * a.heads;
-  return rows <= 16 ? 16 : (rows <= 32 ? 32 : 64);
+  if (rows <= 32) return rows <= 16 ? 16 : 32;
+  const int64_t tiles = (static_cast<int64_t>(a.max_blocks) * a.page + kKeys - 1) / kKeys;
+  return a.num_reqs * ((rows + 63) / 64) * tiles <= 2 * kGroups ? 16 : 64;
 }
 
 // The requests that one launch takes: their tiles (at the most that the tables' sizes allow) are counted in 31 bits.
@@ -776,7 +782,7 @@ LatentPlan plan(const eagle4_latent_attn_args& a) {
   LatentPlan p;
   p.rows = rows_of(a);
   p.groups = kGroups;
-  p.least = 4;
+  p.least = 2;  // against 4: 16 requests of 4 x 16 rows over 1024 keys 39.4 -> 31.3 us, nothing where runs are longer
   p.first = 0;
   p.page_shift = (a.page & (a.page - 1)) == 0 ? __builtin_ctz(a.page) : -1;
   p.page_inv = a.page > 1 ? static_cast<uint32_t>((uint64_t(1) << 32) / a.page) : 0;
