@@ -148,3 +148,47 @@ def test_batches_of_no_rows(dev):
     out = torch.empty(0, 4, 128, dtype=BF16, device=dev)
     read_kv_pages(z["cache"].to(dev), None, z["scale"].to(dev), None, z["table"].to(dev), z["starts"].to(dev), out, None,
                   max_len=8)
+
+
+@pytest.fixture
+def wide_tables(monkeypatch):
+    """Inputs whose tables could hold contexts far longer than they do: what the tables allow decides how many query rows a
+    workgroup takes, so these run the forms of long contexts on the short ones of the tests."""
+    plain = lat.inputs
+
+    def padded(*args, page=16, **kw):
+        x = plain(*args, page=page, **kw)
+        more = torch.zeros(x["table"].shape[0], -(-1100 * 32 // page), dtype=torch.int32)
+        return dict(x, table=torch.cat([x["table"], more], 1))
+
+    monkeypatch.setattr(lat, "inputs", padded)
+
+
+@pytest.mark.parametrize("rank", [512, 256])
+@pytest.mark.parametrize("dtype,cache", [(BF16, "same"), (F16, "same"), (BF16, "fp8"), (F16, "fp8")])
+@pytest.mark.parametrize("heads,sizes", [(16, [3, 4, 1]), (5, [7, 16, 2]), (16, [16, 9, 12]), (128, [1, 1, 1])])
+def test_long_tables(dev, wide_tables, rank, dtype, cache, heads, sizes):
+    lat.test_rows_match_the_oracle(dev, rank, dtype, cache, heads, sizes)
+
+
+@pytest.mark.parametrize("cache", ["same", "fp8"])
+def test_long_tables_of_any_context(dev, wide_tables, cache):
+    for context in (0, 1, 31, 32, 33, 64, 95, 127, 129, 300):
+        lat.test_context_lengths(dev, context, cache)
+    for page in (1, 3, 24, 100):
+        lat.test_page_sizes(dev, page, cache)
+    for sizes in ([64, 33], [40, 64], [32, 1]):
+        lat.test_wide_trees(dev, sizes, cache)
+    test_trees_of_two_tiles_behind_any_context(dev, cache, 512)
+    for value in (float("nan"), float("inf")):
+        lat.test_values_that_are_not_finite_reach_only_rows_that_see_them(dev, value, cache)
+
+
+def test_long_tables_of_every_other_kind(dev, wide_tables):
+    lat.test_scales_of_any_value_and_size(dev)
+    lat.test_masks_that_leave_nothing(dev)
+    lat.test_pages_outside_the_cache_are_not_seen(dev)
+    lat.test_rows_behind_the_last_request_stay(dev)
+    lat.test_strided_operands(dev)
+    lat.test_large_scores(dev)
+    lat.test_streams_and_graphs(dev)
