@@ -650,7 +650,6 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
       if (i < tiles) {
         const uint64_t next_row = row_of(i + 2);
         bits = s_vis[i / kBatch % 2][i % kBatch];
-        lookup(i);
         const Loads to = prepare_next(i + 2, next_row);
         if (!is_ctx(i)) {
           const uint32_t poison = clean(i);
@@ -663,6 +662,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
           if (c % 2 == 1 && c / 2 < kLoads) load_next(to, c / 2);
         });
         if (more) load_next(to, kLoads);
+        lookup(i);
         if constexpr (FP8) next_rows(i + 1);
       }
       const int ln = fresh(lane);
