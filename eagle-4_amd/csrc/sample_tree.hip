@@ -165,11 +165,31 @@ struct QRow {
   }
 };
 
-E4_DEV double wave_sum(double x) {
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) x += __shfl_xor(x, m, 64);
-  return x;
+// A value of another lane of the same 16, by a DPP pattern; of 64 bits in two halves.
+template <int kCtrl>
+E4_DEV double dpp64(double x) {
+  const uint64_t w = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = __builtin_amdgcn_mov_dpp(static_cast<int>(w), kCtrl, 0xF, 0xF, true);
+  const uint32_t hi = __builtin_amdgcn_mov_dpp(static_cast<int>(w >> 32), kCtrl, 0xF, 0xF, true);
+  return __builtin_bit_cast(double, (static_cast<uint64_t>(hi) << 32) | lo);
 }
+// The sum with lane ^ 16 or lane ^ 32: swaps of rows of lanes.
+template <int N>
+E4_DEV double add_row(double x) {
+  const uint64_t w = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = static_cast<uint32_t>(w), hi = static_cast<uint32_t>(w >> 32);
+  const auto a = N == 16 ? __builtin_amdgcn_permlane16_swap(lo, lo, false, false) : __builtin_amdgcn_permlane32_swap(lo, lo, false, false);
+  const auto b = N == 16 ? __builtin_amdgcn_permlane16_swap(hi, hi, false, false) : __builtin_amdgcn_permlane32_swap(hi, hi, false, false);
+  return __builtin_bit_cast(double, (static_cast<uint64_t>(b[0]) << 32) | a[0]) +
+         __builtin_bit_cast(double, (static_cast<uint64_t>(b[1]) << 32) | a[1]);
+}
+E4_DEV double sum16(double x) {  // over the 16 lanes of a row: lane ^ 1, ^ 2, the other quad, the other eight
+  x += dpp64<0xB1>(x);
+  x += dpp64<0x4E>(x);
+  x += dpp64<0x141>(x);
+  return x + dpp64<0x140>(x);
+}
+E4_DEV double wave_sum(double x) { return add_row<32>(add_row<16>(sum16(x))); }
 
 constexpr int kMaxRows = 64;  // of a tree: a lane each
 constexpr int64_t kTwoSteps = 1 << 14;  // chunks of a launch
@@ -214,10 +234,18 @@ E4_DEV int request_of(const eagle4_sample_tree_args& a, int64_t row, int lane) {
   return lo;
 }
 
-E4_DEV float wave_max(float x) {  // NaN the largest
-#pragma unroll
-  for (int k = 1; k < 64; k <<= 1) x = __builtin_elementwise_maximum(x, __shfl_xor(x, k, 64));
-  return x;
+E4_DEV float max16(float x) {  // NaN the largest
+  x = __builtin_elementwise_maximum(x, e4::dpp<0xB1>(x));
+  x = __builtin_elementwise_maximum(x, e4::dpp<0x4E>(x));
+  x = __builtin_elementwise_maximum(x, e4::dpp<0x141>(x));
+  return __builtin_elementwise_maximum(x, e4::dpp<0x140>(x));
+}
+E4_DEV float wave_max(float x) {
+  const uint32_t w = __float_as_uint(max16(x));
+  const auto a = __builtin_amdgcn_permlane16_swap(w, w, false, false);
+  const uint32_t v = __float_as_uint(__builtin_elementwise_maximum(__uint_as_float(a[0]), __uint_as_float(a[1])));
+  const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return __builtin_elementwise_maximum(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
 E4_DEV int wave_min(int x) {
@@ -458,8 +486,7 @@ __global__ __launch_bounds__(kWalkThreads) void sample_walk(const eagle4_sample_
       top = most;
     }
     const float mine = top;
-#pragma unroll
-    for (int k = 1; k < 16; k <<= 1) top = __builtin_elementwise_maximum(top, __shfl_xor(top, k, 64));
+    top = max16(top);
     if (greedy || !(__builtin_fabsf(top) < INFINITY)) {
       int at = INT32_MAX;  // its first chunk's; a row of -inf: 0
       for (int k = l16; k < s.chunks; k += 16)
@@ -472,8 +499,7 @@ __global__ __launch_bounds__(kWalkThreads) void sample_walk(const eagle4_sample_
       total = top == -INFINITY ? 0.0 : w.sums[at];
     } else {
       total *= exp2_64((static_cast<double>(mine) - static_cast<double>(top)) * c);
-#pragma unroll
-      for (int k = 1; k < 16; k <<= 1) total += __shfl_xor(total, k, 64);
+      total = sum16(total);
     }
     if (l16 == 0) {
       s_top[r] = top;
