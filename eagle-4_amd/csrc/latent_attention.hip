@@ -687,12 +687,22 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
     const float inv = sum == 0.f ? 0.f : 1.0f / sum;  // nothing seen: zeros
     int rho, t, head;
     const bool ok = my_row(rho, t, head);
-    if (ok && whole) {
+    if (whole) {
       uint16_t* const o = static_cast<uint16_t*>(a.out) + (u.start + t) * a.stride_ot + head * a.stride_oh + dbase;
+      // Two column tiles at a time: rows of lanes swapped, a lane has 8 adjacent columns of one of them (16 bytes a store).
 #pragma unroll
-      for (int dt = 0; dt < S::DT; ++dt)
-        *reinterpret_cast<u32x2_t*>(o + 16 * dt + 4 * g) =
-            u32x2_t{pack2<T>(acc[dt][0] * inv, acc[dt][1] * inv), pack2<T>(acc[dt][2] * inv, acc[dt][3] * inv)};
+      for (int dt = 0; dt < S::DT; dt += 2) {
+        uint32_t w[2][2];  // [half of a lane's columns][word]
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const auto r = __builtin_amdgcn_permlane16_swap(pack2<T>(acc[dt][2 * k] * inv, acc[dt][2 * k + 1] * inv),
+                                                          pack2<T>(acc[dt + 1][2 * k] * inv, acc[dt + 1][2 * k + 1] * inv),
+                                                          false, false);
+          w[0][k] = r[0];
+          w[1][k] = r[1];
+        }
+        if (ok) *reinterpret_cast<u32x4_t*>(o + 16 * (dt + (g & 1)) + 8 * (g >> 1)) = u32x4_t{w[0][0], w[0][1], w[1][0], w[1][1]};
+      }
     } else if (ok) {
       const int64_t part = (2 * static_cast<int64_t>(wg) + (t0 == 0 ? 1 : 0)) * S::ROWS + rho - rg * S::ROWS;
       float* const o = a.workspace + p.part_off + part * RANK + dbase;
