@@ -531,20 +531,24 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
 
     __syncthreads();  // the last piece's tiles have been read
     // The queries come in through the last two tiles' place, whole lines once for all waves: a lane's own loads would be 16
-    // bytes of every row, twice. 8 rows x 64 columns an instruction, in the layout of a tile.
+    // bytes of every row, twice. 8 rows x 64 columns an instruction, in the layout of a tile. Waves 4-7 have these loads, as
+    // waves 0-3 have the lookups, whose waits would take them in.
     char* const s_q = smem[S::NBUF - 2];
     static_assert(S::KC / 2 * S::ROWS * 128 <= 2 * S::TILE, "the queries' place");
-    {
-      const int ln = fresh(lane), row = 8 * (wave % (2 * RW)) + (ln >> 3), rho = rg * S::ROWS + row;
-      const bool ok = rho < u.width * a.heads;
-      const int t = ok ? rho / a.heads : 0, head = ok ? rho - t * a.heads : 0;
-      const char* const src = ok ? reinterpret_cast<const char*>(static_cast<const uint16_t*>(a.q) + (u.start + t) * a.stride_qt +
-                                                                 head * a.stride_qh)
-                                 : reinterpret_cast<const char*>(zero_row);
-      const int chunk = 16 * ((ln & 7) ^ swz(row % kKeys));
-      const uint32_t dst = uniform(lds_addr(s_q) + 1024 * (wave % (2 * RW)));
+    if (second_half) {
 #pragma unroll 1
-      for (int cb = wave / (2 * RW); cb < S::KC / 2; cb += 4 / RW) dma16(src + 128 * cb + chunk, dst + cb * S::ROWS * 128);
+      for (int part = wave - 4; part < 2 * RW; part += 4) {
+        const int ln = fresh(lane), row = 8 * part + (ln >> 3), rho = rg * S::ROWS + row;
+        const bool ok = rho < u.width * a.heads;
+        const int t = ok ? rho / a.heads : 0, head = ok ? rho - t * a.heads : 0;
+        const char* const src = ok ? reinterpret_cast<const char*>(static_cast<const uint16_t*>(a.q) +
+                                                                   (u.start + t) * a.stride_qt + head * a.stride_qh)
+                                   : reinterpret_cast<const char*>(zero_row);
+        const int chunk = 16 * ((ln & 7) ^ swz(row % kKeys));
+        const uint32_t dst = uniform(lds_addr(s_q) + 1024 * part);
+#pragma unroll 1
+        for (int cb = 0; cb < S::KC / 2; ++cb) dma16(src + 128 * cb + chunk, dst + cb * S::ROWS * 128);
+      }
     }
     if (tid < 2 * kBatchKeys) {  // batches 0 and 1
       const int n = tid / kBatchKeys, i = tid % kBatchKeys;
@@ -554,7 +558,6 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
       if (FP8 && blk >= 0 && blk < a.num_blocks) scale = a.scale_page[blk * a.stride_sp];
       fill(n, i, blk, scale);
     }
-    wait_vm<0>();
     __syncthreads();
 #pragma unroll 1
     for (int i = 0; i < 2; ++i) load_all(prepare_next(i, row_of(i)));
@@ -562,6 +565,9 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
       wait_vm<0>();
       __syncthreads();
       next_rows(0);
+    } else {  // the queries are there; the two tiles may be on their way
+      if (second_half) wait_vm<2 * S::CB1>();
+      __syncthreads();
     }
     // Waits until tile i (fp8: the codes of the one after it too) is there for every wave, the last tile's weights too; the
     // buffer of the tile before that is free.
