@@ -19,12 +19,12 @@
 // lengths fill the chip. A row group cut by a run's end leaves normalised fp32 partials with their log2-sum-exps (at most two
 // a workgroup), which a second kernel merges.
 //
-// Measured (RANK 512, ROPE 64, graph replays). 64 trees of up to 16 tokens, 16 heads, contexts of 1024 to 8192, bf16: 234 us,
+// Measured (RANK 512, ROPE 64, graph replays). 64 trees of up to 16 tokens, 16 heads, contexts of 1024 to 8192, bf16: 233 us,
 // 500 TFLOP/s; four waves that each take all scores of their rows: 455. A tile of 64 rows costs about 3300 cycles, of which
 // the products are 1100 and their operands' LDS reads about as much; the rest is the barrier (250 to 650), the exchange of
 // weights and the lookups (900 to 1600, with the lookups of each tile on their own instead of four tiles at once: 281 us).
-// 128 requests of 4 tokens, 16 heads, fp8 pages: 177 us; widening the codes is a fourth of a tile. 64 single tokens of 16
-// heads: 68 us, 4.5 TB/s. One token of 128 heads over 2048 keys: 26 us, a chain of lookups, queries and first tiles, two tiles
+// 128 requests of 4 tokens, 16 heads, fp8 pages: 172 us; widening the codes is a fourth of a tile. 64 single tokens of 16
+// heads: 67 us, 4.5 TB/s. One token of 128 heads over 2048 keys: 25 us, a chain of lookups, queries and first tiles, two tiles
 // a workgroup, the partials, and 6 us of merge. Queries loaded by each lane on its own, 16 bytes of every row: 6 us more.
 
 #include "attention_tile.h"
