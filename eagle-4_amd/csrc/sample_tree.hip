@@ -258,6 +258,12 @@ E4_DEV int wave_min(int x) {
 }
 
 E4_DEV double scale_of(float temperature) { return 1.4426950408889634 / static_cast<double>(temperature); }
+// exp2((x - top) c), exactly 1 at the maximum: the difference of two logits is taken before it is scaled. (One fma of x c and
+// a rounded -top c would be an operation less, but its error is 2^-53 of |top| c: from 2^53 on, as with logits of a type's
+// lowest value or temperatures below 1e-15, that is no error but the result.)
+E4_DEV double weight_of(float x, float top, double c) {
+  return exp2_64((static_cast<double>(x) - static_cast<double>(top)) * c);
+}
 
 // Maximum and mass of a chunk of row n, by one wave, from its vectors as loaded. Where all mass is on one element (T = 0, a
 // maximum of +inf or NaN) the place of the sum holds the first index of the maximum.
@@ -286,11 +292,11 @@ E4_DEV void chunk_statistics(const eagle4_sample_tree_args& a, const Split& s, i
       }
     sum = wave_min(at);
   } else {
-    const double c = scale_of(temperature), off = -static_cast<double>(m) * c;
+    const double c = scale_of(temperature);
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) sum += exp2_64(__builtin_fma(static_cast<double>(x[i][k]), c, off));
+      for (int k = 0; k < VEC; ++k) sum += weight_of(x[i][k], m, c);
     sum = wave_sum(sum);
   }
   if (lane == 0) {
@@ -336,21 +342,21 @@ __global__ __launch_bounds__(kThreads) void sample_chunks_of(const eagle4_sample
   chunk_statistics<T, NV>(a, s, n, chunk, row, w, a.temperature[b], lane);
 }
 
-// The residual of a vector's elements out of its logits, times the row's total: off = -maximum c.
+// The residual of a vector's elements out of its logits, times the row's total; `top` is the row's maximum.
 template <typename Q, int VEC>
-E4_DEV void residual(const float (&x)[VEC], const QRow<Q, VEC>& qrow, int first, int vocab, double c, double off, double spent,
+E4_DEV void residual(const float (&x)[VEC], const QRow<Q, VEC>& qrow, int first, int vocab, double c, float top, double spent,
                      double (&r)[VEC]) {
   if constexpr (Q::code >= 0) {
     float q[VEC];
     if (spent > 0.0) qrow.load(first, vocab, q);
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
-      r[i] = exp2_64(__builtin_fma(static_cast<double>(x[i]), c, off));
+      r[i] = weight_of(x[i], top, c);
       if (spent > 0.0) r[i] = __builtin_fmax(r[i] - spent * static_cast<double>(q[i]), 0.0);
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) r[i] = exp2_64(__builtin_fma(static_cast<double>(x[i]), c, off));
+    for (int i = 0; i < VEC; ++i) r[i] = weight_of(x[i], top, c);
   }
 }
 
@@ -372,7 +378,7 @@ E4_DEV void take_out(float (&x)[VEC], int first, uint64_t gone, int token) {
 // The mass of it in 64 NV vectors from v0 on, by one wave; their loads are in flight together. `gone`: the lanes whose `token`
 // is taken out.
 template <typename T, typename Q, int NV>
-E4_DEV double residual_mass(const Row<T>& row, const QRow<Q, Row<T>::VEC>& qrow, int v0, double c, double off, double spent,
+E4_DEV double residual_mass(const Row<T>& row, const QRow<Q, Row<T>::VEC>& qrow, int v0, double c, float top, double spent,
                             int lane, uint64_t gone, int token) {
   constexpr int VEC = Row<T>::VEC;
   u32x4 w[NV];
@@ -385,7 +391,7 @@ E4_DEV double residual_mass(const Row<T>& row, const QRow<Q, Row<T>::VEC>& qrow,
     Row<T>::widen(w[i], x);
     if constexpr (Q::code < 0) take_out<VEC>(x, first, gone, token);
     double r[VEC];
-    residual<Q, VEC>(x, qrow, first, row.vocab, c, off, spent, r);
+    residual<Q, VEC>(x, qrow, first, row.vocab, c, top, spent, r);
 #pragma unroll
     for (int k = 0; k < VEC; ++k) sum += r[k];
   }
@@ -404,8 +410,7 @@ __global__ __launch_bounds__(kThreads) void sample_residual(const eagle4_sample_
   const Row<T> row(a.logits, n, a.stride_row, a.vocab);
   const QRow<Q, Row<T>::VEC> qrow(a.probs, n, a.stride_prob, row.past);
   const double c = scale_of(a.temperature[b]);
-  const double off = -static_cast<double>(st.top) * c;
-  const double mass = residual_mass<T, Q, kPart / VEC / 64>(row, qrow, part * (kPart / VEC), c, off, st.spent, lane, 0, 0);
+  const double mass = residual_mass<T, Q, kPart / VEC / 64>(row, qrow, part * (kPart / VEC), c, st.top, st.spent, lane, 0, 0);
   if (lane == 0) masses_of(a, s, b)[part] = mass;
 }
 
@@ -480,9 +485,9 @@ __global__ __launch_bounds__(kWalkThreads) void sample_walk(const eagle4_sample_
         sum[i] = in ? w.sums[k0 + 16 * i] : 0.0;
         most = __builtin_elementwise_maximum(most, m[i]);
       }
-      total *= exp2_64((static_cast<double>(top) - static_cast<double>(most)) * c);
+      total *= weight_of(top, most, c);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) total += sum[i] * exp2_64((static_cast<double>(m[i]) - static_cast<double>(most)) * c);
+      for (int i = 0; i < 4; ++i) total += sum[i] * weight_of(m[i], most, c);
       top = most;
     }
     const float mine = top;
@@ -498,7 +503,7 @@ __global__ __launch_bounds__(kWalkThreads) void sample_walk(const eagle4_sample_
       }
       total = top == -INFINITY ? 0.0 : w.sums[at];
     } else {
-      total *= exp2_64((static_cast<double>(mine) - static_cast<double>(top)) * c);
+      total *= weight_of(mine, top, c);
       total = sum16(total);
     }
     if (l16 == 0) {
@@ -507,9 +512,8 @@ __global__ __launch_bounds__(kWalkThreads) void sample_walk(const eagle4_sample_
     }
   }
   __syncthreads();
-  // exp2((l - top) c), the parent's p of the token times the parent's total
-  const double p = exp2_64(__builtin_fma(static_cast<double>(logit), c,
-                                         child ? -static_cast<double>(s_top[parent]) * c : 0.0));
+  // the parent's p of the token times the parent's total
+  const double p = weight_of(logit, child ? s_top[parent] : 0.f, c);
 
   const auto lane_f64 = [](double x, int j) {
     const uint64_t bits = __builtin_bit_cast(uint64_t, x);
@@ -531,7 +535,7 @@ __global__ __launch_bounds__(kWalkThreads) void sample_walk(const eagle4_sample_
     const QRow<Q, VEC> qrow(a.probs, start + node, a.stride_prob, row.past);
     const Work w(a, s, start + node);
     const float top = s_top[node];
-    const double total = s_total[node], off = -static_cast<double>(top) * c;
+    const double total = s_total[node];
     const bool single = greedy || !(__builtin_fabsf(top) < INFINITY);
     double mass = total;   // Z, and above s, times the total
     uint64_t rejected = 0; // tokens taken out of the residual (no draft probabilities)
@@ -577,7 +581,7 @@ __global__ __launch_bounds__(kWalkThreads) void sample_walk(const eagle4_sample_
         }
         __syncthreads();  // the last masses have been read
         for (int k = wave; k < s.chunks * kParts; k += kWalkWaves) {
-          const double m = residual_mass<T, Q, kPart / VEC / 64>(row, qrow, k * (kPart / VEC), c, off, spent, lane, 0, 0);
+          const double m = residual_mass<T, Q, kPart / VEC / 64>(row, qrow, k * (kPart / VEC), c, top, spent, lane, 0, 0);
           if (lane == 0) masses[k] = m;
         }
         __syncthreads();
@@ -613,7 +617,7 @@ __global__ __launch_bounds__(kWalkThreads) void sample_walk(const eagle4_sample_
           const int k = __builtin_amdgcn_readlane(my_chunk, __builtin_ctzll(left));
           left &= ~__ballot(my_chunk == k);
           if (lost % kWalkWaves == wave) {
-            const double sum = residual_mass<T, Q, kChunk / VEC / 64>(row, qrow, k * (kChunk / VEC), c, off, 0.0, lane, rejected,
+            const double sum = residual_mass<T, Q, kChunk / VEC / 64>(row, qrow, k * (kChunk / VEC), c, top, 0.0, lane, rejected,
                                                                                static_cast<int>(token));
             if (lane == 0) {
               s_lost_chunk[lost] = k;
@@ -627,7 +631,7 @@ __global__ __launch_bounds__(kWalkThreads) void sample_walk(const eagle4_sample_
       // a chunk's mass, or of a residual a part's
       const auto mass_of = [&](int k) {
         if (spent > 0.0) return masses[k];
-        double m = w.sums[k] * exp2_64((static_cast<double>(w.maxes[k]) - static_cast<double>(top)) * c);
+        double m = w.sums[k] * weight_of(w.maxes[k], top, c);
         for (int i = 0; i < lost; ++i)
           if (s_lost_chunk[i] == k) m = s_lost_mass[i];
         return m;
@@ -685,7 +689,7 @@ __global__ __launch_bounds__(kWalkThreads) void sample_walk(const eagle4_sample_
           for (int k = 0; k < VEC; ++k) x[k] = -INFINITY;
         }
         if constexpr (!kProbs) take_out<VEC>(x, row.first(v0 + i), rejected, static_cast<int>(token));
-        residual<Q, VEC>(x, qrow, row.first(v0 + i), row.vocab, c, off, spent, r[i]);
+        residual<Q, VEC>(x, qrow, row.first(v0 + i), row.vocab, c, top, spent, r[i]);
 #pragma unroll
         for (int k = 0; k < VEC; ++k) {
           mine += r[i][k];
