@@ -664,7 +664,7 @@ __global__ __launch_bounds__(kWalkThreads) void sample_walk(const eagle4_sample_
         if (passed != 0) {
           const int f = __builtin_ctzll(passed);
           at = k0 + f;
-          base += lane_f64(run, f) - lane_f64(m, f);
+          if (f > 0) base += lane_f64(run, f - 1);  // not run - m: rounded, that may pass the target
         } else {
           base += lane_f64(run, 63);
         }

@@ -74,3 +74,20 @@ def test_logits_far_from_zero(dev, dtype, probs):
     x["logits"] = ((x["logits"] * 4).round() * step + torch.tensor([far, -far]).repeat(12)[:, None]).to(dtype)
     x["temperature"] = torch.full((4,), step * 4.0)
     st.check(x, st.launch(x, dev))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("probs", [None, F32])
+def test_a_coin_on_the_border_of_two_pieces(dev, dtype, probs):
+    """Rows whose second half repeats the first, and a final coin of a half: the running sum reaches it exactly where a piece
+    ends, and the next token is the first one past it (or, by the sums' rounding, the last one before)."""
+    announce(f"sample tree border {dtype} probs {probs}")
+    n, vocab = 96, 16384
+    x = st.inputs([1] * n, 1, vocab, dtype, probs, seed=54)
+    half = torch.randn(n, vocab // 2, generator=torch.Generator().manual_seed(54)).to(dtype)
+    x["logits"] = torch.cat([half, half], 1)
+    x["final"][:] = 0.5
+    x["temperature"][:] = 1.0
+    sampled, count, _ = st.launch(x, dev)
+    assert count.tolist() == [1] * n
+    assert {int(t) for t in sampled[:, 0].cpu()} <= {vocab // 2 - 1, vocab // 2}
