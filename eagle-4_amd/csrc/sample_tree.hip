@@ -708,7 +708,10 @@ __global__ __launch_bounds__(kWalkThreads) void sample_walk(const eagle4_sample_
       for (int k = 0; k < wave; ++k) from += s_scan[k];
       const double left = __shfl_up(run, 1, 64);
       const double begin = lane == 0 ? from : from + left, stop = from + run;
-      if (sought && begin <= target && stop > target) {
+      // A wave's first lane past the target: not only the one that the target lies in, as the scan's sums are rounded each in its
+      // own order, and a lane without mass may seem to take the sum across it.
+      const uint64_t past = __ballot(sought && stop > target && end >= 0);
+      if (past != 0 && lane == __builtin_ctzll(past)) {
         double acc = begin;
         int hit = end;
         bool open = true;

@@ -91,3 +91,20 @@ def test_a_coin_on_the_border_of_two_pieces(dev, dtype, probs):
     sampled, count, _ = st.launch(x, dev)
     assert count.tolist() == [1] * n
     assert {int(t) for t in sampled[:, 0].cpu()} <= {vocab // 2 - 1, vocab // 2}
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("probs", [None, F32])
+def test_a_coin_on_the_border_of_two_halves_with_masked_tokens_between(dev, dtype, probs):
+    """As above within a piece: the second half begins with eight tokens that may not be drawn."""
+    announce(f"sample tree border and masks {dtype} probs {probs}")
+    n, vocab = 256, 512
+    x = st.inputs([1] * n, 1, vocab, dtype, probs, seed=55)
+    half = torch.randn(n, vocab // 2, generator=torch.Generator().manual_seed(55)).to(dtype)
+    half[:, :8] = -float("inf")
+    x["logits"] = torch.cat([half, half], 1)
+    x["final"][:] = 0.5
+    x["temperature"][:] = 1.0
+    sampled, count, _ = st.launch(x, dev)
+    assert count.tolist() == [1] * n
+    assert {int(t) for t in sampled[:, 0].cpu()} <= {vocab // 2 - 1, vocab // 2 + 8}
