@@ -175,7 +175,9 @@ __global__ __launch_bounds__(256) void write_kernel(const eagle4_write_kv_args a
   for (int i = 0; i < kHeld; ++i)
     if (from[i] != nullptr) held[i].load(from[i]);
   float amax = 0.f;
+  bool any = false;  // a row goes to the page
   auto most = [&](const Chunk<T, N>& ch) {
+    any = true;
     float x[N];
     ch.widen(x);
 #pragma unroll
@@ -191,6 +193,7 @@ __global__ __launch_bounds__(256) void write_kernel(const eagle4_write_kv_args a
     ch.load(s);
     most(ch);
   }
+  if (!__any(any)) return;  // (a request padded into the batch has another's path and no rows: the page is not its own)
   amax = e4::group_max<64>(amax);
 
   const int kept = static_cast<int>(lo - first);  // earlier rows of the page

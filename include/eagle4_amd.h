@@ -461,7 +461,8 @@ int eagle4_mamba2_tree_state_update(const eagle4_mamba2_args* args, void* stream
  * position context_lens[b] + j. The scale of a page that rows go to is the least power of two s with amax <= 448 s over
  * those rows, or the page's own where earlier positions of it are below the context and its scale is larger; where it
  * grows, those positions are re-encoded. Infinities saturate and take no part in amax; NaN stays NaN. A row whose page
- * the table does not hold, or names outside num_blocks, is not written. A page belongs to one request. */
+ * the table does not hold, or names outside num_blocks, is not written, and neither is a path entry that names no row of the
+ * request. A page that no row goes to keeps its scale. A page belongs to one request. */
 typedef struct eagle4_write_kv_args {
   const void* key;   /* [tokens, heads, dim], dtype, unit stride over dim */
   const void* value; /* like key, or null: one matrix (latent rows) */

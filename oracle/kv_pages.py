@@ -46,6 +46,8 @@ def write_rows(rows, cache, scale, table, context: int) -> None:
         block = int(table[index])
         for h in range(heads):
             data = [None if r is None else r[h].double() for r in part]
+            if all(d is None for d in data):  # no row goes to the page
+                continue
             amax = max([float(torch.where(torch.isfinite(d), d.abs(), 0.0).max()) for d in data if d is not None] + [0.0])
             old = float(scale[block, h]) if lead else 0.0
             now = max(old, page_scale(amax))
