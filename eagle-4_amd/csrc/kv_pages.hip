@@ -195,10 +195,32 @@ __global__ __launch_bounds__(256) void write_kernel(const eagle4_write_kv_args a
   }
   if (!__any(any)) return;  // (a request padded into the batch has another's path and no rows: the page is not its own)
   amax = e4::group_max<64>(amax);
+  // Whether the rows hold an infinity: looked for only where no other value gives the page a scale.
+  auto infinite = [&] {
+    bool inf = false;
+    auto look = [&](const Chunk<T, N>& ch) {
+      float x[N];
+      ch.widen(x);
+#pragma unroll
+      for (int i = 0; i < N; ++i) inf = inf || __builtin_fabsf(x[i]) == INFINITY;
+    };
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i)
+      if (from[i] != nullptr) look(held[i]);
+    for (int c = lane + 64 * kHeld; c < chunks; c += 64) {
+      const S* const s = source(c);
+      if (s == nullptr) continue;
+      Chunk<T, N> ch;
+      ch.load(s);
+      look(ch);
+    }
+    return __any(inf) != 0;
+  };
 
   const int kept = static_cast<int>(lo - first);  // earlier rows of the page
   const float old = kept > 0 ? held_scale : 0.f;
-  const float now = fmaxf(old, page_scale(amax));
+  float now = fmaxf(old, page_scale(amax));
+  if (now == 0.f && infinite()) now = 1.f;  // else they would read back as zeros
   const float inv = now > 0.f ? 1.0f / now : 0.f;
   if (kept > 0 && now > old) {
     const float ratio = old * inv;

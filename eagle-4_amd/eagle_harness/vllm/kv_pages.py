@@ -92,8 +92,8 @@ def write_kv_pages(
 
     The scale of a page that rows go to becomes the least power of two ``s`` with ``amax <= 448 s`` over them; a page that
     keeps earlier positions (below the context) keeps its scale if that is larger, and has them re-encoded if it is smaller.
-    Positions behind a request's last row keep their bytes. Infinities saturate and do not count in ``amax``. A page
-    belongs to one request. Rows whose page the table lacks, or names outside the cache, are not written, and neither is a
+    Positions behind a request's last row keep their bytes. Infinities saturate (at 448 times the scale) and do not
+    count in ``amax``; a page of nothing else but zeros gets a scale of 1. A page belongs to one request. Rows whose page the table lacks, or names outside the cache, are not written, and neither is a
     path entry that names no row of its request; a page that no row goes to keeps its scale.
     """
     pages, (heads, dim, page, blocks) = _pages_args("write_kv_pages", key, value, key_cache, value_cache, k_scale, v_scale,

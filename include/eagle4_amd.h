@@ -460,7 +460,8 @@ int eagle4_mamba2_tree_state_update(const eagle4_mamba2_args* args, void* stream
  * Request b's row j (j < its rows, or < path_len[slot] with `path`, whose entry j names the row that it takes) goes to
  * position context_lens[b] + j. The scale of a page that rows go to is the least power of two s with amax <= 448 s over
  * those rows, or the page's own where earlier positions of it are below the context and its scale is larger; where it
- * grows, those positions are re-encoded. Infinities saturate and take no part in amax; NaN stays NaN. A row whose page
+ * grows, those positions are re-encoded. Infinities saturate and take no part in amax (where nothing else gives a scale
+ * above 0 it is 1); NaN stays NaN. A row whose page
  * the table does not hold, or names outside num_blocks, is not written, and neither is a path entry that names no row of the
  * request. A page that no row goes to keeps its scale. A page belongs to one request. */
 typedef struct eagle4_write_kv_args {

@@ -51,12 +51,14 @@ def write_rows(rows, cache, scale, table, context: int) -> None:
             amax = max([float(torch.where(torch.isfinite(d), d.abs(), 0.0).max()) for d in data if d is not None] + [0.0])
             old = float(scale[block, h]) if lead else 0.0
             now = max(old, page_scale(amax))
+            if now == 0 and any(bool(torch.isinf(d).any()) for d in data if d is not None):
+                now = 1.0  # an infinity saturates at a value, not at 0
             if lead and now > old:
                 cache[block, :lead, h] = encode(cache[block, :lead, h].double() * (old / now))
             for j, d in enumerate(data):
                 if d is None:
                     continue
-                y = d / now if now > 0 else torch.where(torch.isinf(d), d, d * 0.0)
+                y = d / now if now > 0 else d * 0.0  # (no infinities then)
                 cache[block, lead + j, h] = encode(y)
             scale[block, h] = now
 
