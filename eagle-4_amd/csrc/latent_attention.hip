@@ -446,9 +446,10 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
       const int n = i / kBatch, key = fresh(tid), k0 = 64 * wave;
       if (i % kBatch == 2) {
         if ((t0 + kBatch * (n + 2)) * kKeys < u.context) dma4(entry_of(n + 2, key), uniform(lds_addr(&s_ent[k0])));
-      } else if (FP8 && i % kBatch == 3) {  // (an entry that was not loaded is none of a key's, and in its bounds or not used)
+      } else if (FP8 && i % kBatch == 3) {  // (an entry that was not loaded is none of a key's: in bounds, or taken for none)
         const int32_t blk = s_ent[key];
-        dma4(a.scale_page + (blk >= 0 && blk < a.num_blocks ? blk : 0) * a.stride_sp,
+        const void* const none = zero_row;  // not page 0's scale: a cache of no pages has none
+        dma4(blk >= 0 && blk < a.num_blocks ? a.scale_page + blk * a.stride_sp : none,
              uniform(lds_addr(&s_entscale[FP8 ? k0 : 0])));
       } else if (i % kBatch == 0 && i > 0) {
         fill(n + 1, key, s_ent[key], FP8 ? s_entscale[FP8 ? key : 0] : 1.f);
