@@ -41,7 +41,7 @@ struct LatentPlan {
   int first, reqs;       // requests of this launch
   int groups;            // workgroups
   int least;             // tiles of a workgroup's run at least
-  int rows;              // query rows of a workgroup
+  int rows;              // query rows of a workgroup at most
   int page_shift;        // of a page size that is a power of two, else -1
   uint32_t page_inv;     // floor(2^32 / page) of any other
   int64_t pre_off, lse_off, part_off;  // float offsets into the workspace
@@ -56,10 +56,10 @@ struct Unit {
   int64_t start;          // first token
   int width, context;     // rows, committed positions
   int ctx_tiles, tiles;   // tiles of a row group
-  int row_groups;
+  E4_DEV int row_groups(int heads, int rows) const { return (width * heads + rows - 1) / rows; }
 };
 
-E4_DEV Unit unit_of(const eagle4_latent_attn_args& a, int b, int rows) {
+E4_DEV Unit unit_of(const eagle4_latent_attn_args& a, int b) {
   Unit u;
   u.start = e4::ld(a.query_start_loc, b);
   int64_t width = e4::ld(a.query_start_loc, b + 1) - u.start;
@@ -71,7 +71,6 @@ E4_DEV Unit unit_of(const eagle4_latent_attn_args& a, int b, int rows) {
   u.context = static_cast<int>(context);
   u.ctx_tiles = (u.context + kKeys - 1) / kKeys;
   u.tiles = u.ctx_tiles + (u.width + kKeys - 1) / kKeys;
-  u.row_groups = (u.width * a.heads + rows - 1) / rows;
   return u;
 }
 
@@ -141,11 +140,11 @@ E4_DEV int swz(int key) { return 2 * ((key >> 1) & 3) | ((key >> 3) & 1); }
 
 constexpr int kWaves = 8, kThreads = 64 * kWaves;
 
-template <int RANK, int ROPE, typename T_, bool FP8_, int RW_>
+template <int RANK_, int ROPE, typename T_, bool FP8_, int RW_>
 struct Shape {
   using T = T_;
   static constexpr bool FP8 = FP8_;
-  static constexpr int RW = RW_, DW = kWaves / RW, DT = RANK / 16 / DW;
+  static constexpr int RANK = RANK_, RW = RW_, DW = kWaves / RW, DT = RANK / 16 / DW;
   static constexpr int DIM = RANK + ROPE, CB = DIM / 64, KC = DIM / 32, ROWS = RW * 16, TILE = CB * 4096;
   // 16-bit pages: a ring of four tiles, two in use and two on their way. fp8 pages: a ring of three, two in use and one being
   // widened, and one of two tiles of codes, the one that is widened and one on its way.
@@ -199,13 +198,13 @@ E4_DEV f32x4_t score_step(const char* tile, const u32x4_t (&q)[S::KC], int kt, i
 
 // The weights of those scores into `to`, relative to the rows' maximum m; l takes their sum. Bit k of bits: key k of the tile
 // is visible to the lane's row. In kPhases phases without a branch, for the places between the products of the output.
-template <typename S>
+template <typename S, typename W>
 struct WeightStep {
   using T = typename S::T;
   static constexpr int kPhases = 8;
   f32x4_t s, ks;
   float top, p[4];
-  E4_DEV void phase(int i, Weights<S::RW>& to, int row_wave, int kt, bool writes, float& m, float& l, float scale_log2,
+  E4_DEV void phase(int i, W& to, int row_wave, int kt, bool writes, float& m, float& l, float scale_log2,
                     const float* key_scale, int lane, uint32_t bits) {
     const int g = lane >> 4;
     if (i == 0) {
@@ -254,8 +253,8 @@ E4_DEV uint32_t scale2(uint32_t w, float f) {
 // The weights of a tile as the operand of its output. macc is what acc is relative to, m what the wave's own next weights
 // are: both move to the largest maximum that the tile's weights bring. (In front of the scores, where no operand of a product
 // is in registers: the compiler then keeps one copy of acc over the branch.)
-template <typename S>
-E4_DEV u32x4_t take_weights(const Weights<S::RW>& from, int row_wave, f32x4_t (&acc)[S::DT], float& macc, float& m, float& l,
+template <typename S, typename W>
+E4_DEV u32x4_t take_weights(const W& from, int row_wave, f32x4_t (&acc)[S::DT], float& macc, float& m, float& l,
                             int lane) {
   using T = typename S::T;
   const int g = lane >> 4, l16 = lane & 15;
@@ -308,51 +307,49 @@ E4_DEV void value_step(const char* tile, u32x4_t pb, f32x4_t (&acc)[S::DT], int 
   }
 }
 
-template <int RANK, int ROPE, typename T, bool FP8, int RW>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void latent_kernel(
-    const eagle4_latent_attn_args a, const LatentPlan p) {
-  using S = Shape<RANK, ROPE, T, FP8, RW>;
-  __shared__ __attribute__((aligned(1024))) char smem[S::NBUF][S::TILE];
-  __shared__ __attribute__((aligned(1024))) char s_raw[FP8 ? 2 : 1][FP8 ? S::RAW : 16];
-  __shared__ Weights<RW> s_w[2];
+// What a workgroup keeps in LDS, for S the shape of the most rows that it may take.
+template <typename S>
+struct Lds {
+  // (sizes are of every shape with these columns and pages, but those of the weights and sums)
+  static constexpr int kBatchKeys = kBatch * kKeys, kRowWaves = S::RW;
+  __attribute__((aligned(1024))) char smem[S::NBUF][S::TILE];
+  __attribute__((aligned(1024))) char s_raw[S::FP8 ? 2 : 1][S::FP8 ? S::RAW : 16];
+  Weights<S::RW> s_w[2];
   // The keys of two batches of tiles: their table entries and scales as loaded, then the addresses of their rows, a bit a key
   // that is there, and the two parts of its scale.
-  constexpr int kBatchKeys = kBatch * kKeys;
-  __shared__ __attribute__((aligned(16))) int32_t s_ent[kBatchKeys];
-  __shared__ __attribute__((aligned(16))) float s_entscale[FP8 ? kBatchKeys : 1];
-  __shared__ uint64_t s_row[2][kBatchKeys];
-  __shared__ uint32_t s_vis[2][kBatch];
-  __shared__ __attribute__((aligned(16))) float s_rest[FP8 ? 2 : 1][kBatchKeys], s_pow2[FP8 ? 2 : 1][kBatchKeys];
-  __shared__ uint32_t s_bad;           // a bit a new key: it holds a value that is not finite
-  __shared__ uint32_t s_tot[kWaves];
-  __shared__ float s_sum[RW][2][16];
-  __shared__ int s_at;
-  __shared__ uint32_t s_before;
+  __attribute__((aligned(16))) int32_t s_ent[kBatchKeys];
+  __attribute__((aligned(16))) float s_entscale[S::FP8 ? kBatchKeys : 1];
+  uint64_t s_row[2][kBatchKeys];
+  uint32_t s_vis[2][kBatch];
+  __attribute__((aligned(16))) float s_rest[S::FP8 ? 2 : 1][kBatchKeys], s_pow2[S::FP8 ? 2 : 1][kBatchKeys];
+  uint32_t s_bad;  // a bit a new key: it holds a value that is not finite
+  uint32_t s_tot[2][kWaves];
+  float s_sum[S::RW][2][16];
+  int s_at;
+  uint32_t s_before;
+};
+
+// The workgroup's run, S::ROWS rows at a time: `total` tiles in all, `sum_tiles` of the requests up to the thread's and `mine`
+// of that one.
+template <typename S, typename L>
+E4_DEV void latent_rows(const eagle4_latent_attn_args& a, const LatentPlan& p, L& lds, uint32_t total, uint32_t sum_tiles,
+                        uint32_t mine) {
+  using T = typename S::T;
+  constexpr bool FP8 = S::FP8;
+  constexpr int RW = S::RW, RANK = S::RANK, kBatchKeys = L::kBatchKeys;
+  auto& smem = lds.smem;
+  auto& s_raw = lds.s_raw;
+  auto& s_w = lds.s_w;
+  auto& s_ent = lds.s_ent;
+  auto& s_entscale = lds.s_entscale;
+  auto& s_row = lds.s_row;
+  auto& s_vis = lds.s_vis;
+  auto& s_rest = lds.s_rest;
+  auto& s_pow2 = lds.s_pow2;
+  auto& s_bad = lds.s_bad;
+  auto& s_sum = lds.s_sum;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l16 = lane & 15;
-
-  // tiles before each request (one a thread)
-  static_assert(kMaxReqs <= kThreads, "requests of a launch");
-  uint32_t mine = 0, sum_tiles = 0;
-  if (tid < p.reqs) {
-    const Unit u = unit_of(a, p.first + tid, S::ROWS);
-    mine = static_cast<uint32_t>(u.tiles) * static_cast<uint32_t>(u.row_groups);
-  }
-  sum_tiles = mine;
-#pragma unroll
-  for (int k = 1; k < 64; k <<= 1) {
-    const uint32_t o = __shfl_up(sum_tiles, k, 64);
-    if (lane >= k) sum_tiles += o;
-  }
-  if (lane == 63) s_tot[wave] = sum_tiles;
-  __syncthreads();
-  uint32_t all_tiles = 0;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
-    if (w < wave) sum_tiles += s_tot[w];
-    all_tiles += s_tot[w];
-  }
-  const uint32_t total = uniform(all_tiles);
   uint32_t share = (total + p.groups - 1) / p.groups;
   share = share < static_cast<uint32_t>(p.least) ? p.least : share;
   // adjacent runs on one XCD (workgroups go to the eight in turn): row groups of a request share its tiles in the L2
@@ -360,18 +357,21 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
   uint32_t pos = wg * share;
   const uint32_t stop = pos + share < total ? pos + share : total;
   if (sum_tiles - mine <= pos && pos < sum_tiles) {  // the request of tile `pos`
-    s_at = tid;
-    s_before = sum_tiles - mine;
+    lds.s_at = tid;
+    lds.s_before = sum_tiles - mine;
   }
   if (wg == 0 && tid < p.reqs) {  // for the merge
     uint32_t* const pre = reinterpret_cast<uint32_t*>(a.workspace + p.pre_off);
     pre[tid + 1] = sum_tiles;
-    if (tid == 0) pre[0] = 0;
+    if (tid == 0) {
+      pre[0] = 0;
+      pre[p.reqs + 1] = S::ROWS;
+    }
   }
   __syncthreads();
   if (pos >= stop) return;
-  int at = uniform(s_at);
-  uint32_t before = uniform(s_before);  // tiles before request `at`
+  int at = uniform(lds.s_at);
+  uint32_t before = uniform(lds.s_before);  // tiles before request `at`
 
   const int row_wave = wave / S::DW, column_wave = wave % S::DW, kt = column_wave % 2, dbase = column_wave * S::DT * 16;
   const float scale_log2 = a.scale * 1.4426950408889634f;
@@ -390,10 +390,10 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
 
   while (pos < stop) {
     const int b = p.first + at;
-    Unit u = unit_of(a, b, S::ROWS);
-    u = Unit{uniform(u.start), uniform(u.width), uniform(u.context), uniform(u.ctx_tiles), uniform(u.tiles),
-             uniform(u.row_groups)};
-    const uint32_t within = pos - before, its_tiles = static_cast<uint32_t>(u.tiles) * static_cast<uint32_t>(u.row_groups);
+    Unit u = unit_of(a, b);
+    u = Unit{uniform(u.start), uniform(u.width), uniform(u.context), uniform(u.ctx_tiles), uniform(u.tiles)};
+    const uint32_t within = pos - before;
+    const uint32_t its_tiles = static_cast<uint32_t>(u.tiles) * static_cast<uint32_t>(uniform(u.row_groups(a.heads, S::ROWS)));
     if (within >= its_tiles) {
       before += its_tiles;
       ++at;
@@ -651,7 +651,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
     for (int i = 0; i <= tiles; ++i) {
       arrive(i);
       const u32x4_t pb = take_weights<S>(s_w[(i + 1) % 2], row_wave, acc, macc, m, l, fresh(lane));
-      WeightStep<S> w;
+      using Step = WeightStep<S, Weights<L::kRowWaves>>;
+      Step w;
       w.s = f32x4_t{0.f, 0.f, 0.f, 0.f};
       uint32_t bits = 0;
       if (i < tiles) {
@@ -675,7 +676,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
       const int ln = fresh(lane);
       const float* const rest = s_rest[FP8 ? i / kBatch % 2 : 0] + i % kBatch * kKeys;
       value_step<S>(smem[(i + S::NBUF - 1) % S::NBUF], pb, acc, dbase, ln, [&](int dt) {
-        constexpr int kPhases = WeightStep<S>::kPhases;
+        constexpr int kPhases = Step::kPhases;
 #pragma unroll
         for (int ph = 0; ph < kPhases; ++ph)
           if (ph * S::DT / kPhases == dt)
@@ -721,6 +722,64 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
   }
 }
 
+// Tiles of 64 rows up to which a launch takes 16 rows a workgroup: 2.5 a workgroup. 64 rows share a tile's loads best, but where
+// there is so little work 16 spread it over more workgroups, with less to bring in, to leave and to merge (RANK 512; the times
+// with 64 and 16 rows: one token of 128 heads over 2048 keys, 130 tiles: 34.5 and 25.4 us; 8192 keys, 514: 45.4 and 34.1;
+// 16384 keys, 1026: 52.2 and 46.2; 32768 keys, 2050: 60.8 and 66.4; a tree of 16 x 16 heads over 4096 keys, 516: 34.0 and
+// 31.3; 4 such trees over 512 keys, 272: 36.3 and 27.0; over 2048 keys, 1040: 34.1 and 40.6). The contexts decide, not the
+// tables' width, which in an engine is that of its longest context: chosen on the GPU, in one kernel that holds both forms.
+constexpr uint32_t kFewTiles = 640;
+
+// Of 16 (FORM 1) or 32 rows (2) a workgroup, or (4) of 64 or 16, by the tiles that there are.
+template <int RANK, int ROPE, typename T, bool FP8, int FORM>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void latent_kernel(
+    const eagle4_latent_attn_args a, const LatentPlan p) {
+  using S = Shape<RANK, ROPE, T, FP8, FORM>;
+  __shared__ Lds<S> lds;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  // tiles before each request (one a thread), and the same of 16 rows
+  static_assert(kMaxReqs <= kThreads, "requests of a launch");
+  uint32_t mine = 0, few = 0;
+  if (tid < p.reqs) {
+    const Unit u = unit_of(a, p.first + tid);
+    mine = static_cast<uint32_t>(u.tiles) * static_cast<uint32_t>(u.row_groups(a.heads, S::ROWS));
+    if constexpr (FORM == 4) few = static_cast<uint32_t>(u.tiles) * static_cast<uint32_t>(u.row_groups(a.heads, 16));
+  }
+  uint32_t sum = mine, sum_few = few;
+#pragma unroll
+  for (int k = 1; k < 64; k <<= 1) {
+    const uint32_t o = __shfl_up(sum, k, 64);
+    if (lane >= k) sum += o;
+    if constexpr (FORM == 4) {
+      const uint32_t f = __shfl_up(sum_few, k, 64);
+      if (lane >= k) sum_few += f;
+    }
+  }
+  if (lane == 63) {
+    lds.s_tot[0][wave] = sum;
+    lds.s_tot[1][wave] = sum_few;
+  }
+  __syncthreads();
+  uint32_t total = 0, total_few = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    if (w < wave) sum += lds.s_tot[0][w];
+    total += lds.s_tot[0][w];
+    if constexpr (FORM == 4) {
+      if (w < wave) sum_few += lds.s_tot[1][w];
+      total_few += lds.s_tot[1][w];
+    }
+  }
+  total = uniform(total);
+  if constexpr (FORM == 4) {
+    if (total <= kFewTiles) {
+      latent_rows<Shape<RANK, ROPE, T, FP8, 1>>(a, p, lds, uniform(total_few), sum_few, few);
+      return;
+    }
+  }
+  latent_rows<S>(a, p, lds, total, sum, mine);
+}
+
 // Rows of row groups that were cut: their partials by log2-sum-exp. One workgroup per 2 / SG rows.
 template <int RANK, int SG, typename T>
 __global__ __launch_bounds__(256) void latent_merge(const eagle4_latent_attn_args a, const LatentPlan p) {
@@ -728,11 +787,12 @@ __global__ __launch_bounds__(256) void latent_merge(const eagle4_latent_attn_arg
   const uint32_t* const pre = reinterpret_cast<const uint32_t*>(a.workspace + p.pre_off);
   const int at = blockIdx.y, b = p.first + at;
   const uint32_t first = pre[at], total = pre[p.reqs];
+  const int rows = static_cast<int>(pre[p.reqs + 1]);  // of a workgroup
   if (pre[at + 1] == first) return;
-  const Unit u = unit_of(a, b, p.rows);
+  const Unit u = unit_of(a, b);
   uint32_t share = (total + p.groups - 1) / p.groups;
   share = share < static_cast<uint32_t>(p.least) ? p.least : share;
-  const int rho0 = blockIdx.x * RPB, rg = rho0 / p.rows;  // p.rows is a multiple of RPB: one row group
+  const int rho0 = blockIdx.x * RPB, rg = rho0 / rows;  // rows is a multiple of RPB: one row group
   if (rho0 >= u.width * a.heads) return;
   const uint32_t begin = first + rg * u.tiles, end = begin + u.tiles;
   const int w0 = static_cast<int>(begin / share), w1 = static_cast<int>((end - 1) / share);
@@ -743,7 +803,7 @@ __global__ __launch_bounds__(256) void latent_merge(const eagle4_latent_attn_arg
   float wsum;
   const bool mine = merge_partials<RANK, SG>(
       ok ? w1 - w0 + 1 : 0,
-      [&](int i) { return (2 * static_cast<int64_t>(w0 + i) + (i == 0 ? 1 : 0)) * p.rows + (rho - rg * p.rows); },
+      [&](int i) { return (2 * static_cast<int64_t>(w0 + i) + (i == 0 ? 1 : 0)) * rows + (rho - rg * rows); },
       a.workspace + p.part_off, a.workspace + p.lse_off, sum, wsum);
   if (!mine || !ok) return;
   const float inv = wsum == 0.f ? 0.f : 1.0f / wsum;
@@ -775,16 +835,10 @@ bool covered(const eagle4_latent_attn_args& a) {
   return true;
 }
 
-// Query rows of a workgroup: 64 share a tile's loads best, but where the tables leave at most two such tiles a workgroup, 16
-// rows spread the work over more of them, with less to bring in, to leave and to merge (RANK 512; the tiles of 64 rows, the
-// times with 64 and 16: one token of 128 heads over 2048 keys, 128 tiles: 36.7 and 26.2 us; 8192 keys, 512: 47.1 and 36.0;
-// 16384 keys, 1024: 52.2 and 46.2; 32768 keys, 2048: 60.8 and 66.4; 4 trees of 16 x 16 heads over 512 keys, 256: 36.3 and
-// 27.0; over 2048 keys, 1024: 34.1 and 40.6).
+// Query rows of a workgroup at most: as the widest request's rows fill them.
 int rows_of(const eagle4_latent_attn_args& a) {
   const int rows = a.max_query_len * a.heads;
-  if (rows <= 32) return rows <= 16 ? 16 : 32;
-  const int64_t tiles = (static_cast<int64_t>(a.max_blocks) * a.page + kKeys - 1) / kKeys;
-  return a.num_reqs * ((rows + 63) / 64) * tiles <= 2 * kGroups ? 16 : 64;
+  return rows <= 16 ? 16 : (rows <= 32 ? 32 : 64);
 }
 
 // The requests that one launch takes: their tiles (at the most that the tables' sizes allow) are counted in 31 bits.
@@ -806,7 +860,7 @@ LatentPlan plan(const eagle4_latent_attn_args& a) {
   const int fit = reqs_of(a, p.rows);
   p.reqs = a.num_reqs < fit ? a.num_reqs : fit;
   p.pre_off = 0;
-  p.lse_off = (p.reqs + 1 + 3) / 4 * 4;
+  p.lse_off = (p.reqs + 2 + 3) / 4 * 4;
   p.part_off = p.lse_off + 2 * static_cast<int64_t>(p.groups) * p.rows;
   return p;
 }
