@@ -816,8 +816,10 @@ extern "C" int64_t eagle4_sample_tree_workspace(const eagle4_sample_tree_args* a
 
 extern "C" int eagle4_sample_tree(const eagle4_sample_tree_args* a, void* stream) {
   if (a->num_reqs == 0) return EAGLE4_OK;
-  if (!covered(a) || a->workspace == nullptr || a->workspace_bytes < workspace_of(*a) || !tab_ok(a->cu_num_logits) ||
-      !tab_ok(a->idx_mapping) || !tab_ok(a->parents) || a->final_coins == nullptr || a->temperature == nullptr)
+  if (!covered(a) || a->workspace == nullptr || reinterpret_cast<uintptr_t>(a->workspace) % 16 != 0 ||
+      a->workspace_bytes < workspace_of(*a) || !tab_ok(a->cu_num_logits) || !tab_ok(a->idx_mapping) || !tab_ok(a->parents) ||
+      a->final_coins == nullptr || a->temperature == nullptr || a->sampled == nullptr || a->num_sampled == nullptr ||
+      a->path == nullptr || a->path_len == nullptr)
     return EAGLE4_NOT_COVERED;
   // (of no rows nothing is read)
   if (a->rows > 0 && (a->logits == nullptr || a->coins == nullptr || !tab_ok(a->drafted))) return EAGLE4_NOT_COVERED;
