@@ -832,6 +832,8 @@ bool covered(const eagle4_latent_attn_args& a) {
   if (a.cache_dtype == EAGLE4_FP8_E4M3 && (a.stride_cb % 16 != 0 || a.stride_cs % 16 != 0)) return false;
   for (const void* p : {a.q, a.latent_new, a.cache, static_cast<const void*>(a.out)})
     if (reinterpret_cast<uintptr_t>(p) % 16 != 0) return false;
+  if (a.tokens > 0 && (a.q == nullptr || a.latent_new == nullptr || a.out == nullptr)) return false;
+  if (a.num_blocks > 0 && a.cache == nullptr) return false;
   return true;
 }
 

@@ -44,3 +44,27 @@ def test_sizes_that_the_sampled_walk_does_not_cover(over):
                                   dict(idx_mapping=_native.itab(None))])
 def test_arguments_that_the_sampled_walk_refuses(over):
     assert _native.library().eagle4_sample_tree(sampled(**over), None) == NOT_COVERED
+
+
+def latent(**over):
+    tab = _native.itab(torch.zeros(4, 4, dtype=I32))
+    return _native.LatentAttnArgs(**{**dict(
+        q=ON, stride_qt=4096, stride_qh=576, latent_new=ON, stride_nt=576, cache=ON, stride_cb=576 * 16, stride_cs=576,
+        block_table=tab, context_lens=tab, query_start_loc=tab, masks=ON, stride_mask=1, out=ON, stride_ot=4096, stride_oh=512,
+        workspace=ON, workspace_bytes=1 << 40, tokens=1, scale=1.0, num_reqs=1, heads=16, rank=512, rope=64, page=16,
+        max_query_len=1, max_blocks=4, num_blocks=4), **over})
+
+
+def test_latent_attentions_base_comes_to_a_launch():
+    lib = _native.library()
+    assert lib.eagle4_latent_attention(latent(), None) not in (0, NOT_COVERED)
+    assert lib.eagle4_latent_attention(latent(cache_dtype=3, scale_page=ON), None) not in (0, NOT_COVERED)
+    assert lib.eagle4_latent_attention(latent(tokens=0, q=0, latent_new=0, out=0), None) not in (0, NOT_COVERED)
+    assert lib.eagle4_latent_attention(latent(num_blocks=0, cache=0), None) not in (0, NOT_COVERED)
+
+
+@pytest.mark.parametrize("over", [dict(q=0), dict(latent_new=0), dict(out=0), dict(cache=0), dict(masks=0), dict(workspace=0),
+                                  dict(workspace=ON + 8), dict(q=ON + 8), dict(stride_cb=4), dict(cache_dtype=3),
+                                  dict(cache_dtype=3, scale_page=ON, stride_cs=584), dict(block_table=_native.itab(None))])
+def test_arguments_that_latent_attention_refuses(over):
+    assert _native.library().eagle4_latent_attention(latent(**over), None) == NOT_COVERED
