@@ -55,8 +55,8 @@ def latent_verify_attention(
         if latent_scale is None:
             raise ValueError("an fp8-e4m3 cache needs latent_scale ([blocks] fp32)")
         if latent_scale.dtype != torch.float32 or latent_scale.dim() not in (1, 2) or latent_scale.shape[0] < blocks or (
-                latent_scale.dim() == 2 and latent_scale.shape[1] < 1):
-            raise ValueError(f"latent_scale must be fp32 [blocks >= {blocks}], got {tuple(latent_scale.shape)}")
+                latent_scale.dim() == 2 and latent_scale.shape[1] != 1):
+            raise ValueError(f"latent_scale must be fp32 [blocks >= {blocks}] or [.., 1], got {tuple(latent_scale.shape)}")
         if latent_scale.device != device:
             raise ValueError("latent_verify_attention: every tensor must be on q's device")
     if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.stride(1) != 1:
