@@ -257,7 +257,7 @@ template <typename S, typename W>
 E4_DEV u32x4_t take_weights(const W& from, int row_wave, f32x4_t (&acc)[S::DT], float& macc, float& m, float& l,
                             int lane) {
   using T = typename S::T;
-  const int g = lane >> 4, l16 = lane & 15;
+  const int l16 = lane & 15;
   // element i of P^T's operand is key 16 (i / 4) + 4 g + i % 4
   u32x2_t p0 = from.p[row_wave][0][lane], p1 = from.p[row_wave][1][lane];
   const float m0 = from.m[row_wave][0][l16], m1 = from.m[row_wave][1][l16];
@@ -780,10 +780,10 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
   latent_rows<S>(a, p, lds, total, sum, mine);
 }
 
-// Rows of row groups that were cut: their partials by log2-sum-exp. One workgroup per 2 / SG rows.
-template <int RANK, int SG, typename T>
+// Rows of row groups that were cut: their partials by log2-sum-exp, a thread four columns: 1024 / RANK rows a workgroup.
+template <int RANK, typename T>
 __global__ __launch_bounds__(256) void latent_merge(const eagle4_latent_attn_args a, const LatentPlan p) {
-  constexpr int LP = RANK / 4, RPB = 256 / LP / SG;
+  constexpr int LP = RANK / 4, RPB = 256 / LP;
   const uint32_t* const pre = reinterpret_cast<const uint32_t*>(a.workspace + p.pre_off);
   const int at = blockIdx.y, b = p.first + at;
   const uint32_t first = pre[at], total = pre[p.reqs];
@@ -797,15 +797,15 @@ __global__ __launch_bounds__(256) void latent_merge(const eagle4_latent_attn_arg
   const uint32_t begin = first + rg * u.tiles, end = begin + u.tiles;
   const int w0 = static_cast<int>(begin / share), w1 = static_cast<int>((end - 1) / share);
   if (w0 == w1) return;
-  const int rho = rho0 + threadIdx.x / (LP * SG);
+  const int rho = rho0 + threadIdx.x / LP;
   const bool ok = rho < u.width * a.heads;
   f32x4_t sum;
   float wsum;
-  const bool mine = merge_partials<RANK, SG>(
+  merge_partials<RANK, 1>(
       ok ? w1 - w0 + 1 : 0,
       [&](int i) { return (2 * static_cast<int64_t>(w0 + i) + (i == 0 ? 1 : 0)) * rows + (rho - rg * rows); },
       a.workspace + p.part_off, a.workspace + p.lse_off, sum, wsum);
-  if (!mine || !ok) return;
+  if (!ok) return;
   const float inv = wsum == 0.f ? 0.f : 1.0f / wsum;
   const int t = rho / a.heads, head = rho % a.heads, d = 4 * (threadIdx.x % LP);
   uint16_t* const o = static_cast<uint16_t*>(a.out) + (u.start + t) * a.stride_ot + head * a.stride_oh + d;
@@ -878,7 +878,7 @@ int launch(const eagle4_latent_attn_args& a, const LatentPlan& p, hipStream_t s)
   if (status != EAGLE4_OK) return status;
   constexpr int RPB = 1024 / RANK;
   const dim3 grid(e4::ceil_div(int64_t(a.max_query_len) * a.heads, RPB), p.reqs);
-  latent_merge<RANK, 1, T><<<grid, 256, 0, s>>>(a, p);
+  latent_merge<RANK, T><<<grid, 256, 0, s>>>(a, p);
   return E4_LAUNCH_STATUS();
 }
 
