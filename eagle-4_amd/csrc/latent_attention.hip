@@ -90,7 +90,7 @@ E4_DEV void wait_vm() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
-// 8 fp8 codes times a power of two, as 16-bit T (exact but beyond T's range).
+// 8 fp8 codes times a power of two, as 16-bit T: exact within split_scale's limits.
 template <typename T>
 E4_DEV u32x4_t widen8(u32x2_t raw, float pow2) {
   u32x4_t w;
@@ -108,11 +108,14 @@ E4_DEV u32x4_t widen8(u32x2_t raw, float pow2) {
 }
 // A page's scale as pow2 x rest, 1 <= |rest| < 2: the power goes into the codes as they are widened, the rest (1 for the
 // scales that the cache's writer makes) onto the key's score and weight. Neither takes a 16-bit weight out of its range,
-// as the whole scale would.
+// as the whole scale would. The power stays where the largest code (448) and the smallest (2^-9) times it are numbers of T; what
+// is beyond joins the rest. (fp16: rows of up to 65504 have scales of up to 2^8, and 256 x 2^8 would be an infinity.)
+template <typename T>
 E4_DEV void split_scale(float scale, float& pow2, float& rest) {
+  constexpr float kLeast = T::code == EAGLE4_BF16 ? 0x1p-117f : 0x1p-15f, kMost = T::code == EAGLE4_BF16 ? 0x1p119f : 0x1p7f;
   const uint32_t e = __float_as_uint(scale) & 0x7f800000u;
   const bool plain = e != 0 && e != 0x7f800000u;
-  pow2 = plain ? __uint_as_float(e) : 1.f;
+  pow2 = plain ? fminf(fmaxf(__uint_as_float(e), kLeast), kMost) : 1.f;
   rest = plain ? scale / pow2 : scale;
 }
 
@@ -438,7 +441,7 @@ E4_DEV void latent_rows(const eagle4_latent_attn_args& a, const LatentPlan& p, L
       const uint64_t there = __ballot(row != nullptr);
       if (key == 0) s_vis[n % 2][i / kKeys] = static_cast<uint32_t>(there >> (i & 32));
       s_row[n % 2][i] = reinterpret_cast<uint64_t>(row != nullptr ? row : reinterpret_cast<const char*>(zero_row));
-      if constexpr (FP8) split_scale(scale, s_pow2[n % 2][i], s_rest[n % 2][i]);
+      if constexpr (FP8) split_scale<T>(scale, s_pow2[n % 2][i], s_rest[n % 2][i]);
     };
     // In the loop the lookups are direct loads too, two iterations ahead of the fill, which is two ahead of the first use.
     const auto lookup = [&](int i) {

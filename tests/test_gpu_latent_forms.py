@@ -5,6 +5,7 @@ import torch
 
 import test_gpu_latent_attention as lat
 from conftest import announce
+from oracle import latent as olat
 
 pytestmark = pytest.mark.gpu
 
@@ -161,3 +162,67 @@ def test_a_captured_call_takes_each_batch_in_its_own_form(dev):
         assert torch.equal(out, want[i])
     lat.check(xs[0], want[0])
     lat.check(xs[2], want[2])
+
+
+@pytest.mark.parametrize("power", [7, 8, 9, 12, 14])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_scales_of_large_values(dev, dtype, power):
+    """A page scaled for values near fp16's largest, and beyond, in a column that no query looks at."""
+    announce(f"latent large scales 2^{power} {dtype}")
+    x = lat.inputs([320, 50], [4, 2], 16, dtype, "fp8", seed=82)
+    x["q"][..., 5] = 0
+    block = int(x["table"][0, 3])
+    codes = torch.zeros(16, 576)
+    codes[:, ::7] = 2.0 ** -9  # the smallest code
+    codes[2, 5] = 256.0 if power == 8 else 448.0
+    x["cache"][block] = codes.to(x["cache"].dtype)
+    x["page_scale"][block] = 2.0 ** power
+    want, bound = olat.latent_attention(x["q"], x["new"], x["cache"], x["table"], x["context"], x["starts"], x["masks"],
+                                        x["scale"], x["rank"], x["page_scale"])
+    # Outputs beyond the type: fp16 ends at 65504, its step there is 32, and from 65520, half a step on, a value rounds to infinity.
+    beyond = (want.abs() + bound >= 65520) & (dtype == F16)
+    for got in (lat.launch(x, dev), lat.launch(crowded(x), dev)[:-1]):
+        g = got.cpu().double()
+        g = torch.where(beyond & torch.isinf(g) & (g * want > 0), want, g)
+        assert float(((g - want).abs() - bound).max()) <= 0
+
+
+@pytest.mark.parametrize("dtype,powers", [(F16, (-14, -20, -26, -33)), (BF16, (-60, -100, -110, -118))])
+def test_scales_of_small_values(dev, dtype, powers):
+    """Values below fp16's subnormals still make scores: queries and scale as large as the values are small."""
+    for power in powers:
+        announce(f"latent small scales 2^{power} {dtype}")
+        x = lat.inputs([320, 50], [4, 2], 16, dtype, "fp8", seed=83)
+        x["page_scale"][:] = 2.0 ** power
+        x["cache"] = (torch.randn(x["cache"].shape, generator=torch.Generator().manual_seed(83)) * 20).to(x["cache"].dtype)
+        x["new"] = x["new"] * 0
+        x["scale"] = 0.002 * 2.0 ** -power
+        small_check(x, dev)
+
+
+def small_check(x, dev):
+    """Within the oracle's bound and, in fp16, what its subnormals allow: an output below 2^-14 is rounded to a multiple of 2^-24,
+    off by 2^-25 at most; and a weight p times the part r of its scale below 2^-15 is, so o is off by at most 2^-25 / r a key, of
+    the values' r |c| = 2^-15 |code|, over a sum of weights of at least 1/2."""
+    want, bound = olat.latent_attention(x["q"], x["new"], x["cache"], x["table"], x["context"], x["starts"], x["masks"],
+                                        x["scale"], x["rank"], x["page_scale"])
+    if x["q"].dtype == F16:
+        keys = int(x["context"].max()) + x["width"]
+        bound = bound + 2.0 ** -25 + 2 * keys * 2.0 ** -25 * 2.0 ** -15 * float(x["cache"].float().abs().max())
+    for got in (lat.launch(x, dev), lat.launch(crowded(x), dev)[:-1]):
+        assert float(((got.cpu().double() - want).abs() - bound).max()) <= 0
+
+
+@pytest.mark.parametrize("dtype,powers", [(F16, (-14, -20, -26, -33)), (BF16, (-60, -100, -110, -118))])
+def test_keys_of_small_values_beside_ordinary_ones(dev, dtype, powers):
+    """Queries look at one half of the columns, the round's rows have values in the other: what the small keys' scores take from
+    the rows' weights shows in ordinary numbers."""
+    for power in powers:
+        announce(f"latent small scales 2^{power} beside ordinary rows {dtype}")
+        x = lat.inputs([320, 50], [4, 2], 16, dtype, "fp8", seed=84)
+        x["page_scale"][:] = 2.0 ** power
+        x["cache"] = (torch.randn(x["cache"].shape, generator=torch.Generator().manual_seed(84)) * 20).to(x["cache"].dtype)
+        x["q"][..., :288] = 0
+        x["new"][:, 288:] = 0
+        x["scale"] = 0.006 * 2.0 ** -power
+        small_check(x, dev)
