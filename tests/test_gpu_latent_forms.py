@@ -226,3 +226,11 @@ def test_keys_of_small_values_beside_ordinary_ones(dev, dtype, powers):
         x["new"][:, 288:] = 0
         x["scale"] = 0.006 * 2.0 ** -power
         small_check(x, dev)
+
+
+def test_launches_of_many_requests_choose_for_themselves(dev):
+    """More requests than one launch takes, the first launch with much to do and the last with little."""
+    announce("latent forms over several launches")
+    n = 1100
+    x = lat.inputs([(37 * b) % 60 for b in range(n)], [b % 3 for b in range(n)], 24, BF16, rank=256, seed=85)
+    lat.check(x, lat.launch(x, dev))
