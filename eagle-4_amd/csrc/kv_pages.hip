@@ -10,8 +10,10 @@
 // Both directions are bound by HBM where there is much to move, and by one chain of dependent loads (lengths, page
 // table, rows, scale) where there is little. Measured (bf16 rows): 4 prompts of 8 heads x 128, K and V, written in 22 us (3.3
 // TB/s read and written, latency's more than HBM's: each wave's chain is five loads long, and 28 waves a CU hide most of
-// it); 64 rounds' accepted rows in 6.4 us, nearly all of it that chain and the launch; 8 long requests read in 35 us (5.6
-// TB/s, what a large copy reaches; with one chunk a lane in flight 56 us); one latent request in 5.4 us.
+// it); 64 rounds' accepted rows in 6.3 us, nearly all of it that chain and the launch; 8 long requests read in 35 us where
+// half of the pages lie in the last-level cache, as in a replay (5.7 TB/s read and written, 32 of 66 MB from HBM; with one
+// chunk a lane in flight 56 us), and in 45 us from cold caches (4.4 TB/s; a copy of 1 GiB reaches 5.15); one latent request in
+// 5.2 us.
 
 #include "common.h"
 

@@ -15,17 +15,23 @@
 //     O^T = C^T P^T in the registers' own order; C^T is read by transposing LDS loads of the same tile: a row of the cache
 //     is brought in once for both products;
 //   - a tile's scores are computed beside the last tile's output, so that the exchange costs no wait: one barrier a tile.
+// Scores, maxima, sums and outputs are in 32 bits. The weights alone are rounded to the rows' type, as the matrix cores take them
+// (relative to a maximum that moves by whole powers of two): each is off by half a step at most, as the outputs are when they
+// are stored, and the two together make the error against 64 bits 0.0023 in bf16 where the outputs' rounding makes 0.0017.
 // The launch is one workgroup a CU; each takes an equal run of all (request, row group, tile)s, so requests of any
 // lengths fill the chip. A row group cut by a run's end leaves normalised fp32 partials with their log2-sum-exps (at most two
 // a workgroup), which a second kernel merges.
 //
-// Measured (RANK 512, ROPE 64, graph replays). 64 trees of up to 16 tokens, 16 heads, contexts of 1024 to 8192, bf16: 233 us,
-// 500 TFLOP/s; four waves that each take all scores of their rows: 455. A tile of 64 rows costs about 3300 cycles, of which
+// Measured (RANK 512, ROPE 64, graph replays). 64 trees of up to 16 tokens, 16 heads, contexts of 1024 to 8192, bf16: 231 us,
+// 505 TFLOP/s; four waves that each take all scores of their rows: 455. A tile of 64 rows costs about 3300 cycles, of which
 // the products are 1100 and their operands' LDS reads about as much; the rest is the barrier (250 to 650), the exchange of
 // weights and the lookups (900 to 1600, with the lookups of each tile on their own instead of four tiles at once: 281 us).
-// 128 requests of 4 tokens, 16 heads, fp8 pages: 172 us; widening the codes is a fourth of a tile. 64 single tokens of 16
-// heads: 67 us, 4.5 TB/s. One token of 128 heads over 2048 keys: 25 us, a chain of lookups, queries and first tiles, two tiles
-// a workgroup, the partials, and 6 us of merge. Queries loaded by each lane on its own, 16 bytes of every row: 6 us more.
+// 128 requests of 4 tokens, 16 heads, fp8 pages: 175 us; widening the codes is a fourth of a tile. 64 single tokens of 16
+// heads: 67 us, 4.5 TB/s. One token of 128 heads over 2048 keys: 25.5 us. By stamps in the kernel 15.9 of them lie between the
+// first workgroup's start and the last one's end: 1.0 for the counts of tiles, 1.2 to the piece's request, 1.6 for lookups,
+// queries and first tiles, 0.7 for the zeroed tile, 1.2 an iteration (16 rows; of 2 to 4), 0.7 for the output, and in runs that
+// reach into a second row group the last four again. Launch and drain are some 4, the merge 6. Queries loaded by each lane on its
+// own, 16 bytes of every row: 6 us more.
 
 #include "attention_tile.h"
 

@@ -10,7 +10,7 @@
 // (Z = 0, which only rounding or a q that is no distribution leaves: p again.) T = 0, or a row whose maximum is not
 // finite: all mass on the argmax (first index, NaN the largest), as greedy acceptance has it.
 //
-// Decisions are comparisons, so everything that enters them is held in 64 bits: exp2 is a polynomial there (15 operations
+// Decisions are comparisons, so everything that enters them is held in 64 bits: exp2 is a polynomial there (16 operations
 // an element at the rate of 32-bit ones, against about 10 with the hardware's 32-bit exp2, whose error would flip one
 // comparison in 10^7, and of a flat row's running sums far more).
 //
@@ -18,7 +18,7 @@
 //   - statistics: of every chunk of a row its maximum and its mass relative to that. All rows of all trees at once, or the
 //     trees' first rows and later those that may still be visited: the walk visits a few of them, but one after another,
 //     and a workgroup that reads its request's rows on its own has one CU's rate (vocabulary 151936, bf16: one tree of
-//     16 rows 105 to 232 us that way, by the walk's length, against 19; 64 trees of up to 16 rows 228 against 85);
+//     16 rows 105 to 232 us that way, by the walk's length, against 20; 64 trees of up to 16 rows 228 against 87);
 //   - the walk, a workgroup per request: the rows' sums out of the chunks', then the decisions, a lane a child. Ends with the
 //     final token: the chunks' running sum leads to one chunk, which is read. With draft probabilities a rejection needs the
 //     residual's mass: the walk stops there and leaves its state;
@@ -28,9 +28,9 @@
 // for 16 trees of 16 over 151936. Continuing the walk in the residual's last workgroup instead of a launch of its own takes a
 // fence of every workgroup, and those cost more (95 us instead of 71). The walk's workgroup has 512 threads for those rows:
 // with 256, 89 us instead of 76 for the 12 trees; with 1024, 3% off the trees and 10% on single users' walks.
-// What bounds it: the statistics by their 64-bit operations (82 us for 750 rows, 44 of them the logits' own; a table
+// What bounds it: the statistics by their 64-bit operations (87 us for 750 rows, 44 of them the logits' own; a table
 // of 32 roots with a polynomial of degree 4 has a third fewer operations and is no faster for its lookups; one chunk
-// loaded ahead of another, 93 us), the walk by its chain of dependent loads (12 us for one request, 22 among 64).
+// loaded ahead of another, 93 us), the walk by its chain of dependent loads (13 us for one request, 21 among 64).
 
 #include "common.h"
 
@@ -769,7 +769,7 @@ int launch(const eagle4_sample_tree_args& a, hipStream_t s) {
   const int pairs = a.probs == nullptr ? 0 : (a.width - 1 < kPairs ? a.width - 1 : kPairs);
   // Without draft probabilities a walk of many rows goes in two: the trees' first rows, then what is left of each tree under
   // the child that was accepted. Two launches more, but a fraction of the rows (64 requests, vocabulary 151936, trees of
-  // 16, 39000 chunks: 95 instead of 135 us; trees of 8, 19000: 76 and 79; 16 requests, trees of 16, 9700: 58 and 51).
+  // 16 rows each, 39000 chunks: 95 instead of 135 us; trees of 8, 19000: 76 and 79; 16 requests, trees of 16, 9700: 58 and 51).
   const bool two = a.probs == nullptr && a.width > 1 && stats >= kTwoSteps;
   const auto chunks_of = [&](int rows, int first) {
     sample_chunks_of<T><<<dim3(e4::ceil_div(split.chunks, kWaves), rows, a.num_reqs), kThreads, 0, s>>>(a, split, first);

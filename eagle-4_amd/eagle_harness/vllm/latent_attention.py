@@ -38,6 +38,10 @@ def latent_verify_attention(
     ``max_query_len`` (<= 64) rows. bf16 or fp16, the cache of the rows' dtype or fp8-e4m3 with ``latent_scale``, one fp32
     scale a page (``[blocks]``, or ``[blocks, 1]`` as :func:`~eagle_harness.vllm.kv_pages.write_kv_pages` keeps it). rank 256 or
     512, rope 64. A row that sees no key gives zeros; a position whose page id lies outside the cache is not seen.
+
+    Scores, sums and outputs are held in 32 bits; the softmax's weights are rounded to the rows' dtype for the second
+    product, as :func:`verify_attention`'s are. The contexts decide how the work is shared out: a block table may be as wide
+    as the longest model length, at no cost and with the same bits.
     """
     if q.dim() != 3 or latent_new.dim() != 2 or latent_cache.dim() != 3 or out.dim() != 3:
         raise ValueError("latent_verify_attention: q [tokens, heads, dim], latent_new [tokens, dim], latent_cache "

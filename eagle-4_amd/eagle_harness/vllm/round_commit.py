@@ -24,6 +24,9 @@ class KvCompactor:
     2 * head_dim) with K then V of a token and head adjacent; ``block_tables[i]`` and ``table_block_sizes[i]``: that
     layer's KV cache group's persistent [num_reqs, max_blocks] int32 block table (the batch's rows, as the forward got
     them) and its tokens per block.
+
+    Rows are moved byte for byte. In an fp8 cache with a scale per page they would change their value between pages: there
+    :func:`~eagle_harness.vllm.kv_pages.write_kv_pages` puts the accepted rows in place instead, from the round's 16-bit rows.
     """
 
     def __init__(
