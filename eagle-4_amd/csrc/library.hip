@@ -27,6 +27,7 @@ extern "C" int64_t eagle4_args_size(int which) {
     case 18: return sizeof(eagle4_read_kv_args);
     case 19: return sizeof(eagle4_sample_tree_args);
     case 20: return sizeof(eagle4_latent_attn_args);
+    case 21: return sizeof(eagle4_sample_rows_args);
     default: return -1;
   }
 }

@@ -1,0 +1,733 @@
+// Rows of logits under temperature, top-k, top-p and min-p on gfx950: tokens drawn from given uniform numbers, the
+// distribution they are drawn from, or the row with what the rules leave out at -inf.
+//
+// Mathematics. w_i = exp((l_i - max l) / T). The order: logits descending, the lower index first among equals. Every rule
+// keeps a beginning of it: top-k its first k tokens, min-p those with w >= min_p, top-p, of what these two leave, with mass
+// Z1, the tokens with less than top_p Z1 before them. The first token is always kept. So a row's outcome is one place of the
+// order, the cut (a logit and, among its equals, an index), and the mass Z up to it. A draw is the first token of the
+// order whose running mass exceeds coin Z. T not above 0, or a maximum that is not finite: the argmax alone.
+//
+// Masses are whole numbers, w in units of 2^-45 rounded once from 64 bits: their sums are exact, the same in any order
+// and by any path below, and a row of 2^18 tokens stays under 2^64. What a token's rounding (2^-46 of the row's largest
+// mass) can move is a comparison whose two sides are that close.
+//
+// A workgroup takes a row. Where top-k or min-p leave few tokens, they bound the row's kept part by a logit before any weight
+// is computed: the k-th largest of the threads' own maxima is not above the row's k-th logit, and min_p is one. What lies
+// above the bound is gathered into LDS, sorted, and everything is decided there. Otherwise the row's masses are summed
+// into 2048 bins of log2 w (1/32 each), and a place of the order is found in its bin: gathered and sorted where the
+// bin holds few tokens, divided into 2048 ranges of logits again where it holds many.
+
+#include "vocab_row.h"
+
+namespace {
+
+using namespace e4vocab;
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int NT = 1024, kWaves = NT / 64;
+constexpr int kBins = 2048, kList = 2048;
+constexpr float kBinsPerOctave = 32.f;
+constexpr double kUnit = 0x1p45;
+constexpr uint32_t kLowestKey = 0x007fffffu;  // of -inf
+
+// A logit as a whole number of the same order; NaN the largest, both zeros alike.
+E4_DEV uint32_t key_of(float x) {
+  if (x != x) return 0xffffffffu;
+  const uint32_t b = __float_as_uint(x + 0.f);
+  return b ^ (b >> 31 ? 0xffffffffu : 0x80000000u);
+}
+E4_DEV float value_of(uint32_t key) { return __uint_as_float(key ^ (key >> 31 ? 0x80000000u : 0xffffffffu)); }
+
+// A token's mass in units of 2^-45.
+E4_DEV uint64_t mass_of(float x, float top, double c) {
+  const double y = __builtin_fma(weight_of(x, top, c), kUnit, 0x1p52);  // rounds to a whole number in the low 52 bits
+  return __builtin_bit_cast(uint64_t, y) & 0xfffffffffffffull;
+}
+// Its bin; not decreasing as x falls.
+E4_DEV int bin_of(float x, float top, double c) {
+  const double t = (static_cast<double>(x) - static_cast<double>(top)) * (c * -static_cast<double>(kBinsPerOctave));
+  return static_cast<int>(__builtin_fmin(t == t ? t : 1e9, kBins - 1));  // (NaN: -inf times a scale of 0)
+}
+
+struct Shared {
+  uint64_t mass[kBins];   // running sums over the bins
+  uint32_t count[kBins];
+  union {
+    struct {
+      uint64_t entry[kList];  // (~key << 32) | index: ascending is the order
+      uint64_t run[kList];    // running masses
+    } list;
+    struct {
+      uint64_t mass[kBins];
+      uint32_t count[kBins];
+    } sub;
+    float maxima[NT];
+  };
+  u32x4 ends[2];
+  uint64_t wave64[kWaves];
+  uint32_t wave32[kWaves];
+  uint32_t listed;
+  int found;
+  float thr;
+  uint64_t sum;
+};
+
+E4_DEV bool in_row(int e, int vocab) { return static_cast<uint32_t>(e) < static_cast<uint32_t>(vocab); }
+
+// A row as a workgroup's threads pass over it: the vectors wholly inside it from memory, the elements before the first and
+// behind the last of those (at most one vector at each end) out of LDS, where they are put once.
+template <typename T>
+struct Rows {
+  static constexpr int VEC = Row<T>::VEC, U = 4;  // U vectors of a thread on their way together
+  using S = typename T::storage;
+  Row<T> row;
+  int begin, end;  // whole vectors
+  u32x4* ends;     // LDS, two
+  float top;
+  double c;
+  int tid;
+
+  E4_DEV Rows(const void* logits, int64_t n, int64_t stride, int vocab, float temperature, u32x4* lds, int tid_)
+      : row(logits, n, stride, vocab), ends(lds), top(0.f), c(scale_of(temperature)), tid(tid_) {
+    begin = row.past > 0 ? 1 : 0;
+    end = (vocab + row.past) / VEC;
+    if (tid < 2 * VEC) {
+      const int e = end_first(tid / VEC) + tid % VEC;
+      reinterpret_cast<S*>(ends)[tid] = in_row(e, vocab) ? row.p[e] : T::from_f32(-INFINITY);
+    }
+    __syncthreads();
+  }
+  // The first element of an end's vector; the row's size where there is none.
+  E4_DEV int end_first(int side) const {
+    if (side == 0) return row.past > 0 ? row.first(0) : row.vocab;
+    return end >= begin && end < row.vectors ? row.first(end) : row.vocab;
+  }
+
+  // f(first element, vector) for every vector, a thread's in ascending order; -inf outside the row.
+  template <typename F>
+  E4_DEV void each_vector(F&& f) const {
+    const float none = -INFINITY;
+    uint32_t low = __float_as_uint(none);
+    if constexpr (VEC == 8) low = T::pack(none, none);
+    for (int v0 = begin; v0 < end; v0 += U * NT) {
+      u32x4 w[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int v = v0 + u * NT + tid;
+        w[u] = u32x4{low, low, low, low};
+        if (v < end) w[u] = row.raw(v);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int v = v0 + u * NT + tid;
+        f(v < end ? row.first(v) : row.vocab, w[u]);
+      }
+    }
+    if (tid < 2) f(end_first(tid), ends[tid]);
+  }
+
+  // f(first element, values)
+  template <typename F>
+  E4_DEV void each(F&& f) const {
+    each_vector([&](int e0, const u32x4& w) {
+      float x[VEC];
+      Row<T>::widen(w, x);
+      f(e0, x);
+    });
+  }
+
+  // f(element, value) for every element of the row, a word of a vector at a time: what takes a weight of each element would
+  // not fit the registers for a whole vector at once.
+  template <typename F>
+  E4_DEV void each_element(F&& f) const {
+    each_vector([&](int e0, u32x4 now) {
+#pragma unroll 1
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (VEC == 4) {
+          if (in_row(e0 + i, row.vocab)) f(e0 + i, __uint_as_float(now[0]));
+        } else {
+          const int e = e0 + 2 * i;
+          if (in_row(e, row.vocab)) f(e, T::to_f32(static_cast<uint16_t>(now[0])));
+          if (in_row(e + 1, row.vocab)) f(e + 1, T::to_f32(static_cast<uint16_t>(now[0] >> 16)));
+        }
+        now = u32x4{now[1], now[2], now[3], now[0]};
+      }
+    });
+  }
+};
+
+E4_DEV uint64_t shfl_up64(uint64_t x, int d) {
+  const uint32_t lo = __shfl_up(static_cast<uint32_t>(x), d, 64), hi = __shfl_up(static_cast<uint32_t>(x >> 32), d, 64);
+  return (static_cast<uint64_t>(hi) << 32) | lo;
+}
+template <typename U>
+E4_DEV U wave_scan(U x, int lane) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    U o;
+    if constexpr (sizeof(U) == 8)
+      o = shfl_up64(x, d);
+    else
+      o = __shfl_up(x, d, 64);
+    if (lane >= d) x += o;
+  }
+  return x;
+}
+// Inclusive running sum over the workgroup's threads; every thread calls it.
+template <typename U>
+E4_DEV U block_scan(U x, U* part, int tid) {
+  const int lane = tid & 63, wave = tid >> 6;
+  x = wave_scan(x, lane);
+  __syncthreads();  // (part may still be read)
+  if (lane == 63) part[wave] = x;
+  __syncthreads();
+  for (int i = 0; i < wave; ++i) x += part[i];
+  return x;
+}
+
+// The bins' counts and masses become running sums.
+E4_DEV void scan_bins(uint64_t* mass, uint32_t* count, Shared& s, int tid) {
+  constexpr int P = kBins / NT;
+  uint64_t m[P], ms = 0;
+  uint32_t k[P], ks = 0;
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    ms += mass[P * tid + i];
+    m[i] = ms;
+    ks += count[P * tid + i];
+    k[i] = ks;
+  }
+  const uint64_t mb = block_scan(ms, s.wave64, tid) - ms;
+  const uint32_t kb = block_scan(ks, s.wave32, tid) - ks;
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    mass[P * tid + i] = mb + m[i];
+    count[P * tid + i] = kb + k[i];
+  }
+  __syncthreads();
+}
+
+// The first bin whose running sum exceeds `target` (the last bin where none does).
+template <typename U>
+E4_DEV int find_bin(const U* run, U target, Shared& s, int tid) {
+  constexpr int P = kBins / NT;
+  if (tid == 0) s.found = kBins - 1;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    const int b = P * tid + i;
+    if (run[b] > target && (b == 0 || run[b - 1] <= target)) s.found = b;
+  }
+  __syncthreads();
+  const int b = s.found;
+  __syncthreads();
+  return b;
+}
+
+// The lowest key in [lo, hi] for which `ok` holds, given that it holds for hi and for every key above one that it
+// holds for. By one wave: 64 probes a round.
+template <typename F>
+E4_DEV uint32_t lowest_key(uint32_t lo, uint32_t hi, int lane, F&& ok) {
+  while (lo < hi) {
+    const uint64_t span = static_cast<uint64_t>(hi) - lo;
+    const uint32_t at = lo + static_cast<uint32_t>(span * lane / 64);  // lane 0: lo; below hi
+    const uint64_t good = __ballot(ok(at));
+    if (good & 1) return lo;
+    const int first = good == 0 ? 64 : __builtin_ctzll(good);
+    hi = first == 64 ? hi : lo + static_cast<uint32_t>(span * first / 64);
+    lo = lo + static_cast<uint32_t>(span * (first - 1) / 64) + 1;
+  }
+  return hi;
+}
+
+// Sorts s.list.entry[0 .. n) ascending; n at most kList. Every thread calls it.
+E4_DEV void sort_list(Shared& s, int n, int tid) {
+  int size = 64;
+  while (size < n) size <<= 1;
+  for (int i = n + tid; i < size; i += NT) s.list.entry[i] = ~0ull;
+  __syncthreads();
+  if (size == 64) {  // one wave, in registers
+    if (tid < 64) {
+      uint64_t x = s.list.entry[tid];
+#pragma unroll
+      for (int k = 2; k <= 64; k <<= 1)
+#pragma unroll
+        for (int j = k >> 1; j > 0; j >>= 1) {
+          const uint32_t lo = __shfl_xor(static_cast<uint32_t>(x), j, 64), hi = __shfl_xor(static_cast<uint32_t>(x >> 32), j, 64);
+          const uint64_t o = (static_cast<uint64_t>(hi) << 32) | lo;
+          const bool keep_low = ((tid & j) == 0) == ((tid & k) == 0);
+          x = keep_low == (o < x) ? o : x;
+        }
+      s.list.entry[tid] = x;
+    }
+    __syncthreads();
+    return;
+  }
+  for (int k = 2; k <= size; k <<= 1)
+    for (int j = k >> 1; j > 0; j >>= 1) {
+      for (int p = tid; p < size / 2; p += NT) {
+        const int i = 2 * p - (p & (j - 1)), o = i + j;
+        const uint64_t a = s.list.entry[i], b = s.list.entry[o];
+        if ((a > b) == ((i & k) == 0)) {
+          s.list.entry[i] = b;
+          s.list.entry[o] = a;
+        }
+      }
+      __syncthreads();
+    }
+}
+
+E4_DEV uint32_t entry_key(uint64_t e) { return ~static_cast<uint32_t>(e >> 32); }
+
+// Gathers the elements with lo <= value <= hi, sorts them and leaves their running masses from `base` on. How many there
+// are (past kList: nothing is listed).
+template <typename T>
+E4_DEV int list_range(const Rows<T>& r, Shared& s, float lo, float hi, uint64_t base) {
+  const int tid = r.tid;
+  __syncthreads();
+  if (tid == 0) s.listed = 0;
+  __syncthreads();
+  r.each([&](int e0, const float(&x)[Row<T>::VEC]) {
+#pragma unroll
+    for (int i = 0; i < Row<T>::VEC; ++i)
+      if (x[i] >= lo && x[i] <= hi && in_row(e0 + i, r.row.vocab)) {
+        const uint32_t at = atomicAdd(&s.listed, 1u);
+        if (at < kList) s.list.entry[at] = (static_cast<uint64_t>(~key_of(x[i])) << 32) | static_cast<uint32_t>(e0 + i);
+      }
+  });
+  __syncthreads();
+  const int n = s.listed;
+  if (n > kList) return n;
+  sort_list(s, n, tid);
+  constexpr int P = kList / NT;
+  uint64_t m[P], sum = 0;
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    const int at = P * tid + i;
+    sum += at < n ? mass_of(value_of(entry_key(s.list.entry[at])), r.top, r.c) : 0;
+    m[i] = sum;
+  }
+  const uint64_t before = block_scan(sum, s.wave64, tid) - sum + base;
+#pragma unroll
+  for (int i = 0; i < P; ++i) s.list.run[P * tid + i] = before + m[i];
+  __syncthreads();
+  return n;
+}
+
+// The first of the list's n entries whose running mass exceeds `target`; n - 1 where none does.
+E4_DEV int list_find(const Shared& s, int n, uint64_t target) {
+  int lo = 0, hi = n - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (s.list.run[mid] > target)
+      hi = mid;
+    else
+      lo = mid + 1;
+  }
+  return lo;
+}
+
+struct Place {
+  float x;
+  int index;
+  uint64_t run;  // mass up to it, its own with it
+};
+
+// The element of the row that is `rank`-th (from 0) by index among those equal to x.
+template <typename T>
+E4_DEV int nth_equal(const Rows<T>& r, Shared& s, float x, uint32_t rank) {
+  constexpr int VEC = Row<T>::VEC;
+  const int tid = r.tid;
+  uint32_t before = 0;
+  if (tid == 0) s.found = 0;
+  for (int v0 = 0; v0 < r.row.vectors; v0 += NT) {
+    const int v = v0 + tid;
+    u32x4 w = r.ends[v == 0 && r.begin == 1 ? 0 : 1];
+    if (v >= r.begin && v < r.end) w = r.row.raw(v);
+    const int e0 = v < r.row.vectors ? r.row.first(v) : r.row.vocab;
+    float y[VEC];
+    Row<T>::widen(w, y);
+    uint32_t k = 0;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) k += y[i] == x && in_row(e0 + i, r.row.vocab);
+    uint32_t at = before + block_scan(k, s.wave32, tid) - k;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i)
+      if (y[i] == x && in_row(e0 + i, r.row.vocab)) {
+        if (at == rank) s.found = e0 + i;
+        ++at;
+      }
+    __syncthreads();
+    uint32_t all = 0;
+    for (int i = 0; i < kWaves; ++i) all += s.wave32[i];
+    before += all;
+    if (before > rank) break;
+  }
+  __syncthreads();
+  const int e = s.found;
+  __syncthreads();
+  return e;
+}
+
+// The first element of the order whose running mass (kByMass) or count exceeds `target`, which is below the row's.
+template <bool kByMass, typename T>
+E4_DEV Place locate(const Rows<T>& r, Shared& s, uint64_t target) {
+  const int tid = r.tid, lane = tid & 63;
+  int b = kByMass ? find_bin(s.mass, target, s, tid) : find_bin(s.count, static_cast<uint32_t>(target), s, tid);
+  uint64_t mass = b > 0 ? s.mass[b - 1] : 0;  // before the range
+  uint32_t count = b > 0 ? s.count[b - 1] : 0, inside = s.count[b] - count;
+  const uint32_t top = key_of(r.top);
+  // the bin's keys; every wave finds them for itself
+  uint32_t lo = b == kBins - 1 ? kLowestKey
+                               : lowest_key(kLowestKey, top, lane, [&](uint32_t k) { return bin_of(value_of(k), r.top, r.c) <= b; });
+  uint32_t hi = b == 0 ? top
+                       : lowest_key(kLowestKey, top, lane, [&](uint32_t k) { return bin_of(value_of(k), r.top, r.c) < b; }) - 1;
+  while (inside > kList && lo < hi) {
+    const int shift = 32 - __builtin_clz(hi - lo) > 11 ? 32 - __builtin_clz(hi - lo) - 11 : 0;
+    __syncthreads();
+    for (int i = tid; i < kBins; i += NT) {
+      s.sub.mass[i] = 0;
+      s.sub.count[i] = 0;
+    }
+    __syncthreads();
+    r.each_element([&](int, float x) {
+      const uint32_t k = key_of(x);
+      if (k >= lo && k <= hi) {
+        const uint32_t at = (hi - k) >> shift;
+        atomicAdd(reinterpret_cast<unsigned long long*>(&s.sub.mass[at]), mass_of(x, r.top, r.c));
+        atomicAdd(&s.sub.count[at], 1u);
+      }
+    });
+    __syncthreads();
+    scan_bins(s.sub.mass, s.sub.count, s, tid);
+    const int at = kByMass ? find_bin(s.sub.mass, target - mass, s, tid) : find_bin(s.sub.count, static_cast<uint32_t>(target) - count, s, tid);
+    const uint64_t m0 = at > 0 ? s.sub.mass[at - 1] : 0;
+    const uint32_t c0 = at > 0 ? s.sub.count[at - 1] : 0;
+    inside = s.sub.count[at] - c0;
+    mass += m0;
+    count += c0;
+    const uint32_t first = hi - (static_cast<uint32_t>(at) << shift);  // the range's highest key
+    const uint32_t wide = (1u << shift) - 1;
+    lo = first - lo < wide ? lo : first - wide;
+    hi = first;
+    __syncthreads();
+  }
+  Place p;
+  if (inside > kList) {  // one logit, many times
+    p.x = value_of(lo);
+    const uint64_t each = mass_of(p.x, r.top, r.c);
+    uint64_t rank = kByMass ? (each > 0 ? (target - mass) / each : 0) : target - count;
+    if (rank >= inside) rank = inside - 1;
+    p.run = mass + (rank + 1) * each;
+    p.index = nth_equal(r, s, p.x, static_cast<uint32_t>(rank));
+    return p;
+  }
+  // (-0's key belongs to no element, but -0 >= 0)
+  const int n = list_range(r, s, value_of(lo), value_of(hi == 0x7fffffffu ? hi - 1 : hi), mass);
+  int at = kByMass ? list_find(s, n, target) : static_cast<int>(static_cast<uint32_t>(target) - count);
+  at = at < n ? at : n - 1;
+  p.x = value_of(entry_key(s.list.entry[at]));
+  p.index = static_cast<int>(static_cast<uint32_t>(s.list.entry[at]));
+  p.run = s.list.run[at];
+  __syncthreads();
+  return p;
+}
+
+// The place of a draw's running mass: what exceeds coin Z (whole masses: what exceeds its whole part).
+E4_DEV uint64_t target_of(float coin, uint64_t z) {
+  const double t = static_cast<double>(coin) * static_cast<double>(z);
+  if (!(t > 0.0)) return 0;
+  const uint64_t u = t < 0x1p63 ? static_cast<uint64_t>(t) : z;
+  return u < z ? u : z - 1;
+}
+// The mass that top-p asks for: the first token whose running mass exceeds this is the last one kept.
+E4_DEV uint64_t nucleus_of(float p, uint64_t z) {
+  const double t = __builtin_ceil(static_cast<double>(p) * static_cast<double>(z));
+  if (!(t > 1.0)) return 0;
+  const uint64_t u = t < 0x1p63 ? static_cast<uint64_t>(t) : z;
+  return (u < z ? u : z) - 1;
+}
+
+struct Cut {
+  float x;  // kept: logits above it, and its equals up to the index
+  int index;
+  bool single;  // the index alone
+};
+
+// Writes a vector's worth of outputs: 16-byte stores where all of them are inside and lie on 16 bytes.
+template <typename U, int N>
+E4_DEV void store_vector(U* out, int e0, int vocab, const U (&y)[N]) {
+  U* const p = out + e0;
+  if (e0 >= 0 && e0 + N <= vocab && reinterpret_cast<uintptr_t>(p) % 16 == 0 && N * sizeof(U) % 16 == 0) {
+    constexpr int W = N * sizeof(U) / 16 > 0 ? N * sizeof(U) / 16 : 1;
+#pragma unroll
+    for (int k = 0; k < W; ++k) {
+      u32x4 w;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (sizeof(U) == 4)
+          w[i] = __builtin_bit_cast(uint32_t, y[(4 * k + i) % N]);
+        else
+          w[i] = static_cast<uint32_t>(y[(8 * k + 2 * i) % N]) | static_cast<uint32_t>(y[(8 * k + 2 * i + 1) % N]) << 16;
+      }
+      __builtin_nontemporal_store(w, reinterpret_cast<u32x4*>(p) + k);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (in_row(e0 + i, vocab)) p[i] = y[i];
+  }
+}
+
+template <typename T, typename P>
+E4_DEV void write_probs(const Rows<T>& r, const Cut& cut, uint64_t z, typename P::storage* out) {
+  constexpr int VEC = Row<T>::VEC;
+  const double share = kUnit / static_cast<double>(z);
+  r.each([&](int e0, const float(&x)[VEC]) {
+    typename P::storage y[VEC];
+    float left[VEC];  // the kept logits, the others at -inf
+    bool any = false;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      const bool kept = cut.single ? e0 + i == cut.index : x[i] > cut.x || (x[i] == cut.x && e0 + i <= cut.index);
+      any |= kept;
+      left[i] = !kept ? -INFINITY : cut.single ? 0.f : x[i];
+      y[i] = P::from_f32(0.f);
+    }
+    if (any) {
+#pragma unroll 1
+      for (int j = 0; j < VEC; ++j) {  // one weight at a time, for the registers
+        const float w = left[0] == -INFINITY ? 0.f : cut.single ? 1.f : static_cast<float>(weight_of(left[0], r.top, r.c) * share);
+#pragma unroll
+        for (int i = 0; i + 1 < VEC; ++i) {
+          left[i] = left[i + 1];
+          y[i] = y[i + 1];
+        }
+        y[VEC - 1] = P::from_f32(w);
+      }
+    }
+    store_vector(out, e0, r.row.vocab, y);
+  });
+}
+
+template <typename T>
+E4_DEV void write_logits(const Rows<T>& r, const Cut& cut, typename T::storage* out) {
+  constexpr int VEC = Row<T>::VEC;
+  r.each([&](int e0, const float(&x)[VEC]) {
+    typename T::storage y[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      const bool kept = cut.single ? e0 + i == cut.index : x[i] > cut.x || (x[i] == cut.x && e0 + i <= cut.index);
+      y[i] = T::from_f32(kept ? x[i] : -INFINITY);
+    }
+    store_vector(out, e0, r.row.vocab, y);
+  });
+}
+
+template <typename T>
+__global__ __launch_bounds__(NT) void sample_rows_kernel(const eagle4_sample_rows_args a) {
+  __shared__ Shared s;
+  constexpr int VEC = Row<T>::VEC;
+  const int64_t n = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t entry = a.entries.ptr != nullptr ? e4::ld(a.entries, n) : n;
+  if (entry < 0 || entry >= a.num_entries) return;  // a padded row
+  const float temperature = a.temperature[entry];
+  const int k = a.top_k != nullptr ? a.top_k[entry] : 0;
+  const float p = a.top_p != nullptr ? a.top_p[entry] : 1.f, m = a.min_p != nullptr ? a.min_p[entry] : 0.f;
+
+  Rows<T> r(a.logits, n, a.stride_row, a.vocab, temperature, s.ends, tid);
+  float mine = -INFINITY;
+  r.each([&](int, const float(&x)[VEC]) {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) mine = __builtin_elementwise_maximum(mine, x[i]);
+  });
+  {
+    const float w = wave_max(mine);
+    if (lane == 0) s.wave32[wave] = __float_as_uint(w);
+    __syncthreads();
+    float top = __uint_as_float(s.wave32[0]);
+    for (int i = 1; i < kWaves; ++i) top = __builtin_elementwise_maximum(top, __uint_as_float(s.wave32[i]));
+    r.top = top;
+    __syncthreads();
+  }
+  Cut cut{-INFINITY, INT32_MAX, false};
+  uint64_t z = static_cast<uint64_t>(kUnit);
+  int64_t* const tokens = a.tokens != nullptr ? a.tokens + n * a.draws : nullptr;
+  const float* const coins = a.coins != nullptr ? a.coins + n * a.draws : nullptr;
+
+  if (!(temperature > 0.f) || !(r.top < INFINITY) || r.top == -INFINITY) {  // the argmax alone
+    if (tid == 0) s.found = INT32_MAX;
+    __syncthreads();
+    int at = INT32_MAX;
+    r.each([&](int e0, const float(&x)[VEC]) {
+#pragma unroll
+      for (int i = VEC - 1; i >= 0; --i) {
+        const bool hit = r.top != r.top ? x[i] != x[i] : x[i] == r.top;
+        if (hit && in_row(e0 + i, a.vocab) && e0 + i < at) at = e0 + i;
+      }
+    });
+    if (at != INT32_MAX) atomicMin(&s.found, at);
+    __syncthreads();
+    cut.single = true;
+    cut.index = s.found;
+    if (tokens != nullptr && tid < a.draws) tokens[tid] = cut.index;
+  } else {
+    const bool by_k = k > 0 && k < a.vocab, by_m = m > 0.f, by_p = p < 1.f;
+    // min-p: the lowest logit whose weight reaches it
+    float lowest = -INFINITY;
+    if (by_m) {
+      const double want = m < 1.f ? static_cast<double>(m) : 1.0;
+      lowest = value_of(lowest_key(kLowestKey, key_of(r.top), lane,
+                                   [&](uint32_t key) { return weight_of(value_of(key), r.top, r.c) >= want; }));
+    }
+    int listed = kList + 1;  // the list holds the order's beginning
+    uint64_t z1 = 0;         // the mass that top-p is taken of, where it is known
+    float bound = lowest;
+    if (by_k && k <= NT) {  // the k-th largest of the threads' maxima
+      s.maxima[tid] = mine;
+      __syncthreads();
+      int rank = 0;
+      for (int i = 0; i < NT; i += 4) {
+        const f32x4 o = *reinterpret_cast<const f32x4*>(&s.maxima[i]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) rank += o[j] > mine || (o[j] == mine && i + j < tid);
+      }
+      if (rank == k - 1) s.thr = mine;
+      __syncthreads();
+      bound = s.thr > bound ? s.thr : bound;
+      __syncthreads();
+    }
+    if (by_m || (by_k && k <= NT)) listed = list_range(r, s, bound, r.top, 0);
+    const bool asked = by_k || by_m || by_p || tokens != nullptr || a.out_kind == EAGLE4_ROWS_PROBS;
+    if (asked && listed > kList) {
+      for (int i = tid; i < kBins; i += NT) {
+        s.mass[i] = 0;
+        s.count[i] = 0;
+      }
+      __syncthreads();
+      r.each_element([&](int, float x) {
+        const int b = bin_of(x, r.top, r.c);
+        atomicAdd(reinterpret_cast<unsigned long long*>(&s.mass[b]), mass_of(x, r.top, r.c));
+        atomicAdd(&s.count[b], 1u);
+      });
+      __syncthreads();
+      scan_bins(s.mass, s.count, s, tid);
+      z1 = s.mass[kBins - 1];
+      if (!by_k && !by_m && by_p) {  // the bins say where top-p's cut is at most
+        const int b = find_bin(s.mass, nucleus_of(p, z1), s, tid);
+        if (s.count[b] <= kList) {
+          const uint32_t low = lowest_key(kLowestKey, key_of(r.top), lane,
+                                          [&](uint32_t key) { return bin_of(value_of(key), r.top, r.c) <= b; });
+          listed = list_range(r, s, value_of(low), r.top, 0);
+        }
+      }
+    }
+    if (listed <= kList) {  // everything is decided in the list
+      int kept = listed;
+      if (by_k && k < kept) kept = k;
+      if (by_m) {
+        int lo = 0, hi = kept;  // the entries that min-p leaves
+        while (lo < hi) {
+          const int mid = (lo + hi) >> 1;
+          if (value_of(entry_key(s.list.entry[mid])) >= lowest)
+            lo = mid + 1;
+          else
+            hi = mid;
+        }
+        kept = m > 1.f ? 1 : lo;
+      }
+      if (kept < 1) kept = 1;
+      if (by_k || by_m) z1 = s.list.run[kept - 1];
+      if (by_p) kept = list_find(s, kept, nucleus_of(p, z1)) + 1;
+      z = s.list.run[kept - 1];
+      const uint64_t last = s.list.entry[kept - 1];
+      cut.x = value_of(entry_key(last));
+      cut.index = static_cast<int>(static_cast<uint32_t>(last));
+      if (tokens != nullptr && tid < a.draws) {
+        const int at = list_find(s, kept, target_of(coins[tid], z));
+        tokens[tid] = static_cast<int64_t>(static_cast<uint32_t>(s.list.entry[at]));
+      }
+    } else if (asked) {
+      if (by_k) {
+        const Place at = locate<false>(r, s, static_cast<uint64_t>(k) - 1);
+        cut.x = at.x;
+        cut.index = at.index;
+        z1 = at.run;
+      }
+      if (by_m && (cut.x < lowest || m > 1.f)) {  // min-p's cut comes first (its first token is the order's)
+        uint64_t sum = 0;
+        r.each_element([&](int, float x) {
+          if (x >= lowest) sum += mass_of(x, r.top, r.c);
+        });
+        sum = block_scan(sum, s.wave64, tid);
+        if (tid == NT - 1) s.sum = sum;
+        __syncthreads();
+        cut.x = lowest;
+        cut.index = INT32_MAX;
+        z1 = s.sum;
+        __syncthreads();
+        if (m > 1.f) {
+          const Place at = locate<false>(r, s, 0);
+          cut.index = at.index;
+          z1 = at.run;
+        }
+      }
+      z = z1;
+      if (by_p) {
+        const Place at = locate<true>(r, s, nucleus_of(p, z1));
+        cut.x = at.x;
+        cut.index = at.index;
+        z = at.run;
+      }
+      if (tokens != nullptr)
+        for (int d = 0; d < a.draws; ++d) {
+          const Place at = locate<true>(r, s, target_of(coins[d], z));
+          if (tid == 0) tokens[d] = at.index;
+        }
+    }
+  }
+  if (a.out == nullptr) return;
+  if (a.out_kind == EAGLE4_ROWS_LOGITS) {
+    write_logits(r, cut, static_cast<typename T::storage*>(a.out) + n * a.stride_out);
+  } else if (a.out_dtype == EAGLE4_F32) {
+    write_probs<T, e4::F32>(r, cut, z, static_cast<float*>(a.out) + n * a.stride_out);
+  } else if (a.out_dtype == EAGLE4_BF16) {
+    write_probs<T, e4::Bf16>(r, cut, z, static_cast<uint16_t*>(a.out) + n * a.stride_out);
+  } else {
+    write_probs<T, e4::F16>(r, cut, z, static_cast<uint16_t*>(a.out) + n * a.stride_out);
+  }
+}
+
+template <typename T>
+int launch(const eagle4_sample_rows_args& a, hipStream_t s) {
+  sample_rows_kernel<T><<<static_cast<unsigned>(a.rows), NT, 0, s>>>(a);
+  return E4_LAUNCH_STATUS();
+}
+
+}  // namespace
+
+extern "C" int eagle4_sample_rows(const eagle4_sample_rows_args* a, void* stream) {
+  if (a->rows == 0) return EAGLE4_OK;
+  const auto lies = [](const void* p, int64_t stride, int dtype) {  // elements on their own size
+    return reinterpret_cast<uintptr_t>(p) % (dtype == EAGLE4_F32 ? 4 : 2) == 0 && stride >= 0;
+  };
+  if (a->rows < 0 || a->rows > (1 << 20) || a->vocab < 1 || a->vocab > EAGLE4_ROWS_MAX_VOCAB || a->num_entries < 1 ||
+      a->logits == nullptr || a->temperature == nullptr || !e4::is_float_dtype(a->dtype) ||
+      !lies(a->logits, a->stride_row, a->dtype) || a->draws < 0 || a->draws > EAGLE4_ROWS_MAX_DRAWS ||
+      (a->entries.ptr != nullptr && !e4::is_index_dtype(a->entries.dtype)) || (a->tokens == nullptr) != (a->draws == 0) ||
+      (a->coins == nullptr) != (a->draws == 0) || (a->tokens == nullptr && a->out == nullptr))
+    return EAGLE4_NOT_COVERED;
+  if (a->out != nullptr &&
+      ((a->out_kind != EAGLE4_ROWS_PROBS && a->out_kind != EAGLE4_ROWS_LOGITS) || !e4::is_float_dtype(a->out_dtype) ||
+       (a->out_kind == EAGLE4_ROWS_LOGITS && a->out_dtype != a->dtype) || !lies(a->out, a->stride_out, a->out_dtype) ||
+       (a->rows > 1 && a->stride_out < a->vocab)))
+    return EAGLE4_NOT_COVERED;
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  switch (a->dtype) {
+    case EAGLE4_BF16: return launch<e4::Bf16>(*a, s);
+    case EAGLE4_F16: return launch<e4::F16>(*a, s);
+    default: return launch<e4::F32>(*a, s);
+  }
+}

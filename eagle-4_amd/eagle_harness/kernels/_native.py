@@ -257,6 +257,13 @@ class LatentAttnArgs(ctypes.Structure):
     )
 
 
+class SampleRowsArgs(ctypes.Structure):
+    _fields_ = _fields(
+        "logits:p stride_row:q entries:t temperature:p top_k:p top_p:p min_p:p coins:p tokens:p out:p stride_out:q rows:q "
+        "num_entries:q vocab:i draws:i dtype:i out_kind:i out_dtype:i reserved:i"
+    )
+
+
 # entry name -> (args struct, index in eagle4_args_size)
 ENTRIES = {
     "eagle4_stage_tree": (StageTreeArgs, 0),
@@ -281,6 +288,7 @@ ENTRIES = {
     "eagle4_read_kv_pages": (ReadKvArgs, 18),
     "eagle4_sample_tree": (SampleTreeArgs, 19),
     "eagle4_latent_attention": (LatentAttnArgs, 20),
+    "eagle4_sample_rows": (SampleRowsArgs, 21),
 }
 EXTRA_SYMBOLS = ("eagle4_verify_attention_workspace", "eagle4_verify_attention_static_bytes",
                  "eagle4_latent_attention_workspace", "eagle4_sample_tree_workspace", "eagle4_version",

@@ -564,6 +564,34 @@ typedef struct eagle4_latent_attn_args {
 int64_t eagle4_latent_attention_workspace(const eagle4_latent_attn_args* args); /* bytes; -1: not covered */
 int eagle4_latent_attention(const eagle4_latent_attn_args* args, void* stream);
 
+/* ---- rows of logits under temperature, top-k, top-p and min-p (no counterpart in the reference's own sources) -------- */
+/* w_i = exp((l_i - max) / temperature). The order: logits descending, the lower index first among equals. Kept: of the first
+ * top_k of the order (0: all) those with w >= min_p, and of these, of mass Z1, the ones with less than top_p Z1 before them
+ * (top_p from 1 on: all); the first one always. With Z the mass kept, tokens[row, d] is the first of the order whose running mass
+ * exceeds coins[row, d] Z. out: w / Z on the kept and 0 elsewhere (PROBS), or the logits with -inf outside the kept (LOGITS;
+ * may be the logits themselves). temperature not above 0, or a row whose maximum is not finite: its argmax alone (first
+ * index; NaN the largest). Rows whose entry is negative or past num_entries are left alone. */
+#define EAGLE4_ROWS_PROBS 1
+#define EAGLE4_ROWS_LOGITS 2
+#define EAGLE4_ROWS_MAX_VOCAB (1 << 18)
+#define EAGLE4_ROWS_MAX_DRAWS 64
+typedef struct eagle4_sample_rows_args {
+  const void* logits; /* [rows, vocab], unit column stride */
+  int64_t stride_row;
+  eagle4_itab entries;      /* [rows] each row's entry in the vectors below, or null: its own index */
+  const float* temperature; /* [num_entries] contiguous */
+  const int32_t* top_k;     /* like temperature, or null: off */
+  const float* top_p;       /* or null */
+  const float* min_p;       /* or null */
+  const float* coins;       /* [rows, draws] contiguous, or null without draws */
+  int64_t* tokens;          /* [rows, draws] contiguous, or null without draws */
+  void* out;                /* [rows, vocab] or null, unit column stride */
+  int64_t stride_out;
+  int64_t rows, num_entries;
+  int32_t vocab, draws, dtype, out_kind, out_dtype, reserved;
+} eagle4_sample_rows_args;
+int eagle4_sample_rows(const eagle4_sample_rows_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -83,3 +83,35 @@ def sample_tree(logits, drafted, cu_num_logits, idx_mapping, parents, coins, fin
         path[slot, : len(taken)] = path.new_tensor(taken)
         path_len[slot] = len(taken)
     return sampled, count
+
+
+def kept_part(logits: np.ndarray, temperature: float, top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0):
+    """One row ``[vocab]`` under the rules: (the kept tokens in their order, their masses), in 64 bits."""
+    x = logits.astype(np.float64)
+    top = np.max(x)
+    if not temperature > 0 or not np.isfinite(top):
+        at = int(np.argmax(np.isnan(x))) if np.isnan(x).any() else int(np.argmax(x))
+        return np.array([at]), np.ones(1)
+    order = np.argsort(-x, kind="stable")
+    with np.errstate(invalid="ignore"):
+        mass = np.exp((x[order] - top) / temperature)
+    mass = np.where(np.isneginf(x[order]), 0.0, mass)
+    n = len(order)
+    if min_p > 0:
+        n = int((mass >= min_p).sum())
+    if top_k > 0:
+        n = min(n, top_k)
+    n = max(n, 1)
+    order, mass = order[:n], mass[:n]
+    if top_p < 1:
+        before = np.concatenate([[0.0], np.cumsum(mass)[:-1]])
+        n = max(1, int((before < top_p * mass.sum()).sum()))
+        order, mass = order[:n], mass[:n]
+    return order, mass
+
+
+def drawn(order: np.ndarray, mass: np.ndarray, coin: float) -> int:
+    """The first token whose running mass exceeds ``coin`` of all."""
+    run = np.cumsum(mass)
+    at = int(np.searchsorted(run, coin * run[-1], side="right"))
+    return int(order[min(at, len(order) - 1)])
