@@ -28,6 +28,9 @@ extern "C" int64_t eagle4_args_size(int which) {
     case 19: return sizeof(eagle4_sample_tree_args);
     case 20: return sizeof(eagle4_latent_attn_args);
     case 21: return sizeof(eagle4_sample_rows_args);
+    case 22: return sizeof(eagle4_rotary_args);
+    case 23: return sizeof(eagle4_resize_tables_args);
+    case 24: return sizeof(eagle4_slot_maps_args);
     default: return -1;
   }
 }

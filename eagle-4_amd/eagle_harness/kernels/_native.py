@@ -78,8 +78,8 @@ def itab(t: Optional[torch.Tensor]) -> ITab:
 
 def _fields(spec: str) -> list:
     """Fields from a compact spec: ``name:type`` pairs, type one of p (pointer), q (int64), i (int32), f (float),
-    t (ITab)."""
-    types = {"p": _ptr, "q": _i64, "i": _i32, "f": _f32, "t": ITab}
+    d (double), t (ITab)."""
+    types = {"p": _ptr, "q": _i64, "i": _i32, "f": _f32, "d": ctypes.c_double, "t": ITab}
     out = []
     for item in spec.split():
         name, kind = item.split(":")
@@ -264,6 +264,27 @@ class SampleRowsArgs(ctypes.Structure):
     )
 
 
+class RotaryArgs(ctypes.Structure):
+    _fields_ = _fields(
+        "q:p k:p q_out:p k_out:p stride_qt:q stride_qh:q stride_kt:q stride_kh:q stride_qot:q stride_qoh:q stride_kot:q "
+        "stride_koh:q positions:t frequencies:p factor:d tokens:q q_heads:i k_heads:i dim:i half:i paired:i dtype:i"
+    )
+
+
+class ResizeTablesArgs(ctypes.Structure):
+    _fields_ = _fields(
+        "block_table:p stride_table:q num_pages:p idx_mapping:t lens:t free_pages:p num_free:p capacity:q num_reqs:i slots:i "
+        "max_pages:i page:i"
+    )
+
+
+class SlotMapsArgs(ctypes.Structure):
+    _fields_ = _fields(
+        "block_table:p stride_table:q num_pages:p idx_mapping:t context_lens:t query_start_loc:t slots:p batch_table:p "
+        "stride_batch:q rows:q num_reqs:i state_slots:i max_pages:i page:i"
+    )
+
+
 # entry name -> (args struct, index in eagle4_args_size)
 ENTRIES = {
     "eagle4_stage_tree": (StageTreeArgs, 0),
@@ -289,6 +310,9 @@ ENTRIES = {
     "eagle4_sample_tree": (SampleTreeArgs, 19),
     "eagle4_latent_attention": (LatentAttnArgs, 20),
     "eagle4_sample_rows": (SampleRowsArgs, 21),
+    "eagle4_rotary": (RotaryArgs, 22),
+    "eagle4_resize_tables": (ResizeTablesArgs, 23),
+    "eagle4_slot_maps": (SlotMapsArgs, 24),
 }
 EXTRA_SYMBOLS = ("eagle4_verify_attention_workspace", "eagle4_verify_attention_static_bytes",
                  "eagle4_latent_attention_workspace", "eagle4_sample_tree_workspace", "eagle4_version",

@@ -1,0 +1,152 @@
+"""Rotary positions of queries and keys (``csrc/rotary.hip``), before :func:`~eagle_harness.vllm.verify_attention.verify_attention`,
+``rows_attention`` or a page write: a tree's rows at the positions that :func:`~eagle_harness.vllm.verify_layout.stage_tree` leaves.
+
+The angles come from 64-bit frequencies, ``position * frequency`` in 64 bits: there is no table of cosines whose length bounds the
+context, and far positions keep their angle. :func:`rotary_frequencies` makes the frequencies, plain or scaled for long contexts.
+"""
+
+from __future__ import annotations
+
+import math
+from typing import Optional
+
+import torch
+
+from eagle_harness.kernels import _native
+
+_DTYPES = {torch.bfloat16: _native.BF16, torch.float16: _native.F16, torch.float32: _native.F32}
+
+
+def rotary_frequencies(
+    dim: int,
+    base: float = 10000.0,
+    *,
+    scaling: str = "none",
+    stretch: float = 1.0,
+    trained: int = 0,
+    fast: float = 32.0,
+    slow: float = 1.0,
+    device: torch.device | str | None = None,
+) -> tuple[torch.Tensor, float]:
+    """``(frequencies [dim / 2] fp64 in radians a position, factor)`` for :func:`rotate_rows`: ``base ** (-2 i / dim)`` for the pair
+    ``i`` of the ``dim`` turned elements, for contexts of ``stretch`` times the trained length by
+
+    - ``"none"``: as trained;
+    - ``"linear"``: every frequency divided by ``stretch``;
+    - ``"ntk"``: the base times ``stretch ** (dim / (dim - 2))``, which leaves the fastest pair and divides the slowest by
+      ``stretch``;
+    - ``"yarn"``: pairs that turn at least ``fast`` times within the ``trained`` positions stay, those that turn at most ``slow``
+      times are divided by ``stretch``, evenly over the pair's number in between; ``factor`` is ``0.1 ln(stretch) + 1``.
+    """
+    if dim < 2 or dim % 2:
+        raise ValueError(f"rotary_frequencies: dim must be even and positive, got {dim}")
+    if not base > 1.0 or not stretch >= 1.0:
+        raise ValueError(f"rotary_frequencies: base must be above 1 and stretch at least 1, got {base}, {stretch}")
+    half, factor = dim // 2, 1.0
+    if scaling == "ntk":
+        if dim < 4:
+            raise ValueError("rotary_frequencies: 'ntk' needs at least two pairs")
+        base = base * stretch ** (dim / (dim - 2))
+    pair = torch.arange(half, dtype=torch.float64)
+    frequencies = torch.pow(torch.tensor(base, dtype=torch.float64), -pair / half)
+    if scaling == "linear":
+        frequencies = frequencies / stretch
+    elif scaling == "yarn":
+        if trained < 1 or not fast > slow > 0:
+            raise ValueError("rotary_frequencies: 'yarn' needs the trained length, and fast > slow > 0")
+        # the pair that turns so many times within the trained positions
+        place = lambda turns: half * math.log(trained / (turns * 2 * math.pi)) / math.log(base)  # noqa: E731
+        low, high = max(math.floor(place(fast)), 0), min(math.ceil(place(slow)), dim - 1)
+        slowed = ((pair - low) / max(high - low, 1e-3)).clamp(0, 1)
+        frequencies = frequencies * (1 - slowed) + frequencies / stretch * slowed
+        factor = 0.1 * math.log(stretch) + 1.0
+    elif scaling not in ("none", "ntk"):
+        raise ValueError(f"rotary_frequencies: scaling {scaling!r} is none of 'none', 'linear', 'ntk', 'yarn'")
+    return frequencies.to(device) if device is not None else frequencies, factor
+
+
+_NONE = (0, 0)
+
+
+def _bytes(t: torch.Tensor) -> tuple[int, int]:
+    """The addresses that a [tokens, heads, dim] tensor of non-negative strides spans."""
+    first = t.data_ptr()
+    return first, first + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
+
+
+def _half(name: str, x: torch.Tensor, out: Optional[torch.Tensor], dtype, tokens: int, dim: int, device) -> tuple:
+    """Checks queries or keys and their output: (output, strides of x, strides of the output)."""
+    if x.dim() != 3 or x.shape[0] != tokens or x.shape[2] != dim:
+        raise ValueError(f"rotate_rows: {name} must be [{tokens}, heads, {dim}], got {tuple(x.shape)}")
+    if x.dtype != dtype or x.device != device:
+        raise ValueError(f"rotate_rows: {name} must be {dtype} on {device}")
+    stride = x.stride()
+    if stride[2] != 1 and dim > 1:
+        raise _native.NotCovered(f"rotate_rows: {name} must have a unit stride over the head dim")
+    to = stride
+    if out is None:
+        out = x
+    elif out is not x:
+        if out.shape != x.shape or out.dtype != dtype or out.device != device:
+            raise ValueError(f"rotate_rows: {name}_out must have {name}'s shape, dtype and device")
+        to = out.stride()
+        if to[2] != 1 and dim > 1:
+            raise _native.NotCovered(f"rotate_rows: {name}_out must have a unit stride over the head dim")
+        if x.numel():
+            (a, b), (c, d) = _bytes(x), _bytes(out)
+            if a < d and c < b and (a != c or to != stride):
+                raise ValueError(f"rotate_rows: {name}_out may be {name} itself, but not overlap it otherwise")
+    if (to[0] == 0 and tokens > 1) or (to[1] == 0 and x.shape[1] > 1):
+        raise ValueError(f"rotate_rows: the output of {name} is an expanded view: every head needs its own storage")
+    return out, stride, to
+
+
+def rotate_rows(
+    q: torch.Tensor,
+    k: Optional[torch.Tensor],
+    positions: torch.Tensor,
+    frequencies: torch.Tensor,
+    *,
+    interleaved: bool = False,
+    factor: float = 1.0,
+    q_out: Optional[torch.Tensor] = None,
+    k_out: Optional[torch.Tensor] = None,
+) -> tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """Turns the first ``2 len(frequencies)`` elements of every head by its row's position, in place without outputs.
+
+    ``q`` [tokens, heads, D] and ``k`` [tokens, kv_heads, D] (None: queries alone) in bf16, fp16 or fp32, any strides
+    over tokens and heads (so the parts of one packed projection); ``positions`` [tokens] int32 / int64; ``frequencies`` fp64
+    radians a position, at most 512. Pair ``i`` is the elements ``(i, half + i)``, or ``(2 i, 2 i + 1)`` where ``interleaved``:
+    ``(x, y) -> factor (x cos - y sin, y cos + x sin)`` of ``position * frequencies[i]``. The elements behind the turned ones
+    are copied. Outputs for both or for neither; angles are computed in 64 bits, products in 32, each rounded once to the
+    rows' dtype. Returns ``(q_out, k_out)``.
+    """
+    code = _DTYPES.get(q.dtype)
+    if code is None:
+        raise _native.NotCovered(f"rotate_rows: rows must be bf16, fp16 or fp32, got {q.dtype}")
+    if q.dim() != 3:
+        raise ValueError(f"rotate_rows: q must be [tokens, heads, D], got {tuple(q.shape)}")
+    (tokens, heads, dim), device = q.shape, q.device
+    if frequencies.dtype != torch.float64 or frequencies.dim() != 1 or not frequencies.is_contiguous() or frequencies.device != device:
+        raise ValueError(f"rotate_rows: frequencies must be a contiguous fp64 vector on {device}")
+    half = frequencies.shape[0]
+    if not 0 < half <= 512 or 2 * half > dim:
+        raise ValueError(f"rotate_rows: {half} pairs do not fit heads of {dim} (at most 512 pairs)")
+    if positions.dim() != 1 or positions.shape[0] < tokens or positions.device != device:
+        raise ValueError(f"rotate_rows: positions must be [{tokens}] on {device}")
+    if k is None and k_out is not None:
+        raise ValueError("rotate_rows: k_out without k")
+    q_out, qs, qo = _half("q", q, q_out, q.dtype, tokens, dim, device)
+    ks, ko, kv_heads = _NONE, _NONE, 0
+    if k is not None:
+        k_out, ks, ko = _half("k", k, k_out, q.dtype, tokens, dim, device)
+        kv_heads = k.shape[1]
+        if (q_out.data_ptr() == q.data_ptr()) != (k_out.data_ptr() == k.data_ptr()) and heads and kv_heads:
+            raise ValueError("rotate_rows: q_out and k_out go together")
+    if tokens == 0:
+        return q_out, k_out
+    args = _native.RotaryArgs(q.data_ptr(), _native.ptr(k), q_out.data_ptr(), _native.ptr(k_out), qs[0], qs[1], ks[0], ks[1], qo[0],
+                              qo[1], ko[0], ko[1], _native.itab(positions), frequencies.data_ptr(), factor, tokens, heads, kv_heads,
+                              dim, half, interleaved, code)
+    _native.launch("eagle4_rotary", args, device)
+    return q_out, k_out

@@ -592,6 +592,58 @@ typedef struct eagle4_sample_rows_args {
 } eagle4_sample_rows_args;
 int eagle4_sample_rows(const eagle4_sample_rows_args* args, void* stream);
 
+/* ---- rotary positions (no counterpart in the reference's own sources) ------------------------------------------------ */
+/* Pair i of a head, elements (i, half + i) or, paired, (2i, 2i + 1), is turned by positions[t] * frequencies[i] and multiplied by
+ * factor; elements from 2 half on are copied. Angles in 64 bits. In place where the outputs are the inputs (both, or neither). */
+typedef struct eagle4_rotary_args {
+  const void *q, *k; /* [tokens, heads, dim], unit stride over dim; k_heads 0: no keys */
+  void *q_out, *k_out;
+  int64_t stride_qt, stride_qh, stride_kt, stride_kh, stride_qot, stride_qoh, stride_kot, stride_koh;
+  eagle4_itab positions;     /* [tokens] */
+  const double* frequencies; /* [half] radians a position */
+  double factor;
+  int64_t tokens;
+  int32_t q_heads, k_heads, dim, half, paired, dtype; /* half <= 512 */
+} eagle4_rotary_args;
+int eagle4_rotary(const eagle4_rotary_args* args, void* stream);
+
+/* ---- block tables from lengths, and the slots of a batch's rows (no counterpart in the reference's own sources) ------ */
+/* Request r, of state slot idx_mapping[r], comes to ceil(lens[r] / page) pages of block_table[slot]. First every request that has
+ * more gives the rest back onto the stack free_pages[0 .. num_free), the last request's last page first; then those that need
+ * more take from its top, in order, as long as the sum of what they and those before them need is there. Others keep what
+ * they have, as do requests with a slot outside the table, and those whose length does not fit it. num_pages and num_free follow.
+ * Giving back what was just taken, in the same batch order, leaves the stack as it was. */
+typedef struct eagle4_resize_tables_args {
+  int32_t* block_table; /* [slots, max_pages], unit column stride */
+  int64_t stride_table;
+  int32_t* num_pages;      /* [slots] contiguous */
+  eagle4_itab idx_mapping; /* [R], each slot once */
+  eagle4_itab lens;        /* [R] */
+  int32_t* free_pages;     /* [capacity] contiguous: as many as there are pages */
+  int32_t* num_free;       /* [1] */
+  int64_t capacity;
+  int32_t num_reqs, slots, max_pages, page;
+} eagle4_resize_tables_args;
+int eagle4_resize_tables(const eagle4_resize_tables_args* args, void* stream);
+
+/* Row j of request r (rows query_start_loc[r] .. of the batch) is position context_lens[r] + j: slots[row] is its place in the
+ * cache, block_table[slot, position / page] * page + position % page, or -1 where the request holds no such page, and for rows behind
+ * the last request's. batch_table[r]: the request's pages, 0 behind them. */
+typedef struct eagle4_slot_maps_args {
+  const int32_t* block_table; /* [state_slots, max_pages], unit column stride */
+  int64_t stride_table;
+  const int32_t* num_pages;    /* [state_slots] contiguous */
+  eagle4_itab idx_mapping;     /* [R] */
+  eagle4_itab context_lens;    /* [R] */
+  eagle4_itab query_start_loc; /* [R + 1] */
+  int64_t* slots;              /* [rows] contiguous */
+  int32_t* batch_table;        /* [R, max_pages] or null, unit column stride */
+  int64_t stride_batch;
+  int64_t rows;
+  int32_t num_reqs, state_slots, max_pages, page;
+} eagle4_slot_maps_args;
+int eagle4_slot_maps(const eagle4_slot_maps_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
