@@ -31,6 +31,7 @@ extern "C" int64_t eagle4_args_size(int which) {
     case 22: return sizeof(eagle4_rotary_args);
     case 23: return sizeof(eagle4_resize_tables_args);
     case 24: return sizeof(eagle4_slot_maps_args);
+    case 25: return sizeof(eagle4_row_attn_fp8_args);
     default: return -1;
   }
 }

@@ -285,6 +285,12 @@ class SlotMapsArgs(ctypes.Structure):
     )
 
 
+class RowAttnFp8Args(ctypes.Structure):
+    _fields_ = [("rows", RowAttnArgs)] + _fields(
+        "k_scale:p v_scale:p stride_ksb:q stride_ksh:q stride_vsb:q stride_vsh:q table_height:q table_width:i num_blocks:i"
+    )
+
+
 # entry name -> (args struct, index in eagle4_args_size)
 ENTRIES = {
     "eagle4_stage_tree": (StageTreeArgs, 0),
@@ -313,6 +319,7 @@ ENTRIES = {
     "eagle4_rotary": (RotaryArgs, 22),
     "eagle4_resize_tables": (ResizeTablesArgs, 23),
     "eagle4_slot_maps": (SlotMapsArgs, 24),
+    "eagle4_row_attention_fp8": (RowAttnFp8Args, 25),
 }
 EXTRA_SYMBOLS = ("eagle4_verify_attention_workspace", "eagle4_verify_attention_static_bytes",
                  "eagle4_latent_attention_workspace", "eagle4_sample_tree_workspace", "eagle4_version",

@@ -19,6 +19,7 @@ from __future__ import annotations
 import functools
 import math
 from dataclasses import dataclass
+from typing import Optional
 
 import torch
 
@@ -79,6 +80,21 @@ def _cache_strides(cache: torch.Tensor) -> tuple[int, int, int]:
     return per_page, per_slot, per_head
 
 
+def _check_fp8(q, keys, values, out, k_scale, v_scale) -> None:
+    if keys.dtype != torch.float8_e4m3fn or values is None or values.dtype != torch.float8_e4m3fn:
+        raise _native.NotCovered("caches with scales must be float8_e4m3fn keys and values")
+    if q.dtype not in (torch.bfloat16, torch.float16) or out.dtype != q.dtype:
+        raise _native.NotCovered("q and out over fp8 pages must share one 16-bit dtype")
+    if values.shape != keys.shape:
+        raise ValueError(f"values {tuple(values.shape)} are not shaped as keys {tuple(keys.shape)}")
+    pages, heads = keys.shape[0], keys.shape[-2]
+    for name, scale in (("k_scale", k_scale), ("v_scale", v_scale)):
+        if scale.dtype != torch.float32 or scale.dim() != 2 or scale.shape[0] < pages or scale.shape[1] < heads:
+            raise ValueError(f"{name} must be fp32 [pages >= {pages}, kv_heads >= {heads}], got {scale.dtype} {tuple(scale.shape)}")
+        if scale.device != q.device:
+            raise ValueError(f"{name} must be on {q.device}")
+
+
 def rows_attention(
     q: torch.Tensor,
     keys: torch.Tensor,
@@ -97,6 +113,8 @@ def rows_attention(
     launch: RowsLaunch,
     table_rows: torch.Tensor | None = None,
     table_page: int = 1,
+    k_scale: Optional[torch.Tensor] = None,
+    v_scale: Optional[torch.Tensor] = None,
 ) -> None:
     """Attention of ``q`` ``[bs * rows_per_request, heads, D]`` into ``out`` (same shape).
 
@@ -108,6 +126,10 @@ def rows_attention(
     ``table[table_rows[b], p // table_page] * table_page + p % table_page`` (row ``b`` without ``table_rows``).
     ``part_out`` / ``part_lse``: scratch of at least ``bs * heads * (launch.splits + 1) *
     rows_padded(rows_per_request)`` rows (kernels/row_attention.py:251-328).
+
+    Beyond the reference: ``float8_e4m3fn`` caches (``keys`` and ``values``, as ``write_kv_pages`` fills them) with
+    ``k_scale`` / ``v_scale`` fp32 ``[pages, kv_heads]`` (any strides), under bf16 or fp16 rows. Value scales below 2^-100 count
+    as 0. A row that sees no key gives zeros.
     """
     rows, heads, head_dim = q.shape
     kv_heads = keys.shape[-2]
@@ -115,7 +137,11 @@ def rows_attention(
         raise ValueError(f"query heads ({heads}) must be divisible by KV heads ({kv_heads})")
     if step > 0 and ancestors is None:
         raise ValueError("a draft step needs its rows' ancestors")
-    if q.dtype != keys.dtype or out.dtype != q.dtype or (values is not None and values.dtype != q.dtype):
+    if (k_scale is None) != (v_scale is None):
+        raise ValueError("k_scale and v_scale go together")
+    if k_scale is not None:
+        _check_fp8(q, keys, values, out, k_scale, v_scale)
+    elif q.dtype != keys.dtype or out.dtype != q.dtype or (values is not None and values.dtype != q.dtype):
         raise _native.NotCovered("q, the caches and out must share one 16-bit dtype")
     for name, t in (("q", q), ("out", out), ("keys", keys)) + ((("values", values),) if values is not None else ()):
         if t.stride(-1) != 1:
@@ -169,4 +195,11 @@ def rows_attention(
         splits=launch.splits,
         scale=scale,
     )
-    _native.launch("eagle4_row_attention", args, q.device)
+    if k_scale is None:
+        _native.launch("eagle4_row_attention", args, q.device)
+        return
+    if table.dim() != 2 or 0 in table.shape or keys.shape[0] == 0:
+        raise ValueError("the page table must be [requests, entries], and the caches hold pages")
+    fp8 = _native.RowAttnFp8Args(args, k_scale.data_ptr(), v_scale.data_ptr(), k_scale.stride(0), k_scale.stride(1), v_scale.stride(0),
+                                 v_scale.stride(1), table.shape[0], table.shape[1], keys.shape[0])
+    _native.launch("eagle4_row_attention_fp8", fp8, q.device)
