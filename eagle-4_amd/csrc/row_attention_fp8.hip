@@ -12,7 +12,7 @@
 // Split: a workgroup takes a key split (or the ancestors) of a request's KV head and up to 16 RT of its rows (request rows x
 // query heads of the group); its four waves take every fourth tile of 32 keys on their own, each with its own softmax, and
 // join at the end: no barrier is in the loop. K goes from memory into the registers that the matrix instructions read: a
-// lane takes 16 bytes of its key, which are two steps of the product (the order of d is the queries' own). V has to be
+// lane takes 16 bytes of its key, which are two steps of the product (the queries, in LDS, are read in that order of d). V has to be
 // transposed and goes through the wave's own LDS. The next tile's loads start when this tile's K is used up and its V is in LDS, so
 // one set of registers does; page entries are looked up a tile further ahead. Splits are joined by a second kernel.
 
@@ -39,6 +39,13 @@ E4_DEV uint2 lds_tr8(const char* p) {
 // The bytes of w that hold an e4m3 NaN (0x7f, 0xff), as 0x80 each.
 E4_DEV uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
 
+// A value as one that the compiler knows nothing of: addresses made from it are made where they are used, and not kept in registers
+// over the loop.
+E4_DEV int here(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
 struct WaveMeta {
   int64_t koff[32], voff[32];  // byte offsets of the tile's key and value rows
   float ks[32], lv[32], iv[32];  // scale log2(e) k_j, log2 v_j, 1 / v_j
@@ -46,48 +53,61 @@ struct WaveMeta {
 
 template <int D, int RT>
 struct Smem {
+  static constexpr int kHalves = D >= 128 ? 2 : 1;  // the join takes the columns in so many parts
   union {
     struct {
-      char v[NW][32 * D];  // a wave's tile of values, rows of D codes in 16-byte chunks swizzled as Tile8's
+      char q[RT * 16 * 2 * D];  // the rows, 16-byte chunks swizzled as Tile's keys
+      char v[NW][32 * D];       // a wave's tile of values, rows of D codes in 16-byte chunks swizzled as Tile8's
       WaveMeta meta[NW];
     } loop;
     struct {
-      f32x4_t acc[NW][D / 16][64];
+      f32x4_t acc[NW][D / 16 / kHalves][64];
       float m[NW][RT * 16], l[NW][RT * 16];
     } join;
   };
 };
 
+// Waves a SIMD that the registers are kept for: the loads of one wave's tile do not cover its latency.
+template <int D, int RT>
+constexpr int kResident = D * RT <= 64 ? 5 : D * RT <= 128 ? 4 : D == 128 && RT == 2 ? 3 : 2;
+
 template <int D, typename T, int RT>
-__global__ __launch_bounds__(NT) void row_attention_fp8_kernel(const eagle4_row_attn_fp8_args x, int groups) {
+__global__ __launch_bounds__(NT, (kResident<D, RT>)) void row_attention_fp8_kernel(const eagle4_row_attn_fp8_args x, int groups, int splits) {
   const eagle4_row_attn_args& a = x.rows;
   using T8 = Tile8<D>;
+  constexpr bool kEarly = D * RT <= 256;  // the next loads before the softmax; else behind it, for the registers
   constexpr int CH = D / 16, KJ = D / 64, NI = D / 32, RPI = 1024 / D;
   __shared__ __attribute__((aligned(1024))) Smem<D, RT> sm;
-  const int split = blockIdx.x, kvh = blockIdx.y / groups, grp = blockIdx.y % groups, b = blockIdx.z;
+  // The row groups of a unit (a split of a request's KV head) run on one XCD (workgroup i on XCD i % 8) one after another, so that
+  // its second one finds the keys in that XCD's cache; rows of units over the XCDs are skewed, so that no XCD has the same head
+  // every time (its rows lie in a part of the cache's channels).
+  const uint32_t at_xcd = blockIdx.x / 8u, turn = at_xcd / groups;
+  const uint32_t unit = turn * 8u + ((blockIdx.x + turn) & 7u);
+  if (unit >= static_cast<uint32_t>(splits) * a.kv_heads * a.bs) return;
+  const int grp = at_xcd % groups, split = unit % splits, kvh = unit / splits % a.kv_heads, b = unit / splits / a.kv_heads;
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4, l16 = lane & 15;
-  const int G = a.heads / a.kv_heads, R = a.rows_per_request * G, NS = a.splits;
+  const int G = a.heads / a.kv_heads, R = a.rows_per_request * G;
   const bool extend = a.step == 0;
+  const int NS = extend ? splits : splits - 1;  // of the shared range; a draft step's ancestors are one more
   const int64_t seq_len = e4::ld(a.seq_lens, b);
   int64_t trow = a.table_rows.ptr != nullptr ? e4::ld(a.table_rows, b) : b;
   trow = trow < 0 ? 0 : trow < x.table_height ? trow : x.table_height - 1;
   const int32_t* const table = a.table + trow * a.stride_table;
 
-  // this lane's rows
-  int t[RT];
-  bool row_ok[RT];
-  u32x4_t q[RT][D / 32];
+  // the queries of all rows go to LDS
+  {
+    constexpr int QC = D / 8, ALL = RT * 16 * QC;
 #pragma unroll
-  for (int r = 0; r < RT; ++r) {
-    const int rho = (grp * RT + r) * 16 + l16;
-    t[r] = rho / G;
-    row_ok[r] = rho < R;
-    const uint16_t* const qp = static_cast<const uint16_t*>(a.q) +
-                               (static_cast<int64_t>(b) * a.rows_per_request + (row_ok[r] ? t[r] : 0)) * a.stride_q_row +
-                               static_cast<int64_t>(kvh * G + (row_ok[r] ? rho % G : 0)) * a.stride_q_head;
-#pragma unroll
-    for (int c = 0; c < D / 32; ++c)  // step c of the product: d = 64 (c / 2) + 16 g + 8 (c % 2) + 0 .. 7
-      q[r][c] = row_ok[r] ? *reinterpret_cast<const u32x4_t*>(qp + 64 * (c / 2) + 16 * g + 8 * (c % 2)) : u32x4_t{0u, 0u, 0u, 0u};
+    for (int i = 0; i < (ALL + NT - 1) / NT; ++i) {
+      const int at = tid + i * NT, row = at / QC, chunk = at % QC, rho = grp * RT * 16 + row;
+      if (ALL % NT != 0 && at >= ALL) break;
+      const uint16_t* const p = static_cast<const uint16_t*>(a.q) +
+                                (static_cast<int64_t>(b) * a.rows_per_request + rho / G) * a.stride_q_row +
+                                static_cast<int64_t>(kvh * G + rho % G) * a.stride_q_head + 8 * chunk;
+      u32x4_t w = {0u, 0u, 0u, 0u};
+      if (rho < R) w = *reinterpret_cast<const u32x4_t*>(p);
+      *reinterpret_cast<u32x4_t*>(sm.loop.q + row * 2 * D + 16 * (chunk ^ Tile<D>::kswz(row))) = w;
+    }
   }
 
   // The split's keys: `count` positions from `start` on, or the rows' ancestor columns; row r sees keys lo[r] .. hi[r] of
@@ -109,21 +129,22 @@ __global__ __launch_bounds__(NT) void row_attention_fp8_kernel(const eagle4_row_
     if (all_hi >= count) all_hi = count - 1;
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
-      lo[r] = extend ? within(window_start(seq_len + t[r], a.window)) : 0;
-      hi[r] = extend ? within(seq_len + t[r]) : count - 1;
+      const int t = ((grp * RT + r) * 16 + l16) / G;
+      lo[r] = extend ? within(window_start(seq_len + t, a.window)) : 0;
+      hi[r] = extend ? within(seq_len + t) : count - 1;
     }
   } else {
     count = a.rows_per_request * a.max_depth;
     all_lo = count;
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
-      lo[r] = t[r] * a.max_depth;
+      lo[r] = ((grp * RT + r) * 16 + l16) / G * a.max_depth;
       hi[r] = lo[r] + a.step - 1;
     }
   }
 #pragma unroll
   for (int r = 0; r < RT; ++r) {
-    if (!row_ok[r]) hi[r] = -1;
+    if ((grp * RT + r) * 16 + l16 >= R) hi[r] = -1;  // no such row
     hi[r] = hi[r] < count ? hi[r] : count - 1;
   }
   const int ntiles = (count + 31) / 32;
@@ -134,18 +155,17 @@ __global__ __launch_bounds__(NT) void row_attention_fp8_kernel(const eagle4_row_
   WaveMeta& meta = sm.loop.meta[wave];
 
   // lane j (and j + 32) looks after key j of a tile: its position (past the split: the last key, which is masked)
-  const int j32 = lane & 31;
   auto key_at = [&](int tile) {
-    const int c = tile * 32 + j32;
+    const int c = tile * 32 + (here(lane) & 31);
     return c < count ? c : count - 1;
   };
   auto lookup = [&](int tile) {
     const int c = key_at(tile);
     if (anc) {  // a column past the row's `step` ancestors takes its first one (masked)
-      const int owner = c / a.max_depth, dep = c - owner * a.max_depth;
+      const int owner = c / here(a.max_depth), dep = c - owner * a.max_depth;
       return a.ancestors[(static_cast<int64_t>(b) * a.rows_per_request + owner) * a.max_depth + (dep < a.step ? dep : 0)];
     }
-    const uint32_t pos = static_cast<uint32_t>(start + c), pg = tp_shift >= 0 ? pos >> tp_shift : pos / tp;
+    const uint32_t pos = static_cast<uint32_t>(start + c), pg = tp_shift >= 0 ? pos >> tp_shift : pos / static_cast<uint32_t>(here(a.table_page));
     return table[pg < static_cast<uint32_t>(x.table_width) ? pg : x.table_width - 1];
   };
   u32x4_t kraw[2][KJ], vraw[NI];
@@ -154,25 +174,31 @@ __global__ __launch_bounds__(NT) void row_attention_fp8_kernel(const eagle4_row_
     uint32_t slot = static_cast<uint32_t>(ent);
     if (!anc) {
       const uint32_t pos = static_cast<uint32_t>(start + key_at(tile));
-      slot = slot * tp + (pos - (tp_shift >= 0 ? pos >> tp_shift : pos / tp) * tp);
+      slot = slot * tp + (pos - (tp_shift >= 0 ? pos >> tp_shift : pos / static_cast<uint32_t>(here(a.table_page))) * tp);
     }
-    uint32_t blk = cp_shift >= 0 ? slot >> cp_shift : slot / cpg;
+    uint32_t blk = cp_shift >= 0 ? slot >> cp_shift : slot / static_cast<uint32_t>(here(a.cache_page));
     const uint32_t in = slot - blk * cpg;
     blk = blk < static_cast<uint32_t>(x.num_blocks) ? blk : x.num_blocks - 1;  // (nothing outside the cache is read)
+    const int j32 = here(lane) & 31;
     meta.koff[j32] = static_cast<int64_t>(blk) * a.k_stride_page + in * a.k_stride_slot;
     meta.voff[j32] = static_cast<int64_t>(blk) * a.v_stride_page + in * a.v_stride_slot;
     ks = x.k_scale[static_cast<int64_t>(blk) * x.stride_ksb + kvh * x.stride_ksh];
     vs = x.v_scale[static_cast<int64_t>(blk) * x.stride_vsb + kvh * x.stride_vsh];
-    const char* const kc = static_cast<const char*>(a.keys) + kvh * a.k_stride_head + 16 * g;
-    const char* const vc = static_cast<const char*>(a.values) + kvh * a.v_stride_head + 16 * (lane % CH);
+    const int me = here(lane);
+    const char* const kc = static_cast<const char*>(a.keys) + kvh * a.k_stride_head + 16 * (me >> 4);
+    const char* const vc = static_cast<const char*>(a.values) + kvh * a.v_stride_head + 16 * (me % CH);
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt) {
-      const char* const p = kc + meta.koff[16 * kt + l16];
+      const char* const p = kc + meta.koff[16 * kt + (me & 15)];
 #pragma unroll
       for (int j = 0; j < KJ; ++j) kraw[kt][j] = *reinterpret_cast<const u32x4_t*>(p + 64 * j);
+      if constexpr (!kEarly) __builtin_amdgcn_sched_barrier(0);
     }
 #pragma unroll
-    for (int n = 0; n < NI; ++n) vraw[n] = *reinterpret_cast<const u32x4_t*>(vc + meta.voff[n * RPI + lane / CH]);
+    for (int n = 0; n < NI; ++n) {
+      vraw[n] = *reinterpret_cast<const u32x4_t*>(vc + meta.voff[n * RPI + me / CH]);
+      if constexpr (!kEarly) __builtin_amdgcn_sched_barrier(0);
+    }
   };
 
   f32x4_t acc[RT][D / 16];
@@ -186,45 +212,61 @@ __global__ __launch_bounds__(NT) void row_attention_fp8_kernel(const eagle4_row_
   }
   const float scale_log2 = a.scale * 1.4426950408889634f;
 
-  // transposing reads of V (Tile8): lane l16 gets d = 16 dt + l16 of keys 16 (k / 4) + 4 g + k % 4
-  const int vk = l16 >> 1, vkey = 16 * (vk >> 2) + 4 * g + (vk & 3);
-  const char* const vrow = sv + vkey * D + 8 * (l16 & 1);
-  const int vsw = T8::vswz(vkey);
-
+  // transposing reads of V (Tile8): lane l16 gets d = 16 dt + l16 of keys 16 (k / 4) + 4 g + k % 4, k = l16 / 2
+  const auto vread = [](int ln) {
+    const int key = 16 * ((ln & 15) >> 3) + 4 * (ln >> 4) + ((ln & 7) >> 1);
+    return key * D + 16 * T8::vswz(key) + 8 * (ln & 1);
+  };
+  // the queries' reads: chunk 8 (c / 2) + 2 g + c % 2 of a row at the chunk xor the row's swizzle (alike for rows 16 apart)
+  const auto qread = [](int ln) { return (ln & 15) * 2 * D + 16 * ((2 * (ln >> 4)) ^ Tile<D>::kswz(ln & 15)); };
   if (wave < ntiles) issue(wave, lookup(wave));
+  __syncthreads();  // the queries
   int32_t ent = wave + NW < ntiles ? lookup(wave + NW) : 0;
   for (int tile = wave; tile < ntiles; tile += NW) {
-    const int base = tile * 32;
+    const int base = tile * 32, qnow = qread(here(lane));
     f32x4_t s[RT][2];
 #pragma unroll
-    for (int kt = 0; kt < 2; ++kt) {
+    for (int r = 0; r < RT; ++r)
 #pragma unroll
-      for (int r = 0; r < RT; ++r) s[r][kt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+      for (int kt = 0; kt < 2; ++kt) s[r][kt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int c = 0; c < D / 32; ++c) {
-        const u32x4_t& w = kraw[kt][c / 2];
-        const u32x4_t k16 = __builtin_bit_cast(u32x4_t, widen_fp8x8<T>(c % 2 ? make_uint2(w[2], w[3]) : make_uint2(w[0], w[1])));
+    for (int j = 0; j < KJ; ++j) {  // steps 2 j and 2 j + 1 take d = 64 j + 16 g + 0 .. 7 and + 8 .. 15
 #pragma unroll
-        for (int r = 0; r < RT; ++r) s[r][kt] = mfma16<T>(k16, q[r][c], s[r][kt]);
+      for (int c = 0; c < 2; ++c) {
+        u32x4_t q[RT];
+        const int qc = qnow ^ 16 * ((8 * j + c) & 15);
+#pragma unroll
+        for (int r = 0; r < RT; ++r) q[r] = *reinterpret_cast<const u32x4_t*>(sm.loop.q + qc + r * 32 * D + 256 * (j / 2));
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) {
+          const u32x4_t k16 = __builtin_bit_cast(
+              u32x4_t, widen_fp8x8<T>(c ? make_uint2(kraw[kt][j][2], kraw[kt][j][3]) : make_uint2(kraw[kt][j][0], kraw[kt][j][1])));
+#pragma unroll
+          for (int r = 0; r < RT; ++r) s[r][kt] = mfma16<T>(k16, q[r], s[r][kt]);
+        }
+        if constexpr (!kEarly) __builtin_amdgcn_sched_barrier(0);
       }
     }
     // a tile that every row sees whole, or not
     const bool full = base >= all_lo && base + 31 <= all_hi;
+    const int j32 = here(lane) & 31;
     const bool none = __builtin_fabsf(vs) < 0x1p-100f;
     meta.ks[j32] = ks * scale_log2;
     meta.lv[j32] = none ? 0.f : log2f(vs);
     meta.iv[j32] = none ? 1.f : 1.f / vs;
     if (__any(none)) {  // such a page's values are zeros whatever its codes
-      const uint64_t which = __ballot(none);
+      const uint32_t which = static_cast<uint32_t>(__ballot(none));
+      const int first = here(lane) / CH;
 #pragma unroll
       for (int n = 0; n < NI; ++n)
-        if ((which >> (n * RPI + lane / CH)) & 1) vraw[n] = u32x4_t{0u, 0u, 0u, 0u};
+        if ((which >> (n * RPI + first)) & 1) vraw[n] = u32x4_t{0u, 0u, 0u, 0u};
     }
     auto put_v = [&]() {
+      const int me = here(lane);
 #pragma unroll
       for (int n = 0; n < NI; ++n) {
-        const int row = n * RPI + lane / CH;
-        *reinterpret_cast<u32x4_t*>(sv + row * D + 16 * ((lane % CH) ^ T8::vswz(row))) = vraw[n];
+        const int row = n * RPI + me / CH;
+        *reinterpret_cast<u32x4_t*>(sv + row * D + 16 * ((me % CH) ^ T8::vswz(row))) = vraw[n];
       }
     };
     put_v();
@@ -236,7 +278,7 @@ __global__ __launch_bounds__(NT) void row_attention_fp8_kernel(const eagle4_row_
 #pragma unroll
         for (int i = 0; i < 4; ++i) odd |= nan_bytes(vraw[n][i]);
       if (__any(odd != 0)) {
-        for (int k = 0; k < 32; ++k)
+        for (int k = here(0); k < 32; ++k)
 #pragma unroll
           for (int dt = 0; dt < D / 16; ++dt) {
             const uint32_t w = *reinterpret_cast<const uint32_t*>(sv + k * D + 16 * (dt ^ T8::vswz(k)) + 4 * g);
@@ -252,16 +294,22 @@ __global__ __launch_bounds__(NT) void row_attention_fp8_kernel(const eagle4_row_
 #pragma unroll
         for (int n = 0; n < NI; ++n)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) vraw[n][i] &= ~((nan_bytes(vraw[n][i]) >> 7) * 0xffu);
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t w = here(vraw[n][i]);
+            vraw[n][i] = w & ~((nan_bytes(w) >> 7) * 0xffu);
+          }
         put_v();
       }
     }
-    __builtin_amdgcn_sched_barrier(0);
-    if (tile + NW < ntiles) {
-      issue(tile + NW, ent);
-      if (tile + 2 * NW < ntiles) ent = lookup(tile + 2 * NW);
-    }
-    __builtin_amdgcn_sched_barrier(0);
+    const auto next = [&]() {
+      __builtin_amdgcn_sched_barrier(0);
+      if (tile + NW < ntiles) {
+        issue(tile + NW, ent);
+        if (tile + 2 * NW < ntiles) ent = lookup(tile + 2 * NW);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    if constexpr (kEarly) next();
 
     u32x4_t pb[RT];
 #pragma unroll
@@ -302,11 +350,15 @@ __global__ __launch_bounds__(NT) void row_attention_fp8_kernel(const eagle4_row_
         pb[r][2 * kt + 1] = pack2<T>(p[2], p[3]);
       }
     }
+    if constexpr (!kEarly) next();
+    const int vnow = vread(here(lane));
 #pragma unroll
     for (int dt = 0; dt < D / 16; ++dt) {
-      const u32x4_t v16 = __builtin_bit_cast(u32x4_t, widen_fp8x8<T>(lds_tr8(vrow + 16 * (dt ^ vsw))));
+      const u32x4_t v16 = __builtin_bit_cast(u32x4_t, widen_fp8x8<T>(lds_tr8(sv + (vnow ^ 16 * (dt & 7)) + 128 * (dt / 8))));
 #pragma unroll
       for (int r = 0; r < RT; ++r) acc[r][dt] = mfma16<T>(v16, pb[r], acc[r][dt]);
+      if constexpr (!kEarly)
+        if (dt % 4 == 3) __builtin_amdgcn_sched_barrier(0);
     }
   }
 
@@ -337,23 +389,28 @@ __global__ __launch_bounds__(NT) void row_attention_fp8_kernel(const eagle4_row_
     }
     const float mine = m[r] > -INFINITY ? exp2f(m[r] - top) : 0.f;
     const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
+    const int rho = (grp * RT + r) * 16 + here(l16);
+    const bool row_in = rho < R;
+    const int64_t part = ((static_cast<int64_t>(b) * a.heads + kvh * G + (row_in ? rho % G : 0)) * (a.splits + 1) + split) * a.rows_padded + rho / G;
+    if (row_in && wave == 0 && g == 0) a.part_lse[part] = sum != 0.f ? top + log2f(sum) : -INFINITY;
+    constexpr int H = Smem<D, RT>::kHalves, C = D / 16 / H;
 #pragma unroll
-    for (int dt = 0; dt < D / 16; ++dt) sm.join.acc[wave][dt][lane] = acc[r][dt] * (mine * inv);
-    const int rho = (grp * RT + r) * 16 + l16;
-    const int64_t part = ((static_cast<int64_t>(b) * a.heads + kvh * G + (row_ok[r] ? rho % G : 0)) * (NS + 1) + split) * a.rows_padded + t[r];
-    if (row_ok[r] && wave == 0 && g == 0) a.part_lse[part] = sum != 0.f ? top + log2f(sum) : -INFINITY;
-    __syncthreads();
-    if (row_ok[r]) {
+    for (int h = 0; h < H; ++h) {
 #pragma unroll
-      for (int i = 0; i < D / 16 / NW; ++i) {
-        const int dt = wave + NW * i;
-        f32x4_t o = sm.join.acc[0][dt][lane];
+      for (int dt = 0; dt < C; ++dt) sm.join.acc[wave][dt][lane] = acc[r][C * h + dt] * (mine * inv);
+      __syncthreads();
+      if (row_in) {
 #pragma unroll
-        for (int w = 1; w < NW; ++w) o += sm.join.acc[w][dt][lane];
-        *reinterpret_cast<f32x4_t*>(a.part_out + part * D + 16 * dt + 4 * g) = o;
+        for (int i = 0; i < C / NW; ++i) {
+          const int dt = wave + NW * i;
+          f32x4_t o = sm.join.acc[0][dt][lane];
+#pragma unroll
+          for (int w = 1; w < NW; ++w) o += sm.join.acc[w][dt][lane];
+          *reinterpret_cast<f32x4_t*>(a.part_out + part * D + 16 * (C * h + dt) + 4 * g) = o;
+        }
       }
+      __syncthreads();
     }
-    __syncthreads();
   }
 }
 
@@ -378,14 +435,29 @@ __global__ __launch_bounds__(256) void row_merge_fp8_kernel(const eagle4_row_att
   *reinterpret_cast<uint2*>(o) = make_uint2(T::pack(acc.x * inv, acc.y * inv), T::pack(acc.z * inv, acc.w * inv));
 }
 
+// The splits that are used of those that the caller has scratch for: as many as fill the GPU's 256 CUs with resident workgroups
+// once, but none of fewer than 256 keys, as far as the window or the page table bound them. A workgroup's start and
+// end cost as much as some tiles: 32 requests' extends (54 rows a head, D 256, window 2048) 48 us with 2 splits, 87 with 8; 64 draft
+// steps (16 rows, D 128, window 4096) 134 with 2, 132 with 4, 135 with 8, 193 with 1 or 32; one over 4096 keys 39 with 1, 11 with 16.
+int used_splits(const eagle4_row_attn_fp8_args& x, int resident, int groups) {
+  const eagle4_row_attn_args& a = x.rows;
+  const int64_t bound = a.window > 0 ? static_cast<int64_t>(a.window) + a.rows_per_request : static_cast<int64_t>(x.table_width) * a.table_page;
+  const int64_t programs = static_cast<int64_t>(a.bs) * a.kv_heads * groups;
+  int64_t n = (256 * resident + programs / 2) / programs;
+  n = n < (bound + 255) / 256 ? n : (bound + 255) / 256;
+  n = n < a.splits ? n : a.splits;
+  return n > 1 ? static_cast<int>(n) : 1;
+}
+
 template <int D, typename T, int RT>
 int launch(const eagle4_row_attn_fp8_args& x, hipStream_t s) {
   const eagle4_row_attn_args& a = x.rows;
   const int R = a.rows_per_request * (a.heads / a.kv_heads);
   const int groups = (R + 16 * RT - 1) / (16 * RT);
-  const int splits = a.splits + (a.step == 0 ? 0 : 1);
-  if (static_cast<int64_t>(a.kv_heads) * groups > 65535) return EAGLE4_NOT_COVERED;
-  row_attention_fp8_kernel<D, T, RT><<<dim3(splits, a.kv_heads * groups, a.bs), NT, 0, s>>>(x, groups);
+  const int splits = used_splits(x, kResident<D, RT>, groups) + (a.step == 0 ? 0 : 1);
+  const int64_t grid = (static_cast<int64_t>(splits) * a.kv_heads * a.bs + 7) / 8 * 8 * groups;
+  if (grid >= (1 << 24)) return EAGLE4_NOT_COVERED;  // (256 threads each: under 2^32)
+  row_attention_fp8_kernel<D, T, RT><<<static_cast<unsigned>(grid), NT, 0, s>>>(x, groups, splits);
   const int64_t pairs = static_cast<int64_t>(a.bs) * a.rows_per_request * a.heads;
   return with_merge_runs<D>(splits, pairs, [&](auto runs) {
     constexpr int SG = decltype(runs)::value;
@@ -399,7 +471,8 @@ template <int D, typename T>
 int launch_rows(const eagle4_row_attn_fp8_args& x, hipStream_t s) {
   const int R = x.rows.rows_per_request * (x.rows.heads / x.rows.kv_heads);
   if (R <= 16) return launch<D, T, 1>(x, s);
-  return launch<D, T, 2>(x, s);
+  if (R <= 32 || D == 256) return launch<D, T, 2>(x, s);
+  if constexpr (D < 256) return launch<D, T, 4>(x, s);
 }
 
 template <typename T>
