@@ -26,10 +26,23 @@ using namespace e4vocab;
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int NT = 1024, kWaves = NT / 64;
-constexpr int kBins = 2048, kList = 2048;
-constexpr float kBinsPerOctave = 32.f;
+constexpr int kBins = 4096, kList = 2048;
+constexpr float kBinsPerOctave = 64.f;
 constexpr double kUnit = 0x1p45;
 constexpr uint32_t kLowestKey = 0x007fffffu;  // of -inf
+
+// A value that all threads have alike, in scalar registers.
+template <typename U>
+E4_DEV U uniform(U x) {
+  static_assert(sizeof(U) == 4 || sizeof(U) == 8, "one word or two");
+  if constexpr (sizeof(U) == 4) {
+    return __builtin_bit_cast(U, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, x)));
+  } else {
+    const uint64_t w = __builtin_bit_cast(uint64_t, x);
+    const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<int>(w)), hi = __builtin_amdgcn_readfirstlane(static_cast<int>(w >> 32));
+    return __builtin_bit_cast(U, static_cast<uint64_t>(hi) << 32 | lo);
+  }
+}
 
 // A logit as a whole number of the same order; NaN the largest, both zeros alike.
 E4_DEV uint32_t key_of(float x) {
@@ -44,11 +57,43 @@ E4_DEV uint64_t mass_of(float x, float top, double c) {
   const double y = __builtin_fma(weight_of(x, top, c), kUnit, 0x1p52);  // rounds to a whole number in the low 52 bits
   return __builtin_bit_cast(uint64_t, y) & 0xfffffffffffffull;
 }
-// Its bin; not decreasing as x falls.
-E4_DEV int bin_of(float x, float top, double c) {
-  const double t = (static_cast<double>(x) - static_cast<double>(top)) * (c * -static_cast<double>(kBinsPerOctave));
-  return static_cast<int>(__builtin_fmin(t == t ? t : 1e9, kBins - 1));  // (NaN: -inf times a scale of 0)
-}
+// Bins of a row's logits, their numbers rising as the logits fall. By weight: 64 a factor of two. By value (bf16): a bin for every
+// value of magnitude from 2^(high - 15) to below 2^high, one for the smaller ones and one for what lies below -2^high, which
+// weighs nothing. There a row is counted, and every value weighed once.
+struct Bins {
+  static constexpr int kOctaves = 15, kValues = kOctaves * 128, kSmall = kValues, kRest = 2 * kValues + 1;
+  bool by_value;
+  float top;
+  double c;
+  uint32_t low16, high16;  // bf16 patterns of 2^(high - 15) and 2^high
+
+  E4_DEV Bins(bool values, float top_, double c_) : by_value(false), top(top_), c(c_), low16(0), high16(0) {
+    if (!values) return;
+    // nothing below top - 32 T has a mass (e^-32 is 2^-46.2); magnitudes up to 2^10 leave few of a row's logits among the small
+    const float reach = __builtin_fmaxf(__builtin_fabsf(top), __builtin_fabsf(top - static_cast<float>(32.0 * 1.4426950408889634 / c)));
+    if (!(reach < 1024.f)) return;
+    by_value = true;
+    high16 = ((__float_as_uint(reach) >> 23) + 1) << 7;
+    high16 = uniform(high16);
+    high16 = high16 > 64 * 128 ? high16 : 64 * 128;
+    low16 = high16 - kValues;
+  }
+  E4_DEV int of(float x) const {
+    if (by_value) {
+      const uint32_t m = __float_as_uint(x) >> 16 & 0x7fffu;
+      if (m < low16) return kSmall;
+      const int at = m < high16 ? static_cast<int>(m - low16) : kValues;
+      return x > 0.f ? kValues - 1 - at : kValues + 1 + at;
+    }
+    const double t = (static_cast<double>(x) - static_cast<double>(top)) * (c * -static_cast<double>(kBinsPerOctave));
+    return static_cast<int>(__builtin_fmin(t == t ? t : 1e9, kBins - 1));  // (NaN: -inf times a scale of 0)
+  }
+  E4_DEV bool one_value(int b) const { return by_value && b != kSmall && b < kRest; }
+  E4_DEV float value(int b) const {
+    const uint32_t w = b < kValues ? low16 + (kValues - 1 - b) : 0x8000u | (low16 + (b - kValues - 1));
+    return __uint_as_float(w << 16);
+  }
+};
 
 struct Shared {
   uint64_t mass[kBins];   // running sums over the bins
@@ -62,7 +107,7 @@ struct Shared {
       uint64_t mass[kBins];
       uint32_t count[kBins];
     } sub;
-    float maxima[NT];
+    uint32_t maxima[NT];
   };
   u32x4 ends[2];
   uint64_t wave64[kWaves];
@@ -79,7 +124,7 @@ E4_DEV bool in_row(int e, int vocab) { return static_cast<uint32_t>(e) < static_
 // behind the last of those (at most one vector at each end) out of LDS, where they are put once.
 template <typename T>
 struct Rows {
-  static constexpr int VEC = Row<T>::VEC, U = 4;  // U vectors of a thread on their way together
+  static constexpr int VEC = Row<T>::VEC, kAhead = 4;  // vectors of a thread on their way together
   using S = typename T::storage;
   Row<T> row;
   int begin, end;  // whole vectors
@@ -89,7 +134,7 @@ struct Rows {
   int tid;
 
   E4_DEV Rows(const void* logits, int64_t n, int64_t stride, int vocab, float temperature, u32x4* lds, int tid_)
-      : row(logits, n, stride, vocab), ends(lds), top(0.f), c(scale_of(temperature)), tid(tid_) {
+      : row(logits, n, stride, vocab), ends(lds), top(0.f), c(uniform(scale_of(temperature))), tid(tid_) {
     begin = row.past > 0 ? 1 : 0;
     end = (vocab + row.past) / VEC;
     if (tid < 2 * VEC) {
@@ -98,50 +143,68 @@ struct Rows {
     }
     __syncthreads();
   }
+  static E4_DEV uint32_t lowest() {
+    const float none = -INFINITY;
+    if constexpr (VEC == 8)
+      return T::pack(none, none);
+    else
+      return __float_as_uint(none);
+  }
   // The first element of an end's vector; the row's size where there is none.
   E4_DEV int end_first(int side) const {
     if (side == 0) return row.past > 0 ? row.first(0) : row.vocab;
     return end >= begin && end < row.vectors ? row.first(end) : row.vocab;
   }
 
-  // f(first element, vector) for every vector, a thread's in ascending order; -inf outside the row.
-  template <typename F>
-  E4_DEV void each_vector(F&& f) const {
-    const float none = -INFINITY;
-    uint32_t low = __float_as_uint(none);
-    if constexpr (VEC == 8) low = T::pack(none, none);
-    for (int v0 = begin; v0 < end; v0 += U * NT) {
-      u32x4 w[U];
+  template <int U>
+  E4_DEV void fetch(int v0, u32x4 (&w)[U]) const {
+    const uint32_t low = lowest();
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int v = v0 + u * NT + tid;
+      w[u] = u32x4{low, low, low, low};
+      if (v < end) w[u] = row.raw(v);
+    }
+  }
+
+  // f(first element, vector) for every vector, a thread's in ascending order; -inf outside the row. Of `shares` workgroups the one
+  // with number `share` has every shares-th U NT vectors.
+  template <int U, typename F>
+  E4_DEV void each_vector(F&& f, int share = 0, int shares = 1) const {
+    const int step = shares * U * NT;
+    u32x4 w[U];
+    fetch(begin + share * U * NT, w);
+    for (int v0 = begin + share * U * NT; v0 < end; v0 += step) {
+      u32x4 now[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) now[u] = w[u];
+      if (v0 + step < end) fetch(v0 + step, w);  // on their way beside this batch's work
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int v = v0 + u * NT + tid;
-        w[u] = u32x4{low, low, low, low};
-        if (v < end) w[u] = row.raw(v);
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int v = v0 + u * NT + tid;
-        f(v < end ? row.first(v) : row.vocab, w[u]);
+        f(v < end ? row.first(v) : row.vocab, now[u]);
       }
     }
-    if (tid < 2) f(end_first(tid), ends[tid]);
+    if (tid < 2 && share == 0) f(end_first(tid), ends[tid]);
   }
 
   // f(first element, values)
-  template <typename F>
-  E4_DEV void each(F&& f) const {
-    each_vector([&](int e0, const u32x4& w) {
-      float x[VEC];
-      Row<T>::widen(w, x);
-      f(e0, x);
-    });
+  template <int U = kAhead, typename F>
+  E4_DEV void each(F&& f, int share = 0, int shares = 1) const {
+    each_vector<U>(
+        [&](int e0, const u32x4& w) {
+          float x[VEC];
+          Row<T>::widen(w, x);
+          f(e0, x);
+        },
+        share, shares);
   }
 
   // f(element, value) for every element of the row, a word of a vector at a time: what takes a weight of each element would
   // not fit the registers for a whole vector at once.
   template <typename F>
   E4_DEV void each_element(F&& f) const {
-    each_vector([&](int e0, u32x4 now) {
+    each_vector<kAhead / 2>([&](int e0, u32x4 now) {
 #pragma unroll 1
       for (int i = 0; i < 4; ++i) {
         if constexpr (VEC == 4) {
@@ -208,19 +271,21 @@ E4_DEV void scan_bins(uint64_t* mass, uint32_t* count, Shared& s, int tid) {
   __syncthreads();
 }
 
-// The first bin whose running sum exceeds `target` (the last bin where none does).
-template <typename U>
-E4_DEV int find_bin(const U* run, U target, Shared& s, int tid) {
+// The first bin whose running mass, or count, exceeds `target` (the last bin where none does).
+E4_DEV int find_bin(const uint64_t* mass, const uint32_t* count, bool by_mass, uint64_t target, Shared& s, int tid) {
   constexpr int P = kBins / NT;
   if (tid == 0) s.found = kBins - 1;
   __syncthreads();
+  uint64_t before = 0;
+  if (tid > 0) before = by_mass ? mass[P * tid - 1] : count[P * tid - 1];
 #pragma unroll
   for (int i = 0; i < P; ++i) {
-    const int b = P * tid + i;
-    if (run[b] > target && (b == 0 || run[b - 1] <= target)) s.found = b;
+    const uint64_t run = by_mass ? mass[P * tid + i] : count[P * tid + i];
+    if (run > target && (P * tid + i == 0 || before <= target)) s.found = P * tid + i;
+    before = run;
   }
   __syncthreads();
-  const int b = s.found;
+  const int b = uniform(s.found);
   __syncthreads();
   return b;
 }
@@ -233,12 +298,12 @@ E4_DEV uint32_t lowest_key(uint32_t lo, uint32_t hi, int lane, F&& ok) {
     const uint64_t span = static_cast<uint64_t>(hi) - lo;
     const uint32_t at = lo + static_cast<uint32_t>(span * lane / 64);  // lane 0: lo; below hi
     const uint64_t good = __ballot(ok(at));
-    if (good & 1) return lo;
+    if (good & 1) return uniform(lo);
     const int first = good == 0 ? 64 : __builtin_ctzll(good);
     hi = first == 64 ? hi : lo + static_cast<uint32_t>(span * first / 64);
     lo = lo + static_cast<uint32_t>(span * (first - 1) / 64) + 1;
   }
-  return hi;
+  return uniform(hi);
 }
 
 // Sorts s.list.entry[0 .. n) ascending; n at most kList. Every thread calls it.
@@ -297,7 +362,7 @@ E4_DEV int list_range(const Rows<T>& r, Shared& s, float lo, float hi, uint64_t 
       }
   });
   __syncthreads();
-  const int n = s.listed;
+  const int n = uniform(s.listed);
   if (n > kList) return n;
   sort_list(s, n, tid);
   constexpr int P = kList / NT;
@@ -370,19 +435,22 @@ E4_DEV int nth_equal(const Rows<T>& r, Shared& s, float x, uint32_t rank) {
   return e;
 }
 
-// The first element of the order whose running mass (kByMass) or count exceeds `target`, which is below the row's.
-template <bool kByMass, typename T>
-E4_DEV Place locate(const Rows<T>& r, Shared& s, uint64_t target) {
+// The first element of the order whose running mass (by_mass) or count exceeds `target`, which is below the row's.
+template <typename T>
+E4_DEV Place locate(const Rows<T>& r, const Bins& bins, Shared& s, bool by_mass, uint64_t target) {
   const int tid = r.tid, lane = tid & 63;
-  int b = kByMass ? find_bin(s.mass, target, s, tid) : find_bin(s.count, static_cast<uint32_t>(target), s, tid);
-  uint64_t mass = b > 0 ? s.mass[b - 1] : 0;  // before the range
-  uint32_t count = b > 0 ? s.count[b - 1] : 0, inside = s.count[b] - count;
-  const uint32_t top = key_of(r.top);
+  const int b = find_bin(s.mass, s.count, by_mass, target, s, tid);
+  uint64_t mass = uniform(b > 0 ? s.mass[b - 1] : uint64_t{0});  // before the range
+  uint32_t count = uniform(b > 0 ? s.count[b - 1] : 0u), inside = uniform(s.count[b]) - count;
   // the bin's keys; every wave finds them for itself
-  uint32_t lo = b == kBins - 1 ? kLowestKey
-                               : lowest_key(kLowestKey, top, lane, [&](uint32_t k) { return bin_of(value_of(k), r.top, r.c) <= b; });
-  uint32_t hi = b == 0 ? top
-                       : lowest_key(kLowestKey, top, lane, [&](uint32_t k) { return bin_of(value_of(k), r.top, r.c) < b; }) - 1;
+  const uint32_t top = key_of(r.top);
+  uint32_t lo = kLowestKey, hi = top;
+  if (bins.one_value(b)) {
+    lo = hi = key_of(bins.value(b));
+  } else {
+    if (b != kBins - 1) lo = lowest_key(kLowestKey, top, lane, [&](uint32_t k) { return bins.of(value_of(k)) <= b; });
+    if (bins.of(r.top) < b) hi = lowest_key(kLowestKey, top, lane, [&](uint32_t k) { return bins.of(value_of(k)) < b; }) - 1;
+  }
   while (inside > kList && lo < hi) {
     const int shift = 32 - __builtin_clz(hi - lo) > 11 ? 32 - __builtin_clz(hi - lo) - 11 : 0;
     __syncthreads();
@@ -401,10 +469,10 @@ E4_DEV Place locate(const Rows<T>& r, Shared& s, uint64_t target) {
     });
     __syncthreads();
     scan_bins(s.sub.mass, s.sub.count, s, tid);
-    const int at = kByMass ? find_bin(s.sub.mass, target - mass, s, tid) : find_bin(s.sub.count, static_cast<uint32_t>(target) - count, s, tid);
-    const uint64_t m0 = at > 0 ? s.sub.mass[at - 1] : 0;
-    const uint32_t c0 = at > 0 ? s.sub.count[at - 1] : 0;
-    inside = s.sub.count[at] - c0;
+    const int at = find_bin(s.sub.mass, s.sub.count, by_mass, target - (by_mass ? mass : count), s, tid);
+    const uint64_t m0 = uniform(at > 0 ? s.sub.mass[at - 1] : uint64_t{0});
+    const uint32_t c0 = uniform(at > 0 ? s.sub.count[at - 1] : 0u);
+    inside = uniform(s.sub.count[at]) - c0;
     mass += m0;
     count += c0;
     const uint32_t first = hi - (static_cast<uint32_t>(at) << shift);  // the range's highest key
@@ -417,7 +485,7 @@ E4_DEV Place locate(const Rows<T>& r, Shared& s, uint64_t target) {
   if (inside > kList) {  // one logit, many times
     p.x = value_of(lo);
     const uint64_t each = mass_of(p.x, r.top, r.c);
-    uint64_t rank = kByMass ? (each > 0 ? (target - mass) / each : 0) : target - count;
+    uint64_t rank = by_mass ? (each > 0 ? (target - mass) / each : 0) : target - count;
     if (rank >= inside) rank = inside - 1;
     p.run = mass + (rank + 1) * each;
     p.index = nth_equal(r, s, p.x, static_cast<uint32_t>(rank));
@@ -425,7 +493,7 @@ E4_DEV Place locate(const Rows<T>& r, Shared& s, uint64_t target) {
   }
   // (-0's key belongs to no element, but -0 >= 0)
   const int n = list_range(r, s, value_of(lo), value_of(hi == 0x7fffffffu ? hi - 1 : hi), mass);
-  int at = kByMass ? list_find(s, n, target) : static_cast<int>(static_cast<uint32_t>(target) - count);
+  int at = by_mass ? list_find(s, n, target) : static_cast<int>(static_cast<uint32_t>(target) - count);
   at = at < n ? at : n - 1;
   p.x = value_of(entry_key(s.list.entry[at]));
   p.index = static_cast<int>(static_cast<uint32_t>(s.list.entry[at]));
@@ -447,6 +515,37 @@ E4_DEV uint64_t nucleus_of(float p, uint64_t z) {
   if (!(t > 1.0)) return 0;
   const uint64_t u = t < 0x1p63 ? static_cast<uint64_t>(t) : z;
   return (u < z ? u : z) - 1;
+}
+
+// A logit that at least k of the row's reach, from the threads' own maxima: about the k-th largest of them. Of M threads' parts of
+// a row some -M ln(1 - k / M) logits reach it, so beyond kMostByMaxima the list would not hold them.
+constexpr int kMostByMaxima = 768;
+E4_DEV float bound_of(Shared& s, float mine, int k, int tid) {
+  s.maxima[tid] = key_of(mine);
+  __syncthreads();
+  if (tid < 64) {
+    uint32_t x[kWaves];
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) x[i] = s.maxima[64 * i + tid];
+    uint32_t lo = kLowestKey, hi = 0xff7fffffu;  // at least k maxima reach lo; hi: the largest finite logit
+    while (lo < hi) {
+      const uint32_t mid = lo + (hi - lo + 1) / 2;
+      int n = 0;
+#pragma unroll
+      for (int i = 0; i < kWaves; ++i) n += __popcll(__ballot(x[i] >= mid));
+      if (n >= k) {
+        lo = mid;
+        if (n <= k + k / 8 + 16) break;
+      } else {
+        hi = mid - 1;
+      }
+    }
+    if (tid == 0) s.thr = value_of(lo);
+  }
+  __syncthreads();
+  const float b = uniform(s.thr);
+  __syncthreads();
+  return b;
 }
 
 struct Cut {
@@ -480,11 +579,11 @@ E4_DEV void store_vector(U* out, int e0, int vocab, const U (&y)[N]) {
   }
 }
 
-template <typename T, typename P>
-E4_DEV void write_probs(const Rows<T>& r, const Cut& cut, uint64_t z, typename P::storage* out) {
+template <typename P, typename T>
+E4_DEV void write_probs(const Rows<T>& r, const Cut& cut, uint64_t z, typename P::storage* out, int share, int shares) {
   constexpr int VEC = Row<T>::VEC;
-  const double share = kUnit / static_cast<double>(z);
-  r.each([&](int e0, const float(&x)[VEC]) {
+  const double unit = kUnit / static_cast<double>(z);
+  r.template each<Rows<T>::kAhead / 2>([&](int e0, const float(&x)[VEC]) {
     typename P::storage y[VEC];
     float left[VEC];  // the kept logits, the others at -inf
     bool any = false;
@@ -498,7 +597,7 @@ E4_DEV void write_probs(const Rows<T>& r, const Cut& cut, uint64_t z, typename P
     if (any) {
 #pragma unroll 1
       for (int j = 0; j < VEC; ++j) {  // one weight at a time, for the registers
-        const float w = left[0] == -INFINITY ? 0.f : cut.single ? 1.f : static_cast<float>(weight_of(left[0], r.top, r.c) * share);
+        const float w = left[0] == -INFINITY ? 0.f : cut.single ? 1.f : static_cast<float>(weight_of(left[0], r.top, r.c) * unit);
 #pragma unroll
         for (int i = 0; i + 1 < VEC; ++i) {
           left[i] = left[i + 1];
@@ -508,11 +607,11 @@ E4_DEV void write_probs(const Rows<T>& r, const Cut& cut, uint64_t z, typename P
       }
     }
     store_vector(out, e0, r.row.vocab, y);
-  });
+  }, share, shares);
 }
 
 template <typename T>
-E4_DEV void write_logits(const Rows<T>& r, const Cut& cut, typename T::storage* out) {
+E4_DEV void write_logits(const Rows<T>& r, const Cut& cut, typename T::storage* out, int share, int shares) {
   constexpr int VEC = Row<T>::VEC;
   r.each([&](int e0, const float(&x)[VEC]) {
     typename T::storage y[VEC];
@@ -522,20 +621,21 @@ E4_DEV void write_logits(const Rows<T>& r, const Cut& cut, typename T::storage* 
       y[i] = T::from_f32(kept ? x[i] : -INFINITY);
     }
     store_vector(out, e0, r.row.vocab, y);
-  });
+  }, share, shares);
 }
 
 template <typename T>
-__global__ __launch_bounds__(NT) void sample_rows_kernel(const eagle4_sample_rows_args a) {
+__global__ __launch_bounds__(NT) void sample_rows_kernel(const eagle4_sample_rows_args a, int shares) {
   __shared__ Shared s;
   constexpr int VEC = Row<T>::VEC;
-  const int64_t n = blockIdx.x;
+  const int64_t n = blockIdx.x / static_cast<uint32_t>(shares);
+  const int share = blockIdx.x % static_cast<uint32_t>(shares);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t entry = a.entries.ptr != nullptr ? e4::ld(a.entries, n) : n;
+  const int64_t entry = uniform(a.entries.ptr != nullptr ? e4::ld(a.entries, n) : n);
   if (entry < 0 || entry >= a.num_entries) return;  // a padded row
-  const float temperature = a.temperature[entry];
-  const int k = a.top_k != nullptr ? a.top_k[entry] : 0;
-  const float p = a.top_p != nullptr ? a.top_p[entry] : 1.f, m = a.min_p != nullptr ? a.min_p[entry] : 0.f;
+  const float temperature = uniform(a.temperature[entry]);
+  const int k = uniform(a.top_k != nullptr ? a.top_k[entry] : 0);
+  const float p = uniform(a.top_p != nullptr ? a.top_p[entry] : 1.f), m = uniform(a.min_p != nullptr ? a.min_p[entry] : 0.f);
 
   Rows<T> r(a.logits, n, a.stride_row, a.vocab, temperature, s.ends, tid);
   float mine = -INFINITY;
@@ -549,12 +649,12 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const eagle4_sample_row
     __syncthreads();
     float top = __uint_as_float(s.wave32[0]);
     for (int i = 1; i < kWaves; ++i) top = __builtin_elementwise_maximum(top, __uint_as_float(s.wave32[i]));
-    r.top = top;
+    r.top = uniform(top);
     __syncthreads();
   }
   Cut cut{-INFINITY, INT32_MAX, false};
   uint64_t z = static_cast<uint64_t>(kUnit);
-  int64_t* const tokens = a.tokens != nullptr ? a.tokens + n * a.draws : nullptr;
+  int64_t* const tokens = a.tokens != nullptr && share == 0 ? a.tokens + n * a.draws : nullptr;
   const float* const coins = a.coins != nullptr ? a.coins + n * a.draws : nullptr;
 
   if (!(temperature > 0.f) || !(r.top < INFINITY) || r.top == -INFINITY) {  // the argmax alone
@@ -585,43 +685,47 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const eagle4_sample_row
     int listed = kList + 1;  // the list holds the order's beginning
     uint64_t z1 = 0;         // the mass that top-p is taken of, where it is known
     float bound = lowest;
-    if (by_k && k <= NT) {  // the k-th largest of the threads' maxima
-      s.maxima[tid] = mine;
-      __syncthreads();
-      int rank = 0;
-      for (int i = 0; i < NT; i += 4) {
-        const f32x4 o = *reinterpret_cast<const f32x4*>(&s.maxima[i]);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) rank += o[j] > mine || (o[j] == mine && i + j < tid);
-      }
-      if (rank == k - 1) s.thr = mine;
-      __syncthreads();
-      bound = s.thr > bound ? s.thr : bound;
-      __syncthreads();
+    if (by_k && k <= kMostByMaxima) {
+      const float b = bound_of(s, mine, k, tid);
+      bound = b > bound ? b : bound;
     }
-    if (by_m || (by_k && k <= NT)) listed = list_range(r, s, bound, r.top, 0);
     const bool asked = by_k || by_m || by_p || tokens != nullptr || a.out_kind == EAGLE4_ROWS_PROBS;
-    if (asked && listed > kList) {
+    const Bins bins(T::code == EAGLE4_BF16, r.top, r.c);
+    bool bounded = by_m || (by_k && k <= kMostByMaxima);
+    for (bool binned = !asked;;) {
+      if (bounded) listed = list_range(r, s, bound, r.top, 0);
+      if (listed <= kList || binned) break;
       for (int i = tid; i < kBins; i += NT) {
         s.mass[i] = 0;
         s.count[i] = 0;
       }
       __syncthreads();
-      r.each_element([&](int, float x) {
-        const int b = bin_of(x, r.top, r.c);
-        atomicAdd(reinterpret_cast<unsigned long long*>(&s.mass[b]), mass_of(x, r.top, r.c));
-        atomicAdd(&s.count[b], 1u);
-      });
+      if (bins.by_value) {
+        r.each_element([&](int, float x) {
+          const int b = bins.of(x);
+          atomicAdd(&s.count[b], 1u);
+          if (b == Bins::kSmall) atomicAdd(reinterpret_cast<unsigned long long*>(&s.mass[b]), mass_of(x, r.top, r.c));
+        });
+        __syncthreads();
+        for (int i = tid; i < Bins::kRest; i += NT)
+          if (i != Bins::kSmall && s.count[i] > 0) s.mass[i] = s.count[i] * mass_of(bins.value(i), r.top, r.c);
+      } else {
+        r.each_element([&](int, float x) {
+          const int b = bins.of(x);
+          atomicAdd(reinterpret_cast<unsigned long long*>(&s.mass[b]), mass_of(x, r.top, r.c));
+          atomicAdd(&s.count[b], 1u);
+        });
+      }
       __syncthreads();
       scan_bins(s.mass, s.count, s, tid);
-      z1 = s.mass[kBins - 1];
+      z1 = uniform(s.mass[kBins - 1]);
+      binned = true;
+      bounded = false;
       if (!by_k && !by_m && by_p) {  // the bins say where top-p's cut is at most
-        const int b = find_bin(s.mass, nucleus_of(p, z1), s, tid);
-        if (s.count[b] <= kList) {
-          const uint32_t low = lowest_key(kLowestKey, key_of(r.top), lane,
-                                          [&](uint32_t key) { return bin_of(value_of(key), r.top, r.c) <= b; });
-          listed = list_range(r, s, value_of(low), r.top, 0);
-        }
+        const int b = find_bin(s.mass, s.count, true, nucleus_of(p, z1), s, tid);
+        bounded = s.count[b] <= kList;
+        if (bounded)
+          bound = value_of(lowest_key(kLowestKey, key_of(r.top), lane, [&](uint32_t key) { return bins.of(value_of(key)) <= b; }));
       }
     }
     if (listed <= kList) {  // everything is decided in the list
@@ -649,60 +753,73 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const eagle4_sample_row
         const int at = list_find(s, kept, target_of(coins[tid], z));
         tokens[tid] = static_cast<int64_t>(static_cast<uint32_t>(s.list.entry[at]));
       }
-    } else if (asked) {
-      if (by_k) {
-        const Place at = locate<false>(r, s, static_cast<uint64_t>(k) - 1);
+    } else if (asked) {  // one place after another: top-k's cut, min-p's, top-p's, the draws'
+      int d = -3;
+      while (d < 0 || (tokens != nullptr && d < a.draws)) {
+        const int step = d++;
+        bool by_mass = true;
+        uint64_t target = 0;
+        if (step == -3) {
+          if (!by_k) continue;
+          by_mass = false;
+          target = static_cast<uint64_t>(k) - 1;
+        } else if (step == -2) {
+          if (!by_m || (cut.x >= lowest && m <= 1.f)) continue;
+          if (m > 1.f) {  // the first token alone
+            by_mass = false;
+          } else {
+            uint64_t sum = 0;
+            r.each_element([&](int, float x) {
+              if (x >= lowest) sum += mass_of(x, r.top, r.c);
+            });
+            sum = block_scan(sum, s.wave64, tid);
+            if (tid == NT - 1) s.sum = sum;
+            __syncthreads();
+            cut.x = lowest;
+            cut.index = INT32_MAX;
+            z1 = uniform(s.sum);
+            __syncthreads();
+            continue;
+          }
+        } else if (step == -1) {
+          z = z1;
+          if (!by_p) continue;
+          target = nucleus_of(p, z1);
+        } else {
+          target = target_of(coins[step], z);
+        }
+        const Place at = locate(r, bins, s, by_mass, target);
+        if (step >= 0) {
+          if (tid == 0) tokens[step] = at.index;
+          continue;
+        }
         cut.x = at.x;
         cut.index = at.index;
-        z1 = at.run;
+        z1 = z = at.run;
       }
-      if (by_m && (cut.x < lowest || m > 1.f)) {  // min-p's cut comes first (its first token is the order's)
-        uint64_t sum = 0;
-        r.each_element([&](int, float x) {
-          if (x >= lowest) sum += mass_of(x, r.top, r.c);
-        });
-        sum = block_scan(sum, s.wave64, tid);
-        if (tid == NT - 1) s.sum = sum;
-        __syncthreads();
-        cut.x = lowest;
-        cut.index = INT32_MAX;
-        z1 = s.sum;
-        __syncthreads();
-        if (m > 1.f) {
-          const Place at = locate<false>(r, s, 0);
-          cut.index = at.index;
-          z1 = at.run;
-        }
-      }
-      z = z1;
-      if (by_p) {
-        const Place at = locate<true>(r, s, nucleus_of(p, z1));
-        cut.x = at.x;
-        cut.index = at.index;
-        z = at.run;
-      }
-      if (tokens != nullptr)
-        for (int d = 0; d < a.draws; ++d) {
-          const Place at = locate<true>(r, s, target_of(coins[d], z));
-          if (tid == 0) tokens[d] = at.index;
-        }
     }
   }
   if (a.out == nullptr) return;
   if (a.out_kind == EAGLE4_ROWS_LOGITS) {
-    write_logits(r, cut, static_cast<typename T::storage*>(a.out) + n * a.stride_out);
+    write_logits(r, cut, static_cast<typename T::storage*>(a.out) + n * a.stride_out, share, shares);
   } else if (a.out_dtype == EAGLE4_F32) {
-    write_probs<T, e4::F32>(r, cut, z, static_cast<float*>(a.out) + n * a.stride_out);
+    write_probs<e4::F32>(r, cut, z, static_cast<float*>(a.out) + n * a.stride_out, share, shares);
   } else if (a.out_dtype == EAGLE4_BF16) {
-    write_probs<T, e4::Bf16>(r, cut, z, static_cast<uint16_t*>(a.out) + n * a.stride_out);
+    write_probs<e4::Bf16>(r, cut, z, static_cast<uint16_t*>(a.out) + n * a.stride_out, share, shares);
   } else {
-    write_probs<T, e4::F16>(r, cut, z, static_cast<uint16_t*>(a.out) + n * a.stride_out);
+    write_probs<e4::F16>(r, cut, z, static_cast<uint16_t*>(a.out) + n * a.stride_out, share, shares);
   }
 }
 
 template <typename T>
 int launch(const eagle4_sample_rows_args& a, hipStream_t s) {
-  sample_rows_kernel<T><<<static_cast<unsigned>(a.rows), NT, 0, s>>>(a);
+  // Few rows with an output: several workgroups a row find the same cut, and each writes its part (not in place, where one
+  // would write what another still reads).
+  constexpr int kPart = Rows<T>::kAhead * NT * Row<T>::VEC;
+  const int parts = (a.vocab + kPart - 1) / kPart;
+  int shares = 1;
+  if (a.out != nullptr && a.out != a.logits && a.rows <= 128) shares = static_cast<int>(256 / a.rows < parts ? 256 / a.rows : parts);
+  sample_rows_kernel<T><<<static_cast<unsigned>(a.rows * shares), NT, 0, s>>>(a, shares);
   return E4_LAUNCH_STATUS();
 }
 
