@@ -70,7 +70,7 @@ struct Bins {
   E4_DEV Bins(bool values, float top_, double c_) : by_value(false), top(top_), c(c_), low16(0), high16(0) {
     if (!values) return;
     // nothing below top - 32 T has a mass (e^-32 is 2^-46.2); magnitudes up to 2^10 leave few of a row's logits among the small
-    const float reach = __builtin_fmaxf(__builtin_fabsf(top), __builtin_fabsf(top - static_cast<float>(32.0 * 1.4426950408889634 / c)));
+    const float reach = uniform(__builtin_fmaxf(__builtin_fabsf(top), __builtin_fabsf(top - static_cast<float>(32.0 * 1.4426950408889634 / c))));
     if (!(reach < 1024.f)) return;
     by_value = true;
     high16 = ((__float_as_uint(reach) >> 23) + 1) << 7;
@@ -124,7 +124,7 @@ E4_DEV bool in_row(int e, int vocab) { return static_cast<uint32_t>(e) < static_
 // behind the last of those (at most one vector at each end) out of LDS, where they are put once.
 template <typename T>
 struct Rows {
-  static constexpr int VEC = Row<T>::VEC, kAhead = 4;  // vectors of a thread on their way together
+  static constexpr int VEC = Row<T>::VEC, kAhead = 3, kAheadWeighed = 2;  // a thread's vectors on their way
   using S = typename T::storage;
   Row<T> row;
   int begin, end;  // whole vectors
@@ -156,34 +156,42 @@ struct Rows {
     return end >= begin && end < row.vectors ? row.first(end) : row.vocab;
   }
 
-  template <int U>
-  E4_DEV void fetch(int v0, u32x4 (&w)[U]) const {
-    const uint32_t low = lowest();
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int v = v0 + u * NT + tid;
-      w[u] = u32x4{low, low, low, low};
-      if (v < end) w[u] = row.raw(v);
-    }
+  // This thread's vector of chunk c: NT vectors from `begin` on, all of them in the row.
+  E4_DEV u32x4 load(int c) const {  // (passes read a row again: temporal)
+    return *reinterpret_cast<const u32x4*>(row.p + row.first(begin + tid) + static_cast<int64_t>(c) * (NT * VEC));
   }
 
-  // f(first element, vector) for every vector, a thread's in ascending order; -inf outside the row. Of `shares` workgroups the one
-  // with number `share` has every shares-th U NT vectors.
+  // f(first element, vector) for every vector, a thread's in ascending order but for the row's two ends; -inf outside the row. Of
+  // `shares` workgroups the one with number `share` has every shares-th chunk. U chunks are on their way all the time: each
+  // load takes the place of the one that is used up.
   template <int U, typename F>
   E4_DEV void each_vector(F&& f, int share = 0, int shares = 1) const {
-    const int step = shares * U * NT;
-    u32x4 w[U];
-    fetch(begin + share * U * NT, w);
-    for (int v0 = begin + share * U * NT; v0 < end; v0 += step) {
-      u32x4 now[U];
+    const int whole = end > begin ? (end - begin) / NT : 0;
+    const int n = whole > share ? (whole - share + shares - 1) / shares : 0;  // chunks of this workgroup
+    const int e0 = row.first(begin + tid);
+    const auto chunk = [&](int j) { return share + shares * j; };
+    const auto first = [&](int j) { return e0 + chunk(j) * (NT * VEC); };
+    if (n > 0) {  // (past the last chunk: the last again, so that the loads on their way are U at every step)
+      const auto ahead = [&](int j) { return load(chunk(j < n ? j : n - 1)); };
+      u32x4 w[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) now[u] = w[u];
-      if (v0 + step < end) fetch(v0 + step, w);  // on their way beside this batch's work
+      for (int u = 0; u < U; ++u) w[u] = ahead(u);
+      for (int j = 0; j < n; j += U) {
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int v = v0 + u * NT + tid;
-        f(v < end ? row.first(v) : row.vocab, now[u]);
+        for (int u = 0; u < U; ++u) {
+          const u32x4 now = w[u];
+          w[u] = ahead(j + U + u);
+          if (j + u < n) f(first(j + u), now);
+        }
       }
+    }
+    // what is left: less than a chunk of whole vectors, and the ends
+    if (whole % shares == share) {
+      const int v = begin + whole * NT + tid;
+      const uint32_t low = lowest();
+      u32x4 last = {low, low, low, low};
+      if (v < end) last = load(whole);
+      f(v < end ? row.first(v) : row.vocab, last);
     }
     if (tid < 2 && share == 0) f(end_first(tid), ends[tid]);
   }
@@ -200,23 +208,25 @@ struct Rows {
         share, shares);
   }
 
-  // f(element, value) for every element of the row, a word of a vector at a time: what takes a weight of each element would
-  // not fit the registers for a whole vector at once.
+  // f(element, value) for every element of a vector, a word at a time: what takes a weight of each element would not fit the
+  // registers for a whole vector at once.
+  template <typename F>
+  E4_DEV void elements(int e0, u32x4 now, F&& f) const {
+#pragma unroll 1
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (VEC == 4) {
+        if (in_row(e0 + i, row.vocab)) f(e0 + i, __uint_as_float(now[0]));
+      } else {
+        const int e = e0 + 2 * i;
+        if (in_row(e, row.vocab)) f(e, T::to_f32(static_cast<uint16_t>(now[0])));
+        if (in_row(e + 1, row.vocab)) f(e + 1, T::to_f32(static_cast<uint16_t>(now[0] >> 16)));
+      }
+      now = u32x4{now[1], now[2], now[3], now[0]};
+    }
+  }
   template <typename F>
   E4_DEV void each_element(F&& f) const {
-    each_vector<kAhead / 2>([&](int e0, u32x4 now) {
-#pragma unroll 1
-      for (int i = 0; i < 4; ++i) {
-        if constexpr (VEC == 4) {
-          if (in_row(e0 + i, row.vocab)) f(e0 + i, __uint_as_float(now[0]));
-        } else {
-          const int e = e0 + 2 * i;
-          if (in_row(e, row.vocab)) f(e, T::to_f32(static_cast<uint16_t>(now[0])));
-          if (in_row(e + 1, row.vocab)) f(e + 1, T::to_f32(static_cast<uint16_t>(now[0] >> 16)));
-        }
-        now = u32x4{now[1], now[2], now[3], now[0]};
-      }
-    });
+    each_vector<kAheadWeighed>([&](int e0, const u32x4& w) { elements(e0, w, f); });
   }
 };
 
@@ -293,7 +303,8 @@ E4_DEV int find_bin(const uint64_t* mass, const uint32_t* count, bool by_mass, u
 // The lowest key in [lo, hi] for which `ok` holds, given that it holds for hi and for every key above one that it
 // holds for. By one wave: 64 probes a round.
 template <typename F>
-E4_DEV uint32_t lowest_key(uint32_t lo, uint32_t hi, int lane, F&& ok) {
+E4_DEV uint32_t lowest_key(uint32_t lo, uint32_t hi, F&& ok) {
+  const int lane = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
   while (lo < hi) {
     const uint64_t span = static_cast<uint64_t>(hi) - lo;
     const uint32_t at = lo + static_cast<uint32_t>(span * lane / 64);  // lane 0: lo; below hi
@@ -353,13 +364,18 @@ E4_DEV int list_range(const Rows<T>& r, Shared& s, float lo, float hi, uint64_t 
   __syncthreads();
   if (tid == 0) s.listed = 0;
   __syncthreads();
-  r.each([&](int e0, const float(&x)[Row<T>::VEC]) {
+  r.template each_vector<Rows<T>::kAhead>([&](int e0, const u32x4& w) {
+    float x[Row<T>::VEC];
+    Row<T>::widen(w, x);
+    bool any = false;
 #pragma unroll
-    for (int i = 0; i < Row<T>::VEC; ++i)
-      if (x[i] >= lo && x[i] <= hi && in_row(e0 + i, r.row.vocab)) {
+    for (int i = 0; i < Row<T>::VEC; ++i) any |= x[i] >= lo && x[i] <= hi;
+    if (any)
+      r.elements(e0, w, [&](int e, float y) {
+        if (!(y >= lo && y <= hi)) return;
         const uint32_t at = atomicAdd(&s.listed, 1u);
-        if (at < kList) s.list.entry[at] = (static_cast<uint64_t>(~key_of(x[i])) << 32) | static_cast<uint32_t>(e0 + i);
-      }
+        if (at < kList) s.list.entry[at] = (static_cast<uint64_t>(~key_of(y)) << 32) | static_cast<uint32_t>(e);
+      });
   });
   __syncthreads();
   const int n = uniform(s.listed);
@@ -438,7 +454,7 @@ E4_DEV int nth_equal(const Rows<T>& r, Shared& s, float x, uint32_t rank) {
 // The first element of the order whose running mass (by_mass) or count exceeds `target`, which is below the row's.
 template <typename T>
 E4_DEV Place locate(const Rows<T>& r, const Bins& bins, Shared& s, bool by_mass, uint64_t target) {
-  const int tid = r.tid, lane = tid & 63;
+  const int tid = r.tid;
   const int b = find_bin(s.mass, s.count, by_mass, target, s, tid);
   uint64_t mass = uniform(b > 0 ? s.mass[b - 1] : uint64_t{0});  // before the range
   uint32_t count = uniform(b > 0 ? s.count[b - 1] : 0u), inside = uniform(s.count[b]) - count;
@@ -448,8 +464,8 @@ E4_DEV Place locate(const Rows<T>& r, const Bins& bins, Shared& s, bool by_mass,
   if (bins.one_value(b)) {
     lo = hi = key_of(bins.value(b));
   } else {
-    if (b != kBins - 1) lo = lowest_key(kLowestKey, top, lane, [&](uint32_t k) { return bins.of(value_of(k)) <= b; });
-    if (bins.of(r.top) < b) hi = lowest_key(kLowestKey, top, lane, [&](uint32_t k) { return bins.of(value_of(k)) < b; }) - 1;
+    if (b != kBins - 1) lo = lowest_key(kLowestKey, top, [&](uint32_t k) { return bins.of(value_of(k)) <= b; });
+    if (bins.of(r.top) < b) hi = lowest_key(kLowestKey, top, [&](uint32_t k) { return bins.of(value_of(k)) < b; }) - 1;
   }
   while (inside > kList && lo < hi) {
     const int shift = 32 - __builtin_clz(hi - lo) > 11 ? 32 - __builtin_clz(hi - lo) - 11 : 0;
@@ -583,7 +599,7 @@ template <typename P, typename T>
 E4_DEV void write_probs(const Rows<T>& r, const Cut& cut, uint64_t z, typename P::storage* out, int share, int shares) {
   constexpr int VEC = Row<T>::VEC;
   const double unit = kUnit / static_cast<double>(z);
-  r.template each<Rows<T>::kAhead / 2>([&](int e0, const float(&x)[VEC]) {
+  r.template each<Rows<T>::kAheadWeighed>([&](int e0, const float(&x)[VEC]) {
     typename P::storage y[VEC];
     float left[VEC];  // the kept logits, the others at -inf
     bool any = false;
@@ -613,7 +629,7 @@ E4_DEV void write_probs(const Rows<T>& r, const Cut& cut, uint64_t z, typename P
 template <typename T>
 E4_DEV void write_logits(const Rows<T>& r, const Cut& cut, typename T::storage* out, int share, int shares) {
   constexpr int VEC = Row<T>::VEC;
-  r.each([&](int e0, const float(&x)[VEC]) {
+  r.template each<Rows<T>::kAheadWeighed>([&](int e0, const float(&x)[VEC]) {
     typename T::storage y[VEC];
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
@@ -661,12 +677,14 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const eagle4_sample_row
     if (tid == 0) s.found = INT32_MAX;
     __syncthreads();
     int at = INT32_MAX;
-    r.each([&](int e0, const float(&x)[VEC]) {
+    const auto hit = [&](float x) { return r.top != r.top ? x != x : x == r.top; };
+    r.template each_vector<Rows<T>::kAhead>([&](int e0, const u32x4& w) {
+      float x[VEC];
+      Row<T>::widen(w, x);
+      bool any = false;
 #pragma unroll
-      for (int i = VEC - 1; i >= 0; --i) {
-        const bool hit = r.top != r.top ? x[i] != x[i] : x[i] == r.top;
-        if (hit && in_row(e0 + i, a.vocab) && e0 + i < at) at = e0 + i;
-      }
+      for (int i = 0; i < VEC; ++i) any |= hit(x[i]);
+      if (any) r.elements(e0, w, [&](int e, float y) { at = hit(y) && e < at ? e : at; });
     });
     if (at != INT32_MAX) atomicMin(&s.found, at);
     __syncthreads();
@@ -679,15 +697,15 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const eagle4_sample_row
     float lowest = -INFINITY;
     if (by_m) {
       const double want = m < 1.f ? static_cast<double>(m) : 1.0;
-      lowest = value_of(lowest_key(kLowestKey, key_of(r.top), lane,
-                                   [&](uint32_t key) { return weight_of(value_of(key), r.top, r.c) >= want; }));
+      lowest = uniform(value_of(lowest_key(kLowestKey, key_of(r.top),
+                                   [&](uint32_t key) { return weight_of(value_of(key), r.top, r.c) >= want; })));
     }
     int listed = kList + 1;  // the list holds the order's beginning
     uint64_t z1 = 0;         // the mass that top-p is taken of, where it is known
     float bound = lowest;
     if (by_k && k <= kMostByMaxima) {
       const float b = bound_of(s, mine, k, tid);
-      bound = b > bound ? b : bound;
+      bound = uniform(b > bound ? b : bound);
     }
     const bool asked = by_k || by_m || by_p || tokens != nullptr || a.out_kind == EAGLE4_ROWS_PROBS;
     const Bins bins(T::code == EAGLE4_BF16, r.top, r.c);
@@ -725,7 +743,7 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const eagle4_sample_row
         const int b = find_bin(s.mass, s.count, true, nucleus_of(p, z1), s, tid);
         bounded = s.count[b] <= kList;
         if (bounded)
-          bound = value_of(lowest_key(kLowestKey, key_of(r.top), lane, [&](uint32_t key) { return bins.of(value_of(key)) <= b; }));
+          bound = uniform(value_of(lowest_key(kLowestKey, key_of(r.top), [&](uint32_t key) { return bins.of(value_of(key)) <= b; })));
       }
     }
     if (listed <= kList) {  // everything is decided in the list
@@ -815,7 +833,7 @@ template <typename T>
 int launch(const eagle4_sample_rows_args& a, hipStream_t s) {
   // Few rows with an output: several workgroups a row find the same cut, and each writes its part (not in place, where one
   // would write what another still reads).
-  constexpr int kPart = Rows<T>::kAhead * NT * Row<T>::VEC;
+  constexpr int kPart = NT * Row<T>::VEC;
   const int parts = (a.vocab + kPart - 1) / kPart;
   int shares = 1;
   if (a.out != nullptr && a.out != a.logits && a.rows <= 128) shares = static_cast<int>(256 / a.rows < parts ? 256 / a.rows : parts);
