@@ -17,13 +17,16 @@
 // into 2048 bins of log2 w (1/32 each), and a place of the order is found in its bin: gathered and sorted where the
 // bin holds few tokens, divided into 2048 ranges of logits again where it holds many.
 
+#include <type_traits>
+
 #include "vocab_row.h"
 
 namespace {
 
 using namespace e4vocab;
 
-typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+typedef int16_t i16x2 __attribute__((ext_vector_type(2)));
 
 constexpr int NT = 1024, kWaves = NT / 64;
 constexpr int kBins = 4096, kList = 2048;
@@ -61,16 +64,16 @@ E4_DEV uint64_t mass_of(float x, float top, double c) {
 // value of magnitude from 2^(high - 15) to below 2^high, one for the smaller ones and one for what lies below -2^high, which
 // weighs nothing. There a row is counted, and every value weighed once.
 struct Bins {
-  static constexpr int kOctaves = 15, kValues = kOctaves * 128, kSmall = kValues, kRest = 2 * kValues + 1;
+  static constexpr int kOctaves = 15, kValues = kOctaves * 128, kSmall = kValues, kRest = 2 * kValues + 1;  // bins of values: 0 .. kRest - 1
   bool by_value;
   float top;
   double c;
   uint32_t low16, high16;  // bf16 patterns of 2^(high - 15) and 2^high
 
-  E4_DEV Bins(bool values, float top_, double c_) : by_value(false), top(top_), c(c_), low16(0), high16(0) {
+  E4_DEV Bins(bool values, float top_, float temperature, double c_) : by_value(false), top(top_), c(c_), low16(0), high16(0) {
     if (!values) return;
     // nothing below top - 32 T has a mass (e^-32 is 2^-46.2); magnitudes up to 2^10 leave few of a row's logits among the small
-    const float reach = uniform(__builtin_fmaxf(__builtin_fabsf(top), __builtin_fabsf(top - static_cast<float>(32.0 * 1.4426950408889634 / c))));
+    const float reach = uniform(__builtin_fmaxf(__builtin_fabsf(top), __builtin_fabsf(top - 32.5f * temperature)));
     if (!(reach < 1024.f)) return;
     by_value = true;
     high16 = ((__float_as_uint(reach) >> 23) + 1) << 7;
@@ -78,34 +81,45 @@ struct Bins {
     high16 = high16 > 64 * 128 ? high16 : 64 * 128;
     low16 = high16 - kValues;
   }
+  // A bf16 pattern's magnitude as steps from the small ones: 0 for them, kValues + 1 from 2^high on. (Positive ones do not come there.)
+  E4_DEV int steps(uint32_t w) const {
+    const int m = w & 0x7fffu, lo = static_cast<int>(low16) - 1, hi = high16;
+    return (m < lo ? lo : m < hi ? m : hi) - lo;
+  }
   E4_DEV int of(float x) const {
     if (by_value) {
-      const uint32_t m = __float_as_uint(x) >> 16 & 0x7fffu;
-      if (m < low16) return kSmall;
-      const int at = m < high16 ? static_cast<int>(m - low16) : kValues;
-      return x > 0.f ? kValues - 1 - at : kValues + 1 + at;
+      const int up = steps(__float_as_uint(x) >> 16);
+      return kSmall + (x < 0.f ? up : -up);
     }
     const double t = (static_cast<double>(x) - static_cast<double>(top)) * (c * -static_cast<double>(kBinsPerOctave));
     return static_cast<int>(__builtin_fmin(t == t ? t : 1e9, kBins - 1));  // (NaN: -inf times a scale of 0)
   }
+  // Two patterns at once: their steps, and their bins' places in an array of words, in bytes.
+  E4_DEV void places(uint32_t w, u16x2& up, u16x2& at) const {
+    const uint16_t lo = static_cast<uint16_t>(low16 - 1), hi = static_cast<uint16_t>(high16);
+    const u16x2 m = __builtin_bit_cast(u16x2, w & 0x7fff7fffu);
+    up = __builtin_elementwise_min(__builtin_elementwise_max(m, u16x2{lo, lo}), u16x2{hi, hi}) - u16x2{lo, lo};
+    const u16x2 sign = __builtin_bit_cast(u16x2, __builtin_bit_cast(i16x2, w) >> 15);  // all ones below 0
+    at = ((up ^ ~sign) - ~sign + u16x2{kSmall, kSmall}) << 2;
+  }
   E4_DEV bool one_value(int b) const { return by_value && b != kSmall && b < kRest; }
   E4_DEV float value(int b) const {
-    const uint32_t w = b < kValues ? low16 + (kValues - 1 - b) : 0x8000u | (low16 + (b - kValues - 1));
+    const uint32_t w = b < kSmall ? low16 + (kSmall - 1 - b) : 0x8000u | (low16 + (b - kSmall - 1));
     return __uint_as_float(w << 16);
   }
 };
 
 struct Shared {
-  uint64_t mass[kBins];   // running sums over the bins
-  uint32_t count[kBins];
+  alignas(16) uint64_t mass[kBins];  // running sums over the bins
+  alignas(16) uint32_t count[kBins];
   union {
     struct {
       uint64_t entry[kList];  // (~key << 32) | index: ascending is the order
       uint64_t run[kList];    // running masses
     } list;
     struct {
-      uint64_t mass[kBins];
-      uint32_t count[kBins];
+      alignas(16) uint64_t mass[kBins];
+      alignas(16) uint32_t count[kBins];
     } sub;
     uint32_t maxima[NT];
   };
@@ -133,8 +147,8 @@ struct Rows {
   double c;
   int tid;
 
-  E4_DEV Rows(const void* logits, int64_t n, int64_t stride, int vocab, float temperature, u32x4* lds, int tid_)
-      : row(logits, n, stride, vocab), ends(lds), top(0.f), c(uniform(scale_of(temperature))), tid(tid_) {
+  E4_DEV Rows(const void* logits, int64_t n, int64_t stride, int vocab, u32x4* lds, int tid_)
+      : row(logits, n, stride, vocab), ends(lds), top(0.f), c(0.0), tid(tid_) {
     begin = row.past > 0 ? 1 : 0;
     end = (vocab + row.past) / VEC;
     if (tid < 2 * VEC) {
@@ -161,7 +175,7 @@ struct Rows {
     return *reinterpret_cast<const u32x4*>(row.p + row.first(begin + tid) + static_cast<int64_t>(c) * (NT * VEC));
   }
 
-  // f(first element, vector) for every vector, a thread's in ascending order but for the row's two ends; -inf outside the row. Of
+  // f(first element, vector, whether it is known to be inside the row) for every vector, a thread's in ascending order but for the row's two ends; -inf outside the row. Of
   // `shares` workgroups the one with number `share` has every shares-th chunk. U chunks are on their way all the time: each
   // load takes the place of the one that is used up.
   template <int U, typename F>
@@ -181,7 +195,7 @@ struct Rows {
         for (int u = 0; u < U; ++u) {
           const u32x4 now = w[u];
           w[u] = ahead(j + U + u);
-          if (j + u < n) f(first(j + u), now);
+          if (j + u < n) f(first(j + u), now, std::true_type{});
         }
       }
     }
@@ -191,16 +205,16 @@ struct Rows {
       const uint32_t low = lowest();
       u32x4 last = {low, low, low, low};
       if (v < end) last = load(whole);
-      f(v < end ? row.first(v) : row.vocab, last);
+      f(v < end ? row.first(v) : row.vocab, last, std::false_type{});
     }
-    if (tid < 2 && share == 0) f(end_first(tid), ends[tid]);
+    if (tid < 2 && share == 0) f(end_first(tid), ends[tid], std::false_type{});
   }
 
   // f(first element, values)
   template <int U = kAhead, typename F>
   E4_DEV void each(F&& f, int share = 0, int shares = 1) const {
     each_vector<U>(
-        [&](int e0, const u32x4& w) {
+        [&](int e0, const u32x4& w, auto) {
           float x[VEC];
           Row<T>::widen(w, x);
           f(e0, x);
@@ -210,23 +224,38 @@ struct Rows {
 
   // f(element, value) for every element of a vector, a word at a time: what takes a weight of each element would not fit the
   // registers for a whole vector at once.
-  template <typename F>
-  E4_DEV void elements(int e0, u32x4 now, F&& f) const {
+  template <typename Inside, typename F>
+  E4_DEV void elements(int e0, u32x4 now, Inside, F&& f) const {
 #pragma unroll 1
     for (int i = 0; i < 4; ++i) {
       if constexpr (VEC == 4) {
-        if (in_row(e0 + i, row.vocab)) f(e0 + i, __uint_as_float(now[0]));
+        if (Inside::value || in_row(e0 + i, row.vocab)) f(e0 + i, __uint_as_float(now[0]));
       } else {
         const int e = e0 + 2 * i;
-        if (in_row(e, row.vocab)) f(e, T::to_f32(static_cast<uint16_t>(now[0])));
-        if (in_row(e + 1, row.vocab)) f(e + 1, T::to_f32(static_cast<uint16_t>(now[0] >> 16)));
+        if (Inside::value || in_row(e, row.vocab)) f(e, T::to_f32(static_cast<uint16_t>(now[0])));
+        if (Inside::value || in_row(e + 1, row.vocab)) f(e + 1, T::to_f32(static_cast<uint16_t>(now[0] >> 16)));
       }
       now = u32x4{now[1], now[2], now[3], now[0]};
     }
   }
   template <typename F>
   E4_DEV void each_element(F&& f) const {
-    each_vector<kAheadWeighed>([&](int e0, const u32x4& w) { elements(e0, w, f); });
+    each_vector<kAheadWeighed>([&](int e0, const u32x4& w, auto inside) { elements(e0, w, inside, f); });
+  }
+
+  // f(element, value) for the elements of a vector that `hits` has a bit for, few of them.
+  template <typename F>
+  E4_DEV void hit_elements(int e0, const u32x4& w, uint32_t hits, F&& f) const {
+    while (hits != 0) {
+      const int i = __builtin_ctz(hits), k = VEC == 4 ? i : i / 2;
+      hits &= hits - 1;
+      const uint32_t one = k & 1 ? w[1] : w[0], two = k & 1 ? w[3] : w[2], word = k & 2 ? two : one;
+      if (!in_row(e0 + i, row.vocab)) continue;
+      if constexpr (VEC == 4)
+        f(e0 + i, __uint_as_float(word));
+      else
+        f(e0 + i, T::to_f32(static_cast<uint16_t>(i & 1 ? word >> 16 : word)));
+    }
   }
 };
 
@@ -259,25 +288,45 @@ E4_DEV U block_scan(U x, U* part, int tid) {
   return x;
 }
 
+E4_DEV void clear(uint64_t* mass, uint32_t* count, int tid) {
+  constexpr u32x4 none = {0u, 0u, 0u, 0u};
+  for (int i = tid; i < kBins / 2; i += NT) reinterpret_cast<u32x4*>(mass)[i] = none;
+  for (int i = tid; i < kBins / 4; i += NT) reinterpret_cast<u32x4*>(count)[i] = none;
+}
+
 // The bins' counts and masses become running sums.
 E4_DEV void scan_bins(uint64_t* mass, uint32_t* count, Shared& s, int tid) {
   constexpr int P = kBins / NT;
-  uint64_t m[P], ms = 0;
-  uint32_t k[P], ks = 0;
-#pragma unroll
-  for (int i = 0; i < P; ++i) {
-    ms += mass[P * tid + i];
-    m[i] = ms;
-    ks += count[P * tid + i];
-    k[i] = ks;
+  static_assert(P == 4, "a 16-byte piece of counts a thread");
+  const int lane = tid & 63, wave = tid >> 6;
+  typedef uint64_t u64x2 __attribute__((ext_vector_type(2)));
+  u64x2* const m = reinterpret_cast<u64x2*>(mass) + 2 * tid;
+  u32x4* const k = reinterpret_cast<u32x4*>(count) + tid;
+  u64x2 a = m[0], b = m[1];
+  u32x4 c = *k;
+  a[1] += a[0];
+  b[0] += a[1];
+  b[1] += b[0];
+  c[1] += c[0];
+  c[2] += c[1];
+  c[3] += c[2];
+  uint64_t mb = wave_scan(b[1], lane);
+  uint32_t kb = wave_scan(c[3], lane);
+  __syncthreads();
+  if (lane == 63) {
+    s.wave64[wave] = mb;
+    s.wave32[wave] = kb;
   }
-  const uint64_t mb = block_scan(ms, s.wave64, tid) - ms;
-  const uint32_t kb = block_scan(ks, s.wave32, tid) - ks;
-#pragma unroll
-  for (int i = 0; i < P; ++i) {
-    mass[P * tid + i] = mb + m[i];
-    count[P * tid + i] = kb + k[i];
+  __syncthreads();
+  mb -= b[1];
+  kb -= c[3];
+  for (int i = 0; i < wave; ++i) {
+    mb += s.wave64[i];
+    kb += s.wave32[i];
   }
+  m[0] = u64x2{a[0] + mb, a[1] + mb};
+  m[1] = u64x2{b[0] + mb, b[1] + mb};
+  *k = u32x4{c[0] + kb, c[1] + kb, c[2] + kb, c[3] + kb};
   __syncthreads();
 }
 
@@ -317,18 +366,64 @@ E4_DEV uint32_t lowest_key(uint32_t lo, uint32_t hi, F&& ok) {
   return uniform(hi);
 }
 
-// Sorts s.list.entry[0 .. n) ascending; n at most kList. Every thread calls it.
+// The lowest key of the bins up to b, given the row's largest.
+E4_DEV uint32_t lowest_of(const Bins& bins, int b, uint32_t top) {
+  if (!bins.by_value) return b == kBins - 1 ? kLowestKey : lowest_key(kLowestKey, top, [&](uint32_t k) { return bins.of(value_of(k)) <= b; });
+  if (b >= Bins::kRest) return kLowestKey;
+  return b == Bins::kSmall ? key_of(bins.value(b + 1)) + 1 : key_of(bins.value(b));
+}
+
+// Sorts s.list.entry[0 .. n) ascending; n at most kList. Every thread calls it. A bitonic network over the next power of two: an entry
+// a thread (two beyond NT), partners in the same wave by lane exchanges, those of other waves through LDS. (Every step through LDS
+// behind a barrier: 256 entries 16 us instead of 5.)
+template <int E>
+E4_DEV void sort_entries(Shared& s, int n, int size, int tid) {
+  uint64_t x[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) x[e] = tid + NT * e < n ? s.list.entry[tid + NT * e] : ~0ull;
+  for (int k = 2; k <= size; k <<= 1)
+    for (int j = k >> 1; j > 0; j >>= 1) {
+      if (E == 2 && j == NT) {  // the thread's own two (the last merge: ascending)
+        const uint64_t lo = x[0] < x[E - 1] ? x[0] : x[E - 1];
+        x[E - 1] = x[0] < x[E - 1] ? x[E - 1] : x[0];
+        x[0] = lo;
+        continue;
+      }
+      uint64_t o[E];
+      if (j < 64) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const uint32_t lo = __shfl_xor(static_cast<uint32_t>(x[e]), j, 64), hi = __shfl_xor(static_cast<uint32_t>(x[e] >> 32), j, 64);
+          o[e] = (static_cast<uint64_t>(hi) << 32) | lo;
+        }
+      } else {
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < E; ++e) s.list.entry[tid + NT * e] = x[e];
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] = s.list.entry[(tid ^ j) + NT * e];
+      }
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const bool keep_low = ((tid & j) == 0) == (((tid + NT * e) & k) == 0);
+        x[e] = keep_low == (o[e] < x[e]) ? o[e] : x[e];
+      }
+    }
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < E; ++e) s.list.entry[tid + NT * e] = x[e];
+  __syncthreads();
+}
 E4_DEV void sort_list(Shared& s, int n, int tid) {
   int size = 64;
   while (size < n) size <<= 1;
-  for (int i = n + tid; i < size; i += NT) s.list.entry[i] = ~0ull;
-  __syncthreads();
-  if (size == 64) {  // one wave, in registers
+  if (size == 64) {  // by one wave alone
     if (tid < 64) {
-      uint64_t x = s.list.entry[tid];
-#pragma unroll
+      uint64_t x = tid < n ? s.list.entry[tid] : ~0ull;
+#pragma unroll 1
       for (int k = 2; k <= 64; k <<= 1)
-#pragma unroll
+#pragma unroll 1
         for (int j = k >> 1; j > 0; j >>= 1) {
           const uint32_t lo = __shfl_xor(static_cast<uint32_t>(x), j, 64), hi = __shfl_xor(static_cast<uint32_t>(x >> 32), j, 64);
           const uint64_t o = (static_cast<uint64_t>(hi) << 32) | lo;
@@ -340,18 +435,10 @@ E4_DEV void sort_list(Shared& s, int n, int tid) {
     __syncthreads();
     return;
   }
-  for (int k = 2; k <= size; k <<= 1)
-    for (int j = k >> 1; j > 0; j >>= 1) {
-      for (int p = tid; p < size / 2; p += NT) {
-        const int i = 2 * p - (p & (j - 1)), o = i + j;
-        const uint64_t a = s.list.entry[i], b = s.list.entry[o];
-        if ((a > b) == ((i & k) == 0)) {
-          s.list.entry[i] = b;
-          s.list.entry[o] = a;
-        }
-      }
-      __syncthreads();
-    }
+  if (size <= NT)
+    sort_entries<1>(s, n, size, tid);
+  else
+    sort_entries<2>(s, n, size, tid);
 }
 
 E4_DEV uint32_t entry_key(uint64_t e) { return ~static_cast<uint32_t>(e >> 32); }
@@ -364,18 +451,31 @@ E4_DEV int list_range(const Rows<T>& r, Shared& s, float lo, float hi, uint64_t 
   __syncthreads();
   if (tid == 0) s.listed = 0;
   __syncthreads();
-  r.template each_vector<Rows<T>::kAhead>([&](int e0, const u32x4& w) {
-    float x[Row<T>::VEC];
+  const bool from_top = hi >= r.top;
+  r.template each_vector<Rows<T>::kAhead>([&](int e0, const u32x4& w, auto) {
+    constexpr int VEC = Row<T>::VEC;
+    float x[VEC];
     Row<T>::widen(w, x);
-    bool any = false;
+    bool any;
+    if (from_top) {
+      float most = x[0];
 #pragma unroll
-    for (int i = 0; i < Row<T>::VEC; ++i) any |= x[i] >= lo && x[i] <= hi;
-    if (any)
-      r.elements(e0, w, [&](int e, float y) {
-        if (!(y >= lo && y <= hi)) return;
+      for (int i = 1; i < VEC; ++i) most = __builtin_elementwise_maximum(most, x[i]);
+      any = most >= lo;
+    } else {
+      any = false;
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) any |= x[i] >= lo && x[i] <= hi;
+    }
+    if (any) {
+      uint32_t hits = 0;
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) hits |= x[i] >= lo && x[i] <= hi ? 1u << i : 0u;
+      r.hit_elements(e0, w, hits, [&](int e, float y) {
         const uint32_t at = atomicAdd(&s.listed, 1u);
         if (at < kList) s.list.entry[at] = (static_cast<uint64_t>(~key_of(y)) << 32) | static_cast<uint32_t>(e);
       });
+    }
   });
   __syncthreads();
   const int n = uniform(s.listed);
@@ -464,16 +564,13 @@ E4_DEV Place locate(const Rows<T>& r, const Bins& bins, Shared& s, bool by_mass,
   if (bins.one_value(b)) {
     lo = hi = key_of(bins.value(b));
   } else {
-    if (b != kBins - 1) lo = lowest_key(kLowestKey, top, [&](uint32_t k) { return bins.of(value_of(k)) <= b; });
-    if (bins.of(r.top) < b) hi = lowest_key(kLowestKey, top, [&](uint32_t k) { return bins.of(value_of(k)) < b; }) - 1;
+    lo = lowest_of(bins, b, top);
+    if (bins.of(r.top) < b) hi = lowest_of(bins, b - 1, top) - 1;
   }
   while (inside > kList && lo < hi) {
     const int shift = 32 - __builtin_clz(hi - lo) > 11 ? 32 - __builtin_clz(hi - lo) - 11 : 0;
     __syncthreads();
-    for (int i = tid; i < kBins; i += NT) {
-      s.sub.mass[i] = 0;
-      s.sub.count[i] = 0;
-    }
+    clear(s.sub.mass, s.sub.count, tid);
     __syncthreads();
     r.each_element([&](int, float x) {
       const uint32_t k = key_of(x);
@@ -543,7 +640,24 @@ E4_DEV float bound_of(Shared& s, float mine, int k, int tid) {
     uint32_t x[kWaves];
 #pragma unroll
     for (int i = 0; i < kWaves; ++i) x[i] = s.maxima[64 * i + tid];
-    uint32_t lo = kLowestKey, hi = 0xff7fffffu;  // at least k maxima reach lo; hi: the largest finite logit
+    // at least k maxima reach lo: the least of them that is a number, where there are k; none passes hi
+    uint32_t lo = 0xff7fffffu, hi = 0;
+    int numbers = 0;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) {
+      lo = x[i] > kLowestKey && x[i] < lo ? x[i] : lo;
+      hi = x[i] > hi ? x[i] : hi;
+      numbers += __popcll(__ballot(x[i] > kLowestKey));
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const uint32_t l = __shfl_xor(lo, d, 64), h = __shfl_xor(hi, d, 64);
+      lo = l < lo ? l : lo;
+      hi = h > hi ? h : hi;
+    }
+    lo = uniform(lo);
+    hi = uniform(hi);
+    if (numbers < k) lo = hi = kLowestKey;
     while (lo < hi) {
       const uint32_t mid = lo + (hi - lo + 1) / 2;
       int n = 0;
@@ -653,7 +767,10 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const eagle4_sample_row
   const int k = uniform(a.top_k != nullptr ? a.top_k[entry] : 0);
   const float p = uniform(a.top_p != nullptr ? a.top_p[entry] : 1.f), m = uniform(a.min_p != nullptr ? a.min_p[entry] : 0.f);
 
-  Rows<T> r(a.logits, n, a.stride_row, a.vocab, temperature, s.ends, tid);
+  int64_t* const tokens = a.tokens != nullptr && share == 0 ? a.tokens + n * a.draws : nullptr;
+  const float* const coins = a.coins != nullptr ? a.coins + n * a.draws : nullptr;
+  const float coin = tokens != nullptr && tid < a.draws ? coins[tid] : 0.f;  // (here, beside the row's first loads)
+  Rows<T> r(a.logits, n, a.stride_row, a.vocab, s.ends, tid);
   float mine = -INFINITY;
   r.each([&](int, const float(&x)[VEC]) {
 #pragma unroll
@@ -666,25 +783,28 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const eagle4_sample_row
     float top = __uint_as_float(s.wave32[0]);
     for (int i = 1; i < kWaves; ++i) top = __builtin_elementwise_maximum(top, __uint_as_float(s.wave32[i]));
     r.top = uniform(top);
+    r.c = uniform(scale_of(temperature));
     __syncthreads();
   }
   Cut cut{-INFINITY, INT32_MAX, false};
   uint64_t z = static_cast<uint64_t>(kUnit);
-  int64_t* const tokens = a.tokens != nullptr && share == 0 ? a.tokens + n * a.draws : nullptr;
-  const float* const coins = a.coins != nullptr ? a.coins + n * a.draws : nullptr;
 
   if (!(temperature > 0.f) || !(r.top < INFINITY) || r.top == -INFINITY) {  // the argmax alone
     if (tid == 0) s.found = INT32_MAX;
     __syncthreads();
     int at = INT32_MAX;
-    const auto hit = [&](float x) { return r.top != r.top ? x != x : x == r.top; };
-    r.template each_vector<Rows<T>::kAhead>([&](int e0, const u32x4& w) {
+    r.template each_vector<Rows<T>::kAhead>([&](int e0, const u32x4& w, auto) {
       float x[VEC];
       Row<T>::widen(w, x);
-      bool any = false;
+      float most = x[0];
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) any |= hit(x[i]);
-      if (any) r.elements(e0, w, [&](int e, float y) { at = hit(y) && e < at ? e : at; });
+      for (int i = 1; i < VEC; ++i) most = __builtin_elementwise_maximum(most, x[i]);
+      if (most == r.top || most != most) {
+        uint32_t hits = 0;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) hits |= (r.top != r.top ? x[i] != x[i] : x[i] == r.top) ? 1u << i : 0u;
+        r.hit_elements(e0, w, hits, [&](int e, float) { at = e < at ? e : at; });
+      }
     });
     if (at != INT32_MAX) atomicMin(&s.found, at);
     __syncthreads();
@@ -708,22 +828,34 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const eagle4_sample_row
       bound = uniform(b > bound ? b : bound);
     }
     const bool asked = by_k || by_m || by_p || tokens != nullptr || a.out_kind == EAGLE4_ROWS_PROBS;
-    const Bins bins(T::code == EAGLE4_BF16, r.top, r.c);
+    const Bins bins(T::code == EAGLE4_BF16, r.top, temperature, r.c);
     bool bounded = by_m || (by_k && k <= kMostByMaxima);
     for (bool binned = !asked;;) {
       if (bounded) listed = list_range(r, s, bound, r.top, 0);
       if (listed <= kList || binned) break;
-      for (int i = tid; i < kBins; i += NT) {
-        s.mass[i] = 0;
-        s.count[i] = 0;
-      }
+      clear(s.mass, s.count, tid);
       __syncthreads();
       if (bins.by_value) {
-        r.each_element([&](int, float x) {
-          const int b = bins.of(x);
-          atomicAdd(&s.count[b], 1u);
-          if (b == Bins::kSmall) atomicAdd(reinterpret_cast<unsigned long long*>(&s.mass[b]), mass_of(x, r.top, r.c));
-        });
+        if constexpr (T::code == EAGLE4_BF16)
+          r.template each_vector<Rows<T>::kAhead>([&](int e0, const u32x4& w, auto inside) {
+            u16x2 least = {0xffff, 0xffff};  // steps; 0: among the small ones
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              u16x2 up, at;
+              bins.places(w[i], up, at);
+              least = __builtin_elementwise_min(least, up);
+              const uint32_t both = __builtin_bit_cast(uint32_t, at);
+              char* const count = reinterpret_cast<char*>(s.count);
+              if (decltype(inside)::value || in_row(e0 + 2 * i, a.vocab)) atomicAdd(reinterpret_cast<uint32_t*>(count + (both & 0xffffu)), 1u);
+              if (decltype(inside)::value || in_row(e0 + 2 * i + 1, a.vocab)) atomicAdd(reinterpret_cast<uint32_t*>(count + (both >> 16)), 1u);
+            }
+            const bool small = least[0] == 0 || least[1] == 0;
+            if (small)
+              r.elements(e0, w, inside, [&](int, float x) {
+                if (bins.of(x) == Bins::kSmall)
+                  atomicAdd(reinterpret_cast<unsigned long long*>(&s.mass[Bins::kSmall]), mass_of(x, r.top, r.c));
+              });
+          });
         __syncthreads();
         for (int i = tid; i < Bins::kRest; i += NT)
           if (i != Bins::kSmall && s.count[i] > 0) s.mass[i] = s.count[i] * mass_of(bins.value(i), r.top, r.c);
@@ -743,7 +875,7 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const eagle4_sample_row
         const int b = find_bin(s.mass, s.count, true, nucleus_of(p, z1), s, tid);
         bounded = s.count[b] <= kList;
         if (bounded)
-          bound = uniform(value_of(lowest_key(kLowestKey, key_of(r.top), [&](uint32_t key) { return bins.of(value_of(key)) <= b; })));
+          bound = uniform(value_of(lowest_of(bins, b, key_of(r.top))));
       }
     }
     if (listed <= kList) {  // everything is decided in the list
@@ -768,7 +900,7 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const eagle4_sample_row
       cut.x = value_of(entry_key(last));
       cut.index = static_cast<int>(static_cast<uint32_t>(last));
       if (tokens != nullptr && tid < a.draws) {
-        const int at = list_find(s, kept, target_of(coins[tid], z));
+        const int at = list_find(s, kept, target_of(coin, z));
         tokens[tid] = static_cast<int64_t>(static_cast<uint32_t>(s.list.entry[at]));
       }
     } else if (asked) {  // one place after another: top-k's cut, min-p's, top-p's, the draws'
