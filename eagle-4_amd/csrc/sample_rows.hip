@@ -684,23 +684,30 @@ struct Cut {
   bool single;  // the index alone
 };
 
-// Writes a vector's worth of outputs: 16-byte stores where all of them are inside and lie on 16 bytes.
+// Writes N outputs: 16-byte stores (8 bytes of four 16-bit outputs) where all of them are inside and lie on such a boundary.
+// Nontemporal where a wave's stores are whole lines.
 template <typename U, int N>
 E4_DEV void store_vector(U* out, int e0, int vocab, const U (&y)[N]) {
+  typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+  constexpr int kBytes = N * static_cast<int>(sizeof(U));
+  static_assert(kBytes == 8 || kBytes % 16 == 0, "sizes of a vector of rows");
   U* const p = out + e0;
-  if (e0 >= 0 && e0 + N <= vocab && reinterpret_cast<uintptr_t>(p) % 16 == 0 && N * sizeof(U) % 16 == 0) {
-    constexpr int W = N * sizeof(U) / 16 > 0 ? N * sizeof(U) / 16 : 1;
+  if (e0 >= 0 && e0 + N <= vocab && reinterpret_cast<uintptr_t>(p) % (kBytes < 16 ? 8 : 16) == 0) {
+    uint32_t w[kBytes / 4];
 #pragma unroll
-    for (int k = 0; k < W; ++k) {
-      u32x4 w;
+    for (int i = 0; i < kBytes / 4; ++i) {
+      if constexpr (sizeof(U) == 4)
+        w[i] = __builtin_bit_cast(uint32_t, y[i]);
+      else
+        w[i] = static_cast<uint32_t>(y[2 * i]) | static_cast<uint32_t>(y[2 * i + 1]) << 16;
+    }
+    if constexpr (kBytes == 8) {
+      __builtin_nontemporal_store(u32x2{w[0], w[1]}, reinterpret_cast<u32x2*>(p));
+    } else if constexpr (kBytes == 16) {
+      __builtin_nontemporal_store(u32x4{w[0], w[1], w[2], w[3]}, reinterpret_cast<u32x4*>(p));
+    } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if constexpr (sizeof(U) == 4)
-          w[i] = __builtin_bit_cast(uint32_t, y[(4 * k + i) % N]);
-        else
-          w[i] = static_cast<uint32_t>(y[(8 * k + 2 * i) % N]) | static_cast<uint32_t>(y[(8 * k + 2 * i + 1) % N]) << 16;
-      }
-      __builtin_nontemporal_store(w, reinterpret_cast<u32x4*>(p) + k);
+      for (int k = 0; k < kBytes / 16; ++k) reinterpret_cast<u32x4*>(p)[k] = u32x4{w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]};
     }
   } else {
 #pragma unroll
@@ -709,48 +716,82 @@ E4_DEV void store_vector(U* out, int e0, int vocab, const U (&y)[N]) {
   }
 }
 
-template <typename P, typename T>
-E4_DEV void write_probs(const Rows<T>& r, const Cut& cut, uint64_t z, typename P::storage* out, int share, int shares) {
+// What is written in a token's place: its share of the mass, or its logit.
+template <typename T, typename P>
+struct ProbOut {
+  using S = typename P::storage;
+  S* out;
+  float top;
+  double c, unit;
+  bool single;
+  static E4_DEV S none() { return P::from_f32(0.f); }
+  E4_DEV S operator()(float x) const {
+    return P::from_f32(single ? 1.f : static_cast<float>(weight_of(x, top, c) * unit));
+  }
+};
+template <typename T>
+struct LogitOut {
+  using S = typename T::storage;
+  S* out;
+  static E4_DEV S none() { return T::from_f32(-INFINITY); }
+  E4_DEV S operator()(float x) const { return T::from_f32(x); }
+};
+
+// Writes a row of which all that is kept is s.list.entry[0 .. kept) or, kept 0, the token at cut.index alone: nothing of it is read
+// again. The row is filled, then the kept tokens are put in.
+template <typename Out>
+E4_DEV void write_few(const Shared& s, int kept, const Cut& cut, int vocab, const Out& out, int share, int shares, int tid) {
+  using S = typename Out::S;
+  constexpr int N = 16 / sizeof(S);
+  const int past = static_cast<int>(reinterpret_cast<uintptr_t>(out.out) % 16 / sizeof(S)), vectors = (vocab + past + N - 1) / N;
+  S y[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) y[i] = Out::none();
+  for (int v = share * NT + tid; v < vectors; v += shares * NT) store_vector(out.out, v * N - past, vocab, y);
+  // Every wave waits for its own fill to arrive, then for the others', so that no token is overwritten. (A fence that other XCDs
+  // see would write the cache back: 70 us and more.)
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  const auto put = [&](int e, float x) {
+    if ((e + past) / N / NT % shares == share) out.out[e] = out(x);
+  };
+  if (kept == 0) {
+    if (tid == 0) put(cut.index, cut.x);
+  } else {
+    for (int i = tid; i < kept; i += NT)
+      put(static_cast<int>(static_cast<uint32_t>(s.list.entry[i])), value_of(entry_key(s.list.entry[i])));
+  }
+}
+
+// Writes a row of which much is kept.
+template <typename T, typename Out>
+E4_DEV void write_row(const Rows<T>& r, const Cut& cut, const Out& out, int share, int shares) {
   constexpr int VEC = Row<T>::VEC;
-  const double unit = kUnit / static_cast<double>(z);
+  using S = typename Out::S;
   r.template each<Rows<T>::kAheadWeighed>([&](int e0, const float(&x)[VEC]) {
-    typename P::storage y[VEC];
     float left[VEC];  // the kept logits, the others at -inf
+    S y[VEC];
     bool any = false;
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
-      const bool kept = cut.single ? e0 + i == cut.index : x[i] > cut.x || (x[i] == cut.x && e0 + i <= cut.index);
+      const bool kept = x[i] > cut.x || (x[i] == cut.x && e0 + i <= cut.index);
       any |= kept;
-      left[i] = !kept ? -INFINITY : cut.single ? 0.f : x[i];
-      y[i] = P::from_f32(0.f);
+      left[i] = kept ? x[i] : -INFINITY;
+      y[i] = Out::none();
     }
     if (any) {
 #pragma unroll 1
       for (int j = 0; j < VEC; ++j) {  // one weight at a time, for the registers
-        const float w = left[0] == -INFINITY ? 0.f : cut.single ? 1.f : static_cast<float>(weight_of(left[0], r.top, r.c) * unit);
+        const S one = left[0] == -INFINITY ? Out::none() : out(left[0]);
 #pragma unroll
         for (int i = 0; i + 1 < VEC; ++i) {
           left[i] = left[i + 1];
           y[i] = y[i + 1];
         }
-        y[VEC - 1] = P::from_f32(w);
+        y[VEC - 1] = one;
       }
     }
-    store_vector(out, e0, r.row.vocab, y);
-  }, share, shares);
-}
-
-template <typename T>
-E4_DEV void write_logits(const Rows<T>& r, const Cut& cut, typename T::storage* out, int share, int shares) {
-  constexpr int VEC = Row<T>::VEC;
-  r.template each<Rows<T>::kAheadWeighed>([&](int e0, const float(&x)[VEC]) {
-    typename T::storage y[VEC];
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      const bool kept = cut.single ? e0 + i == cut.index : x[i] > cut.x || (x[i] == cut.x && e0 + i <= cut.index);
-      y[i] = T::from_f32(kept ? x[i] : -INFINITY);
-    }
-    store_vector(out, e0, r.row.vocab, y);
+    store_vector(out.out, e0, r.row.vocab, y);
   }, share, shares);
 }
 
@@ -787,6 +828,7 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const eagle4_sample_row
     __syncthreads();
   }
   Cut cut{-INFINITY, INT32_MAX, false};
+  int kept_list = 0;  // kept tokens, where all of them are in the list
   uint64_t z = static_cast<uint64_t>(kUnit);
 
   if (!(temperature > 0.f) || !(r.top < INFINITY) || r.top == -INFINITY) {  // the argmax alone
@@ -810,6 +852,7 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const eagle4_sample_row
     __syncthreads();
     cut.single = true;
     cut.index = s.found;
+    cut.x = r.top;
     if (tokens != nullptr && tid < a.draws) tokens[tid] = cut.index;
   } else {
     const bool by_k = k > 0 && k < a.vocab, by_m = m > 0.f, by_p = p < 1.f;
@@ -896,6 +939,7 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const eagle4_sample_row
       if (by_k || by_m) z1 = s.list.run[kept - 1];
       if (by_p) kept = list_find(s, kept, nucleus_of(p, z1)) + 1;
       z = s.list.run[kept - 1];
+      kept_list = kept;
       const uint64_t last = s.list.entry[kept - 1];
       cut.x = value_of(entry_key(last));
       cut.index = static_cast<int>(static_cast<uint32_t>(last));
@@ -950,15 +994,23 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const eagle4_sample_row
     }
   }
   if (a.out == nullptr) return;
+  const auto write = [&](const auto& out) {
+    if (kept_list > 0 || cut.single)
+      write_few(s, kept_list, cut, a.vocab, out, share, shares, tid);
+    else
+      write_row(r, cut, out, share, shares);
+  };
   if (a.out_kind == EAGLE4_ROWS_LOGITS) {
-    write_logits(r, cut, static_cast<typename T::storage*>(a.out) + n * a.stride_out, share, shares);
-  } else if (a.out_dtype == EAGLE4_F32) {
-    write_probs<e4::F32>(r, cut, z, static_cast<float*>(a.out) + n * a.stride_out, share, shares);
-  } else if (a.out_dtype == EAGLE4_BF16) {
-    write_probs<e4::Bf16>(r, cut, z, static_cast<uint16_t*>(a.out) + n * a.stride_out, share, shares);
-  } else {
-    write_probs<e4::F16>(r, cut, z, static_cast<uint16_t*>(a.out) + n * a.stride_out, share, shares);
+    write(LogitOut<T>{static_cast<typename T::storage*>(a.out) + n * a.stride_out});
+    return;
   }
+  const double unit = kUnit / static_cast<double>(z);
+  if (a.out_dtype == EAGLE4_F32)
+    write(ProbOut<T, e4::F32>{static_cast<float*>(a.out) + n * a.stride_out, r.top, r.c, unit, cut.single});
+  else if (a.out_dtype == EAGLE4_BF16)
+    write(ProbOut<T, e4::Bf16>{static_cast<uint16_t*>(a.out) + n * a.stride_out, r.top, r.c, unit, cut.single});
+  else
+    write(ProbOut<T, e4::F16>{static_cast<uint16_t*>(a.out) + n * a.stride_out, r.top, r.c, unit, cut.single});
 }
 
 template <typename T>
