@@ -73,26 +73,36 @@ def step_splits(programs: int, device: torch.device) -> int:
 def _cache_strides(cache: torch.Tensor) -> tuple[int, int, int]:
     """Element strides (per page, per slot within its page, per KV head) of a cache view. A ``[pages, page, heads,
     D]`` view has all three; a ``[slots, heads, D]`` view is read as pages of one slot, so its slot stride is 0."""
-    if cache.dim() == 4:
-        per_page, per_slot, per_head = cache.stride(0), cache.stride(1), cache.stride(2)
-    else:
-        per_page, per_slot, per_head = cache.stride(0), 0, cache.stride(1)
-    return per_page, per_slot, per_head
+    stride = cache.stride()
+    if len(stride) == 4:
+        return stride[0], stride[1], stride[2]
+    return stride[0], 0, stride[1]
 
 
-def _check_fp8(q, keys, values, out, k_scale, v_scale) -> None:
+def _check_fp8(q, keys, values, out, k_scale, v_scale, part_out, part_lse, table, seq_lens, ancestors, table_rows, rows_per_request,
+               step) -> None:
     if keys.dtype != torch.float8_e4m3fn or values is None or values.dtype != torch.float8_e4m3fn:
         raise _native.NotCovered("caches with scales must be float8_e4m3fn keys and values")
     if q.dtype not in (torch.bfloat16, torch.float16) or out.dtype != q.dtype:
         raise _native.NotCovered("q and out over fp8 pages must share one 16-bit dtype")
-    if values.shape != keys.shape:
-        raise ValueError(f"values {tuple(values.shape)} are not shaped as keys {tuple(keys.shape)}")
-    pages, heads = keys.shape[0], keys.shape[-2]
+    (rows, _, dim), shape, device = q.shape, keys.shape, q.device
+    if values.shape != shape or len(shape) not in (3, 4) or shape[-1] != dim or shape[0] == 0:
+        raise ValueError(f"keys {tuple(shape)} and values {tuple(values.shape)} must be alike, [pages, page, kv_heads, {dim}]")
+    if out.shape != q.shape:
+        raise ValueError(f"out must be {tuple(q.shape)}, got {tuple(out.shape)}")
+    pages, heads = shape[0], shape[-2]
     for name, scale in (("k_scale", k_scale), ("v_scale", v_scale)):
-        if scale.dtype != torch.float32 or scale.dim() != 2 or scale.shape[0] < pages or scale.shape[1] < heads:
-            raise ValueError(f"{name} must be fp32 [pages >= {pages}, kv_heads >= {heads}], got {scale.dtype} {tuple(scale.shape)}")
-        if scale.device != q.device:
-            raise ValueError(f"{name} must be on {q.device}")
+        have = scale.shape
+        if scale.dtype != torch.float32 or len(have) != 2 or have[0] < pages or have[1] < heads:
+            raise ValueError(f"{name} must be fp32 [pages >= {pages}, kv_heads >= {heads}], got {scale.dtype} {tuple(have)}")
+    bs = rows // rows_per_request if rows_per_request > 0 else 0
+    if table.dim() != 2 or 0 in table.shape or seq_lens.shape[0] < bs or (table_rows is not None and table_rows.shape[0] < bs):
+        raise ValueError(f"the page table must be [requests, entries], seq_lens and table_rows [{bs}]")
+    if step > 0 and (ancestors.shape[-1] < step or ancestors.numel() < bs * rows_per_request * ancestors.shape[-1]):
+        raise ValueError(f"ancestors must be [{bs}, {rows_per_request}, >= {step}], got {tuple(ancestors.shape)}")
+    for t in (keys, values, out, k_scale, v_scale, part_out, part_lse, table, seq_lens, ancestors if step > 0 else None, table_rows):
+        if t is not None and t.device != device:
+            raise ValueError(f"every tensor must be on the rows' device, {device}, got {t.device}")
 
 
 def rows_attention(
@@ -140,7 +150,8 @@ def rows_attention(
     if (k_scale is None) != (v_scale is None):
         raise ValueError("k_scale and v_scale go together")
     if k_scale is not None:
-        _check_fp8(q, keys, values, out, k_scale, v_scale)
+        _check_fp8(q, keys, values, out, k_scale, v_scale, part_out, part_lse, table, seq_lens, ancestors, table_rows,
+                   rows_per_request, step)
     elif q.dtype != keys.dtype or out.dtype != q.dtype or (values is not None and values.dtype != q.dtype):
         raise _native.NotCovered("q, the caches and out must share one 16-bit dtype")
     for name, t in (("q", q), ("out", out), ("keys", keys)) + ((("values", values),) if values is not None else ()):
@@ -157,49 +168,17 @@ def rows_attention(
     if step > 0:
         anc = ancestors if ancestors.dtype == torch.int32 and ancestors.is_contiguous() else ancestors.to(
             torch.int32).contiguous()
-    args = _native.RowAttnArgs(
-        q=q.data_ptr(),
-        stride_q_row=q.stride(0),
-        stride_q_head=q.stride(1),
-        keys=keys.data_ptr(),
-        values=_native.ptr(values),
-        k_stride_page=kst[0],
-        k_stride_slot=kst[1],
-        k_stride_head=kst[2],
-        v_stride_page=vst[0],
-        v_stride_slot=vst[1],
-        v_stride_head=vst[2],
-        out=out.data_ptr(),
-        stride_o_row=out.stride(0),
-        stride_o_head=out.stride(1),
-        part_out=part_out.data_ptr(),
-        part_lse=part_lse.data_ptr(),
-        part_rows=min(part_out.shape[0], part_lse.numel()),
-        table=table.data_ptr(),
-        stride_table=table.stride(0),
-        table_rows=_native.itab(table_rows),
-        seq_lens=_native.itab(seq_lens),
-        ancestors=_native.ptr(anc),
-        max_depth=anc.shape[-1] if anc is not None else 1,
-        table_page=table_page,
-        cache_page=1 if keys.dim() == 3 else keys.shape[1],
-        bs=bs,
-        rows_per_request=rows_per_request,
-        rows_padded=rows_padded(rows_per_request),
-        heads=heads,
-        kv_heads=kv_heads,
-        head_dim=head_dim,
-        dtype=_native.dtype_code(q.dtype),
-        step=step,
-        window=window,
-        splits=launch.splits,
-        scale=scale,
-    )
+    q_stride, out_stride = q.stride(), out.stride()
+    args = _native.RowAttnArgs(  # by position, as the struct has them: by name it costs more than the rest of the call
+        q.data_ptr(), q_stride[0], q_stride[1], keys.data_ptr(), _native.ptr(values), kst[0], kst[1], kst[2], vst[0], vst[1], vst[2],
+        out.data_ptr(), out_stride[0], out_stride[1], part_out.data_ptr(), part_lse.data_ptr(),
+        min(part_out.shape[0], part_lse.numel()), table.data_ptr(), table.stride(0), _native.itab(table_rows),
+        _native.itab(seq_lens), _native.ptr(anc), anc.shape[-1] if anc is not None else 1, table_page,
+        1 if keys.dim() == 3 else keys.shape[1], bs, rows_per_request, rows_padded(rows_per_request), heads, kv_heads, head_dim,
+        _native.dtype_code(q.dtype), step, window, launch.splits, scale)
     if k_scale is None:
         _native.launch("eagle4_row_attention", args, q.device)
         return
-    if table.dim() != 2 or 0 in table.shape or keys.shape[0] == 0:
-        raise ValueError("the page table must be [requests, entries], and the caches hold pages")
-    fp8 = _native.RowAttnFp8Args(args, k_scale.data_ptr(), v_scale.data_ptr(), k_scale.stride(0), k_scale.stride(1), v_scale.stride(0),
-                                 v_scale.stride(1), table.shape[0], table.shape[1], keys.shape[0])
+    ks, vs, (height, width) = k_scale.stride(), v_scale.stride(), table.shape
+    fp8 = _native.RowAttnFp8Args(args, k_scale.data_ptr(), v_scale.data_ptr(), ks[0], ks[1], vs[0], vs[1], height, width, keys.shape[0])
     _native.launch("eagle4_row_attention_fp8", fp8, q.device)

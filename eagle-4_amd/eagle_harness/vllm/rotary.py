@@ -58,7 +58,7 @@ def rotary_frequencies(
         place = lambda turns: half * math.log(trained / (turns * 2 * math.pi)) / math.log(base)  # noqa: E731
         low, high = max(math.floor(place(fast)), 0), min(math.ceil(place(slow)), dim - 1)
         slowed = ((pair - low) / max(high - low, 1e-3)).clamp(0, 1)
-        frequencies = frequencies * (1 - slowed) + frequencies / stretch * slowed
+        frequencies = frequencies * (1 - slowed * (1 - 1 / stretch))
         factor = 0.1 * math.log(stretch) + 1.0
     elif scaling not in ("none", "ntk"):
         raise ValueError(f"rotary_frequencies: scaling {scaling!r} is none of 'none', 'linear', 'ntk', 'yarn'")
@@ -68,37 +68,33 @@ def rotary_frequencies(
 _NONE = (0, 0)
 
 
-def _bytes(t: torch.Tensor) -> tuple[int, int]:
-    """The addresses that a [tokens, heads, dim] tensor of non-negative strides spans."""
-    first = t.data_ptr()
-    return first, first + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
-
-
-def _half(name: str, x: torch.Tensor, out: Optional[torch.Tensor], dtype, tokens: int, dim: int, device) -> tuple:
-    """Checks queries or keys and their output: (output, strides of x, strides of the output)."""
-    if x.dim() != 3 or x.shape[0] != tokens or x.shape[2] != dim:
-        raise ValueError(f"rotate_rows: {name} must be [{tokens}, heads, {dim}], got {tuple(x.shape)}")
+def _half(name: str, x: torch.Tensor, out: Optional[torch.Tensor], like: tuple) -> tuple:
+    """Checks queries or keys and their output: (heads, output, strides of x, strides of the output, addresses of both)."""
+    dtype, tokens, dim, device, size = like
+    shape, stride = x.shape, x.stride()
+    if len(shape) != 3 or shape[0] != tokens or shape[2] != dim:
+        raise ValueError(f"rotate_rows: {name} must be [{tokens}, heads, {dim}], got {tuple(shape)}")
     if x.dtype != dtype or x.device != device:
         raise ValueError(f"rotate_rows: {name} must be {dtype} on {device}")
-    stride = x.stride()
     if stride[2] != 1 and dim > 1:
         raise _native.NotCovered(f"rotate_rows: {name} must have a unit stride over the head dim")
-    to = stride
+    heads, at, to = shape[1], x.data_ptr(), stride
+    out_at = at
     if out is None:
         out = x
     elif out is not x:
-        if out.shape != x.shape or out.dtype != dtype or out.device != device:
+        if out.shape != shape or out.dtype != dtype or out.device != device:
             raise ValueError(f"rotate_rows: {name}_out must have {name}'s shape, dtype and device")
-        to = out.stride()
+        to, out_at = out.stride(), out.data_ptr()
         if to[2] != 1 and dim > 1:
             raise _native.NotCovered(f"rotate_rows: {name}_out must have a unit stride over the head dim")
-        if x.numel():
-            (a, b), (c, d) = _bytes(x), _bytes(out)
-            if a < d and c < b and (a != c or to != stride):
+        if tokens and heads and (at != out_at or to != stride):
+            span = ((tokens - 1) * stride[0] + (heads - 1) * stride[1] + dim) * size
+            if at < out_at + ((tokens - 1) * to[0] + (heads - 1) * to[1] + dim) * size and out_at < at + span:
                 raise ValueError(f"rotate_rows: {name}_out may be {name} itself, but not overlap it otherwise")
-    if (to[0] == 0 and tokens > 1) or (to[1] == 0 and x.shape[1] > 1):
+    if (to[0] == 0 and tokens > 1) or (to[1] == 0 and heads > 1):
         raise ValueError(f"rotate_rows: the output of {name} is an expanded view: every head needs its own storage")
-    return out, stride, to
+    return heads, out, stride, to, at, out_at
 
 
 def rotate_rows(
@@ -118,7 +114,7 @@ def rotate_rows(
     over tokens and heads (so the parts of one packed projection); ``positions`` [tokens] int32 / int64; ``frequencies`` fp64
     radians a position, at most 512. Pair ``i`` is the elements ``(i, half + i)``, or ``(2 i, 2 i + 1)`` where ``interleaved``:
     ``(x, y) -> factor (x cos - y sin, y cos + x sin)`` of ``position * frequencies[i]``. The elements behind the turned ones
-    are copied. Outputs for both or for neither; angles are computed in 64 bits, products in 32, each rounded once to the
+    are copied. Outputs for both or for neither, in memory that no other argument has; angles are computed in 64 bits, products in 32, each rounded once to the
     rows' dtype. Returns ``(q_out, k_out)``.
     """
     code = _DTYPES.get(q.dtype)
@@ -126,7 +122,7 @@ def rotate_rows(
         raise _native.NotCovered(f"rotate_rows: rows must be bf16, fp16 or fp32, got {q.dtype}")
     if q.dim() != 3:
         raise ValueError(f"rotate_rows: q must be [tokens, heads, D], got {tuple(q.shape)}")
-    (tokens, heads, dim), device = q.shape, q.device
+    (tokens, _, dim), device = q.shape, q.device
     if frequencies.dtype != torch.float64 or frequencies.dim() != 1 or not frequencies.is_contiguous() or frequencies.device != device:
         raise ValueError(f"rotate_rows: frequencies must be a contiguous fp64 vector on {device}")
     half = frequencies.shape[0]
@@ -136,17 +132,17 @@ def rotate_rows(
         raise ValueError(f"rotate_rows: positions must be [{tokens}] on {device}")
     if k is None and k_out is not None:
         raise ValueError("rotate_rows: k_out without k")
-    q_out, qs, qo = _half("q", q, q_out, q.dtype, tokens, dim, device)
-    ks, ko, kv_heads = _NONE, _NONE, 0
+    like = (q.dtype, tokens, dim, device, 4 if code == _native.F32 else 2)
+    heads, q_out, qs, qo, q_at, qo_at = _half("q", q, q_out, like)
+    kv_heads, ks, ko, k_at, ko_at = 0, _NONE, _NONE, None, None
     if k is not None:
-        k_out, ks, ko = _half("k", k, k_out, q.dtype, tokens, dim, device)
-        kv_heads = k.shape[1]
-        if (q_out.data_ptr() == q.data_ptr()) != (k_out.data_ptr() == k.data_ptr()) and heads and kv_heads:
+        kv_heads, k_out, ks, ko, k_at, ko_at = _half("k", k, k_out, like)
+        if (q_at == qo_at) != (k_at == ko_at) and heads and kv_heads:
             raise ValueError("rotate_rows: q_out and k_out go together")
     if tokens == 0:
         return q_out, k_out
-    args = _native.RotaryArgs(q.data_ptr(), _native.ptr(k), q_out.data_ptr(), _native.ptr(k_out), qs[0], qs[1], ks[0], ks[1], qo[0],
-                              qo[1], ko[0], ko[1], _native.itab(positions), frequencies.data_ptr(), factor, tokens, heads, kv_heads,
-                              dim, half, interleaved, code)
+    args = _native.RotaryArgs(q_at, k_at, qo_at, ko_at, qs[0], qs[1], ks[0], ks[1], qo[0], qo[1], ko[0], ko[1],
+                              _native.itab(positions), frequencies.data_ptr(), factor, tokens, heads, kv_heads, dim, half, interleaved,
+                              code)
     _native.launch("eagle4_rotary", args, device)
     return q_out, k_out

@@ -65,6 +65,12 @@ def _out_stride(what: str, name: str, out: torch.Tensor, logits: torch.Tensor) -
     return stride
 
 
+def _overlap(logits: torch.Tensor, out: torch.Tensor, out_stride: int) -> bool:
+    (rows, vocab), a, b = logits.shape, logits.data_ptr(), out.data_ptr()
+    return rows > 0 and (a < b + out.element_size() * ((rows - 1) * out_stride + vocab)
+                         and b < a + logits.element_size() * ((rows - 1) * logits.stride(0) + vocab))
+
+
 def draw_tokens(
     logits: torch.Tensor,
     coins: torch.Tensor,
@@ -85,7 +91,7 @@ def draw_tokens(
     padded one) draws nothing: its tokens and ``probs`` are left as they were.
 
     With ``Z`` the mass kept, the token is the first of the order whose running mass exceeds ``coin * Z``. ``probs`` [rows,
-    vocab] (bf16 / fp16 / fp32) is filled with ``w / Z`` on the kept tokens, 0 elsewhere.
+    vocab] (bf16 / fp16 / fp32, memory of its own) is filled with ``w / Z`` on the kept tokens, 0 elsewhere.
     """
     code, fields = _rows_args("draw_tokens", logits, temperature, top_k, top_p, min_p, entries)
     rows, vocab = logits.shape
@@ -99,6 +105,8 @@ def draw_tokens(
         out, stride, kind, out_code = probs.data_ptr(), _out_stride("draw_tokens", "probs", probs, logits), PROBS, _DTYPES.get(probs.dtype)
         if out_code is None:
             raise _native.NotCovered(f"draw_tokens: probs must be bf16, fp16 or fp32, got {probs.dtype}")
+        if _overlap(logits, probs, stride):
+            raise ValueError("draw_tokens: probs must not overlap the logits")
     tokens = torch.empty(coins.shape, dtype=torch.int64, device=logits.device)
     if rows == 0:
         return tokens
@@ -132,11 +140,8 @@ def truncate_logits(
         stride = _out_stride("truncate_logits", "out", out, logits)
         if out.dtype != logits.dtype:
             raise ValueError(f"truncate_logits: out must be {logits.dtype}, got {out.dtype}")
-        if out.data_ptr() != logits.data_ptr() or (rows > 1 and stride != logits.stride(0)):
-            size = logits.element_size()
-            a, b = logits.data_ptr(), out.data_ptr()
-            if rows and a < b + size * ((rows - 1) * stride + vocab) and b < a + size * ((rows - 1) * logits.stride(0) + vocab):
-                raise ValueError("truncate_logits: out may be the logits themselves, but not overlap them otherwise")
+        if (out.data_ptr() != logits.data_ptr() or (rows > 1 and stride != logits.stride(0))) and _overlap(logits, out, stride):
+            raise ValueError("truncate_logits: out may be the logits themselves, but not overlap them otherwise")
     if rows == 0:
         return out
     args = _native.SampleRowsArgs(*fields, None, None, out.data_ptr(), stride, rows, temperature.shape[0], vocab, 0, code, LOGITS,
