@@ -366,9 +366,25 @@ E4_DEV uint32_t lowest_key(uint32_t lo, uint32_t hi, F&& ok) {
   return uniform(hi);
 }
 
+// The same, where `guess` is a logit near that key: one round of probes if it is within 32 keys.
+template <typename F>
+E4_DEV uint32_t lowest_key_near(float guess, uint32_t hi, F&& ok) {
+  const uint32_t at = guess > -INFINITY ? key_of(guess) : 0u;  // (NaN: no guess)
+  if (at > kLowestKey + 32 && at < hi - 32) {
+    const int lane = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
+    const uint64_t good = __ballot(ok(at - 32 + lane));
+    if (good != 0 && !(good & 1)) return uniform(at - 32 + __builtin_ctzll(good));
+  }
+  return lowest_key(kLowestKey, hi, ok);
+}
+
 // The lowest key of the bins up to b, given the row's largest.
 E4_DEV uint32_t lowest_of(const Bins& bins, int b, uint32_t top) {
-  if (!bins.by_value) return b == kBins - 1 ? kLowestKey : lowest_key(kLowestKey, top, [&](uint32_t k) { return bins.of(value_of(k)) <= b; });
+  if (!bins.by_value) {
+    if (b == kBins - 1) return kLowestKey;
+    const float guess = static_cast<float>(static_cast<double>(bins.top) - (b + 1) / (bins.c * static_cast<double>(kBinsPerOctave)));
+    return lowest_key_near(guess, top, [&](uint32_t k) { return bins.of(value_of(k)) <= b; });
+  }
   if (b >= Bins::kRest) return kLowestKey;
   return b == Bins::kSmall ? key_of(bins.value(b + 1)) + 1 : key_of(bins.value(b));
 }
@@ -860,8 +876,8 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const eagle4_sample_row
     float lowest = -INFINITY;
     if (by_m) {
       const double want = m < 1.f ? static_cast<double>(m) : 1.0;
-      lowest = uniform(value_of(lowest_key(kLowestKey, key_of(r.top),
-                                   [&](uint32_t key) { return weight_of(value_of(key), r.top, r.c) >= want; })));
+      lowest = uniform(value_of(lowest_key_near(r.top + logf(static_cast<float>(want)) * temperature, key_of(r.top),
+                                                [&](uint32_t key) { return weight_of(value_of(key), r.top, r.c) >= want; })));
     }
     int listed = kList + 1;  // the list holds the order's beginning
     uint64_t z1 = 0;         // the mass that top-p is taken of, where it is known
