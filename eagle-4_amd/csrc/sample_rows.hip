@@ -138,7 +138,8 @@ E4_DEV bool in_row(int e, int vocab) { return static_cast<uint32_t>(e) < static_
 // behind the last of those (at most one vector at each end) out of LDS, where they are put once.
 template <typename T>
 struct Rows {
-  static constexpr int VEC = Row<T>::VEC, kAhead = 3, kAheadWeighed = 2;  // a thread's vectors on their way
+  // A thread's vectors on their way: what the registers hold (fp16's conversions take a vector's more).
+  static constexpr int VEC = Row<T>::VEC, kAhead = T::code == EAGLE4_F16 ? 2 : 3, kAheadWeighed = 2;
   using S = typename T::storage;
   Row<T> row;
   int begin, end;  // whole vectors
@@ -389,43 +390,82 @@ E4_DEV uint32_t lowest_of(const Bins& bins, int b, uint32_t top) {
   return b == Bins::kSmall ? key_of(bins.value(b + 1)) + 1 : key_of(bins.value(b));
 }
 
+// The value of lane ^ J, by lane patterns: within a quad, a mirrored half row and quad, a row turned by 8, swaps of rows.
+template <int J>
+E4_DEV uint32_t partner32(uint32_t x, int lane) {
+  const int v = static_cast<int>(x);
+  if constexpr (J == 1) return __builtin_amdgcn_mov_dpp(v, 0xB1, 0xF, 0xF, true);
+  if constexpr (J == 2) return __builtin_amdgcn_mov_dpp(v, 0x4E, 0xF, 0xF, true);
+  if constexpr (J == 4) return __builtin_amdgcn_mov_dpp(__builtin_amdgcn_mov_dpp(v, 0x141, 0xF, 0xF, true), 0x1B, 0xF, 0xF, true);
+  if constexpr (J == 8) return __builtin_amdgcn_mov_dpp(v, 0x128, 0xF, 0xF, true);
+  if constexpr (J == 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    return lane & 16 ? r[0] : r[1];
+  }
+  if constexpr (J == 32) {
+    const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return lane & 32 ? r[0] : r[1];
+  }
+}
+template <int J>
+E4_DEV uint64_t ordered(uint64_t x, bool up, int lane) {  // the lower of x and lane ^ J's where `up` and bit J agree
+  const uint64_t o = static_cast<uint64_t>(partner32<J>(static_cast<uint32_t>(x >> 32), lane)) << 32 | partner32<J>(static_cast<uint32_t>(x), lane);
+  const bool low = ((lane & J) == 0) == up;
+  return low == (o < x) ? o : x;
+}
+// The steps of a merge within a wave, from lane distance J down.
+template <int J>
+E4_DEV uint64_t merge_wave(uint64_t x, bool up, int lane) {
+  x = ordered<J>(x, up, lane);
+  if constexpr (J > 1) x = merge_wave<J / 2>(x, up, lane);
+  return x;
+}
+E4_DEV uint64_t sort_wave(uint64_t x, bool up, int lane) {
+  x = merge_wave<1>(x, (lane & 2) == 0, lane);
+  x = merge_wave<2>(x, (lane & 4) == 0, lane);
+  x = merge_wave<4>(x, (lane & 8) == 0, lane);
+  x = merge_wave<8>(x, (lane & 16) == 0, lane);
+  x = merge_wave<16>(x, (lane & 32) == 0, lane);
+  return merge_wave<32>(x, up, lane);
+}
+
 // Sorts s.list.entry[0 .. n) ascending; n at most kList. Every thread calls it. A bitonic network over the next power of two: an entry
-// a thread (two beyond NT), partners in the same wave by lane exchanges, those of other waves through LDS. (Every step through LDS
-// behind a barrier: 256 entries 16 us instead of 5.)
+// a thread (two beyond NT), steps within a wave by lane patterns, those between waves through LDS. (Every step through LDS behind a
+// barrier: 256 entries 16 us.)
 template <int E>
 E4_DEV void sort_entries(Shared& s, int n, int size, int tid) {
+  const int lane = tid & 63;
   uint64_t x[E];
 #pragma unroll
-  for (int e = 0; e < E; ++e) x[e] = tid + NT * e < n ? s.list.entry[tid + NT * e] : ~0ull;
-  for (int k = 2; k <= size; k <<= 1)
-    for (int j = k >> 1; j > 0; j >>= 1) {
+  for (int e = 0; e < E; ++e) {
+    const int at = tid + NT * e;
+    x[e] = at < n ? s.list.entry[at] : ~0ull;
+    if (at < size) x[e] = sort_wave(x[e], (at & 64) == 0, lane);
+  }
+  for (int k = 128; k <= size; k <<= 1) {
+    for (int j = k >> 1; j >= 64; j >>= 1) {
       if (E == 2 && j == NT) {  // the thread's own two (the last merge: ascending)
         const uint64_t lo = x[0] < x[E - 1] ? x[0] : x[E - 1];
         x[E - 1] = x[0] < x[E - 1] ? x[E - 1] : x[0];
         x[0] = lo;
         continue;
       }
-      uint64_t o[E];
-      if (j < 64) {
+      __syncthreads();
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const uint32_t lo = __shfl_xor(static_cast<uint32_t>(x[e]), j, 64), hi = __shfl_xor(static_cast<uint32_t>(x[e] >> 32), j, 64);
-          o[e] = (static_cast<uint64_t>(hi) << 32) | lo;
-        }
-      } else {
-        __syncthreads();
-#pragma unroll
-        for (int e = 0; e < E; ++e) s.list.entry[tid + NT * e] = x[e];
-        __syncthreads();
-#pragma unroll
-        for (int e = 0; e < E; ++e) o[e] = s.list.entry[(tid ^ j) + NT * e];
-      }
+      for (int e = 0; e < E; ++e) s.list.entry[tid + NT * e] = x[e];
+      __syncthreads();
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        const bool keep_low = ((tid & j) == 0) == (((tid + NT * e) & k) == 0);
-        x[e] = keep_low == (o[e] < x[e]) ? o[e] : x[e];
+        const int at = tid + NT * e;
+        const uint64_t o = s.list.entry[at ^ j];
+        const bool low = ((at & j) == 0) == ((at & k) == 0);
+        x[e] = low == (o < x[e]) ? o : x[e];
       }
     }
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (tid + NT * e < size) x[e] = merge_wave<32>(x[e], ((tid + NT * e) & k) == 0, lane);
+  }
   __syncthreads();
 #pragma unroll
   for (int e = 0; e < E; ++e) s.list.entry[tid + NT * e] = x[e];
@@ -434,23 +474,6 @@ E4_DEV void sort_entries(Shared& s, int n, int size, int tid) {
 E4_DEV void sort_list(Shared& s, int n, int tid) {
   int size = 64;
   while (size < n) size <<= 1;
-  if (size == 64) {  // by one wave alone
-    if (tid < 64) {
-      uint64_t x = tid < n ? s.list.entry[tid] : ~0ull;
-#pragma unroll 1
-      for (int k = 2; k <= 64; k <<= 1)
-#pragma unroll 1
-        for (int j = k >> 1; j > 0; j >>= 1) {
-          const uint32_t lo = __shfl_xor(static_cast<uint32_t>(x), j, 64), hi = __shfl_xor(static_cast<uint32_t>(x >> 32), j, 64);
-          const uint64_t o = (static_cast<uint64_t>(hi) << 32) | lo;
-          const bool keep_low = ((tid & j) == 0) == ((tid & k) == 0);
-          x = keep_low == (o < x) ? o : x;
-        }
-      s.list.entry[tid] = x;
-    }
-    __syncthreads();
-    return;
-  }
   if (size <= NT)
     sort_entries<1>(s, n, size, tid);
   else
