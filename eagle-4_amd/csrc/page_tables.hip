@@ -53,18 +53,44 @@ E4_DEV Request request_of(const eagle4_resize_tables_args& a, int r) {
   return q;
 }
 
-// The chunk's request that page f of the running sums belongs to.
-E4_DEV int owner_of(const uint32_t* ends, uint32_t f) {
-  int lo = 0, hi = NT - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (ends[mid] > f)
-      hi = mid;
-    else
-      lo = mid + 1;
+// f(i, request, page of the request's that moves) for this thread's pages of the chunk's `all`, i their number in it. Four of them are
+// looked for, loaded and stored together (one after another: 96 prompts of up to 171 pages 32 us a cycle of taking, mapping and
+// giving back, 21 so).
+template <typename Load, typename Store>
+E4_DEV void each_page(const Chunk& c, uint32_t all, int tid, Load&& load, Store&& store) {
+  constexpr int U = 4;
+  for (uint32_t f0 = tid; f0 < all; f0 += U * NT) {
+    int lo[U], hi[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      lo[u] = 0;
+      hi[u] = NT - 1;
+    }
+#pragma unroll 1
+    for (int step = 0; step < 10; ++step)  // the first request whose running sum passes the page
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int mid = (lo[u] + hi[u]) >> 1;
+        if (c.ends[mid] > f0 + u * NT)
+          hi[u] = mid;
+        else
+          lo[u] = mid < hi[u] ? mid + 1 : hi[u];
+      }
+    int32_t page[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint32_t f = f0 + u * NT < all ? f0 + u * NT : f0;  // (past the last: the first again, not stored)
+      const int r = f == f0 ? lo[0] : lo[u];
+      lo[u] = r;
+      hi[u] = static_cast<int>(f - (r > 0 ? c.ends[r - 1] : 0));
+      page[u] = load(f, r, hi[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (f0 + u * NT < all) store(f0 + u * NT, lo[u], hi[u], page[u]);
   }
-  return lo;
 }
+static_assert(NT == 1 << 10, "ten steps of the search");
 
 __global__ __launch_bounds__(NT) void resize_tables_kernel(const eagle4_resize_tables_args a) {
   __shared__ Chunk c;
@@ -95,11 +121,9 @@ __global__ __launch_bounds__(NT) void resize_tables_kernel(const eagle4_resize_t
     c.ends[tid] = ends;
     __syncthreads();
     const uint32_t all = c.ends[NT - 1];
-    for (uint32_t f = tid; f < all; f += NT) {
-      const int r = owner_of(c.ends, f);
-      const uint32_t first = r > 0 ? c.ends[r - 1] : 0;
-      a.free_pages[top - 1 - (done + f)] = a.block_table[c.slot[r] * a.stride_table + c.from[r] + (f - first)];
-    }
+    each_page(
+        c, all, tid, [&](uint32_t, int r, int i) { return a.block_table[c.slot[r] * a.stride_table + c.from[r] + i]; },
+        [&](uint32_t f, int, int, int32_t page) { a.free_pages[top - 1 - (done + f)] = page; });
     if (n > 0) a.num_pages[q.slot] = q.need;
     done += all;
     __syncthreads();
@@ -117,12 +141,11 @@ __global__ __launch_bounds__(NT) void resize_tables_kernel(const eagle4_resize_t
     c.ends[tid] = ends;
     __syncthreads();
     const uint32_t all = c.ends[NT - 1];
-    for (uint32_t f = tid; f < all; f += NT) {
-      const int r = owner_of(c.ends, f);
-      if (c.slot[r] < 0) continue;
-      const uint32_t first = r > 0 ? c.ends[r - 1] : 0;
-      a.block_table[c.slot[r] * a.stride_table + c.from[r] + (f - first)] = a.free_pages[top - 1 - (wanted + f)];
-    }
+    each_page(
+        c, all, tid, [&](uint32_t f, int r, int) { return c.slot[r] < 0 ? 0 : a.free_pages[top - 1 - (wanted + f)]; },
+        [&](uint32_t, int r, int i, int32_t page) {
+          if (c.slot[r] >= 0) a.block_table[c.slot[r] * a.stride_table + c.from[r] + i] = page;
+        });
     if (served) a.num_pages[q.slot] = q.need;
     if (tid == 0) s_served = 0;
     __syncthreads();

@@ -30,7 +30,6 @@ typedef int16_t i16x2 __attribute__((ext_vector_type(2)));
 
 constexpr int NT = 1024, kWaves = NT / 64;
 constexpr int kBins = 4096, kList = 2048;
-constexpr float kBinsPerOctave = 64.f;
 constexpr double kUnit = 0x1p45;
 constexpr uint32_t kLowestKey = 0x007fffffu;  // of -inf
 
@@ -55,11 +54,28 @@ E4_DEV uint32_t key_of(float x) {
 }
 E4_DEV float value_of(uint32_t key) { return __uint_as_float(key ^ (key >> 31 ? 0x80000000u : 0xffffffffu)); }
 
-// A token's mass in units of 2^-45.
-E4_DEV uint64_t mass_of(float x, float top, double c) {
-  const double y = __builtin_fma(weight_of(x, top, c), kUnit, 0x1p52);  // rounds to a whole number in the low 52 bits
-  return __builtin_bit_cast(uint64_t, y) & 0xfffffffffffffull;
+// A token's mass in units of 2^-45, and -64 log2 w as a whole number. With 64 log2 w = r - (64 q + j), |r| <= 1/2, the mass is roots[j] =
+// 2^(-j/64), times 2^(r/64) by its series (the next term is below 10^-16), times 2^-q.
+struct Weighed {
+  int steps;  // -64 log2 w, rounded
+  uint64_t mass;
+};
+E4_DEV Weighed weigh(float x, float top, double c, const double* roots) {
+  double y = (static_cast<double>(x) - static_cast<double>(top)) * (c * 64.0);
+  y = __builtin_fmax(y, -70400.0);  // (and for the NaN of -inf times a scale of 0)
+  const double n = __builtin_rint(y), r = y - n;
+  constexpr double k = 0.6931471805599453 / 64;
+  double p = k * k * k * k * k / 120;
+  p = __builtin_fma(p, r, k * k * k * k / 24);
+  p = __builtin_fma(p, r, k * k * k / 6);
+  p = __builtin_fma(p, r, k * k / 2);
+  p = __builtin_fma(p, r, k);
+  p = __builtin_fma(p, r, 1.0);
+  const int steps = -static_cast<int>(n);
+  p = __builtin_ldexp(p * roots[steps & 63], 45 - (steps >> 6)) + 0x1p52;  // rounds to a whole number in the low 52 bits
+  return Weighed{steps, __builtin_bit_cast(uint64_t, p) & 0xfffffffffffffull};
 }
+
 // Bins of a row's logits, their numbers rising as the logits fall. By weight: 64 a factor of two. By value (bf16): a bin for every
 // value of magnitude from 2^(high - 15) to below 2^high, one for the smaller ones and one for what lies below -2^high, which
 // weighs nothing. There a row is counted, and every value weighed once.
@@ -91,8 +107,9 @@ struct Bins {
       const int up = steps(__float_as_uint(x) >> 16);
       return kSmall + (x < 0.f ? up : -up);
     }
-    const double t = (static_cast<double>(x) - static_cast<double>(top)) * (c * -static_cast<double>(kBinsPerOctave));
-    return static_cast<int>(__builtin_fmin(t == t ? t : 1e9, kBins - 1));  // (NaN: -inf times a scale of 0)
+    const double y = (static_cast<double>(x) - static_cast<double>(top)) * (c * 64.0);
+    const int steps = -static_cast<int>(__builtin_rint(__builtin_fmax(y, -70400.0)));
+    return steps < kBins - 1 ? steps : kBins - 1;
   }
   // Two patterns at once: their steps, and their bins' places in an array of words, in bytes.
   E4_DEV void places(uint32_t w, u16x2& up, u16x2& at) const {
@@ -123,6 +140,7 @@ struct Shared {
     } sub;
     uint32_t maxima[NT];
   };
+  double roots[64];
   u32x4 ends[2];
   uint64_t wave64[kWaves];
   uint32_t wave32[kWaves];
@@ -390,7 +408,7 @@ E4_DEV uint32_t lowest_key_near(float guess, uint32_t hi, F&& ok) {
 E4_DEV uint32_t lowest_of(const Bins& bins, int b, uint32_t top) {
   if (!bins.by_value) {
     if (b == kBins - 1) return kLowestKey;
-    const float guess = static_cast<float>(static_cast<double>(bins.top) - (b + 1) / (bins.c * static_cast<double>(kBinsPerOctave)));
+    const float guess = static_cast<float>(static_cast<double>(bins.top) - (b + 0.5) / (bins.c * 64.0));
     return lowest_key_near(guess, top, [&](uint32_t k) { return bins.of(value_of(k)) <= b; });
   }
   if (b >= Bins::kRest) return kLowestKey;
@@ -532,7 +550,7 @@ E4_DEV int list_range(const Rows<T>& r, Shared& s, float lo, float hi, uint64_t 
 #pragma unroll
   for (int i = 0; i < P; ++i) {
     const int at = P * tid + i;
-    sum += at < n ? mass_of(value_of(entry_key(s.list.entry[at])), r.top, r.c) : 0;
+    sum += at < n ? weigh(value_of(entry_key(s.list.entry[at])), r.top, r.c, s.roots).mass : 0;
     m[i] = sum;
   }
   const uint64_t before = block_scan(sum, s.wave64, tid) - sum + base;
@@ -622,7 +640,7 @@ E4_DEV Place locate(const Rows<T>& r, const Bins& bins, Shared& s, bool by_mass,
       const uint32_t k = key_of(x);
       if (k >= lo && k <= hi) {
         const uint32_t at = (hi - k) >> shift;
-        atomicAdd(reinterpret_cast<unsigned long long*>(&s.sub.mass[at]), mass_of(x, r.top, r.c));
+        atomicAdd(reinterpret_cast<unsigned long long*>(&s.sub.mass[at]), weigh(x, r.top, r.c, s.roots).mass);
         atomicAdd(&s.sub.count[at], 1u);
       }
     });
@@ -643,7 +661,7 @@ E4_DEV Place locate(const Rows<T>& r, const Bins& bins, Shared& s, bool by_mass,
   Place p;
   if (inside > kList) {  // one logit, many times
     p.x = value_of(lo);
-    const uint64_t each = mass_of(p.x, r.top, r.c);
+    const uint64_t each = weigh(p.x, r.top, r.c, s.roots).mass;
     uint64_t rank = by_mass ? (each > 0 ? (target - mass) / each : 0) : target - count;
     if (rank >= inside) rank = inside - 1;
     p.run = mass + (rank + 1) * each;
@@ -902,6 +920,7 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const eagle4_sample_row
 
   int64_t* const tokens = a.tokens != nullptr && share == 0 ? a.tokens + n * a.draws : nullptr;
   const float* const coins = a.coins != nullptr ? a.coins + n * a.draws : nullptr;
+  if (tid < 64) s.roots[tid] = exp2(tid * -1.0 / 64);
   const float coin = tokens != nullptr && tid < a.draws ? coins[tid] : 0.f;  // (here, beside the row's first loads)
   Rows<T> r(a.logits, n, a.stride_row, a.vocab, s.ends, tid);
   float mine = -INFINITY;
@@ -988,16 +1007,17 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const eagle4_sample_row
             if (small)
               r.elements(e0, w, inside, [&](int, float x) {
                 if (bins.of(x) == Bins::kSmall)
-                  atomicAdd(reinterpret_cast<unsigned long long*>(&s.mass[Bins::kSmall]), mass_of(x, r.top, r.c));
+                  atomicAdd(reinterpret_cast<unsigned long long*>(&s.mass[Bins::kSmall]), weigh(x, r.top, r.c, s.roots).mass);
               });
           });
         __syncthreads();
         for (int i = tid; i < Bins::kRest; i += NT)
-          if (i != Bins::kSmall && s.count[i] > 0) s.mass[i] = s.count[i] * mass_of(bins.value(i), r.top, r.c);
+          if (i != Bins::kSmall && s.count[i] > 0) s.mass[i] = s.count[i] * weigh(bins.value(i), r.top, r.c, s.roots).mass;
       } else {
         r.each_element([&](int, float x) {
-          const int b = bins.of(x);
-          atomicAdd(reinterpret_cast<unsigned long long*>(&s.mass[b]), mass_of(x, r.top, r.c));
+          const Weighed w = weigh(x, r.top, r.c, s.roots);
+          const int b = w.steps < kBins - 1 ? w.steps : kBins - 1;
+          atomicAdd(reinterpret_cast<unsigned long long*>(&s.mass[b]), w.mass);
           atomicAdd(&s.count[b], 1u);
         });
       }
@@ -1056,7 +1076,7 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const eagle4_sample_row
           } else {
             uint64_t sum = 0;
             r.each_element([&](int, float x) {
-              if (x >= lowest) sum += mass_of(x, r.top, r.c);
+              if (x >= lowest) sum += weigh(x, r.top, r.c, s.roots).mass;
             });
             sum = block_scan(sum, s.wave64, tid);
             if (tid == NT - 1) s.sum = sum;
