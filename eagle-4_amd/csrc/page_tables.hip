@@ -53,12 +53,10 @@ E4_DEV Request request_of(const eagle4_resize_tables_args& a, int r) {
   return q;
 }
 
-// f(i, request, page of the request's that moves) for this thread's pages of the chunk's `all`, i their number in it. Four of them are
-// looked for, loaded and stored together (one after another: 96 prompts of up to 171 pages 32 us a cycle of taking, mapping and
-// giving back, 21 so).
-template <typename Load, typename Store>
-E4_DEV void each_page(const Chunk& c, uint32_t all, int tid, Load&& load, Store&& store) {
-  constexpr int U = 4;
+// Moves this thread's pages of the chunk's `all`: load and store get a page's number in the chunk, its request, and its number among
+// the request's that move. U of them are looked for, loaded and stored together.
+template <int U, typename Load, typename Store>
+E4_DEV void move_pages(const Chunk& c, uint32_t all, int tid, Load&& load, Store&& store) {
   for (uint32_t f0 = tid; f0 < all; f0 += U * NT) {
     int lo[U], hi[U];
 #pragma unroll
@@ -91,6 +89,13 @@ E4_DEV void each_page(const Chunk& c, uint32_t all, int tid, Load&& load, Store&
   }
 }
 static_assert(NT == 1 << 10, "ten steps of the search");
+template <typename Load, typename Store>
+E4_DEV void each_page(const Chunk& c, uint32_t all, int tid, Load&& load, Store&& store) {
+  if (all <= NT)
+    move_pages<1>(c, all, tid, load, store);
+  else
+    move_pages<8>(c, all, tid, load, store);
+}
 
 __global__ __launch_bounds__(NT) void resize_tables_kernel(const eagle4_resize_tables_args a) {
   __shared__ Chunk c;
@@ -99,10 +104,11 @@ __global__ __launch_bounds__(NT) void resize_tables_kernel(const eagle4_resize_t
   const int tid = threadIdx.x;
   const int chunks = (a.num_reqs + NT - 1) / NT;
   const int64_t before = *a.num_free;
-  // what comes back in all
+  // what comes back in all (the requests of a batch of one chunk are looked up once)
+  const Request first = request_of(a, tid);
   int64_t back = 0;
   for (int i = 0; i < chunks; ++i) {
-    const Request q = request_of(a, i * NT + tid);
+    const Request q = i == 0 ? first : request_of(a, i * NT + tid);
     const uint32_t ends = block_scan(q.have > q.need ? q.have - q.need : 0, c.part, tid);
     if (tid == NT - 1) s_total = ends;
     __syncthreads();
@@ -113,7 +119,7 @@ __global__ __launch_bounds__(NT) void resize_tables_kernel(const eagle4_resize_t
   // page f that comes back, counted over the batch, lies f below the top
   int64_t done = 0;
   for (int i = 0; back > 0 && i < chunks; ++i) {
-    const Request q = request_of(a, i * NT + tid);
+    const Request q = i == 0 ? first : request_of(a, i * NT + tid);
     const uint32_t n = q.have > q.need ? q.have - q.need : 0;
     const uint32_t ends = block_scan(n, c.part, tid);
     c.slot[tid] = static_cast<int32_t>(q.slot);
@@ -131,8 +137,8 @@ __global__ __launch_bounds__(NT) void resize_tables_kernel(const eagle4_resize_t
   // the stack is whole (the barrier above orders its stores for this workgroup); now it is taken from
   __syncthreads();
   int64_t taken = 0, wanted = 0;
-  for (int i = 0; i < chunks; ++i) {
-    const Request q = request_of(a, i * NT + tid);
+  for (int i = 0; i < chunks; ++i) {  // (a request that gave pages back needs none)
+    const Request q = i == 0 ? first : request_of(a, i * NT + tid);
     const uint32_t n = q.need > q.have ? q.need - q.have : 0;
     const uint32_t ends = block_scan(n, c.part, tid);
     const bool served = n > 0 && wanted + ends <= top;

@@ -81,28 +81,29 @@ def _cache_strides(cache: torch.Tensor) -> tuple[int, int, int]:
 
 def _check_fp8(q, keys, values, out, k_scale, v_scale, part_out, part_lse, table, seq_lens, ancestors, table_rows, rows_per_request,
                step) -> None:
-    if keys.dtype != torch.float8_e4m3fn or values is None or values.dtype != torch.float8_e4m3fn:
+    fp8, dtype, rows_shape, shape = torch.float8_e4m3fn, q.dtype, q.shape, keys.shape
+    if values is None or keys.dtype != fp8 or values.dtype != fp8:
         raise _native.NotCovered("caches with scales must be float8_e4m3fn keys and values")
-    if q.dtype not in (torch.bfloat16, torch.float16) or out.dtype != q.dtype:
+    if (dtype != torch.bfloat16 and dtype != torch.float16) or out.dtype != dtype:
         raise _native.NotCovered("q and out over fp8 pages must share one 16-bit dtype")
-    (rows, _, dim), shape, device = q.shape, keys.shape, q.device
-    if values.shape != shape or len(shape) not in (3, 4) or shape[-1] != dim or shape[0] == 0:
-        raise ValueError(f"keys {tuple(shape)} and values {tuple(values.shape)} must be alike, [pages, page, kv_heads, {dim}]")
-    if out.shape != q.shape:
-        raise ValueError(f"out must be {tuple(q.shape)}, got {tuple(out.shape)}")
+    if values.shape != shape or not 3 <= len(shape) <= 4 or shape[-1] != rows_shape[2] or shape[0] == 0:
+        raise ValueError(f"keys {tuple(shape)} and values {tuple(values.shape)} must be alike, [pages, page, kv_heads, {rows_shape[2]}]")
+    if out.shape != rows_shape:
+        raise ValueError(f"out must be {tuple(rows_shape)}, got {tuple(out.shape)}")
     pages, heads = shape[0], shape[-2]
     for name, scale in (("k_scale", k_scale), ("v_scale", v_scale)):
         have = scale.shape
         if scale.dtype != torch.float32 or len(have) != 2 or have[0] < pages or have[1] < heads:
             raise ValueError(f"{name} must be fp32 [pages >= {pages}, kv_heads >= {heads}], got {scale.dtype} {tuple(have)}")
-    bs = rows // rows_per_request if rows_per_request > 0 else 0
-    if table.dim() != 2 or 0 in table.shape or seq_lens.shape[0] < bs or (table_rows is not None and table_rows.shape[0] < bs):
+    bs = rows_shape[0] // rows_per_request if rows_per_request > 0 else 0
+    if table.dim() != 2 or table.numel() == 0 or seq_lens.shape[0] < bs or (table_rows is not None and table_rows.shape[0] < bs):
         raise ValueError(f"the page table must be [requests, entries], seq_lens and table_rows [{bs}]")
     if step > 0 and (ancestors.shape[-1] < step or ancestors.numel() < bs * rows_per_request * ancestors.shape[-1]):
         raise ValueError(f"ancestors must be [{bs}, {rows_per_request}, >= {step}], got {tuple(ancestors.shape)}")
+    where = q.get_device()
     for t in (keys, values, out, k_scale, v_scale, part_out, part_lse, table, seq_lens, ancestors if step > 0 else None, table_rows):
-        if t is not None and t.device != device:
-            raise ValueError(f"every tensor must be on the rows' device, {device}, got {t.device}")
+        if t is not None and t.get_device() != where:
+            raise ValueError(f"every tensor must be on the rows' device, {q.device}, got {t.device}")
 
 
 def rows_attention(
@@ -154,8 +155,8 @@ def rows_attention(
                    rows_per_request, step)
     elif q.dtype != keys.dtype or out.dtype != q.dtype or (values is not None and values.dtype != q.dtype):
         raise _native.NotCovered("q, the caches and out must share one 16-bit dtype")
-    for name, t in (("q", q), ("out", out), ("keys", keys)) + ((("values", values),) if values is not None else ()):
-        if t.stride(-1) != 1:
+    for name, t in (("q", q), ("out", out), ("keys", keys), ("values", values)):
+        if t is not None and t.stride(-1) != 1:
             raise _native.NotCovered(f"{name} must have a unit stride over the head dim")
     if part_out.dtype != torch.float32 or part_lse.dtype != torch.float32 or not part_out.is_contiguous():
         raise _native.NotCovered("the partials are contiguous fp32 scratch")

@@ -16,10 +16,10 @@ from eagle_harness.kernels import _native
 
 
 def _tables(what: str, block_table: torch.Tensor, num_pages: torch.Tensor, idx_mapping: torch.Tensor, page: int) -> tuple:
-    """Checks what both operators share: (slots, max_pages, row stride, requests, device)."""
+    """Checks what both operators share: (slots, max_pages, row stride, requests, the device's number)."""
     if block_table.dim() != 2 or block_table.dtype != torch.int32 or num_pages.dtype != torch.int32:
         raise ValueError(f"{what}: block_table [slots, pages] and num_pages [slots] must be int32")
-    (slots, most), (stride, column), device = block_table.shape, block_table.stride(), block_table.device
+    (slots, most), (stride, column), where = block_table.shape, block_table.stride(), block_table.get_device()
     if slots < 1 or most < 1:
         raise ValueError(f"{what}: block_table is empty")
     if (column != 1 and most != 1) or (stride < most and slots > 1):
@@ -28,9 +28,9 @@ def _tables(what: str, block_table: torch.Tensor, num_pages: torch.Tensor, idx_m
         raise ValueError(f"{what}: num_pages must be contiguous, one entry for each of the {slots} slots")
     if idx_mapping.dim() != 1 or page < 1:
         raise ValueError(f"{what}: idx_mapping must be a vector and page positive")
-    if num_pages.device != device or idx_mapping.device != device:
-        raise ValueError(f"{what}: every tensor must be on {device}")
-    return slots, most, stride, idx_mapping.shape[0], device
+    if num_pages.get_device() != where or idx_mapping.get_device() != where:
+        raise ValueError(f"{what}: every tensor must be on {block_table.device}")
+    return slots, most, stride, idx_mapping.shape[0], where
 
 
 def resize_tables(
@@ -56,21 +56,21 @@ def resize_tables(
     of its request. Giving back in the same order what was just taken leaves the stack as it was. Table entries behind a
     request's pages are not cleared. Nothing happens at all if ``num_free`` and what comes back are more than ``free_pages`` holds.
     """
-    slots, most, stride, requests, device = _tables("resize_tables", block_table, num_pages, idx_mapping, page)
+    slots, most, stride, requests, where = _tables("resize_tables", block_table, num_pages, idx_mapping, page)
     if lens.dim() != 1 or lens.shape[0] < requests:
         raise ValueError(f"resize_tables: lens must be [{requests}]")
     if free_pages.dtype != torch.int32 or free_pages.dim() != 1 or not free_pages.is_contiguous():
         raise ValueError("resize_tables: free_pages must be a contiguous int32 vector")
     if num_free.dtype != torch.int32 or num_free.numel() != 1:
         raise ValueError("resize_tables: num_free must be one int32")
-    if lens.device != device or free_pages.device != device or num_free.device != device:
-        raise ValueError(f"resize_tables: every tensor must be on {device}")
+    if lens.get_device() != where or free_pages.get_device() != where or num_free.get_device() != where:
+        raise ValueError(f"resize_tables: every tensor must be on {block_table.device}")
     if requests == 0:
         return
     args = _native.ResizeTablesArgs(block_table.data_ptr(), stride, num_pages.data_ptr(), _native.itab(idx_mapping),
                                     _native.itab(lens), free_pages.data_ptr(), num_free.data_ptr(), free_pages.shape[0], requests,
                                     slots, most, page)
-    _native.launch("eagle4_resize_tables", args, device)
+    _native.launch("eagle4_resize_tables", args, block_table.device)
 
 
 def slot_maps(
@@ -91,7 +91,7 @@ def slot_maps(
     page``, -1 where the request holds no such page, and -1 behind the last request's rows. ``batch_table`` [requests, pages] int32
     gets each request's pages and 0 behind them; request rows behind the batch are left as they were.
     """
-    state_slots, most, stride, requests, device = _tables("slot_maps", block_table, num_pages, idx_mapping, page)
+    state_slots, most, stride, requests, where = _tables("slot_maps", block_table, num_pages, idx_mapping, page)
     if query_start_loc.shape[0] < requests + 1 or context_lens.shape[0] < requests:
         raise ValueError(f"slot_maps: query_start_loc must be [{requests + 1}] and context_lens [{requests}]")
     if slots.dtype != torch.int64 or slots.dim() != 1 or not slots.is_contiguous():
@@ -103,14 +103,14 @@ def slot_maps(
         batch_stride, column = batch_table.stride()
         if (column != 1 and most != 1) or (batch_stride < most and requests > 1):
             raise _native.NotCovered("slot_maps: batch_table must have a unit column stride and rows of their own storage")
-        if batch_table.device != device:
-            raise ValueError(f"slot_maps: every tensor must be on {device}")
-    if context_lens.device != device or query_start_loc.device != device or slots.device != device:
-        raise ValueError(f"slot_maps: every tensor must be on {device}")
+        if batch_table.get_device() != where:
+            raise ValueError(f"slot_maps: every tensor must be on {block_table.device}")
+    if context_lens.get_device() != where or query_start_loc.get_device() != where or slots.get_device() != where:
+        raise ValueError(f"slot_maps: every tensor must be on {block_table.device}")
     if requests == 0 and slots.shape[0] == 0:
         return slots, batch_table
     args = _native.SlotMapsArgs(block_table.data_ptr(), stride, num_pages.data_ptr(), _native.itab(idx_mapping),
                                 _native.itab(context_lens), _native.itab(query_start_loc), slots.data_ptr(),
                                 _native.ptr(batch_table), batch_stride, slots.shape[0], requests, state_slots, most, page)
-    _native.launch("eagle4_slot_maps", args, device)
+    _native.launch("eagle4_slot_maps", args, block_table.device)
     return slots, batch_table
