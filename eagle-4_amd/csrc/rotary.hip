@@ -164,7 +164,7 @@ int launch(const eagle4_rotary_args& a, hipStream_t s) {
   // enough tokens for an angle a thread, and for four pieces a thread
   const int heads = a.q_heads + a.k_heads;
   int tokens_of = 1;
-  while (2 * tokens_of * a.half <= kAngles && (tokens_of * a.half < NT || tokens_of * heads * pieces < 4 * NT) &&
+  while (2 * tokens_of * a.half <= kAngles && (tokens_of * a.half < NT || static_cast<int64_t>(heads) * pieces * tokens_of < 4 * NT) &&
          a.tokens > static_cast<int64_t>(512) * tokens_of)
     tokens_of *= 2;
   if (static_cast<int64_t>(heads) * pieces * tokens_of > (1 << 28)) return EAGLE4_NOT_COVERED;

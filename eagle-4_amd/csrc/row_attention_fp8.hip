@@ -89,7 +89,9 @@ __global__ __launch_bounds__(NT, (kResident<D, RT>)) void row_attention_fp8_kern
   const int G = a.heads / a.kv_heads, R = a.rows_per_request * G;
   const bool extend = a.step == 0;
   const int NS = extend ? splits : splits - 1;  // of the shared range; a draft step's ancestors are one more
-  const int64_t seq_len = e4::ld(a.seq_lens, b);
+  int64_t seq_len = e4::ld(a.seq_lens, b);
+  const int64_t room = static_cast<int64_t>(x.table_width) * a.table_page;  // (a padded request's length may be anything)
+  seq_len = seq_len < room ? seq_len : room;
   int64_t trow = a.table_rows.ptr != nullptr ? e4::ld(a.table_rows, b) : b;
   trow = trow < 0 ? 0 : trow < x.table_height ? trow : x.table_height - 1;
   const int32_t* const table = a.table + trow * a.stride_table;

@@ -95,6 +95,8 @@ def _check_fp8(q, keys, values, out, k_scale, v_scale, part_out, part_lse, table
         have = scale.shape
         if scale.dtype != torch.float32 or len(have) != 2 or have[0] < pages or have[1] < heads:
             raise ValueError(f"{name} must be fp32 [pages >= {pages}, kv_heads >= {heads}], got {scale.dtype} {tuple(have)}")
+    if part_out.dim() != 2 or part_out.shape[1] != rows_shape[2] or not part_lse.is_contiguous():
+        raise ValueError(f"part_out must be [rows, {rows_shape[2]}], part_lse contiguous, got {tuple(part_out.shape)}")
     bs = rows_shape[0] // rows_per_request if rows_per_request > 0 else 0
     if table.dim() != 2 or table.numel() == 0 or seq_lens.shape[0] < bs or (table_rows is not None and table_rows.shape[0] < bs):
         raise ValueError(f"the page table must be [requests, entries], seq_lens and table_rows [{bs}]")
@@ -139,8 +141,8 @@ def rows_attention(
     rows_padded(rows_per_request)`` rows (kernels/row_attention.py:251-328).
 
     Beyond the reference: ``float8_e4m3fn`` caches (``keys`` and ``values``, as ``write_kv_pages`` fills them) with
-    ``k_scale`` / ``v_scale`` fp32 ``[pages, kv_heads]`` (any strides), under bf16 or fp16 rows. Value scales below 2^-100 count
-    as 0. A row that sees no key gives zeros.
+    ``k_scale`` / ``v_scale`` fp32 ``[pages, kv_heads]`` (any strides; not negative), under bf16 or fp16 rows. Value scales below
+    2^-100 count as 0. No key is read past the page table's last entry or the cache's last page. A row that sees no key gives zeros.
     """
     rows, heads, head_dim = q.shape
     kv_heads = keys.shape[-2]

@@ -45,7 +45,8 @@ def resize_tables(
     """Brings every request of the batch to the pages that its length needs, in place.
 
     ``block_table`` [slots, pages] and ``num_pages`` [slots] int32: the pages that each state slot holds; ``idx_mapping``
-    [requests] the slots of the batch (each once; a negative one is a padded request), ``lens`` [requests] their lengths
+    [requests] the slots of the batch (each at most once, or its pages are given back or taken twice; a negative one is a
+    padded request), ``lens`` [requests] their lengths
     (int32 / int64), context and the rows to come. ``free_pages`` int32, as long as there are pages, with ``num_free`` [1]
     int32: a stack of the free ones.
 
@@ -92,7 +93,7 @@ def slot_maps(
     gets each request's pages and 0 behind them; request rows behind the batch are left as they were.
     """
     state_slots, most, stride, requests, where = _tables("slot_maps", block_table, num_pages, idx_mapping, page)
-    if query_start_loc.shape[0] < requests + 1 or context_lens.shape[0] < requests:
+    if query_start_loc.dim() != 1 or context_lens.dim() != 1 or query_start_loc.shape[0] < requests + 1 or context_lens.shape[0] < requests:
         raise ValueError(f"slot_maps: query_start_loc must be [{requests + 1}] and context_lens [{requests}]")
     if slots.dtype != torch.int64 or slots.dim() != 1 or not slots.is_contiguous():
         raise ValueError("slot_maps: slots must be a contiguous int64 vector")
@@ -105,6 +106,9 @@ def slot_maps(
             raise _native.NotCovered("slot_maps: batch_table must have a unit column stride and rows of their own storage")
         if batch_table.get_device() != where:
             raise ValueError(f"slot_maps: every tensor must be on {block_table.device}")
+        at, to = block_table.data_ptr(), batch_table.data_ptr()
+        if requests and at < to + 4 * ((requests - 1) * batch_stride + most) and to < at + 4 * ((state_slots - 1) * stride + most):
+            raise ValueError("slot_maps: batch_table must not overlap block_table")
     if context_lens.get_device() != where or query_start_loc.get_device() != where or slots.get_device() != where:
         raise ValueError(f"slot_maps: every tensor must be on {block_table.device}")
     if requests == 0 and slots.shape[0] == 0:

@@ -92,8 +92,9 @@ def _half(name: str, x: torch.Tensor, out: Optional[torch.Tensor], like: tuple) 
             span = ((tokens - 1) * stride[0] + (heads - 1) * stride[1] + dim) * size
             if at < out_at + ((tokens - 1) * to[0] + (heads - 1) * to[1] + dim) * size and out_at < at + span:
                 raise ValueError(f"rotate_rows: {name}_out may be {name} itself, but not overlap it otherwise")
-    if (to[0] == 0 and tokens > 1) or (to[1] == 0 and heads > 1):
-        raise ValueError(f"rotate_rows: the output of {name} is an expanded view: every head needs its own storage")
+    (near, count), (far, others) = ((to[1], heads), (to[0], tokens)) if to[1] <= to[0] else ((to[0], tokens), (to[1], heads))
+    if tokens and heads and ((count > 1 and near < dim) or (others > 1 and far < (near * (count - 1) if count > 1 else 0) + dim)):
+        raise ValueError(f"rotate_rows: heads of the output of {name} overlap: every one needs its own storage")
     return heads, out, stride, to, at, out_at
 
 
@@ -114,8 +115,8 @@ def rotate_rows(
     over tokens and heads (so the parts of one packed projection); ``positions`` [tokens] int32 / int64; ``frequencies`` fp64
     radians a position, at most 512. Pair ``i`` is the elements ``(i, half + i)``, or ``(2 i, 2 i + 1)`` where ``interleaved``:
     ``(x, y) -> factor (x cos - y sin, y cos + x sin)`` of ``position * frequencies[i]``. The elements behind the turned ones
-    are copied. Outputs for both or for neither, in memory that no other argument has; angles are computed in 64 bits, products in 32, each rounded once to the
-    rows' dtype. Returns ``(q_out, k_out)``.
+    are copied. Outputs for both or for neither; what is written is memory that no other argument has. Angles are computed in 64
+    bits, products in 32, each element rounded once to the rows' dtype. Returns ``(q_out, k_out)``.
     """
     code = _DTYPES.get(q.dtype)
     if code is None:

@@ -113,6 +113,10 @@ def shifted():
     (dict(q=torch.zeros(1, 2, 16).expand(4, 2, 16), k=None), ValueError),
     (dict(q_out=torch.zeros(4, 1, 16).expand(4, 2, 16), k=None), ValueError),
     (shifted(), ValueError),
+    (dict(q=torch.zeros(200).as_strided((4, 2, 16), (16, 8, 1)), k=None), ValueError),  # heads that overlap
+    (dict(q=torch.zeros(200).as_strided((4, 2, 16), (24, 16, 1)), k=None), ValueError),  # tokens that do
+    (dict(q=torch.zeros(200).as_strided((4, 2, 16), (16, 56, 1)), k=None), ValueError),
+    (dict(q=torch.zeros(200).as_strided((4, 2, 16), (16, 64, 1)), k=None), RuntimeError),  # heads before tokens: none
     (dict(), RuntimeError),
     (dict(k=None), RuntimeError),
 ])
@@ -209,6 +213,9 @@ def maps(**over):
     (dict(batch=zeros(1, 4)), ValueError),
     (dict(batch=zeros(2, 5)), ValueError),
     (dict(batch=zeros(1, 4).expand(2, 4)), NotCovered),
+    (dict(zip(("table", "batch"), [zeros(3, 4)] * 2)), ValueError),
+    (dict(context=zeros(2, 2)), ValueError),
+    (dict(starts=zeros(3, 2)), ValueError),
     (dict(batch=None), RuntimeError),
 ])
 def test_slot_maps(over, error):
@@ -224,7 +231,8 @@ def rows(**over):
              ks=torch.ones(5, 2), vs=torch.ones(5, 2), table=zeros(1, 3), out=None, seq=zeros(1), step=0, anc=None)
     x.update(over)
     out = torch.zeros_like(x["q"]) if x["out"] is None else x["out"]
-    return rows_attention(x["q"], x["keys"], x["values"], out, torch.zeros(4 * 3 * 16, 64), torch.zeros(4 * 3 * 16), x["table"],
+    part = x.get("part", torch.zeros(4 * 3 * 16, 64))
+    return rows_attention(x["q"], x["keys"], x["values"], out, part, x.get("lse", torch.zeros(4 * 3 * 16)), x["table"],
                           x["seq"], x["anc"], rows_per_request=2, step=x["step"], window=0, scale=1.0, launch=RowsLaunch(splits=2, block_n=32),
                           table_page=16, k_scale=x["ks"], v_scale=x["vs"])
 
@@ -251,6 +259,9 @@ def rows(**over):
     (dict(step=2, anc=None), ValueError),
     (dict(step=2, anc=zeros(1, 2, 2)), RuntimeError),
     (dict(keys=zeros(0, 16, 2, 64, dtype=torch.float8_e4m3fn), values=zeros(0, 16, 2, 64, dtype=torch.float8_e4m3fn)), ValueError),
+    (dict(part=torch.zeros(4 * 3 * 16, 32)), ValueError),
+    (dict(part=torch.zeros(4 * 3 * 16 * 64)), ValueError),
+    (dict(lse=torch.zeros(2 * 4 * 3 * 16)[::2]), ValueError),
     (dict(ks=None, vs=None), NotCovered),  # fp8 caches without scales
     (dict(), RuntimeError),
 ])
