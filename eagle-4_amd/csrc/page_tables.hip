@@ -2,9 +2,10 @@
 // that neither a host's allocator nor its tables are on a round's path.
 //
 // eagle4_resize_tables: one workgroup. The stack of free pages is one sequence, so which entries a request gives or takes follows
-// from running sums over the batch; a chunk of 1024 requests has its sums in LDS, and the threads take the pages that move, one
-// each, finding the request of a page by its place in the sums. What bounds it: three dependent rounds of loads (slots and
-// lengths, page counts, table entries).
+// from running sums over the batch; a chunk of 1024 requests has its sums in LDS, and the threads take the pages that move, finding
+// the request of a page by its place in the sums. What bounds it is latency: rounds of loads that depend on each other (slots and
+// lengths, page counts, then the pages of both directions). 64 requests by a few pages, up and back with both maps of their
+// rows, take 15.3 us in a graph; more workgroups would have to wait for each other's sums, which costs more than this one's loads.
 //
 // eagle4_slot_maps: some workgroups a request, each with its share of the request's rows and table entries; no row is searched for.
 
@@ -54,47 +55,23 @@ E4_DEV Request request_of(const eagle4_resize_tables_args& a, int r) {
 }
 
 // Moves this thread's pages of the chunk's `all`: load and store get a page's number in the chunk, its request, and its number among
-// the request's that move. U of them are looked for, loaded and stored together.
-template <int U, typename Load, typename Store>
-E4_DEV void move_pages(const Chunk& c, uint32_t all, int tid, Load&& load, Store&& store) {
-  for (uint32_t f0 = tid; f0 < all; f0 += U * NT) {
-    int lo[U], hi[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      lo[u] = 0;
-      hi[u] = NT - 1;
-    }
-#pragma unroll 1
-    for (int step = 0; step < 10; ++step)  // the first request whose running sum passes the page
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int mid = (lo[u] + hi[u]) >> 1;
-        if (c.ends[mid] > f0 + u * NT)
-          hi[u] = mid;
-        else
-          lo[u] = mid < hi[u] ? mid + 1 : hi[u];
-      }
-    int32_t page[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const uint32_t f = f0 + u * NT < all ? f0 + u * NT : f0;  // (past the last: the first again, not stored)
-      const int r = f == f0 ? lo[0] : lo[u];
-      lo[u] = r;
-      hi[u] = static_cast<int>(f - (r > 0 ? c.ends[r - 1] : 0));
-      page[u] = load(f, r, hi[u]);
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (f0 + u * NT < all) store(f0 + u * NT, lo[u], hi[u], page[u]);
-  }
-}
+// the request's that move. The search's LDS reads are most of it where many move: 512 prompts' 65 thousand pages, up, mapped and
+// back, take 103 us, and 122 with a loop that ends when the request is found.
 static_assert(NT == 1 << 10, "ten steps of the search");
 template <typename Load, typename Store>
-E4_DEV void each_page(const Chunk& c, uint32_t all, int tid, Load&& load, Store&& store) {
-  if (all <= NT)
-    move_pages<1>(c, all, tid, load, store);
-  else
-    move_pages<8>(c, all, tid, load, store);
+E4_DEV void move_pages(const Chunk& c, uint32_t all, int tid, Load&& load, Store&& store) {
+  for (uint32_t f = tid; f < all; f += NT) {
+    int lo = 0, hi = NT - 1;  // the first request whose running sum passes f: ten steps, and once found it stays
+#pragma unroll
+    for (int step = 0; step < 10; ++step) {
+      const int mid = (lo + hi) >> 1;
+      const bool past = c.ends[mid] > f;
+      hi = past ? mid : hi;
+      lo = past ? lo : mid + 1;
+    }
+    const int i = static_cast<int>(f - (lo > 0 ? c.ends[lo - 1] : 0));
+    store(f, lo, i, load(f, lo, i));
+  }
 }
 
 __global__ __launch_bounds__(NT) void resize_tables_kernel(const eagle4_resize_tables_args a) {
@@ -127,7 +104,7 @@ __global__ __launch_bounds__(NT) void resize_tables_kernel(const eagle4_resize_t
     c.ends[tid] = ends;
     __syncthreads();
     const uint32_t all = c.ends[NT - 1];
-    each_page(
+    move_pages(
         c, all, tid, [&](uint32_t, int r, int i) { return a.block_table[c.slot[r] * a.stride_table + c.from[r] + i]; },
         [&](uint32_t f, int, int, int32_t page) { a.free_pages[top - 1 - (done + f)] = page; });
     if (n > 0) a.num_pages[q.slot] = q.need;
@@ -147,7 +124,7 @@ __global__ __launch_bounds__(NT) void resize_tables_kernel(const eagle4_resize_t
     c.ends[tid] = ends;
     __syncthreads();
     const uint32_t all = c.ends[NT - 1];
-    each_page(
+    move_pages(
         c, all, tid, [&](uint32_t f, int r, int) { return c.slot[r] < 0 ? 0 : a.free_pages[top - 1 - (wanted + f)]; },
         [&](uint32_t, int r, int i, int32_t page) {
           if (c.slot[r] >= 0) a.block_table[c.slot[r] * a.stride_table + c.from[r] + i] = page;
