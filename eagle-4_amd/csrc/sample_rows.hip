@@ -19,13 +19,13 @@
 //    k-th largest of the threads' maxima is not above the row's k-th logit, and min_p is a logit. A pass gathers what
 //    lies above the bound into LDS (up to 2048 tokens), where it is sorted and everything is decided.
 // 3. Otherwise a pass sums the row into bins, ordered by falling logit: 64 of them a factor of two in w, or, of bf16 rows of
-//    magnitudes below 1024, one for each value, which are counted in 32 bits and weighed once each. A place of the order is
-//    found in its bin: by arithmetic where the bin is one value, gathered and sorted where it holds few tokens, divided into 2048 ranges
+//    magnitudes below 1024, one for each value, which are counted in 32 bits and weighed once each; where no rule bounds a
+//    bf16 row, it is counted in pass 1, on the guess that its magnitudes are below 64. A place of the order is found in its bin: by arithmetic where the bin is one value, gathered and sorted where it holds few tokens, divided into 2048 ranges
 //    of logits again where it holds many. Top-p alone takes its list from the bins and decides as in 2.
 // 4. An output is filled and the listed tokens put in, or written in a last pass where no list holds all that is kept.
 //
-// What bounds it: 256 rows of 151936 bf16 logits, 2 draws and fp32 shares each (the least traffic: 233 MB, 45 us) take 66 us where
-// top-k 20 keeps a list, 85 to 93 where top-p or min-p do; 1024 rows cut in place of a copy (92 us) 123 to 130 us: the second pass
+// What bounds it: 256 rows of 151936 bf16 logits, 2 draws and fp32 shares each (the least traffic: 233 MB, 45 us) take 58 us
+// where top-k 20 keeps a list in every row, 69 with top-p 0.95 alone, 86 where all is kept; 1024 rows cut in place of a copy (92 us) 121 to 125 us: the second pass
 // and the bins' LDS additions, beside HBM. A single row takes 16 us: its passes' latency on one CU, where a row split over workgroups
 // would need launches or a wait between them. Few rows with an output are shared by workgroups that all find the cut: 16 rows
 // cut take 22 us.
@@ -93,22 +93,32 @@ E4_DEV Weighed weigh(float x, float top, double c, const double* roots) {
 // value of magnitude from 2^(high - 15) to below 2^high, one for the smaller ones and one for what lies below -2^high, which
 // weighs nothing. There a row is counted, and every value weighed once.
 struct Bins {
+  static constexpr float kFirst = 64.f;
+  static constexpr uint32_t kFirst16 = (127 + 6) << 7;
   static constexpr int kOctaves = 15, kValues = kOctaves * 128, kSmall = kValues, kRest = 2 * kValues + 1;  // bins of values: 0 .. kRest - 1
   bool by_value;
   float top;
   double c;
   uint32_t low16, high16;  // bf16 patterns of 2^(high - 15) and 2^high
 
-  E4_DEV Bins(bool values, float top_, float temperature, double c_) : by_value(false), top(top_), c(c_), low16(0), high16(0) {
+  // Bins of a row that is counted before its maximum is known: of magnitudes below 64.
+  E4_DEV Bins() : by_value(true), top(0.f), c(0.0), low16(kFirst16 - kValues), high16(kFirst16) {}
+  // (`first`: those)
+  E4_DEV Bins(bool values, float top_, float temperature, double c_, bool first) : by_value(false), top(top_), c(c_), low16(0), high16(0) {
     if (!values) return;
-    // nothing below top - 32 T has a mass (e^-32 is 2^-46.2); magnitudes up to 2^10 leave few of a row's logits among the small
-    const float reach = uniform(__builtin_fmaxf(__builtin_fabsf(top), __builtin_fabsf(top - 32.5f * temperature)));
+    // magnitudes up to 2^10 leave few of a row's logits among the small
+    const float reach = reach_of(top, temperature);
     if (!(reach < 1024.f)) return;
     by_value = true;
     high16 = ((__float_as_uint(reach) >> 23) + 1) << 7;
     high16 = uniform(high16);
     high16 = high16 > 64 * 128 ? high16 : 64 * 128;
+    if (first) high16 = kFirst16;
     low16 = high16 - kValues;
+  }
+  // The magnitude that a row's masses end at: nothing below top - 32 T has one (e^-32 is 2^-46.2).
+  static E4_DEV float reach_of(float top, float temperature) {
+    return uniform(__builtin_fmaxf(__builtin_fabsf(top), __builtin_fabsf(top - 32.5f * temperature)));
   }
   // A bf16 pattern's magnitude as steps from the small ones: 0 for them, kValues + 1 from 2^high on. (Positive ones do not come there.)
   E4_DEV int steps(uint32_t w) const {
@@ -131,6 +141,31 @@ struct Bins {
     up = __builtin_elementwise_min(__builtin_elementwise_max(m, u16x2{lo, lo}), u16x2{hi, hi}) - u16x2{lo, lo};
     const u16x2 sign = __builtin_bit_cast(u16x2, __builtin_bit_cast(i16x2, w) >> 15);  // all ones below 0
     at = ((up ^ ~sign) - ~sign + u16x2{kSmall, kSmall}) << 2;
+  }
+  // Counts a vector's logits (those before the row's maximum is known may be above the bins: they go to the first, and the row is
+  // counted again). Bits of those among the small, whose masses are not those of one value.
+  template <bool kAbove, typename Inside>
+  E4_DEV uint32_t count(uint32_t* counts, int e0, const u32x4& w, Inside, int vocab) const {
+    u16x2 least = {0xffff, 0xffff};  // steps; 0: among the small ones
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      u16x2 up, at;
+      places(w[i], up, at);
+      if constexpr (kAbove) at = __builtin_bit_cast(u16x2, __builtin_elementwise_max(__builtin_bit_cast(i16x2, at), i16x2{0, 0}));
+      least = __builtin_elementwise_min(least, up);
+      const uint32_t both = __builtin_bit_cast(uint32_t, at);
+      char* const c8 = reinterpret_cast<char*>(counts);
+      if (Inside::value || static_cast<uint32_t>(e0 + 2 * i) < static_cast<uint32_t>(vocab))
+        atomicAdd(reinterpret_cast<uint32_t*>(c8 + (both & 0xffffu)), 1u);
+      if (Inside::value || static_cast<uint32_t>(e0 + 2 * i + 1) < static_cast<uint32_t>(vocab))
+        atomicAdd(reinterpret_cast<uint32_t*>(c8 + (both >> 16)), 1u);
+    }
+    uint32_t hits = 0;
+    if (least[0] == 0 || least[1] == 0) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) hits |= ((w[i / 2] >> (16 * (i % 2))) & 0x7fffu) < low16 ? 1u << i : 0u;
+    }
+    return hits;
   }
   E4_DEV bool one_value(int b) const { return by_value && b != kSmall && b < kRest; }
   E4_DEV float value(int b) const {
@@ -936,11 +971,36 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const eagle4_sample_row
   if (tid < 64) s.roots[tid] = exp2(tid * -1.0 / 64);
   const float coin = tokens != nullptr && tid < a.draws ? coins[tid] : 0.f;  // (here, beside the row's first loads)
   Rows<T> r(a.logits, n, a.stride_row, a.vocab, s.ends, tid);
+  const bool by_k = k > 0 && k < a.vocab, by_m = m > 0.f, by_p = p < 1.f;
+  const bool asked = by_k || by_m || by_p || tokens != nullptr || a.out_kind == EAGLE4_ROWS_PROBS;
+  bool bounded = by_m || (by_k && k <= kMostByMaxima);
+  // bf16 rows that will need their bins are counted in the pass that finds the maximum: 256 rows drawn from whole 56 -> 48 us, by
+  // top-p 0.95 48 -> 43 (rows with a bound wait for their rules before the first pass: one row's top-k 15.8 -> 16.1)
+  bool counted = T::code == EAGLE4_BF16 && temperature > 0.f && asked && !bounded;
   float mine = -INFINITY;
-  r.each([&](int, const float(&x)[VEC]) {
+  const auto most = [&](const float(&x)[VEC]) {
 #pragma unroll
     for (int i = 0; i < VEC; ++i) mine = __builtin_elementwise_maximum(mine, x[i]);
-  });
+  };
+  if (counted) {
+    if constexpr (T::code == EAGLE4_BF16) {
+      clear(s.mass, s.count, tid);
+      if (tid == 0) s.listed = 0;
+      __syncthreads();
+      const Bins first;
+      r.template each_vector<Rows<T>::kAhead>([&](int e0, const u32x4& w, auto inside) {
+        float x[VEC];
+        Row<T>::widen(w, x);
+        most(x);
+        r.hit_elements(e0, w, first.count<true>(s.count, e0, w, inside, a.vocab), [&](int, float x) {
+          const uint32_t at = atomicAdd(&s.listed, 1u);
+          if (at < kList) s.list.entry[at] = __float_as_uint(x);
+        });
+      });
+    }
+  } else {
+    r.each([&](int, const float(&x)[VEC]) { most(x); });
+  }
   {
     const float w = wave_max(mine);
     if (lane == 0) s.wave32[wave] = __float_as_uint(w);
@@ -979,7 +1039,6 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const eagle4_sample_row
     cut.x = r.top;
     if (tokens != nullptr && tid < a.draws) tokens[tid] = cut.index;
   } else {
-    const bool by_k = k > 0 && k < a.vocab, by_m = m > 0.f, by_p = p < 1.f;
     // min-p: the lowest logit whose weight reaches it
     float lowest = -INFINITY;
     if (by_m) {
@@ -994,35 +1053,27 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const eagle4_sample_row
       const float b = bound_of(s, mine, k, tid);
       bound = uniform(b > bound ? b : bound);
     }
-    const bool asked = by_k || by_m || by_p || tokens != nullptr || a.out_kind == EAGLE4_ROWS_PROBS;
-    const Bins bins(T::code == EAGLE4_BF16, r.top, temperature, r.c);
-    bool bounded = by_m || (by_k && k <= kMostByMaxima);
+    const uint32_t small = counted ? uniform(s.listed) : 0;  // their values are in the list
+    counted = counted && small <= kList && Bins::reach_of(r.top, temperature) < Bins::kFirst;
+    const Bins bins(T::code == EAGLE4_BF16, r.top, temperature, r.c, counted);
     for (bool binned = !asked;;) {
       if (bounded) listed = list_range(r, s, bound, r.top, 0);
       if (listed <= kList || binned) break;
-      clear(s.mass, s.count, tid);
-      __syncthreads();
+      if (!counted) {
+        clear(s.mass, s.count, tid);
+        __syncthreads();
+      }
       if (bins.by_value) {
-        if constexpr (T::code == EAGLE4_BF16)
+        const auto add_small = [&](float x) {
+          atomicAdd(reinterpret_cast<unsigned long long*>(&s.mass[Bins::kSmall]), weigh(x, r.top, r.c, s.roots).mass);
+        };
+        if (counted) {
+          for (uint32_t i = tid; i < small; i += NT) add_small(__uint_as_float(static_cast<uint32_t>(s.list.entry[i])));
+        } else if constexpr (T::code == EAGLE4_BF16) {
           r.template each_vector<Rows<T>::kAhead>([&](int e0, const u32x4& w, auto inside) {
-            u16x2 least = {0xffff, 0xffff};  // steps; 0: among the small ones
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              u16x2 up, at;
-              bins.places(w[i], up, at);
-              least = __builtin_elementwise_min(least, up);
-              const uint32_t both = __builtin_bit_cast(uint32_t, at);
-              char* const count = reinterpret_cast<char*>(s.count);
-              if (decltype(inside)::value || in_row(e0 + 2 * i, a.vocab)) atomicAdd(reinterpret_cast<uint32_t*>(count + (both & 0xffffu)), 1u);
-              if (decltype(inside)::value || in_row(e0 + 2 * i + 1, a.vocab)) atomicAdd(reinterpret_cast<uint32_t*>(count + (both >> 16)), 1u);
-            }
-            const bool small = least[0] == 0 || least[1] == 0;
-            if (small)
-              r.elements(e0, w, inside, [&](int, float x) {
-                if (bins.of(x) == Bins::kSmall)
-                  atomicAdd(reinterpret_cast<unsigned long long*>(&s.mass[Bins::kSmall]), weigh(x, r.top, r.c, s.roots).mass);
-              });
+            r.hit_elements(e0, w, bins.count<false>(s.count, e0, w, inside, a.vocab), [&](int, float x) { add_small(x); });
           });
+        }
         __syncthreads();
         for (int i = tid; i < Bins::kRest; i += NT)
           if (i != Bins::kSmall && s.count[i] > 0) s.mass[i] = s.count[i] * weigh(bins.value(i), r.top, r.c, s.roots).mass;
@@ -1130,7 +1181,7 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const eagle4_sample_row
     return;
   }
   const double unit = kUnit / static_cast<double>(z);
-  const Bins bins(T::code == EAGLE4_BF16, r.top, temperature, r.c);
+  const Bins bins(T::code == EAGLE4_BF16, r.top, temperature, r.c, false);
   const auto write = [&](const auto& out) {
     if constexpr (T::code == EAGLE4_BF16)
       if (kept_list == 0 && !cut.single && bins.by_value) return write_shares(r, cut, s, bins, out, share, shares);

@@ -162,3 +162,30 @@ def test_two_streams_at_a_time(dev):
     for i, result in enumerate(got):
         for one, two in zip(result, want[i % 2]):
             assert torch.equal(one, two), i
+
+
+@pytest.mark.parametrize("p", [0.9, 1.0])
+@pytest.mark.parametrize("kind", ["zeros", "few zeros", "large", "small", "masked", "at 64", "wide", "below"])
+def test_rows_that_no_rule_bounds(dev, kind, p):
+    """Values at the edges of what one pass over a bf16 row can count: many zeros, magnitudes of 64 and more, all of them tiny, masks,
+    a hot temperature, all far below 0."""
+    announce(f"rows that no rule bounds: {kind} p={p}")
+    x, t = sr._logits(3, 20011, "bf16", 17).float(), 1.0
+    if kind == "zeros":
+        x[:, 100:9000] = 0.0
+    elif kind == "few zeros":
+        x[:, 100:700] = 0.0
+        x[:, 700:900] = -0.0
+    elif kind == "large":
+        x, t = x * 20, 8.0
+    elif kind == "small":
+        x = x * 1e-4
+    elif kind == "masked":
+        x[:, ::3], x[:, 1::9] = -torch.inf, torch.finfo(torch.bfloat16).min
+    elif kind == "at 64":
+        x[0, 5], x[1, 5], x[2, 5] = 63.75, 64.0, 500.0
+    elif kind == "wide":
+        t = 3.0
+    elif kind == "below":
+        x = x - 40.0
+    sr._check(dev, x.bfloat16(), t, 0, p, 0.0, probs="f32")
