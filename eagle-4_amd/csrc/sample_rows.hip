@@ -20,15 +20,16 @@
 //    lies above the bound into LDS (up to 2048 tokens), where it is sorted and everything is decided.
 // 3. Otherwise a pass sums the row into bins, ordered by falling logit: 64 of them a factor of two in w, or, of bf16 rows of
 //    magnitudes below 1024, one for each value, which are counted in 32 bits and weighed once each; where no rule bounds a
-//    bf16 row, it is counted in pass 1, on the guess that its magnitudes are below 64. A place of the order is found in its bin: by arithmetic where the bin is one value, gathered and sorted where it holds few tokens, divided into 2048 ranges
-//    of logits again where it holds many. Top-p alone takes its list from the bins and decides as in 2.
+//    bf16 row, it is counted in pass 1, on the guess that its magnitudes are below 64. A place of the order is found in its bin:
+//    by arithmetic, and a count of equals by index, where the bin is one value; gathered and sorted where it holds few tokens;
+//    divided into 2048 ranges of logits again where it holds many. Top-p alone takes its list from the bins and decides as in 2.
 // 4. An output is filled and the listed tokens put in, or written in a last pass where no list holds all that is kept.
 //
-// What bounds it: 256 rows of 151936 bf16 logits, 2 draws and fp32 shares each (the least traffic: 233 MB, 45 us) take 58 us
-// where top-k 20 keeps a list in every row, 69 with top-p 0.95 alone, 86 where all is kept; 1024 rows cut in place of a copy (92 us) 121 to 125 us: the second pass
-// and the bins' LDS additions, beside HBM. A single row takes 16 us: its passes' latency on one CU, where a row split over workgroups
-// would need launches or a wait between them. Few rows with an output are shared by workgroups that all find the cut: 16 rows
-// cut take 22 us.
+// What bounds it: 256 rows of 151936 bf16 logits, a draw and fp32 shares each (the least traffic: 233 MB, 46 us) take 58 us
+// where top-k 20 keeps a list in every row, 69 with top-p 0.95 alone, 86 where all is kept; 1024 rows cut (94 us) 121 to 125 us: the
+// second pass and the bins' LDS additions, beside HBM. A single row takes 16 us: its passes' latency on one CU, where a row
+// split over workgroups would need launches or a wait between them. Few rows with an output are shared by workgroups that all
+// find the cut: 16 rows cut take 22 us.
 
 #include <type_traits>
 
@@ -627,35 +628,51 @@ struct Place {
   uint64_t run;  // mass up to it, its own with it
 };
 
-// The element of the row that is `rank`-th (from 0) by index among those equal to x.
+// The element of the row that is `rank`-th (from 0) by index among those equal to x: a pass counts them by parts of 256 elements, and
+// a wave looks through the part.
+constexpr int kPartBits = 8;
+static_assert(EAGLE4_ROWS_MAX_VOCAB <= NT << kPartBits, "a part a thread");
 template <typename T>
 E4_DEV int nth_equal(const Rows<T>& r, Shared& s, float x, uint32_t rank) {
   constexpr int VEC = Row<T>::VEC;
   const int tid = r.tid;
-  uint32_t before = 0;
+  uint32_t* const part = s.sub.count;
+  __syncthreads();
+  part[tid] = 0;
   if (tid == 0) s.found = 0;
-  for (int v0 = 0; v0 < r.row.vectors; v0 += NT) {
-    const int v = v0 + tid;
-    u32x4 w = r.ends[v == 0 && r.begin == 1 ? 0 : 1];
-    if (v >= r.begin && v < r.end) w = r.row.raw(v);
-    const int e0 = v < r.row.vectors ? r.row.first(v) : r.row.vocab;
+  __syncthreads();
+  r.template each_vector<Rows<T>::kAhead>([&](int e0, const u32x4& w, auto inside) {
     float y[VEC];
     Row<T>::widen(w, y);
-    uint32_t k = 0;
+    uint32_t hits = 0;
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) k += y[i] == x && in_row(e0 + i, r.row.vocab);
-    uint32_t at = before + block_scan(k, s.wave32, tid) - k;
+    for (int i = 0; i < VEC; ++i) hits |= y[i] == x ? 1u << i : 0u;
+    if (hits == 0) return;
+    if (decltype(inside)::value && e0 >> kPartBits == (e0 + VEC - 1) >> kPartBits)
+      atomicAdd(&part[e0 >> kPartBits], static_cast<uint32_t>(__popc(hits)));
+    else
+      r.hit_elements(e0, w, hits, [&](int e, float) { atomicAdd(&part[e >> kPartBits], 1u); });
+  });
+  __syncthreads();
+  const uint32_t own = part[tid], run = block_scan(own, s.wave32, tid);
+  if (run > rank && run - own <= rank) {
+    s.found = tid;
+    s.listed = rank - (run - own);
+  }
+  __syncthreads();
+  const int e1 = uniform(s.found) << kPartBits;
+  uint32_t left = uniform(s.listed);
+  __syncthreads();
+  if (tid < 64) {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i)
-      if (y[i] == x && in_row(e0 + i, r.row.vocab)) {
-        if (at == rank) s.found = e0 + i;
-        ++at;
-      }
-    __syncthreads();
-    uint32_t all = 0;
-    for (int i = 0; i < kWaves; ++i) all += s.wave32[i];
-    before += all;
-    if (before > rank) break;
+    for (int i = 0; i < (1 << kPartBits) / 64; ++i) {
+      const int e = e1 + 64 * i + tid;
+      const bool hit = in_row(e, r.row.vocab) && T::to_f32(r.row.p[e]) == x;
+      const uint64_t all = __ballot(hit);
+      const uint32_t before = __popcll(all & ((uint64_t{1} << tid) - 1));
+      if (hit && before == left) s.found = e;
+      left -= __popcll(all);  // (below 0, a large number: found already)
+    }
   }
   __syncthreads();
   const int e = s.found;
@@ -707,7 +724,7 @@ E4_DEV Place locate(const Rows<T>& r, const Bins& bins, Shared& s, bool by_mass,
     __syncthreads();
   }
   Place p;
-  if (inside > kList) {  // one logit, many times
+  if (lo == hi) {  // one logit, however often
     p.x = value_of(lo);
     const uint64_t each = weigh(p.x, r.top, r.c, s.roots).mass;
     uint64_t rank = by_mass ? (each > 0 ? (target - mass) / each : 0) : target - count;
