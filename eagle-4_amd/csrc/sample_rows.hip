@@ -680,9 +680,10 @@ E4_DEV int nth_equal(const Rows<T>& r, Shared& s, float x, uint32_t rank) {
   return e;
 }
 
-// The first element of the order whose running mass (by_mass) or count exceeds `target`, which is below the row's.
+// The first element of the order whose running mass (by_mass) or count exceeds `target`, which is below the row's. Without
+// `index` the element's place among its equals may stay unknown (-1): a pass less.
 template <typename T>
-E4_DEV Place locate(const Rows<T>& r, const Bins& bins, Shared& s, bool by_mass, uint64_t target) {
+E4_DEV Place locate(const Rows<T>& r, const Bins& bins, Shared& s, bool by_mass, uint64_t target, bool index) {
   const int tid = r.tid;
   const int b = find_bin(s.mass, s.count, by_mass, target, s, tid);
   uint64_t mass = uniform(b > 0 ? s.mass[b - 1] : uint64_t{0});  // before the range
@@ -730,7 +731,8 @@ E4_DEV Place locate(const Rows<T>& r, const Bins& bins, Shared& s, bool by_mass,
     uint64_t rank = by_mass ? (each > 0 ? (target - mass) / each : 0) : target - count;
     if (rank >= inside) rank = inside - 1;
     p.run = mass + (rank + 1) * each;
-    p.index = nth_equal(r, s, p.x, static_cast<uint32_t>(rank));
+    p.index = -1;
+    if (index) p.index = nth_equal(r, s, p.x, static_cast<uint32_t>(rank));
     return p;
   }
   // (-0's key belongs to no element, but -0 >= 0)
@@ -1175,7 +1177,7 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const eagle4_sample_row
         } else {
           target = target_of(coins[step], z);
         }
-        const Place at = locate(r, bins, s, by_mass, target);
+        const Place at = locate(r, bins, s, by_mass, target, step >= 0 || a.out != nullptr);  // draws need no more of a cut than its mass
         if (step >= 0) {
           if (tid == 0) tokens[step] = at.index;
           continue;
