@@ -26,7 +26,7 @@
 // 4. An output is filled and the listed tokens put in, or written in a last pass where no list holds all that is kept.
 //
 // What bounds it: 256 rows of 151936 bf16 logits, a draw and fp32 shares each (the least traffic: 233 MB, 46 us) take 58 us
-// where top-k 20 keeps a list in every row, 69 with top-p 0.95 alone, 86 where all is kept; 1024 rows cut (94 us) 121 to 125 us: the
+// where top-k 20 keeps a list in every row, 70 with top-p 0.95 alone, 86 where all is kept; 1024 rows cut (94 us) 120 to 126 us: the
 // second pass and the bins' LDS additions, beside HBM. A single row takes 16 us: its passes' latency on one CU, where a row
 // split over workgroups would need launches or a wait between them. Few rows with an output are shared by workgroups that all
 // find the cut: 16 rows cut take 22 us.
