@@ -70,10 +70,9 @@ def step_splits(programs: int, device: torch.device) -> int:
     return 2 ** exponent if exponent > 0 else 1
 
 
-def _cache_strides(cache: torch.Tensor) -> tuple[int, int, int]:
-    """Element strides (per page, per slot within its page, per KV head) of a cache view. A ``[pages, page, heads,
-    D]`` view has all three; a ``[slots, heads, D]`` view is read as pages of one slot, so its slot stride is 0."""
-    stride = cache.stride()
+def _cache_strides(stride: tuple) -> tuple[int, int, int]:
+    """Element strides (per page, per slot within its page, per KV head) of a cache view, of its own. A ``[pages, page,
+    heads, D]`` view has all three; a ``[slots, heads, D]`` view is read as pages of one slot, so its slot stride is 0."""
     if len(stride) == 4:
         return stride[0], stride[1], stride[2]
     return stride[0], 0, stride[1]
@@ -98,7 +97,7 @@ def _check_fp8(q, keys, values, out, k_scale, v_scale, part_out, part_lse, table
     if part_out.dim() != 2 or part_out.shape[1] != rows_shape[2] or not part_lse.is_contiguous():
         raise ValueError(f"part_out must be [rows, {rows_shape[2]}], part_lse contiguous, got {tuple(part_out.shape)}")
     bs = rows_shape[0] // rows_per_request if rows_per_request > 0 else 0
-    if table.dim() != 2 or table.numel() == 0 or seq_lens.shape[0] < bs or (table_rows is not None and table_rows.shape[0] < bs):
+    if table.dim() != 2 or table.numel() == 0 or seq_lens.shape[0] < bs or (table if table_rows is None else table_rows).shape[0] < bs:
         raise ValueError(f"the page table must be [requests, entries], seq_lens and table_rows [{bs}]")
     if step > 0 and (ancestors.shape[-1] < step or ancestors.numel() < bs * rows_per_request * ancestors.shape[-1]):
         raise ValueError(f"ancestors must be [{bs}, {rows_per_request}, >= {step}], got {tuple(ancestors.shape)}")
@@ -157,27 +156,27 @@ def rows_attention(
                    rows_per_request, step)
     elif q.dtype != keys.dtype or out.dtype != q.dtype or (values is not None and values.dtype != q.dtype):
         raise _native.NotCovered("q, the caches and out must share one 16-bit dtype")
-    for name, t in (("q", q), ("out", out), ("keys", keys), ("values", values)):
-        if t is not None and t.stride(-1) != 1:
-            raise _native.NotCovered(f"{name} must have a unit stride over the head dim")
+    q_stride, out_stride, k_stride = q.stride(), out.stride(), keys.stride()
+    v_stride = k_stride if values is None else values.stride()
+    if q_stride[-1] != 1 or out_stride[-1] != 1 or k_stride[-1] != 1 or v_stride[-1] != 1:
+        raise _native.NotCovered("q, out, keys and values must have a unit stride over the head dim")
     if part_out.dtype != torch.float32 or part_lse.dtype != torch.float32 or not part_out.is_contiguous():
         raise _native.NotCovered("the partials are contiguous fp32 scratch")
-    if table.dtype != torch.int32 or table.stride(-1) != 1:
+    table_stride = table.stride()
+    if table.dtype != torch.int32 or table_stride[-1] != 1:
         raise _native.NotCovered("the page table must be int32 with unit stride")
     bs = rows // rows_per_request
-    kst = _cache_strides(keys)
-    vst = _cache_strides(values) if values is not None else kst
+    kst, vst = _cache_strides(k_stride), _cache_strides(v_stride)
     anc = None
     if step > 0:
         anc = ancestors if ancestors.dtype == torch.int32 and ancestors.is_contiguous() else ancestors.to(
             torch.int32).contiguous()
-    q_stride, out_stride = q.stride(), out.stride()
     args = _native.RowAttnArgs(  # by position, as the struct has them: by name it costs more than the rest of the call
         q.data_ptr(), q_stride[0], q_stride[1], keys.data_ptr(), _native.ptr(values), kst[0], kst[1], kst[2], vst[0], vst[1], vst[2],
         out.data_ptr(), out_stride[0], out_stride[1], part_out.data_ptr(), part_lse.data_ptr(),
-        min(part_out.shape[0], part_lse.numel()), table.data_ptr(), table.stride(0), _native.itab(table_rows),
+        min(part_out.shape[0], part_lse.numel()), table.data_ptr(), table_stride[0], _native.itab(table_rows),
         _native.itab(seq_lens), _native.ptr(anc), anc.shape[-1] if anc is not None else 1, table_page,
-        1 if keys.dim() == 3 else keys.shape[1], bs, rows_per_request, rows_padded(rows_per_request), heads, kv_heads, head_dim,
+        1 if len(k_stride) == 3 else keys.shape[1], bs, rows_per_request, rows_padded(rows_per_request), heads, kv_heads, head_dim,
         _native.dtype_code(q.dtype), step, window, launch.splits, scale)
     if k_scale is None:
         _native.launch("eagle4_row_attention", args, q.device)

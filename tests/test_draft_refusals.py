@@ -259,6 +259,7 @@ def rows(**over):
     (dict(step=2, anc=None), ValueError),
     (dict(step=2, anc=zeros(1, 2, 2)), RuntimeError),
     (dict(keys=zeros(0, 16, 2, 64, dtype=torch.float8_e4m3fn), values=zeros(0, 16, 2, 64, dtype=torch.float8_e4m3fn)), ValueError),
+    (dict(q=zeros(4, 4, 64, dtype=torch.bfloat16), seq=zeros(2)), ValueError),  # two requests, one row of the table
     (dict(part=torch.zeros(4 * 3 * 16, 32)), ValueError),
     (dict(part=torch.zeros(4 * 3 * 16 * 64)), ValueError),
     (dict(lse=torch.zeros(2 * 4 * 3 * 16)[::2]), ValueError),
