@@ -9,8 +9,8 @@
 //
 // A workgroup takes some tokens; a thread 16 bytes of a head, or the two 16-byte pieces whose elements are paired, several
 // of them on their way together. What bounds it: HBM, one read and one write of each element: 8191 tokens of 32 and 8 heads of
-// 128 (168 MB) take 34 us with their launch, 28 in a graph that finds part of them in the last cache; a copy of them takes 32.5. 16 tokens take 4.8 us
-// in a graph, a launch's latency and that of two loads after each other.
+// 128 (168 MB) take 34 us with their launch, 28 in a graph that finds part of them in the last cache; a copy's rate makes 33.
+// 16 tokens take 4.8 us in a graph, a launch's latency and that of two loads after each other.
 
 #include "common.h"
 

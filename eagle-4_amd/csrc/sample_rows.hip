@@ -1094,8 +1094,12 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const eagle4_sample_row
           });
         }
         __syncthreads();
-        for (int i = tid; i < Bins::kRest; i += NT)
-          if (i != Bins::kSmall && s.count[i] > 0) s.mass[i] = s.count[i] * weigh(bins.value(i), r.top, r.c, s.roots).mass;
+#pragma unroll 2
+        for (int j = 0; j < kBins / NT; ++j) {  // (two together: a weight is a chain of 64-bit operations)
+          const int i = tid + j * NT;
+          const uint64_t mass = s.count[i] * weigh(bins.value(i), r.top, r.c, s.roots).mass;
+          if (i != Bins::kSmall && i < Bins::kRest) s.mass[i] = mass;
+        }
       } else {
         r.each_element([&](int, float x) {
           const Weighed w = weigh(x, r.top, r.c, s.roots);
