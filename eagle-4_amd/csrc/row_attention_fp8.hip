@@ -4,10 +4,14 @@
 // V_j the codes, which the products take exactly (every e4m3 value is a bf16 and an fp16 value). With logarithms to base 2
 // and t_j = s_j + log2 v_j, the weights are w_j = 2^(t_j - m), m a running maximum of t:
 //     out = sum w_j V_j / sum w_j / v_j.
-// So what is rounded to the rows' 16 bits for the second product is at most 2^kSlack and has its largest terms near 1, whatever
-// the scales are; sums, maxima and the denominator are in 32 bits. A page whose value scale is 0, or below 2^-100, counts in the
-// denominator alone (its codes are taken as zeros). The keys that a row does not see weigh 0, and in tiles that hold such keys NaN
-// codes are taken out of the values first (0 times NaN): they are added to the rows that see them.
+// So what is rounded for the second product is at most 2^kSlack and its largest terms are near 1; sums, maxima and the denominator
+// are in 32 bits. Bf16 rows round a weight once to bf16 (2^-8 of it, as the output is rounded anyway). fp16 has not the range:
+// a key without values (zeros under a large scale, or a page of scale 0, which counts as 1 here) may hold the maximum, and the weights
+// that matter lie 2^-20 and more below it. So fp16 rows take each weight as two bf16 parts, 16 bits of it over the range of 32-bit floats;
+// codes are bf16 values too. That costs 1 to 3% of a step, 2 to 15% of an extend (36 rows a head of D 128 over 2048 keys, 32 requests: 47
+// -> 53 us; bf16 rows would pay as much, 47 -> 54). A page whose value scale is 0, or below 2^-100, counts in the denominator alone
+// (its codes are taken as zeros). The keys that a row does not see weigh 0, and in tiles that hold such keys NaN codes are taken
+// out of the values first (0 times NaN): they are added to the rows that see them.
 //
 // Split: a workgroup takes a key split (or the ancestors) of a request's KV head and up to 16 RT of its rows (request rows x
 // query heads of the group); its four waves take every fourth tile of 32 keys on their own, each with its own softmax, and
@@ -59,6 +63,7 @@ struct Smem {
       char q[RT * 16 * 2 * D];  // the rows, 16-byte chunks swizzled as Tile's keys
       char v[NW][32 * D];       // a wave's tile of values, rows of D codes in 16-byte chunks swizzled as Tile8's
       WaveMeta meta[NW];
+      int2 seen[RT * 16];  // the first and the last key that a row sees
     } loop;
     struct {
       f32x4_t acc[NW][D / 16 / kHalves][64];
@@ -75,6 +80,7 @@ template <int D, typename T, int RT>
 __global__ __launch_bounds__(NT, (kResident<D, RT>)) void row_attention_fp8_kernel(const eagle4_row_attn_fp8_args x, int groups, int splits) {
   const eagle4_row_attn_args& a = x.rows;
   using T8 = Tile8<D>;
+  constexpr int kParts = T::code == EAGLE4_F16 ? 2 : 1;  // of a weight, in bf16
   constexpr bool kEarly = D * RT <= 256;  // the next loads before the softmax; else behind it, for the registers
   constexpr int CH = D / 16, KJ = D / 64, NI = D / 32, RPI = 1024 / D;
   __shared__ __attribute__((aligned(1024))) Smem<D, RT> sm;
@@ -116,38 +122,36 @@ __global__ __launch_bounds__(NT, (kResident<D, RT>)) void row_attention_fp8_kern
   // them, and every row sees all_lo .. all_hi.
   const bool anc = !extend && split == NS;
   int64_t start = 0;
-  int count = 0, all_lo = 0, all_hi = -1, lo[RT], hi[RT];
+  int count = 0, all_lo = 0, all_hi = -1;
+  int64_t end = 0;
+  const auto within = [&](int64_t p) { return static_cast<int>(p < start - 1 ? -1 : p < end ? p - start : end - start); };
   if (!anc) {
     const int64_t first = window_start(extend ? seq_len : seq_len - 1, a.window);
     const int64_t last = extend ? seq_len + a.rows_per_request - 1 : seq_len - 1;
     const int64_t span = last + 1 - first;
     const int64_t per = span > 0 ? ((span + NS - 1) / NS + 31) / 32 * 32 : 0;
     start = first + split * per;
-    const int64_t end = start + per < last + 1 ? start + per : last + 1;
+    end = start + per < last + 1 ? start + per : last + 1;
     count = end > start ? static_cast<int>(end - start) : 0;
-    const auto within = [&](int64_t p) { return static_cast<int>(p < start - 1 ? -1 : p < end ? p - start : end - start); };
     all_lo = extend ? within(window_start(last, a.window)) : 0;
     all_hi = extend ? within(seq_len) : count - 1;
     if (all_hi >= count) all_hi = count - 1;
-#pragma unroll
-    for (int r = 0; r < RT; ++r) {
-      const int t = ((grp * RT + r) * 16 + l16) / G;
-      lo[r] = extend ? within(window_start(seq_len + t, a.window)) : 0;
-      hi[r] = extend ? within(seq_len + t) : count - 1;
-    }
   } else {
     count = a.rows_per_request * a.max_depth;
     all_lo = count;
-#pragma unroll
-    for (int r = 0; r < RT; ++r) {
-      lo[r] = ((grp * RT + r) * 16 + l16) / G * a.max_depth;
-      hi[r] = lo[r] + a.step - 1;
-    }
   }
-#pragma unroll
-  for (int r = 0; r < RT; ++r) {
-    if ((grp * RT + r) * 16 + l16 >= R) hi[r] = -1;  // no such row
-    hi[r] = hi[r] < count ? hi[r] : count - 1;
+  if (tid < RT * 16) {
+    const int rho = grp * RT * 16 + tid, t = rho / G;
+    int lo = 0, hi = count - 1;
+    if (anc) {
+      lo = t * a.max_depth;
+      hi = lo + a.step - 1;
+    } else if (extend) {
+      lo = within(window_start(seq_len + t, a.window));
+      hi = within(seq_len + t);
+    }
+    if (rho >= R) hi = -1;  // no such row
+    sm.loop.seen[tid] = make_int2(lo, hi < count ? hi : count - 1);
   }
   const int ntiles = (count + 31) / 32;
 
@@ -276,7 +280,7 @@ __global__ __launch_bounds__(NT, (kResident<D, RT>)) void row_attention_fp8_kern
       }
     };
     put_v();
-    auto visible = [&](int r, int k) { return base + k >= lo[r] && base + k <= hi[r]; };
+    auto visible = [&](int2 seen, int k) { return base + k >= seen.x && base + k <= seen.y; };
     if (!full) {
       uint32_t odd = 0;
 #pragma unroll
@@ -292,7 +296,7 @@ __global__ __launch_bounds__(NT, (kResident<D, RT>)) void row_attention_fp8_kern
             if (bad == 0) continue;
 #pragma unroll
             for (int r = 0; r < RT; ++r)
-              if (visible(r, k))
+              if (visible(sm.loop.seen[16 * r + l16], k))
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
                   if ((bad >> (8 * i)) & 0x80u) acc[r][dt][i] = NAN;
@@ -317,10 +321,12 @@ __global__ __launch_bounds__(NT, (kResident<D, RT>)) void row_attention_fp8_kern
     };
     if constexpr (kEarly) next();
 
-    u32x4_t pb[RT];
+    u32x4_t pb[RT], pl[kParts == 2 ? RT : 1];
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
       float top = -INFINITY;
+      int2 seen = {0, 0};
+      if (!full) seen = sm.loop.seen[16 * r + l16];
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt) {
         const f32x4_t k4 = *reinterpret_cast<const f32x4_t*>(&meta.ks[16 * kt + 4 * g]);
@@ -328,7 +334,7 @@ __global__ __launch_bounds__(NT, (kResident<D, RT>)) void row_attention_fp8_kern
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           s[r][kt][i] = s[r][kt][i] * k4[i] + v4[i];
-          if (!full && !visible(r, 16 * kt + 4 * g + i)) s[r][kt][i] = -INFINITY;
+          if (!full && !visible(seen, 16 * kt + 4 * g + i)) s[r][kt][i] = -INFINITY;
           top = fmaxf(top, s[r][kt][i]);
         }
       }
@@ -352,17 +358,25 @@ __global__ __launch_bounds__(NT, (kResident<D, RT>)) void row_attention_fp8_kern
           p[i] = __builtin_amdgcn_exp2f(s[r][kt][i] - ref);
           l[r] += p[i] == 0.f ? 0.f : p[i] * i4[i];
         }
-        pb[r][2 * kt] = pack2<T>(p[0], p[1]);
-        pb[r][2 * kt + 1] = pack2<T>(p[2], p[3]);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const uint32_t w = pack2<e4::Bf16>(p[2 * i], p[2 * i + 1]);
+          pb[r][2 * kt + i] = w;
+          if constexpr (kParts == 2)
+            pl[r][2 * kt + i] = pack2<e4::Bf16>(p[2 * i] - __uint_as_float(w << 16), p[2 * i + 1] - __uint_as_float(w & 0xffff0000u));
+        }
       }
     }
     if constexpr (!kEarly) next();
     const int vnow = vread(here(lane));
 #pragma unroll
     for (int dt = 0; dt < D / 16; ++dt) {
-      const u32x4_t v16 = __builtin_bit_cast(u32x4_t, widen_fp8x8<T>(lds_tr8(sv + (vnow ^ 16 * (dt & 7)) + 128 * (dt / 8))));
+      const u32x4_t v16 = __builtin_bit_cast(u32x4_t, widen_fp8x8<e4::Bf16>(lds_tr8(sv + (vnow ^ 16 * (dt & 7)) + 128 * (dt / 8))));
 #pragma unroll
-      for (int r = 0; r < RT; ++r) acc[r][dt] = mfma16<T>(v16, pb[r], acc[r][dt]);
+      for (int r = 0; r < RT; ++r) acc[r][dt] = mfma16<e4::Bf16>(v16, pb[r], acc[r][dt]);
+      if constexpr (kParts == 2)
+#pragma unroll
+        for (int r = 0; r < RT; ++r) acc[r][dt] = mfma16<e4::Bf16>(v16, pl[r], acc[r][dt]);
       if constexpr (!kEarly)
         if (dt % 4 == 3) __builtin_amdgcn_sched_barrier(0);
     }
