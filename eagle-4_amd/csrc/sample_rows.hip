@@ -972,6 +972,28 @@ E4_DEV void write_shares(const Rows<T>& r, const Cut& cut, Shared& s, const Bins
   }, share, shares);
 }
 
+// A row without rules: its tokens are 0, a token like any other for what looks them up next, and its logits are copied where that is asked.
+template <typename T>
+E4_DEV void padded_row(const eagle4_sample_rows_args& a, int64_t n, int share, int shares, int64_t* tokens, u32x4* ends, int tid) {
+  constexpr int VEC = Row<T>::VEC;
+  using S = typename T::storage;
+  if (tokens != nullptr && tid < a.draws) tokens[tid] = 0;
+  if (a.copy_padded == 0) return;
+  const Rows<T> r(a.logits, n, a.stride_row, a.vocab, ends, tid);
+  S* const out = static_cast<S*>(a.out) + n * a.stride_out;
+  r.template each_vector<Rows<T>::kAhead>([&](int e0, const u32x4& w, auto) {
+    S y[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      if constexpr (sizeof(S) == 4)
+        y[i] = __uint_as_float(w[i]);
+      else
+        y[i] = static_cast<S>(w[i / 2] >> (16 * (i % 2)));
+    }
+    store_vector(out, e0, a.vocab, y);
+  }, share, shares);
+}
+
 template <typename T>
 __global__ __launch_bounds__(NT) void sample_rows_kernel(const eagle4_sample_rows_args a, int shares) {
   __shared__ Shared s;
@@ -980,12 +1002,15 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const eagle4_sample_row
   const int share = blockIdx.x % static_cast<uint32_t>(shares);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t entry = uniform(a.entries.ptr != nullptr ? e4::ld(a.entries, n) : n);
-  if (entry < 0 || entry >= a.num_entries) return;  // a padded row
+  int64_t* const tokens = a.tokens != nullptr && share == 0 ? a.tokens + n * a.draws : nullptr;
+  if (entry < 0 || entry >= a.num_entries) {
+    padded_row<T>(a, n, share, shares, tokens, s.ends, tid);
+    return;
+  }
   const float temperature = uniform(a.temperature[entry]);
   const int k = uniform(a.top_k != nullptr ? a.top_k[entry] : 0);
   const float p = uniform(a.top_p != nullptr ? a.top_p[entry] : 1.f), m = uniform(a.min_p != nullptr ? a.min_p[entry] : 0.f);
 
-  int64_t* const tokens = a.tokens != nullptr && share == 0 ? a.tokens + n * a.draws : nullptr;
   const float* const coins = a.coins != nullptr ? a.coins + n * a.draws : nullptr;
   if (tid < 64) s.roots[tid] = exp2(tid * -1.0 / 64);
   const float coin = tokens != nullptr && tid < a.draws ? coins[tid] : 0.f;  // (here, beside the row's first loads)
@@ -1248,6 +1273,7 @@ extern "C" int eagle4_sample_rows(const eagle4_sample_rows_args* a, void* stream
        (a->out_kind == EAGLE4_ROWS_LOGITS && a->out_dtype != a->dtype) || !lies(a->out, a->stride_out, a->out_dtype) ||
        (a->rows > 1 && a->stride_out < a->vocab)))
     return EAGLE4_NOT_COVERED;
+  if (a->copy_padded != 0 && (a->out == nullptr || a->out_kind != EAGLE4_ROWS_LOGITS)) return EAGLE4_NOT_COVERED;
   const hipStream_t s = static_cast<hipStream_t>(stream);
   switch (a->dtype) {
     case EAGLE4_BF16: return launch<e4::Bf16>(*a, s);

@@ -260,7 +260,7 @@ class LatentAttnArgs(ctypes.Structure):
 class SampleRowsArgs(ctypes.Structure):
     _fields_ = _fields(
         "logits:p stride_row:q entries:t temperature:p top_k:p top_p:p min_p:p coins:p tokens:p out:p stride_out:q rows:q "
-        "num_entries:q vocab:i draws:i dtype:i out_kind:i out_dtype:i reserved:i"
+        "num_entries:q vocab:i draws:i dtype:i out_kind:i out_dtype:i copy_padded:i"
     )
 
 

@@ -88,7 +88,7 @@ def draw_tokens(
     uniform numbers in [0, 1), contiguous: each draws one token of its row, independently. ``temperature``, ``top_k``
     (int32), ``top_p`` and ``min_p`` (fp32; None: off) are vectors over requests, ``entries`` [rows] (int32 / int64) the
     request of each row; without it row ``n`` takes entry ``n``. A row whose entry is negative or past the vectors (a
-    padded one) draws nothing: its tokens and ``probs`` are left as they were.
+    padded one) gets tokens of 0, which a captured step may look up; its row of ``probs`` is left as it was.
 
     With ``Z`` the mass kept, the token is the first of the order whose running mass exceeds ``coin * Z``. ``probs`` [rows,
     vocab] (bf16 / fp16 / fp32, memory of its own) is filled with ``w / Z`` on the kept tokens, 0 elsewhere.
@@ -130,10 +130,12 @@ def truncate_logits(
     :func:`~eagle_harness.vllm.tree_accept.sample_tree`, with the same temperatures.
 
     Arguments as :func:`draw_tokens`'. ``out`` [rows, vocab] of the logits' dtype takes the rows (``out=logits``: in place;
-    any other overlap is not allowed); None: a new tensor. Rows of entries outside the vectors are not written."""
+    any other overlap is not allowed); None: a new tensor. Rows of entries outside the vectors keep their logits: they are not written in a
+    given ``out``, and copied into a new tensor."""
     code, fields = _rows_args("truncate_logits", logits, temperature, top_k, top_p, min_p, entries)
     rows, vocab = logits.shape
-    if out is None:
+    copy_padded = out is None
+    if copy_padded:
         out = torch.empty((rows, vocab), dtype=logits.dtype, device=logits.device)
         stride = vocab
     else:
@@ -145,6 +147,6 @@ def truncate_logits(
     if rows == 0:
         return out
     args = _native.SampleRowsArgs(*fields, None, None, out.data_ptr(), stride, rows, temperature.shape[0], vocab, 0, code, LOGITS,
-                                  code, 0)
+                                  code, copy_padded)
     _native.launch("eagle4_sample_rows", args, logits.device)
     return out

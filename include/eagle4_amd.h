@@ -570,7 +570,8 @@ int eagle4_latent_attention(const eagle4_latent_attn_args* args, void* stream);
  * (top_p from 1 on: all); the first one always. With Z the mass kept, tokens[row, d] is the first of the order whose running mass
  * exceeds coins[row, d] Z. out: w / Z on the kept and 0 elsewhere (PROBS), or the logits with -inf outside the kept (LOGITS;
  * may be the logits themselves). temperature not above 0, or a row whose maximum is not finite: its argmax alone (first
- * index; NaN the largest). Rows whose entry is negative or past num_entries are left alone. */
+ * index; NaN the largest). A row whose entry is negative or past num_entries draws 0s; its row of out is left alone, or, with
+ * copy_padded (LOGITS), gets the logits as they are. */
 #define EAGLE4_ROWS_PROBS 1
 #define EAGLE4_ROWS_LOGITS 2
 #define EAGLE4_ROWS_MAX_VOCAB (1 << 18)
@@ -588,7 +589,7 @@ typedef struct eagle4_sample_rows_args {
   void* out;                /* [rows, vocab] or null, unit column stride */
   int64_t stride_out;
   int64_t rows, num_entries;
-  int32_t vocab, draws, dtype, out_kind, out_dtype, reserved;
+  int32_t vocab, draws, dtype, out_kind, out_dtype, copy_padded;
 } eagle4_sample_rows_args;
 int eagle4_sample_rows(const eagle4_sample_rows_args* args, void* stream);
 

@@ -1,0 +1,18 @@
+"""More of what the C entries of the sampled draft step's operators check before any launch, beside ``test_draft_entry_checks.py``; its
+calls and its pointers, so only where there is no GPU."""
+
+import pytest
+import torch
+
+from eagle_harness.kernels import _native
+from test_draft_entry_checks import NOT_COVERED, OK, ON, sampled
+
+pytestmark = pytest.mark.skipif(torch.cuda.is_available(), reason="calls that pass the checks would be launched")
+
+
+def test_copies_of_padded_rows_are_truncated_rows():
+    call = _native.library().eagle4_sample_rows
+    cut = dict(coins=0, tokens=0, draws=0, out=ON, stride_out=9, out_kind=2, copy_padded=1)
+    assert call(sampled(**cut), None) not in (OK, NOT_COVERED)
+    assert call(sampled(out=ON, stride_out=9, out_kind=1, copy_padded=1), None) == NOT_COVERED
+    assert call(sampled(copy_padded=1), None) == NOT_COVERED
