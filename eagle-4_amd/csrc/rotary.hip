@@ -170,7 +170,9 @@ int launch(const eagle4_rotary_args& a, hipStream_t s) {
          a.tokens > static_cast<int64_t>(512) * tokens_of)
     tokens_of *= 2;
   if (static_cast<int64_t>(heads) * pieces * tokens_of > (1 << 28)) return EAGLE4_NOT_COVERED;
-  rotary_kernel<T, V, kPaired><<<static_cast<unsigned>((a.tokens + tokens_of - 1) / tokens_of), NT, 0, s>>>(a, tokens_of, pieces, turned);
+  const int64_t grid = (a.tokens + tokens_of - 1) / tokens_of;
+  if (grid >= (1 << 24)) return EAGLE4_NOT_COVERED;  // (256 threads each: under 2^32)
+  rotary_kernel<T, V, kPaired><<<static_cast<unsigned>(grid), NT, 0, s>>>(a, tokens_of, pieces, turned);
   return E4_LAUNCH_STATUS();
 }
 

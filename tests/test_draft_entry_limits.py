@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from eagle_harness.kernels import _native
-from test_draft_entry_checks import NOT_COVERED, OK, ON, sampled
+from test_draft_entry_checks import NOT_COVERED, OK, ON, rotary, sampled
 
 pytestmark = pytest.mark.skipif(torch.cuda.is_available(), reason="calls that pass the checks would be launched")
 
@@ -16,3 +16,13 @@ def test_copies_of_padded_rows_are_truncated_rows():
     assert call(sampled(**cut), None) not in (OK, NOT_COVERED)
     assert call(sampled(out=ON, stride_out=9, out_kind=1, copy_padded=1), None) == NOT_COVERED
     assert call(sampled(copy_padded=1), None) == NOT_COVERED
+
+
+def test_rotary_tokens_past_a_launch():
+    """2^24 workgroups of 256 threads are more than a launch takes; these shapes have 64 tokens a workgroup, and wide heads one."""
+    call = _native.library().eagle4_rotary
+    assert call(rotary(tokens=1 << 30), None) == NOT_COVERED
+    assert call(rotary(tokens=(1 << 30) - 64), None) not in (OK, NOT_COVERED)
+    wide = dict(dim=1024, half=512, q_heads=64, stride_qh=1024, stride_kh=1024, stride_qoh=1024, stride_koh=1024)
+    assert call(rotary(tokens=1 << 24, **wide), None) == NOT_COVERED
+    assert call(rotary(tokens=(1 << 24) - 1, **wide), None) not in (OK, NOT_COVERED)
