@@ -477,9 +477,10 @@ int launch(const eagle4_row_attn_fp8_args& x, hipStream_t s) {
   const int groups = (R + 16 * RT - 1) / (16 * RT);
   const int splits = used_splits(x, kResident<D, RT>, groups) + (a.step == 0 ? 0 : 1);
   const int64_t grid = (static_cast<int64_t>(splits) * a.kv_heads * a.bs + 7) / 8 * 8 * groups;
-  if (grid >= (1 << 24)) return EAGLE4_NOT_COVERED;  // (256 threads each: under 2^32)
-  row_attention_fp8_kernel<D, T, RT><<<static_cast<unsigned>(grid), NT, 0, s>>>(x, groups, splits);
   const int64_t pairs = static_cast<int64_t>(a.bs) * a.rows_per_request * a.heads;
+  // (both launches have 256 threads a workgroup: under 2^32; the merge takes more than one run a row only in small grids)
+  if (grid >= (1 << 24) || (pairs + 1024 / D - 1) / (1024 / D) >= (1 << 24)) return EAGLE4_NOT_COVERED;
+  row_attention_fp8_kernel<D, T, RT><<<static_cast<unsigned>(grid), NT, 0, s>>>(x, groups, splits);
   return with_merge_runs<D>(splits, pairs, [&](auto runs) {
     constexpr int SG = decltype(runs)::value;
     constexpr int64_t per = 256 / (D / 4) / SG;
