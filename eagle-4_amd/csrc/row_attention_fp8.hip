@@ -96,8 +96,10 @@ __global__ __launch_bounds__(NT, (kResident<D, RT>)) void row_attention_fp8_kern
   const bool extend = a.step == 0;
   const int NS = extend ? splits : splits - 1;  // of the shared range; a draft step's ancestors are one more
   int64_t seq_len = e4::ld(a.seq_lens, b);
-  const int64_t room = static_cast<int64_t>(x.table_width) * a.table_page;  // (a padded request's length may be anything)
-  seq_len = seq_len < room ? seq_len : room;
+  // Keys end with the page table: a row past it sees those before. (A padded request's length may be anything; far out it makes no
+  // difference which.)
+  const int64_t room = static_cast<int64_t>(x.table_width) * a.table_page, out = int64_t{1} << 32;
+  seq_len = seq_len < -out ? -out : seq_len < room + out ? seq_len : room + out;
   int64_t trow = a.table_rows.ptr != nullptr ? e4::ld(a.table_rows, b) : b;
   trow = trow < 0 ? 0 : trow < x.table_height ? trow : x.table_height - 1;
   const int32_t* const table = a.table + trow * a.stride_table;
@@ -127,13 +129,13 @@ __global__ __launch_bounds__(NT, (kResident<D, RT>)) void row_attention_fp8_kern
   const auto within = [&](int64_t p) { return static_cast<int>(p < start - 1 ? -1 : p < end ? p - start : end - start); };
   if (!anc) {
     const int64_t first = window_start(extend ? seq_len : seq_len - 1, a.window);
-    const int64_t last = extend ? seq_len + a.rows_per_request - 1 : seq_len - 1;
+    const int64_t newest = extend ? seq_len + a.rows_per_request - 1 : seq_len - 1, last = newest < room ? newest : room - 1;
     const int64_t span = last + 1 - first;
     const int64_t per = span > 0 ? ((span + NS - 1) / NS + 31) / 32 * 32 : 0;
     start = first + split * per;
     end = start + per < last + 1 ? start + per : last + 1;
     count = end > start ? static_cast<int>(end - start) : 0;
-    all_lo = extend ? within(window_start(last, a.window)) : 0;
+    all_lo = extend ? within(window_start(newest, a.window)) : 0;
     all_hi = extend ? within(seq_len) : count - 1;
     if (all_hi >= count) all_hi = count - 1;
   } else {

@@ -141,8 +141,9 @@ def rows_attention(
 
     Beyond the reference: ``float8_e4m3fn`` caches (``keys`` and ``values``, as ``write_kv_pages`` fills them) with
     ``k_scale`` / ``v_scale`` fp32 ``[pages, kv_heads]`` (any strides; not negative), under bf16 or fp16 rows. Value scales below
-    2^-100 count as 0. Softmax weights enter the product with the values in bf16 under bf16 rows (sums and the denominator are in 32 bits),
-    in 16 bits over the range of 32-bit floats under fp16 rows. No key is read past the page table's last entry or the cache's last page. A row that sees no key gives zeros.
+    2^-100 count as 0. Softmax weights enter the product with the values in bf16 under bf16 rows (sums and the denominator are in
+    32 bits), in 16 bits over the range of 32-bit floats under fp16 rows. Keys end with the page table (a row behind it sees those before),
+    and nothing is read past the cache's last page. A row that sees no key gives zeros.
     """
     rows, heads, head_dim = q.shape
     kv_heads = keys.shape[-2]
