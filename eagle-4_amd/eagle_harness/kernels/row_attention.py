@@ -96,8 +96,11 @@ def _check_fp8(q, keys, values, out, k_scale, v_scale, part_out, part_lse, table
             raise ValueError(f"{name} must be fp32 [pages >= {pages}, kv_heads >= {heads}], got {scale.dtype} {tuple(have)}")
     if part_out.dim() != 2 or part_out.shape[1] != rows_shape[2] or not part_lse.is_contiguous():
         raise ValueError(f"part_out must be [rows, {rows_shape[2]}], part_lse contiguous, got {tuple(part_out.shape)}")
-    bs = rows_shape[0] // rows_per_request if rows_per_request > 0 else 0
-    if table.dim() != 2 or table.numel() == 0 or seq_lens.shape[0] < bs or (table if table_rows is None else table_rows).shape[0] < bs:
+    if rows_per_request < 1 or rows_shape[0] % rows_per_request:
+        raise ValueError(f"{rows_shape[0]} rows are not {rows_per_request} a request")
+    bs = rows_shape[0] // rows_per_request
+    if table.dim() != 2 or seq_lens.dim() == 0 or (bs > 0 and table.numel() == 0) or seq_lens.shape[0] < bs \
+            or (table_rows is not None and table_rows.dim() == 0) or (table if table_rows is None else table_rows).shape[0] < bs:
         raise ValueError(f"the page table must be [requests, entries], seq_lens and table_rows [{bs}]")
     if step > 0 and (ancestors.shape[-1] < step or ancestors.numel() < bs * rows_per_request * ancestors.shape[-1]):
         raise ValueError(f"ancestors must be [{bs}, {rows_per_request}, >= {step}], got {tuple(ancestors.shape)}")

@@ -44,3 +44,12 @@ def test_rows_behind_the_table(dev, step, length, window, dtype):
             want = w @ v
             bound = (e + 2.0**-16) * (w @ v.abs()) + e * want.abs() + 2.0**-25
             assert ((got[t, h] - want).abs() <= bound).all(), (t, h)
+
+
+def test_no_requests(dev):
+    announce("fp8 rows: no requests")
+    cache, scales = torch.zeros(4, 16, 2, 64, device=dev).to(torch.float8_e4m3fn), torch.ones(4, 2, device=dev)
+    q = torch.empty(0, 4, 64, dtype=torch.bfloat16, device=dev)
+    none = torch.empty(0, dtype=torch.int32, device=dev)
+    got = rows._launch(dev, q, cache, cache, scales, scales, none.view(0, 6), none, None, rows=2, step=0, window=0, splits=2, table_page=16)
+    assert got.shape == q.shape
