@@ -164,7 +164,9 @@ def rows_attention(
     q_stride, out_stride, k_stride = q.stride(), out.stride(), keys.stride()
     v_stride = k_stride if values is None else values.stride()
     if q_stride[-1] != 1 or out_stride[-1] != 1 or k_stride[-1] != 1 or v_stride[-1] != 1:
-        raise _native.NotCovered("q, out, keys and values must have a unit stride over the head dim")
+        strides = {"q": q_stride, "out": out_stride, "keys": k_stride, "values": v_stride}
+        name = next(n for n, stride in strides.items() if stride[-1] != 1)
+        raise _native.NotCovered(f"{name} must have a unit stride over the head dim")
     if part_out.dtype != torch.float32 or part_lse.dtype != torch.float32 or not part_out.is_contiguous():
         raise _native.NotCovered("the partials are contiguous fp32 scratch")
     table_stride = table.stride()

@@ -35,3 +35,20 @@ def test_rows_a_request(count):
         rows_attention(q, cache, cache, torch.zeros_like(q), torch.zeros(192, 64), torch.zeros(192), known.zeros(1, 3), known.zeros(1), None,
                        rows_per_request=count, step=0, window=0, scale=1.0, launch=RowsLaunch(splits=2, block_n=32), table_page=16,
                        k_scale=torch.ones(5, 2), v_scale=torch.ones(5, 2))
+
+
+@pytest.mark.parametrize("name", ["q", "out", "keys", "values"])
+@pytest.mark.parametrize("scales", [False, True])
+def test_the_tensor_without_a_unit_stride_is_named(name, scales):
+    from eagle_harness.kernels._native import NotCovered
+    from eagle_harness.kernels.row_attention import RowsLaunch, rows_attention
+
+    cached = torch.float8_e4m3fn if scales else BF16
+    x = dict(q=known.zeros(2, 4, 64, dtype=BF16), out=known.zeros(2, 4, 64, dtype=BF16), keys=known.zeros(5, 16, 2, 64, dtype=cached),
+             values=known.zeros(5, 16, 2, 64, dtype=cached))
+    x[name] = torch.zeros(*x[name].shape[:-1], 128, dtype=x[name].dtype)[..., ::2]
+    ks, vs = (torch.ones(5, 2), torch.ones(5, 2)) if scales else (None, None)
+    with pytest.raises(NotCovered, match=f"^{name} must"):
+        rows_attention(x["q"], x["keys"], x["values"], x["out"], torch.zeros(192, 64), torch.zeros(192), known.zeros(1, 3), known.zeros(1), None,
+                       rows_per_request=2, step=0, window=0, scale=1.0, launch=RowsLaunch(splits=2, block_n=32), table_page=16,
+                       k_scale=ks, v_scale=vs)
