@@ -76,6 +76,29 @@ def itab(t: Optional[torch.Tensor]) -> ITab:
     return ITab(t.data_ptr(), strides[0] if n else 0, strides[1] if n > 1 else 0, code, 0)
 
 
+def apart(a: int, a_dims: tuple, a_width: int, b: int, b_dims: tuple, b_width: int) -> bool:
+    """Whether two strided tensors are known to share no byte: pieces of ``width`` bytes from an address on, repeated along ``dims``,
+    (count, stride in bytes) each. Either one ends before the other begins, or, modulo some stride that divides all that are not
+    below it, each lies within a range of its own (columns of one wider row, heads of one packed projection)."""
+
+    def extent(dims, width, step):
+        for count, stride in dims:
+            if count > 1 and stride % step:
+                if stride > step:
+                    return step + 1
+                width += (count - 1) * stride
+        return width
+
+    spans = [width + sum((count - 1) * stride for count, stride in dims) for dims, width in ((a_dims, a_width), (b_dims, b_width))]
+    if any(count == 0 for count, _ in (*a_dims, *b_dims)) or a + spans[0] <= b or b + spans[1] <= a:
+        return True
+    for step in {stride for count, stride in (*a_dims, *b_dims) if count > 1 and stride > 0}:
+        from_a = (b - a) % step
+        if extent(a_dims, a_width, step) <= from_a and from_a + extent(b_dims, b_width, step) <= step:
+            return True
+    return False
+
+
 def _fields(spec: str) -> list:
     """Fields from a compact spec: ``name:type`` pairs, type one of p (pointer), q (int64), i (int32), f (float),
     d (double), t (ITab)."""

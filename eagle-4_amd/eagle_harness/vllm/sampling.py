@@ -66,9 +66,11 @@ def _out_stride(what: str, name: str, out: torch.Tensor, logits: torch.Tensor) -
 
 
 def _overlap(logits: torch.Tensor, out: torch.Tensor, out_stride: int) -> bool:
-    (rows, vocab), a, b = logits.shape, logits.data_ptr(), out.data_ptr()
-    return rows > 0 and (a < b + out.element_size() * ((rows - 1) * out_stride + vocab)
-                         and b < a + logits.element_size() * ((rows - 1) * logits.stride(0) + vocab))
+    (rows, vocab), a, b, size, out_size = logits.shape, logits.data_ptr(), out.data_ptr(), logits.element_size(), out.element_size()
+    stride = logits.stride(0)
+    if rows == 0 or a >= b + out_size * ((rows - 1) * out_stride + vocab) or b >= a + size * ((rows - 1) * stride + vocab):
+        return False
+    return not _native.apart(a, ((rows, size * stride),), size * vocab, b, ((rows, out_size * out_stride),), out_size * vocab)
 
 
 def draw_tokens(
@@ -91,7 +93,7 @@ def draw_tokens(
     padded one) gets tokens of 0, which a captured step may look up; its row of ``probs`` is left as it was.
 
     With ``Z`` the mass kept, the token is the first of the order whose running mass exceeds ``coin * Z``. ``probs`` [rows,
-    vocab] (bf16 / fp16 / fp32, memory of its own) is filled with ``w / Z`` on the kept tokens, 0 elsewhere.
+    vocab] (bf16 / fp16 / fp32, no element shared with the logits) is filled with ``w / Z`` on the kept tokens, 0 elsewhere.
     """
     code, fields = _rows_args("draw_tokens", logits, temperature, top_k, top_p, min_p, entries)
     rows, vocab = logits.shape

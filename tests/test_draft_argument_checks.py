@@ -52,3 +52,44 @@ def test_the_tensor_without_a_unit_stride_is_named(name, scales):
         rows_attention(x["q"], x["keys"], x["values"], x["out"], torch.zeros(192, 64), torch.zeros(192), known.zeros(1, 3), known.zeros(1), None,
                        rows_per_request=2, step=0, window=0, scale=1.0, launch=RowsLaunch(splits=2, block_n=32), table_page=16,
                        k_scale=ks, v_scale=vs)
+
+
+@pytest.mark.parametrize("seed", range(40))
+def test_tensors_known_to_be_apart(seed):
+    """Against the bytes themselves: what is called apart shares none; and layouts that are used are called apart."""
+    import random
+
+    from eagle_harness.kernels._native import apart
+
+    rng = random.Random(seed)
+
+    def touched(at, dims, width):
+        places = [at]
+        for count, stride in dims:
+            places = [p + i * stride for p in places for i in range(count)]
+        return {p + i for p in places for i in range(width)}
+
+    for _ in range(400):
+        steps = rng.choice(([24, 96], [96, 24], [8, 40], [0, 16], [16, 16], [30, 7]))
+        other = steps if rng.random() < 0.7 else [rng.randint(0, 100) for _ in steps]
+        one = (rng.randint(0, 60), tuple((rng.randint(0, 4), s) for s in steps), rng.randint(1, 30))
+        two = (rng.randint(0, 60), tuple((rng.randint(0, 4), s) for s in other), rng.randint(1, 30))
+        if touched(*one) & touched(*two):
+            assert not apart(*one, *two)
+    assert apart(1000, ((5, 80),), 40, 1040, ((5, 80),), 40) and not apart(1000, ((5, 80),), 40, 1038, ((5, 80),), 40)
+    assert apart(0, ((3, 96), (2, 48)), 24, 24, ((3, 96), (2, 48)), 24)  # halves of every head
+    assert apart(0, ((3, 96), (2, 12)), 12, 24, ((3, 96), (2, 12)), 12)  # heads of one packed row
+    assert apart(0, ((1, 7), (4, 16)), 8, 8, ((4, 16),), 8)
+
+
+@pytest.mark.parametrize("at,error", [(10, RuntimeError), (9, ValueError), (5, ValueError), (0, ValueError)])
+def test_outputs_in_other_columns_of_the_logits_store(at, error):
+    """Rows of one wider buffer: columns of their own are taken (and refused by the launch alone), shared ones are not."""
+    wide = torch.zeros(3, 20)
+    with pytest.raises(error):
+        known.draw(logits=wide[:, :10], probs=wide[:, at : at + 10])
+    if at:
+        with pytest.raises(error):
+            known.draw(truncate=True, logits=wide[:, :10], out=wide[:, at : at + 10])
+        with pytest.raises(error):
+            known.draw(truncate=True, logits=wide[:, at : at + 10], out=wide[:, :10])
