@@ -91,7 +91,9 @@ def _half(name: str, x: torch.Tensor, out: Optional[torch.Tensor], like: tuple) 
         if tokens and heads and (at != out_at or to != stride):
             span = ((tokens - 1) * stride[0] + (heads - 1) * stride[1] + dim) * size
             if at < out_at + ((tokens - 1) * to[0] + (heads - 1) * to[1] + dim) * size and out_at < at + span:
-                raise ValueError(f"rotate_rows: {name}_out may be {name} itself, but not overlap it otherwise")
+                layout = lambda strides: ((tokens, strides[0] * size), (heads, strides[1] * size))  # noqa: E731
+                if not _native.apart(at, layout(stride), dim * size, out_at, layout(to), dim * size):
+                    raise ValueError(f"rotate_rows: {name}_out may be {name} itself, but not overlap it otherwise")
     (near, count), (far, others) = ((to[1], heads), (to[0], tokens)) if to[1] <= to[0] else ((to[0], tokens), (to[1], heads))
     if tokens and heads and ((count > 1 and near < dim) or (others > 1 and far < (near * (count - 1) if count > 1 else 0) + dim)):
         raise ValueError(f"rotate_rows: heads of the output of {name} overlap: every one needs its own storage")

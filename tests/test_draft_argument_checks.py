@@ -93,3 +93,23 @@ def test_outputs_in_other_columns_of_the_logits_store(at, error):
             known.draw(truncate=True, logits=wide[:, :10], out=wide[:, at : at + 10])
         with pytest.raises(error):
             known.draw(truncate=True, logits=wide[:, at : at + 10], out=wide[:, :10])
+
+
+def heads_of(first, last, lead=0, tokens=4, heads=5, dim=16):
+    return lambda store: store[lead:].view(-1)[: tokens * heads * dim].view(tokens, heads, dim)[:, first:last]
+
+
+@pytest.mark.parametrize("q,out,error", [
+    (heads_of(0, 2), heads_of(2, 4), RuntimeError),  # other heads of one packed row
+    (heads_of(3, 5), heads_of(0, 2), RuntimeError),
+    (heads_of(0, 2), heads_of(1, 3), ValueError),
+    (heads_of(0, 2), heads_of(2, 4, lead=8), RuntimeError),
+    (heads_of(0, 2), heads_of(1, 3, lead=8), ValueError),
+    (lambda s: s[:320].view(4, 5, 16)[..., :8], lambda s: s[:320].view(4, 5, 16)[..., 8:], RuntimeError),  # halves of every head
+    (lambda s: s[:320].view(5, 4, 16).transpose(0, 1)[:, :2], lambda s: s[:320].view(5, 4, 16).transpose(0, 1)[:, 2:4], RuntimeError),
+    (lambda s: s[:320].view(5, 4, 16).transpose(0, 1)[:, :2], lambda s: s[:320].view(5, 4, 16).transpose(0, 1)[:, 1:3], ValueError),
+])
+def test_rotated_rows_beside_their_inputs(q, out, error):
+    store = torch.zeros(400)
+    with pytest.raises(error):
+        known.rotate(q=q(store), q_out=out(store), k=None)

@@ -28,3 +28,20 @@ def test_columns_beside_the_logits(dev, dtype, vocab):
         assert truncate_logits(x, *rules, out=beside) is beside
         assert torch.equal(beside, truncate_logits(alone, *rules)) and torch.equal(x, alone)
         assert (wide[:, :1] == 9).all() and (wide[:, 2 * vocab + 1 :] == 9).all()
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dim,part", [(128, 128), (96, 64), (20, 6)])
+def test_heads_beside_the_rotated_ones(dev, dim, part, interleaved):
+    """The parts of one packed projection, rotated into other parts of it."""
+    from eagle_harness.vllm.rotary import rotary_frequencies, rotate_rows
+
+    announce(f"rotated beside the inputs {part} of {dim} interleaved={interleaved}")
+    gen = torch.Generator().manual_seed(dim)
+    packed = torch.randn(37, 12, dim, generator=gen).bfloat16().to(dev)
+    k_out = torch.empty(37, 2, dim, dtype=packed.dtype, device=dev)
+    before, at, f = packed.clone(), torch.arange(37, device=dev) * 1001, rotary_frequencies(part, device=dev)[0]
+    rotate_rows(packed[:, 0:4], packed[:, 4:6], at, f, interleaved=interleaved, q_out=packed[:, 7:11], k_out=k_out)
+    q, k = rotate_rows(before[:, 0:4].clone(), before[:, 4:6].clone(), at, f, interleaved=interleaved)
+    assert torch.equal(packed[:, 7:11], q) and torch.equal(k_out, k)
+    assert torch.equal(packed[:, :7], before[:, :7]) and torch.equal(packed[:, 11:], before[:, 11:])
