@@ -108,7 +108,8 @@ def slot_maps(
             raise ValueError(f"slot_maps: every tensor must be on {block_table.device}")
         at, to = block_table.data_ptr(), batch_table.data_ptr()
         if requests and at < to + 4 * ((requests - 1) * batch_stride + most) and to < at + 4 * ((state_slots - 1) * stride + most):
-            raise ValueError("slot_maps: batch_table must not overlap block_table")
+            if not _native.apart(at, ((state_slots, 4 * stride),), 4 * most, to, ((requests, 4 * batch_stride),), 4 * most):
+                raise ValueError("slot_maps: batch_table must not overlap block_table")
     if context_lens.get_device() != where or query_start_loc.get_device() != where or slots.get_device() != where:
         raise ValueError(f"slot_maps: every tensor must be on {block_table.device}")
     if requests == 0 and slots.shape[0] == 0:

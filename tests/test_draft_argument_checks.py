@@ -113,3 +113,10 @@ def test_rotated_rows_beside_their_inputs(q, out, error):
     store = torch.zeros(400)
     with pytest.raises(error):
         known.rotate(q=q(store), q_out=out(store), k=None)
+
+
+@pytest.mark.parametrize("at,error", [(4, RuntimeError), (5, RuntimeError), (3, ValueError), (0, ValueError)])
+def test_a_batch_table_beside_the_block_table(at, error):
+    wide = known.zeros(3, 9)
+    with pytest.raises(error):
+        known.maps(table=wide[:, :4], batch=wide[:2, at : at + 4])

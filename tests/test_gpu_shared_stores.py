@@ -45,3 +45,20 @@ def test_heads_beside_the_rotated_ones(dev, dim, part, interleaved):
     q, k = rotate_rows(before[:, 0:4].clone(), before[:, 4:6].clone(), at, f, interleaved=interleaved)
     assert torch.equal(packed[:, 7:11], q) and torch.equal(k_out, k)
     assert torch.equal(packed[:, :7], before[:, :7]) and torch.equal(packed[:, 11:], before[:, 11:])
+
+
+def test_a_batch_table_beside_the_block_table(dev):
+    from eagle_harness.vllm.page_tables import slot_maps
+
+    announce("a batch table beside the block table")
+    i32 = dict(dtype=torch.int32, device=dev)
+    wide = torch.full((6, 21), -7, **i32)
+    table, batch = wide[:, :10], wide[:3, 10:20]
+    table.copy_(torch.arange(60, **i32).view(6, 10))
+    before, pages = table.clone(), torch.tensor([10, 3, 0, 7, 1, 5], **i32)
+    idx, context, starts = torch.tensor([3, 0, 2], **i32), torch.tensor([100, 20, 0], **i32), torch.tensor([0, 9, 19, 22], **i32)
+    got = slot_maps(table, pages, idx, context, starts, 16, slots=torch.empty(25, dtype=torch.int64, device=dev), batch_table=batch)
+    want = slot_maps(before, pages, idx, context, starts, 16, slots=torch.empty(25, dtype=torch.int64, device=dev),
+                     batch_table=torch.empty(3, 10, **i32))
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and torch.equal(table, before)
+    assert (wide[:, 20] == -7).all() and (wide[3:, 10:] == -7).all()
