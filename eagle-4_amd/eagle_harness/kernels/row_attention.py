@@ -39,6 +39,7 @@ class RowsLaunch:
 
 
 STEP_WAVES = 4.0
+_MOST = (1 << 31) - 1  # of a 32-bit field; a longer window is the whole context
 STEP = RowsLaunch(splits=64, block_n=32, num_warps=2, num_stages=3)
 
 
@@ -172,6 +173,8 @@ def rows_attention(
     table_stride = table.stride()
     if table.dtype != torch.int32 or table_stride[-1] != 1:
         raise _native.NotCovered("the page table must be int32 with unit stride")
+    if abs(table_page) > _MOST:
+        raise ValueError(f"table_page must be at most {_MOST}, got {table_page}")
     bs = rows // rows_per_request
     kst, vst = _cache_strides(k_stride), _cache_strides(v_stride)
     anc = None
@@ -184,7 +187,7 @@ def rows_attention(
         min(part_out.shape[0], part_lse.numel()), table.data_ptr(), table_stride[0], _native.itab(table_rows),
         _native.itab(seq_lens), _native.ptr(anc), anc.shape[-1] if anc is not None else 1, table_page,
         1 if len(k_stride) == 3 else keys.shape[1], bs, rows_per_request, rows_padded(rows_per_request), heads, kv_heads, head_dim,
-        _native.dtype_code(q.dtype), step, window, launch.splits, scale)
+        _native.dtype_code(q.dtype), step, min(window, _MOST), launch.splits, scale)
     if k_scale is None:
         _native.launch("eagle4_row_attention", args, q.device)
         return

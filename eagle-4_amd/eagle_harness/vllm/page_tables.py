@@ -26,8 +26,8 @@ def _tables(what: str, block_table: torch.Tensor, num_pages: torch.Tensor, idx_m
         raise _native.NotCovered(f"{what}: block_table must have a unit column stride and rows of their own storage")
     if num_pages.shape != (slots,) or not num_pages.is_contiguous():
         raise ValueError(f"{what}: num_pages must be contiguous, one entry for each of the {slots} slots")
-    if idx_mapping.dim() != 1 or page < 1:
-        raise ValueError(f"{what}: idx_mapping must be a vector and page positive")
+    if idx_mapping.dim() != 1 or not 0 < page < 1 << 31:
+        raise ValueError(f"{what}: idx_mapping must be a vector and page from 1 to 2^31 - 1")
     if num_pages.get_device() != where or idx_mapping.get_device() != where:
         raise ValueError(f"{what}: every tensor must be on {block_table.device}")
     return slots, most, stride, idx_mapping.shape[0], where

@@ -120,3 +120,33 @@ def test_a_batch_table_beside_the_block_table(at, error):
     wide = known.zeros(3, 9)
     with pytest.raises(error):
         known.maps(table=wide[:, :4], batch=wide[:2, at : at + 4])
+
+
+@pytest.mark.parametrize("page", [(1 << 31), (1 << 32) + 16, -16])
+def test_page_sizes_past_32_bits(page):
+    for call in (known.resize, known.maps):
+        with pytest.raises(ValueError):
+            call(page=page)
+
+
+@pytest.mark.parametrize("scales", [False, True])
+def test_windows_and_table_pages_past_32_bits(monkeypatch, scales):
+    """A window longer than 32 bits is the longest, not what its low bits say; a table page is refused."""
+    from eagle_harness.kernels import _native, row_attention
+
+    given = []
+    monkeypatch.setattr(_native, "launch", lambda name, args, device: given.append(args.rows if scales else args))
+    q, cache = known.zeros(2, 4, 64, dtype=BF16), known.zeros(5, 16, 2, 64, dtype=torch.float8_e4m3fn if scales else BF16)
+    ks, vs = (torch.ones(5, 2), torch.ones(5, 2)) if scales else (None, None)
+
+    def call(window, page=16):
+        row_attention.rows_attention(q, cache, cache, torch.zeros_like(q), torch.zeros(192, 64), torch.zeros(192), known.zeros(1, 3),
+                                     known.zeros(1), None, rows_per_request=2, step=0, window=window, scale=1.0,
+                                     launch=row_attention.RowsLaunch(splits=2, block_n=32), table_page=page, k_scale=ks, v_scale=vs)
+
+    for window, want in ((0, 0), (5, 5), ((1 << 31) - 1, (1 << 31) - 1), (1 << 31, (1 << 31) - 1), ((1 << 32) + 5, (1 << 31) - 1)):
+        call(window)
+        assert given[-1].window == want
+    for page in (1 << 31, (1 << 32) + 16, -(1 << 32) + 16):
+        with pytest.raises(ValueError):
+            call(0, page)
