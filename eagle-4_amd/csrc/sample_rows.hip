@@ -972,28 +972,6 @@ E4_DEV void write_shares(const Rows<T>& r, const Cut& cut, Shared& s, const Bins
   }, share, shares);
 }
 
-// A row without rules: its tokens are 0, a token like any other for what looks them up next, and its logits are copied where that is asked.
-template <typename T>
-E4_DEV void padded_row(const eagle4_sample_rows_args& a, int64_t n, int share, int shares, int64_t* tokens, u32x4* ends, int tid) {
-  constexpr int VEC = Row<T>::VEC;
-  using S = typename T::storage;
-  if (tokens != nullptr && tid < a.draws) tokens[tid] = 0;
-  if (a.copy_padded == 0) return;
-  const Rows<T> r(a.logits, n, a.stride_row, a.vocab, ends, tid);
-  S* const out = static_cast<S*>(a.out) + n * a.stride_out;
-  r.template each_vector<Rows<T>::kAhead>([&](int e0, const u32x4& w, auto) {
-    S y[VEC];
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      if constexpr (sizeof(S) == 4)
-        y[i] = __uint_as_float(w[i]);
-      else
-        y[i] = static_cast<S>(w[i / 2] >> (16 * (i % 2)));
-    }
-    store_vector(out, e0, a.vocab, y);
-  }, share, shares);
-}
-
 template <typename T>
 __global__ __launch_bounds__(NT) void sample_rows_kernel(const eagle4_sample_rows_args a, int shares) {
   __shared__ Shared s;
@@ -1002,15 +980,23 @@ __global__ __launch_bounds__(NT) void sample_rows_kernel(const eagle4_sample_row
   const int share = blockIdx.x % static_cast<uint32_t>(shares);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t entry = uniform(a.entries.ptr != nullptr ? e4::ld(a.entries, n) : n);
-  int64_t* const tokens = a.tokens != nullptr && share == 0 ? a.tokens + n * a.draws : nullptr;
-  if (entry < 0 || entry >= a.num_entries) {
-    padded_row<T>(a, n, share, shares, tokens, s.ends, tid);
+  if (entry < 0 || entry >= a.num_entries) {  // a padded row: tokens of 0, like any other for what looks them up next, and its logits
+    if (a.tokens != nullptr && share == 0 && tid < a.draws) a.tokens[n * a.draws + tid] = 0;
+    // (one by one, 768 such rows 244 us: whole vectors, as the other rows have them, cost those 0.3 us of 16 by their code alone)
+    if (a.copy_padded != 0) {
+      using S = typename T::storage;
+      const S* const from = static_cast<const S*>(a.logits) + n * a.stride_row;
+      S* const to = static_cast<S*>(a.out) + n * a.stride_out;
+#pragma unroll 8
+      for (int i = share * NT + tid; i < a.vocab; i += shares * NT) to[i] = from[i];
+    }
     return;
   }
   const float temperature = uniform(a.temperature[entry]);
   const int k = uniform(a.top_k != nullptr ? a.top_k[entry] : 0);
   const float p = uniform(a.top_p != nullptr ? a.top_p[entry] : 1.f), m = uniform(a.min_p != nullptr ? a.min_p[entry] : 0.f);
 
+  int64_t* const tokens = a.tokens != nullptr && share == 0 ? a.tokens + n * a.draws : nullptr;
   const float* const coins = a.coins != nullptr ? a.coins + n * a.draws : nullptr;
   if (tid < 64) s.roots[tid] = exp2(tid * -1.0 / 64);
   const float coin = tokens != nullptr && tid < a.draws ? coins[tid] : 0.f;  // (here, beside the row's first loads)
