@@ -3,9 +3,10 @@
 //
 // eagle4_resize_tables: one workgroup. The stack of free pages is one sequence, so which entries a request gives or takes follows
 // from running sums over the batch; a chunk of 1024 requests has its sums in LDS, and the threads take the pages that move, finding
-// the request of a page by its place in the sums. What bounds it is latency: rounds of loads that depend on each other (slots and
+// the request of a page by its place in the sums. What bounds a round is latency: loads that depend on each other (slots and
 // lengths, page counts, then the pages of both directions). 64 requests by a few pages, up and back with both maps of their
-// rows, take 15.3 us in a graph; more workgroups would have to wait for each other's sums, which costs more than this one's loads.
+// rows, take 15.3 us in a graph. Where many pages move it is this one workgroup's searches, in proportion to the pages (65 thousand of them
+// 103 us, below): there a launch for the sums and one of many workgroups for the moves would be faster. It is not built.
 //
 // eagle4_slot_maps: some workgroups a request, each with its share of the request's rows and table entries; no row is searched for.
 

@@ -459,9 +459,9 @@ __global__ __launch_bounds__(256) void row_merge_fp8_kernel(const eagle4_row_att
 
 // The splits that are used of those that the caller has scratch for: as many as fill the GPU's 256 CUs with resident workgroups
 // once, but none of fewer than 256 keys, as far as the window or the page table bound them. A workgroup's start and
-// end cost as much as some tiles: 32 requests' extends (54 rows a head, D 256, window 2048) 48 us with 2 splits, 87 with 8; 64 draft
-// steps (16 rows, D 128, window 4096) 134 with 2, 132 with 4, 135 with 8, 193 with 1 or 32; one over 4096 keys 39 with 1, 11 with 16.
-// (Taken without the values' streaming hint, which saves 3 to 5% of each.)
+// end cost as much as some tiles: 32 requests' extends (54 rows a head, D 256, window 2048) 53 us with 2 splits, 60 with 1, 88 with 8; 64
+// draft steps (16 rows, D 128, window 4096) 113 with 2, 112 with 4, 119 with 8, 175 with 1, 171 with 32; one over 4096 keys 39.5 with 1,
+// 11.4 with 16, 13.5 with 64.
 int used_splits(const eagle4_row_attn_fp8_args& x, int resident, int groups) {
   const eagle4_row_attn_args& a = x.rows;
   const int64_t bound = a.window > 0 ? static_cast<int64_t>(a.window) + a.rows_per_request : static_cast<int64_t>(x.table_width) * a.table_page;

@@ -26,10 +26,11 @@
 // 4. An output is filled and the listed tokens put in, or written in a last pass where no list holds all that is kept.
 //
 // What bounds it: 256 rows of 151936 bf16 logits, a draw and fp32 shares each (the least traffic: 233 MB, 46 us) take 58 us
-// where top-k 20 keeps a list in every row, 70 with top-p 0.95 alone, 86 where all is kept; 1024 rows cut (94 us) 120 to 126 us: the
-// second pass and the bins' LDS additions, beside HBM. A single row takes 16 us: its passes' latency on one CU, where a row
-// split over workgroups would need launches or a wait between them. Few rows with an output are shared by workgroups that all
-// find the cut: 16 rows cut take 22 us.
+// where top-k 20 keeps a list in every row, 70 with top-p 0.95 alone, 86 where all is kept; 1024 rows cut (94 us) 118 to 129 us: the
+// second pass and the bins' LDS additions, beside HBM. A single row that top-k, min-p or T bounds takes 9 to 22 us: its passes' latency
+// on one CU. One that no rule bounds takes 34 to 41 us in bf16, 53 to 90 in fp16 and 61 to 83 in fp32, which have no bins by value:
+// all of it is counted or weighed by one CU, where more could share it with launches or a wait between them (not tried).
+// Few rows with an output are shared by workgroups that all find the cut: 16 rows cut take 22 us.
 
 #include <type_traits>
 
@@ -882,7 +883,7 @@ E4_DEV void write_few(const Shared& s, int kept, const Cut& cut, int vocab, cons
   for (int i = 0; i < N; ++i) y[i] = Out::none();
   for (int v = share * NT + tid; v < vectors; v += shares * NT) store_vector(out.out, v * N - past, vocab, y);
   // Every wave waits for its own fill to arrive, then for the others', so that no token is overwritten. (A fence that other XCDs
-  // see would write the cache back: 70 us and more.)
+  // see writes the fill back from the cache: 70 us and more here.)
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
   const auto put = [&](int e, float x) {
