@@ -6,7 +6,7 @@ from __future__ import annotations
 def resized(table, pages, idx, lens, stack, capacity, page):
     """``table`` (lists of pages a slot), ``pages`` and ``stack`` (the free ones) in place."""
     slots, most = len(table), len(table[0])
-    if len(stack) + sum(max(0, pages[s] - -(-n // page)) for s, n in zip(idx, lens) if 0 <= s < slots) > capacity:
+    if len(stack) + sum(max(0, pages[s] - -(-max(n, 0) // page)) for s, n in zip(idx, lens) if 0 <= s < slots) > capacity:
         return
     for s, n in reversed(list(zip(idx, lens))):
         need = -(-max(n, 0) // page)
