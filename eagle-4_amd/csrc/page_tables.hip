@@ -156,6 +156,8 @@ __global__ __launch_bounds__(kMapThreads) void slot_maps_kernel(const eagle4_slo
     held = held < a.max_pages ? held : a.max_pages;
     const int32_t* const table = a.block_table + (known ? slot : 0) * a.stride_table;
     const int64_t last = end < a.rows ? end : a.rows;
+    if (r == 0)  // rows before the first request's
+      for (int64_t row = tid; row < start && row < a.rows; row += step) a.slots[row] = -1;
     const uint32_t page = static_cast<uint32_t>(a.page);
     for (int64_t row = (start > 0 ? start : 0) + tid; row < last; row += step) {
       const int64_t position = context + (row - start);

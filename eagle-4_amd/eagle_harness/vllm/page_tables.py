@@ -89,7 +89,7 @@ def slot_maps(
 
     Row ``j`` of request ``r`` (rows ``query_start_loc[r] ..``) is position ``context_lens[r] + j`` of state slot ``idx_mapping[r]``;
     ``slots`` (contiguous int64, as long as the batch is padded to) gets ``block_table[slot, position // page] * page + position %
-    page``, -1 where the request holds no such page, and -1 behind the last request's rows. ``batch_table`` [requests, pages] int32
+    page``, -1 where the request holds no such page, and -1 before the first and behind the last request's rows. ``batch_table`` [requests, pages] int32
     gets each request's pages and 0 behind them; request rows behind the batch are left as they were.
     """
     state_slots, most, stride, requests, where = _tables("slot_maps", block_table, num_pages, idx_mapping, page)

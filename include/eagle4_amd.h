@@ -641,8 +641,8 @@ typedef struct eagle4_resize_tables_args {
 int eagle4_resize_tables(const eagle4_resize_tables_args* args, void* stream);
 
 /* Row j of request r (rows query_start_loc[r] .. of the batch) is position context_lens[r] + j: slots[row] is its place in the
- * cache, block_table[slot, position / page] * page + position % page, or -1 where the request holds no such page, and for rows behind
- * the last request's. batch_table[r]: the request's pages, 0 behind them. */
+ * cache, block_table[slot, position / page] * page + position % page, or -1 where the request holds no such page, and for rows before
+ * the first request's and behind the last one's. batch_table[r]: the request's pages, 0 behind them. */
 typedef struct eagle4_slot_maps_args {
   const int32_t* block_table; /* [state_slots, max_pages], unit column stride */
   int64_t stride_table;
