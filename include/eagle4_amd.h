@@ -595,8 +595,8 @@ int eagle4_sample_rows(const eagle4_sample_rows_args* args, void* stream);
 
 /* ---- draft-row attention over fp8 pages (no counterpart in the reference's own sources) ----------------------------- */
 /* eagle4_row_attention's rows over e4m3 caches: a key's scores and values take its page's and head's scale. Strides of the caches
- * in elements (bytes); rows.values is not null. Table entries are taken within the table's height and width, pages within num_blocks.
- * A row that sees no key gives zeros. */
+ * in elements (bytes); rows.values is not null. Keys end with the table's width: a row behind it sees those before. Request rows are taken
+ * within the table's height, pages within num_blocks. A row that sees no key gives zeros. */
 typedef struct eagle4_row_attn_fp8_args {
   eagle4_row_attn_args rows;
   const float *k_scale, *v_scale; /* [num_blocks, kv_heads] */
@@ -608,7 +608,8 @@ int eagle4_row_attention_fp8(const eagle4_row_attn_fp8_args* args, void* stream)
 
 /* ---- rotary positions (no counterpart in the reference's own sources) ------------------------------------------------ */
 /* Pair i of a head, elements (i, half + i) or, paired, (2i, 2i + 1), is turned by positions[t] * frequencies[i] and multiplied by
- * factor; elements from 2 half on are copied. Angles in 64 bits. In place where the outputs are the inputs (both, or neither). */
+ * factor; elements from 2 half on are copied. Angles in 64 bits. In place where the outputs are the inputs (both, or neither). Below 2^24
+ * tokens; more where heads are narrow. */
 typedef struct eagle4_rotary_args {
   const void *q, *k; /* [tokens, heads, dim], unit stride over dim; k_heads 0: no keys */
   void *q_out, *k_out;
