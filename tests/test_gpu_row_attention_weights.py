@@ -56,3 +56,22 @@ def test_pages_of_zeros_alone(dev, dtype):
     got = rows._launch(dev, *[t.to(dev) for t in (q, keys, values, ks, vs, table, seq)], None, rows=3, step=0, window=0, splits=2,
                        table_page=16)
     assert (got == 0).all()
+
+
+@pytest.mark.parametrize("dim,hq", [(64, 4), (128, 32), (256, 12)])
+@pytest.mark.parametrize("bad", [5, 66, 97])
+def test_nan_codes_under_fp16_rows(dev, bad, dim, hq):
+    """A NaN code among the values of position 5 or 66 (rows at 95 to 98 see both) or of 97, which rows 2 and 3 alone see."""
+    announce(f"fp8 rows: NaN at {bad} under fp16 rows of {dim}")
+    gen = torch.Generator().manual_seed(dim)
+    page, hkv, n = 16, 2, 4
+    keys, ks = rows._cache(gen, 7, page, hkv, dim, 0.2)
+    values, vs = rows._cache(gen, 7, page, hkv, dim, 0.2)
+    table, seq = torch.arange(7).view(1, 7).int(), torch.tensor([95])
+    q = torch.randn(n, hq, dim, generator=gen).to(torch.float16)
+    run = lambda: rows._launch(dev, *[t.to(dev) for t in (q, keys, values, ks, vs, table, seq)], None, rows=n, step=0, window=0,  # noqa: E731
+                               splits=2, table_page=page).cpu()
+    want = run()
+    values.view(torch.uint8)[bad // page, bad % page, 0, 33] = 0x7F
+    want[2 if bad == 97 else 0 :, : hq // 2, 33] = torch.nan
+    assert torch.equal(run().nan_to_num(99.0), want.nan_to_num(99.0))
